@@ -241,7 +241,7 @@ def _run_own(s):
     outputs = tuple(s[name] for name in _OUTPUTS[op])
     if case["prepared"]:  # a decoding loop binds its buffers once and launches for every token
         if "call" not in s:
-            s["call"] = artifact.prepare_call(inputs, outputs=outputs)
+            s["call"] = artifact.prepare(*inputs, outputs=outputs)
         s["call"].launch()
     else:
         made = artifact.run(*inputs)
