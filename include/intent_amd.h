@@ -671,6 +671,80 @@ int intent_nvfp4_quantize(const void* x, int64_t M, int64_t N, int64_t x_ld, con
 int intent_i8_per_token_quantize(const void* x, int x_is_bf16, int64_t M, int64_t K, int64_t x_ld,
                                  int8_t* q, int64_t q_ld, float* scales, void* stream);
 
+/*
+ * Norms of queries and keys for each head and the position rotation, in one
+ * pass: q [T, HQ, D] and k [T, HK, D], f16 or bf16 (is_bf16), token strides
+ * q_ld and k_ld elements (slices of one projection's rows), to q_out and k_out.
+ *   y = x * rsqrt(mean(x^2) + eps) * weight over the D elements of a head (a
+ *       null weight: no norm; weights [D] of the heads' type),
+ *   then the first R elements rotated as pairs (a, b), (i, i + R/2) or
+ *   (2i, 2i + 1) when `interleaved`: (a cos - b sin, b cos + a sin), with
+ *   cos_sin f32 [P, R] (cos_sin_ld): R/2 cosines, then R/2 sines, of positions[t]
+ *   (i32 [T], clamped to the table). R = 0: no rotation.
+ * f32 throughout, one rounding at the end. D % 8 == 0, D <= 512, R % 16 == 0,
+ * 16-byte aligned heads. No reference counterpart.
+ */
+int intent_qk_norm_rope(const void* q, int64_t T, int64_t HQ, int64_t q_ld,
+                        const void* k, int64_t HK, int64_t k_ld, int64_t D,
+                        const void* q_weight, const void* k_weight, float eps,
+                        const float* cos_sin, int64_t P, int64_t R, int64_t cos_sin_ld,
+                        int interleaved, const int32_t* positions, int is_bf16,
+                        void* q_out, int64_t q_out_ld, void* k_out, int64_t k_out_ld,
+                        void* stream);
+
+/*
+ * The same pass with the keys, and the values v [T, HK, D] (v_ld) as they are,
+ * appended to a paged cache [pages][HK][page_size][D] (k_page_ld, v_page_ld
+ * elements from a page to the next; page_size a power of two): token t goes to
+ * slot slots[t] = page * page_size + place. A negative slot (a padded row) or
+ * one past the cache is skipped; its q_out row is written all the same. Slots
+ * of one call are distinct: one given twice ends with rows of either token.
+ * The cache holds the heads' type, or E4M3FN codes (cache_is_fp8) with scales
+ * f32 [pages][HK][page_size] (k_scales_ld, v_scales_ld from a page to the next):
+ * scale = max(absmax, 1e-12) / 448 of a token's head, code = e4m3fn(clamp(y /
+ * scale, +-448)), the rule of intent_fp8_groupwise_quantize for bf16 with one
+ * group for each head. Everything else in the cache stays as it is.
+ * No reference counterpart.
+ */
+int intent_paged_kv_append(const void* q, int64_t T, int64_t HQ, int64_t q_ld,
+                           const void* k, int64_t HK, int64_t k_ld,
+                           const void* v, int64_t v_ld, int64_t D,
+                           const void* q_weight, const void* k_weight, float eps,
+                           const float* cos_sin, int64_t P, int64_t R, int64_t cos_sin_ld,
+                           int interleaved, const int32_t* positions, const int32_t* slots,
+                           int is_bf16, int cache_is_fp8,
+                           void* k_cache, int64_t k_page_ld, void* v_cache, int64_t v_page_ld,
+                           float* k_scales, int64_t k_scales_ld,
+                           float* v_scales, int64_t v_scales_ld,
+                           int64_t pages, int64_t page_size,
+                           void* q_out, int64_t q_out_ld, void* stream);
+
+/*
+ * Attention of new tokens over the paged cache that intent_paged_kv_append
+ * fills. Sequence s owns the rows q_offsets[s] .. q_offsets[s+1] of q and out
+ * [T, HQ, D] (q_ld, out_ld) and the first kv_lens[s] tokens of its pages
+ * page_table[s][0 .. table_width) (i32, table_ld), its new tokens last. Row i of
+ * n stands at p = kv_len - n + i and sees the tokens t < kv_len with t <= p
+ * (causal) and t > p - window (window > 0):
+ *   out = sum_t softmax_t(scale q.k_t) v_t,  HQ / HK query heads to a cached head;
+ * a row that sees nothing (an empty cache, more new tokens than cached ones)
+ * is zero, rows of no sequence are not written, and what a row does not see
+ * does not reach it, whatever it holds. f32 scores, softmax and sums; the
+ * weights are rounded to q's type for the product with the values.
+ * Lengths, offsets and page ids are clamped to the tensors, never followed out
+ * of them. D % 8 == 0, D <= 512. No reference counterpart.
+ */
+int intent_paged_attention(const void* q, int64_t T, int64_t HQ, int64_t q_ld,
+                           int is_bf16, int cache_is_fp8,
+                           const void* k_cache, int64_t k_page_ld, const void* v_cache, int64_t v_page_ld,
+                           const float* k_scales, int64_t k_scales_ld,
+                           const float* v_scales, int64_t v_scales_ld,
+                           int64_t pages, int64_t HK, int64_t page_size, int64_t D,
+                           const int32_t* page_table, int64_t S, int64_t table_width, int64_t table_ld,
+                           const int32_t* q_offsets, const int32_t* kv_lens,
+                           float scale, int causal, int64_t window,
+                           void* out, int64_t out_ld, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

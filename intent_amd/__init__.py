@@ -53,6 +53,16 @@ from .definitions import (
     w8a8_scaled_matmul,
     weight_only_int4_asym_matmul,
     weight_only_int8_matmul,
+    qk_norm_rope,
+    bf16_qk_norm_rope,
+    paged_kv_append,
+    bf16_paged_kv_append,
+    paged_kv_append_fp8,
+    bf16_paged_kv_append_fp8,
+    paged_attention,
+    bf16_paged_attention,
+    paged_attention_fp8,
+    bf16_paged_attention_fp8,
 )
 from .errors import CompilationStageError, LanguageUseError, NativeLibraryError
 from .interface import DType, PublicInterface, ScalarParameter, ViewKind, ViewParameter
@@ -72,4 +82,7 @@ __all__ = [
     "moe_expert_ffn", "moe_expert_ffn_w4", "moe_gate_up_w4", "moe_route_topk", "q4_k_q8_k_dot", "q8_k_quantize",
     "quantized_projection", "w8a8_scaled_matmul", "weight_only_int4_asym_matmul",
     "weight_only_int8_matmul",
+    "qk_norm_rope", "bf16_qk_norm_rope", "paged_kv_append", "bf16_paged_kv_append", "paged_kv_append_fp8",
+    "bf16_paged_kv_append_fp8", "paged_attention", "bf16_paged_attention", "paged_attention_fp8",
+    "bf16_paged_attention_fp8",
 ]

@@ -1,0 +1,206 @@
+// Attention of new tokens over a paged cache (gfx950): the entry, and the kernel for any head size.
+#include "paged_attn.h"
+
+namespace {
+
+using namespace intent;
+
+template <bool kBf16>
+INTENT_DEVICE float widen1(uint16_t v) {
+  if constexpr (kBf16) return bit_cast<float>((uint32_t)v << 16);
+  else return (float)bit_cast<f16>(v);
+}
+
+template <bool kBf16, bool kFp8>
+INTENT_DEVICE void widen8(const void* p, float (&v)[8]) {
+  if constexpr (kFp8) {
+    const u32x2 raw = *(const u32x2*)p;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)raw[j], false);
+      const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)raw[j], true);
+      v[4 * j] = lo[0], v[4 * j + 1] = lo[1], v[4 * j + 2] = hi[0], v[4 * j + 3] = hi[1];
+    }
+  } else {
+    const u32x4 raw = load16(p);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[2 * j] = widen1<kBf16>((uint16_t)(raw[j] & 0xffffu));
+      v[2 * j + 1] = widen1<kBf16>((uint16_t)(raw[j] >> 16));
+    }
+  }
+}
+
+template <bool kBf16, bool kFp8>
+INTENT_DEVICE float widen_one(const void* cache, int64_t index) {
+  if constexpr (kFp8) return __builtin_amdgcn_cvt_f32_fp8((int)((const uint8_t*)cache)[index], 0);
+  else return widen1<kBf16>(((const uint16_t*)cache)[index]);
+}
+
+INTENT_DEVICE float wave_max(float v) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor(v, off));
+  return v;
+}
+INTENT_DEVICE float wave_sum(float v) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off);
+  return v;
+}
+
+// Any D that is a multiple of 8 up to 512: one wave for each query row. A lane takes one token of 64
+// for the products with the keys, then D / 64 columns of the values, whose tokens the wave goes
+// through one by one; tokens that the row does not see are not read.
+template <bool kBf16, bool kFp8>
+__global__ __launch_bounds__(256) void paged_attn_row_kernel(const AttnArgs a) {
+  __shared__ float qs[4][512];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t item = (int64_t)blockIdx.x * 4 + wave;
+  if (item >= (int64_t)a.T * a.HQ) return;
+  const int row = (int)(item / a.HQ), head = (int)(item - (int64_t)row * a.HQ), kv_head = head / a.group;
+  int s = -1;
+  for (int s0 = 0; s0 < a.S && s < 0; s0 += 64) {
+    bool owns = false;
+    if (s0 + lane < a.S) {
+      const Sequence q = sequence_of(a, s0 + lane);
+      owns = row >= q.start && row < q.start + q.count;
+    }
+    const uint64_t found = __ballot(owns);
+    if (found) s = s0 + __builtin_ctzll(found);
+  }
+  if (s < 0) return;  // a row of no sequence is left as it is
+  const Sequence seq = sequence_of(a, s);
+  const int p = seq.kv - seq.count + (row - seq.start);
+  const int first = first_seen(a, p), end = end_seen(a, p, seq.kv);
+  const uint16_t* q = a.q + (int64_t)row * a.q_ld + (int64_t)head * a.D;
+  for (int d = lane; d < a.D; d += 64) qs[wave][d] = widen1<kBf16>(q[d]) * a.scale_log2;
+  __builtin_amdgcn_wave_barrier();
+
+  constexpr int kBytes = kFp8 ? 1 : 2;
+  float acc[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+  float top = -INFINITY, total = 0.f;
+  for (int t0 = first; t0 < end; t0 += 64) {
+    const int t = t0 + lane;
+    float score = -INFINITY, v_scale = 1.f;
+    int page = 0;
+    if (t < end) {
+      page = page_of(a, s, t);
+      const char* k = (const char*)a.k_cache + row_in_cache(a, page, a.k_page, kv_head, t, a.D) * kBytes;
+      float sum = 0.f;
+      for (int d = 0; d < a.D; d += 8) {
+        float kv[8];
+        widen8<kBf16, kFp8>(k + d * kBytes, kv);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum = __builtin_fmaf(kv[j], qs[wave][d + j], sum);
+      }
+      if constexpr (kFp8) {
+        sum *= a.k_scales[row_in_cache(a, page, a.ks_page, kv_head, t, 1)];
+        v_scale = a.v_scales[row_in_cache(a, page, a.vs_page, kv_head, t, 1)];
+      }
+      score = sum;
+    }
+    const float m = fmaxf(top, wave_max(score));
+    const float base = m == -INFINITY ? 0.f : m;
+    const float keep = __builtin_amdgcn_exp2f(top - base);
+    const float w = t < end ? __builtin_amdgcn_exp2f(score - base) : 0.f;
+    total = total * keep + wave_sum(w);
+    const float wv = w * v_scale;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] *= keep;
+    const int n = min(end - t0, 64);
+    for (int i = 0; i < n; ++i) {
+      const float wi = __shfl(wv, i);
+      const int64_t v = row_in_cache(a, __shfl(page, i), a.v_page, kv_head, t0 + i, a.D);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (lane + 64 * j < a.D)
+          acc[j] = __builtin_fmaf(wi, widen_one<kBf16, kFp8>(a.v_cache, v + lane + 64 * j), acc[j]);
+    }
+    top = m;
+  }
+  const float inv = end > first ? 1.0f / total : 0.f;
+  uint16_t* out = a.out + (int64_t)row * a.out_ld + (int64_t)head * a.D;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (lane + 64 * j < a.D) {
+      const float o = end > first ? acc[j] * inv : 0.f;
+      if constexpr (kBf16) out[lane + 64 * j] = (uint16_t)(bf16x2_rne(o, o) & 0xffffu);
+      else out[lane + 64 * j] = bit_cast<uint16_t>((f16)o);
+    }
+  }
+}
+
+template <bool kBf16, bool kFp8>
+int launch_rows(const AttnArgs& a, hipStream_t stream) {
+  const int64_t blocks = ((int64_t)a.T * a.HQ + 3) / 4;
+  hipLaunchKernelGGL((paged_attn_row_kernel<kBf16, kFp8>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  return launch_status_fmt("paged_attn_row_kernel<%s%s>", kBf16 ? "bf16" : "f16", kFp8 ? ", fp8 cache" : "");
+}
+
+}  // namespace
+
+extern "C" int intent_paged_attention(const void* q, int64_t T, int64_t HQ, int64_t q_ld, int is_bf16,
+                                      int cache_is_fp8, const void* k_cache, int64_t k_page_ld, const void* v_cache,
+                                      int64_t v_page_ld, const float* k_scales, int64_t k_scales_ld,
+                                      const float* v_scales, int64_t v_scales_ld, int64_t pages, int64_t HK,
+                                      int64_t page_size, int64_t D, const int32_t* page_table, int64_t S,
+                                      int64_t table_width, int64_t table_ld, const int32_t* q_offsets,
+                                      const int32_t* kv_lens, float scale, int causal, int64_t window, void* out,
+                                      int64_t out_ld, void* stream) {
+  clear_error();
+  INTENT_REQUIRE(T >= 0 && HQ >= 0 && HK >= 0 && D >= 0 && S >= 0 && pages >= 0 && page_size >= 0 && table_width >= 0 &&
+                     window >= 0 && T <= INT32_MAX && HQ <= 65536 && HK <= 65536 && S < INT32_MAX &&
+                     pages <= INT32_MAX && page_size <= INT32_MAX,
+                 INTENT_ERR_INVALID_ARGUMENT, "bad extents (T=%lld HQ=%lld HK=%lld D=%lld S=%lld pages=%lld of %lld)",
+                 (long long)T, (long long)HQ, (long long)HK, (long long)D, (long long)S, (long long)pages,
+                 (long long)page_size);
+  if (T == 0 || HQ == 0 || D == 0 || S == 0) return INTENT_OK;
+  INTENT_REQUIRE(HK > 0 && HQ % HK == 0, INTENT_ERR_INVALID_ARGUMENT,
+                 "HQ=%lld query heads must be a multiple of the HK=%lld heads of the cache", (long long)HQ, (long long)HK);
+  INTENT_REQUIRE(D % 8 == 0 && D <= 512, INTENT_ERR_UNSUPPORTED, "D must be a multiple of 8 up to 512, got %lld",
+                 (long long)D);
+  const bool any = pages > 0 && page_size > 0 && table_width > 0;
+  INTENT_REQUIRE(!any || (page_size & (page_size - 1)) == 0, INTENT_ERR_UNSUPPORTED,
+                 "the page size must be a power of two, got %lld", (long long)page_size);
+  INTENT_REQUIRE(!any || table_width <= INT32_MAX / page_size, INTENT_ERR_UNSUPPORTED,
+                 "a table of %lld pages of %lld tokens exceeds 2^31 tokens", (long long)table_width,
+                 (long long)page_size);
+  // one wave for each row of a head: the grid's work items stay below 2^32
+  INTENT_REQUIRE(T * HQ < ((int64_t)1 << 26), INTENT_ERR_UNSUPPORTED,
+                 "T * HQ = %lld rows exceed the %lld a launch covers", (long long)(T * HQ), (long long)((int64_t)1 << 26));
+  INTENT_REQUIRE(q && out && q_offsets && kv_lens && (!any || (k_cache && v_cache && page_table)) &&
+                     (!any || !cache_is_fp8 || (k_scales && v_scales)),
+                 INTENT_ERR_INVALID_ARGUMENT, "null pointer argument");
+  INTENT_REQUIRE(T == 1 || (q_ld >= HQ * D && out_ld >= HQ * D), INTENT_ERR_INVALID_ARGUMENT,
+                 "token stride smaller than the heads");
+  INTENT_REQUIRE(intent::aligned16(q) && intent::aligned16(out) && (T == 1 || (q_ld % 8 == 0 && out_ld % 8 == 0)),
+                 INTENT_ERR_ALIGNMENT, "q and out must be 16-byte aligned with token strides %% 8 == 0");
+  if (any) {
+    const int64_t step = cache_is_fp8 ? 16 : 8;
+    INTENT_REQUIRE(S == 1 || table_ld >= table_width, INTENT_ERR_INVALID_ARGUMENT, "table stride smaller than the row");
+    INTENT_REQUIRE(pages == 1 || (k_page_ld >= HK * page_size * D && v_page_ld >= HK * page_size * D &&
+                                  (!cache_is_fp8 || (k_scales_ld >= HK * page_size && v_scales_ld >= HK * page_size))),
+                   INTENT_ERR_INVALID_ARGUMENT, "page stride smaller than the page");
+    INTENT_REQUIRE(intent::aligned16(k_cache) && intent::aligned16(v_cache) &&
+                       (pages == 1 || (k_page_ld % step == 0 && v_page_ld % step == 0)) &&
+                       (!cache_is_fp8 || (intent::aligned4(k_scales) && intent::aligned4(v_scales))),
+                   INTENT_ERR_ALIGNMENT, "the cache must be 16-byte aligned with page strides of whole 16 bytes");
+  }
+  AttnArgs a{};
+  a.q = (const uint16_t*)q, a.q_ld = q_ld;
+  a.k_cache = k_cache, a.v_cache = v_cache, a.k_page = k_page_ld, a.v_page = v_page_ld;
+  a.k_scales = k_scales, a.v_scales = v_scales, a.ks_page = k_scales_ld, a.vs_page = v_scales_ld;
+  a.page_table = page_table, a.table_ld = table_ld;
+  a.q_offsets = q_offsets, a.kv_lens = kv_lens;
+  a.out = (uint16_t*)out, a.out_ld = out_ld;
+  a.scale_log2 = scale * 1.44269504088896340736f;
+  a.T = (int)T, a.S = (int)S, a.HQ = (int)HQ, a.HK = (int)HK, a.group = (int)(HQ / HK), a.D = (int)D;
+  a.pages = any ? (int)pages : 0, a.page_shift = any ? __builtin_ctzll((unsigned long long)page_size) : 0;
+  a.most_kv = any ? (int)(table_width * page_size) : 0;
+  a.causal = causal != 0, a.window = (int)(window < INT32_MAX ? window : INT32_MAX);
+  hipStream_t st = (hipStream_t)stream;
+  if (cache_is_fp8) return is_bf16 ? launch_rows<true, true>(a, st) : launch_rows<false, true>(a, st);
+  return is_bf16 ? launch_rows<true, false>(a, st) : launch_rows<false, false>(a, st);
+}

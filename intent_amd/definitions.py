@@ -27,7 +27,7 @@ class Param:
     dtype: str
     dims: tuple
     access: ViewKind = IN
-    leading_stride: bool = False  # 2-D views may carry a leading stride; others must be contiguous
+    leading_stride: bool = False  # the first axis may carry any stride that holds a row; else contiguous
     free_strides: bool = False    # any strides; the definition's launch adapts the layout
 
 
@@ -1310,6 +1310,187 @@ nvfp4_quantize = KernelDefinition(
 )
 
 
+# ---- attention over a paged cache: norms and rotation, append, attention -----------
+
+def _prefix(dt: str) -> str:
+    return "" if dt == "f16" else dt + "_"
+
+
+def _heads_check(env: dict) -> None:
+    for name, extent in (("q_weight", env["WQ"]), ("k_weight", env["WK"])):
+        if extent not in (0, env["D"]):
+            raise ValueError(f"{name} must have D ({env['D']}) elements, or none for no norm, got {extent}")
+    if env["R"] > env["D"] or env["R"] % 2:
+        raise ValueError(f"cos_sin.shape[1] ({env['R']}) must be even and at most D ({env['D']})")
+    if env["D"] % 8 or env["D"] > 512 or env["R"] % 16:
+        raise NotImplementedError(f"D ({env['D']}) must be a multiple of 8 up to 512 and the rotated elements "
+                                  f"({env['R']}) a multiple of 16")
+    if env["R"] and env["T"] and not env["P"]:
+        raise ValueError("cos_sin must hold at least one position")
+
+
+def _heads_arguments(v: dict, env: dict) -> tuple:
+    """Queries and keys, as both entries take them (values between the two parts)."""
+    q, k, table = v["q"], v["k"], v["cos_sin"]
+    first = (_ptr(q), env["T"], env["HQ"], _ld(q), _ptr(k), env["HK"], _ld(k))
+    rest = (env["D"], _ptr(v["q_weight"]) if env["WQ"] else None, _ptr(v["k_weight"]) if env["WK"] else None,
+            float(env["EPS"]), _ptr(table), env["P"], env["R"], _ld(table), int(bool(env["INTERLEAVED"])),
+            _ptr(v["positions"]))
+    return first, rest
+
+
+_HEADS_CONSTEXPRS = {"EPS": 1e-6, "INTERLEAVED": False}
+
+
+def _norm_rope_definition(dt: str) -> KernelDefinition:
+    def launch(v: dict, env: dict, stream: int, workspace) -> str:
+        first, rest = _heads_arguments(v, env)
+        q_out, k_out = v["q_out"], v["k_out"]
+        _native.call("intent_qk_norm_rope", *first, *rest, int(dt == "bf16"), _ptr(q_out), _ld(q_out), _ptr(k_out),
+                     _ld(k_out), stream)
+        return "intent_qk_norm_rope"
+
+    return KernelDefinition(
+        name=_prefix(dt) + "qk_norm_rope",
+        params=(
+            Param("q", dt, ("T", "HQ", "D"), leading_stride=True),
+            Param("k", dt, ("T", "HK", "D"), leading_stride=True),
+            Param("q_weight", dt, ("WQ",)),
+            Param("k_weight", dt, ("WK",)),
+            Param("cos_sin", "f32", ("P", "R"), leading_stride=True),
+            Param("positions", "i32", ("T",)),
+            Param("q_out", dt, ("T", "HQ", "D"), OUT, leading_stride=True),
+            Param("k_out", dt, ("T", "HK", "D"), OUT, leading_stride=True),
+        ),
+        launch=launch,
+        constexprs=dict(_HEADS_CONSTEXPRS),
+        check=_heads_check,
+        reference="no kernel of the reference's quantized path; the pass between its projections and the attention",
+        doc="per head: x * rsqrt(mean(x^2) + EPS) * weight (no norm with an empty weight), then the first R elements "
+            "rotated by cos_sin[position] = (cosines, sines) of R / 2 pairs (i, i + R/2), or (2i, 2i + 1) INTERLEAVED",
+    )
+
+
+qk_norm_rope = _norm_rope_definition("f16")
+bf16_qk_norm_rope = _norm_rope_definition("bf16")
+
+
+def _page_check(env: dict) -> None:
+    if env["PAGE"] & (env["PAGE"] - 1):
+        raise NotImplementedError(f"the page size ({env['PAGE']}) must be a power of two")
+
+
+def _append_check(env: dict) -> None:
+    _heads_check(env)
+    _page_check(env)
+
+
+def _cache_params(dt: str, fp8: bool, access: ViewKind) -> tuple:
+    cache = "f8e4m3fn" if fp8 else dt
+    params = tuple(Param(f"{name}_cache", cache, ("PAGES", "HK", "PAGE", "D"), access, leading_stride=True)
+                   for name in ("k", "v"))
+    if fp8:
+        params += tuple(Param(f"{name}_scales", "f32", ("PAGES", "HK", "PAGE"), access, leading_stride=True)
+                        for name in ("k", "v"))
+    return params
+
+
+def _cache_arguments(v: dict, fp8: bool) -> tuple:
+    k, kv = v["k_cache"], v["v_cache"]
+    scales = (_ptr(v["k_scales"]), _ld(v["k_scales"]), _ptr(v["v_scales"]), _ld(v["v_scales"])) if fp8 else (None, 0, None, 0)
+    return (_ptr(k), _ld(k), _ptr(kv), _ld(kv), *scales)
+
+
+_CACHE_DOC = "E4M3FN codes with a scale per token and head, max(absmax, 1e-12) / 448"
+
+
+def _append_definition(dt: str, fp8: bool) -> KernelDefinition:
+    def launch(v: dict, env: dict, stream: int, workspace) -> str:
+        first, rest = _heads_arguments(v, env)
+        value, q_out = v["v"], v["q_out"]
+        _native.call("intent_paged_kv_append", *first, _ptr(value), _ld(value), *rest, _ptr(v["slots"]),
+                     int(dt == "bf16"), int(fp8), *_cache_arguments(v, fp8), env["PAGES"], env["PAGE"], _ptr(q_out),
+                     _ld(q_out), stream)
+        return "intent_paged_kv_append"
+
+    return KernelDefinition(
+        name=_prefix(dt) + "paged_kv_append" + ("_fp8" if fp8 else ""),
+        params=(
+            Param("q", dt, ("T", "HQ", "D"), leading_stride=True),
+            Param("k", dt, ("T", "HK", "D"), leading_stride=True),
+            Param("v", dt, ("T", "HK", "D"), leading_stride=True),
+            Param("q_weight", dt, ("WQ",)),
+            Param("k_weight", dt, ("WK",)),
+            Param("cos_sin", "f32", ("P", "R"), leading_stride=True),
+            Param("positions", "i32", ("T",)),
+            Param("slots", "i32", ("T",)),
+            *_cache_params(dt, fp8, INOUT),
+            Param("q_out", dt, ("T", "HQ", "D"), OUT, leading_stride=True),
+        ),
+        launch=launch,
+        constexprs=dict(_HEADS_CONSTEXPRS),
+        check=_append_check,
+        reference="examples/kernels/quantization/fp8.py:11-39 (the quantizer's rule, one group for each head)" if fp8 else
+                  "no kernel of the reference's quantized path; the producer of the paged attention's cache",
+        doc="q_out, and keys as qk_norm_rope, values as they are, at token slots[t] (page * PAGE + place) of the cache"
+            + (f": {_CACHE_DOC}" if fp8 else "") + "; a negative slot (padding) or one past the cache is skipped",
+    )
+
+
+paged_kv_append = _append_definition("f16", False)
+bf16_paged_kv_append = _append_definition("bf16", False)
+paged_kv_append_fp8 = _append_definition("f16", True)
+bf16_paged_kv_append_fp8 = _append_definition("bf16", True)
+
+
+def _attention_check(env: dict) -> None:
+    if env["S_PLUS_1"] != env["S"] + 1:
+        raise ValueError(f"q_offsets has {env['S_PLUS_1']} entries; {env['S'] + 1} are needed for {env['S']} sequences")
+    if env["T"] and env["HQ"] and (not env["HK"] or env["HQ"] % env["HK"]):
+        raise ValueError(f"HQ ({env['HQ']}) must be a multiple of HK ({env['HK']})")
+    if env["D"] % 8 or env["D"] > 512:
+        raise NotImplementedError(f"D ({env['D']}) must be a multiple of 8 up to 512")
+    if env["WINDOW"] < 0:
+        raise ValueError(f"WINDOW must not be negative, got {env['WINDOW']}")
+    _page_check(env)
+
+
+def _attention_definition(dt: str, fp8: bool) -> KernelDefinition:
+    def launch(v: dict, env: dict, stream: int, workspace) -> str:
+        q, out, table = v["q"], v["out"], v["page_table"]
+        _native.call("intent_paged_attention", _ptr(q), env["T"], env["HQ"], _ld(q), int(dt == "bf16"), int(fp8),
+                     *_cache_arguments(v, fp8), env["PAGES"], env["HK"], env["PAGE"], env["D"], _ptr(table), env["S"],
+                     env["MAX_PAGES"], _ld(table), _ptr(v["q_offsets"]), _ptr(v["kv_lens"]), float(env["scale"]),
+                     int(bool(env["CAUSAL"])), int(env["WINDOW"]), _ptr(out), _ld(out), stream)
+        return "intent_paged_attention"
+
+    return KernelDefinition(
+        name=_prefix(dt) + "paged_attention" + ("_fp8" if fp8 else ""),
+        params=(
+            Param("q", dt, ("T", "HQ", "D"), leading_stride=True),
+            *_cache_params(dt, fp8, IN),
+            Param("page_table", "i32", ("S", "MAX_PAGES"), leading_stride=True),
+            Param("q_offsets", "i32", ("S_PLUS_1",)),
+            Param("kv_lens", "i32", ("S",)),
+            Param("out", dt, ("T", "HQ", "D"), OUT, leading_stride=True),
+            Scalar("scale", "f32"),
+        ),
+        launch=launch,
+        constexprs={"CAUSAL": True, "WINDOW": 0},
+        check=_attention_check,
+        reference="no kernel of the reference's quantized path; I.matmul contractions over a paged operand",
+        doc="rows q_offsets[s] .. q_offsets[s+1] attend the kv_lens[s] tokens of sequence s's pages (the new ones last): "
+            "out = softmax(scale q.k) v over the seen tokens, zeros where none is seen"
+            + (f"; cache: {_CACHE_DOC}" if fp8 else ""),
+    )
+
+
+paged_attention = _attention_definition("f16", False)
+bf16_paged_attention = _attention_definition("bf16", False)
+paged_attention_fp8 = _attention_definition("f16", True)
+bf16_paged_attention_fp8 = _attention_definition("bf16", True)
+
+
 ALL_DEFINITIONS = (
     weight_only_int4_matmul, weight_only_int4_asym_matmul, weight_only_int8_matmul, w8a8_scaled_matmul, gemm_i8_nt,
     gemm_i8,
@@ -1319,4 +1500,6 @@ ALL_DEFINITIONS = (
     deepgemm_fp8_2xacc, fp8_e4m3_matmul, fp8_e5m2_matmul, dequant_bf16_fp4_matmul, quantized_gemm,
     ragged_grouped_gemm, ragged_grouped_gemm_bf16, routed_expert_projection_bf16, gemm, bf16_gemm,
     nvfp4_quantize, per_token_int8_quantize, bf16_per_token_int8_quantize,
+    qk_norm_rope, bf16_qk_norm_rope, paged_kv_append, bf16_paged_kv_append, paged_kv_append_fp8,
+    bf16_paged_kv_append_fp8, paged_attention, bf16_paged_attention, paged_attention_fp8, bf16_paged_attention_fp8,
 )

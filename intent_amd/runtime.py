@@ -269,6 +269,11 @@ class HIPRuntime:
                 raise ValueError(f"{p.name}.strides[1] violates the declared interface relation (must be 1)")
             if t.stride(0) < t.shape[1] and t.shape[0] > 1:
                 raise ValueError(f"{p.name}.strides[0] is smaller than the row")
+        elif p.leading_stride and t.dim() > 2:
+            if not t[0].is_contiguous():
+                raise ValueError(f"{p.name} must be contiguous behind its first axis")
+            if t.stride(0) < t[0].numel() and t.shape[0] > 1:
+                raise ValueError(f"{p.name}.strides[0] is smaller than the row")
         elif not t.is_contiguous():
             raise ValueError(f"{p.name} must be contiguous")
 
