@@ -732,7 +732,12 @@ int intent_paged_kv_append(const void* q, int64_t T, int64_t HQ, int64_t q_ld,
  * does not reach it, whatever it holds. f32 scores, softmax and sums; the
  * weights are rounded to q's type for the product with the values.
  * Lengths, offsets and page ids are clamped to the tensors, never followed out
- * of them. D % 8 == 0, D <= 512. No reference counterpart.
+ * of them. D % 8 == 0, D <= 512 (heads of 64, 96, 128 and 256 run the MFMA
+ * kernels, others one wave for each row). No reference counterpart.
+ * workspace: where few rows attend many tokens, their tokens are split over
+ * workgroups, whose f32 sums pass through it; _workspace_size gives the bytes
+ * that a call of these extents can use (0: none). With less, null or one that is
+ * not 16-byte aligned the call runs without a split.
  */
 int intent_paged_attention(const void* q, int64_t T, int64_t HQ, int64_t q_ld,
                            int is_bf16, int cache_is_fp8,
@@ -743,7 +748,10 @@ int intent_paged_attention(const void* q, int64_t T, int64_t HQ, int64_t q_ld,
                            const int32_t* page_table, int64_t S, int64_t table_width, int64_t table_ld,
                            const int32_t* q_offsets, const int32_t* kv_lens,
                            float scale, int causal, int64_t window,
-                           void* out, int64_t out_ld, void* stream);
+                           void* out, int64_t out_ld,
+                           void* workspace, size_t workspace_bytes, void* stream);
+size_t intent_paged_attention_workspace_size(int64_t T, int64_t HQ, int64_t HK, int64_t D, int64_t S,
+                                             int64_t table_width, int64_t page_size);
 
 #ifdef __cplusplus
 }

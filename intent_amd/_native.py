@@ -92,7 +92,8 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "intent_paged_kv_append": ([P, I64, I64, I64, P, I64, I64, P, I64, I64, P, P, F32, P, I64, I64, I64, INT, P, P, INT,
                                 INT, P, I64, P, I64, P, I64, P, I64, I64, I64, P, I64, P], INT),
     "intent_paged_attention": ([P, I64, I64, I64, INT, INT, P, I64, P, I64, P, I64, P, I64, I64, I64, I64, I64, P, I64,
-                                I64, I64, P, P, F32, INT, I64, P, I64, P], INT),
+                                I64, I64, P, P, F32, INT, I64, P, I64, P, SIZE, P], INT),
+    "intent_paged_attention_workspace_size": ([I64, I64, I64, I64, I64, I64, I64], SIZE),
     "intent_hbm_read_probe": ([P, I64, INT, INT, P, I64, P], INT),
     "intent_mfma_peak_probe": ([INT, I64, I64, P, P], INT),
 }

@@ -5,6 +5,8 @@ namespace {
 
 using namespace intent;
 
+constexpr int64_t kMostTokens = (int64_t)1 << 30;  // of a sequence: positions stay far inside 32 bits
+
 template <bool kBf16>
 INTENT_DEVICE float widen1(uint16_t v) {
   if constexpr (kBf16) return bit_cast<float>((uint32_t)v << 16);
@@ -139,7 +141,107 @@ int launch_rows(const AttnArgs& a, hipStream_t stream) {
   return launch_status_fmt("paged_attn_row_kernel<%s%s>", kBf16 ? "bf16" : "f16", kFp8 ? ", fp8 cache" : "");
 }
 
+// ---- which kernel, and into how many parts --------------------------------------------
+
+// Workgroups that the tiles are split for: two for each of the 256 CUs.
+constexpr int kFill = 512;
+
+struct Part {
+  int tiles;  // 16-row tiles of the kernel with the tokens over the waves; 0: 128 rows
+  int min_rows, max_rows;
+  int rows() const { return tiles > 0 ? 16 * tiles : 128; }
+  int unit() const { return tiles > 0 ? 128 : 64; }
+};
+
+struct Plan {
+  Part part[2];
+  int parts;
+};
+
+bool tiled(int64_t D) { return D == 64 || D == 96 || D == 128 || D == 256; }
+
+// The host knows the rows of all sequences together. Up to 64 for each on average, they go to the
+// kernel that spreads the tokens over the waves, with the tile that holds the average; beyond, each
+// sequence goes by its own: up to 32 rows there, more to the 128-row tile.
+Plan plan_of(int64_t T, int64_t S, int64_t group) {
+  const int64_t rows = T * group, mean = (rows + S - 1) / S;
+  Plan p{};
+  p.parts = 1;
+  if (mean <= 64) {
+    p.part[0] = {mean <= 16 ? 1 : mean <= 32 ? 2 : 4, 0, INT32_MAX};
+  } else if (S == 1) {
+    p.part[0] = {0, 0, INT32_MAX};
+  } else {
+    p.parts = 2;
+    p.part[0] = {0, 32, INT32_MAX};
+    p.part[1] = {2, 0, 32};
+  }
+  return p;
+}
+
+int64_t tiles_bound(const Part& p, int64_t T, int64_t S, int64_t group) {
+  return T * group / p.rows() + (S < T ? S : T);
+}
+
+// Parts of all split tiles of one head: fewer than twice the target (each of two parts at least has
+// more than half its share), and at most every tile's most.
+int64_t slots_bound(const Part& p, int64_t T, int64_t S, int64_t group, int64_t HK, int64_t most_kv) {
+  const int64_t target = (kFill + HK - 1) / HK;
+  int64_t splits = (most_kv + p.unit() - 1) / p.unit();
+  if (splits > kMostSplits) splits = kMostSplits;
+  if (splits < 2) return 0;
+  const int64_t all = tiles_bound(p, T, S, group) * splits;
+  return all < 2 * target ? all : 2 * target;
+}
+
+size_t part_bytes(const Part& p, int64_t T, int64_t S, int64_t group, int64_t HK, int64_t D, int64_t most_kv) {
+  return (size_t)(slots_bound(p, T, S, group, HK, most_kv) * HK * p.rows() * (D + 2) * 4);
+}
+
+int launch_tiled(AttnArgs a, bool bf16, bool fp8, float* workspace, size_t bytes, hipStream_t stream) {
+  const Plan plan = plan_of(a.T, a.S, a.group);
+  int status = INTENT_OK;
+  for (int i = 0; i < plan.parts && status == INTENT_OK; ++i) {
+    const Part& p = plan.part[i];
+    const size_t need = part_bytes(p, a.T, a.S, a.group, a.HK, a.D, a.most_kv);
+    const bool split = need > 0 && workspace != nullptr && bytes >= need;
+    AttnLaunch l{};
+    a.min_rows = p.min_rows, a.max_rows = p.max_rows;
+    a.target = split ? (kFill + a.HK - 1) / a.HK : 0;
+    a.partial = workspace;
+    a.partial_stats = split ? workspace + slots_bound(p, a.T, a.S, a.group, a.HK, a.most_kv) * a.HK * p.rows() * a.D : nullptr;
+    const int64_t tiles = tiles_bound(p, a.T, a.S, a.group);
+    const int64_t joins = split ? (tiles < a.target ? tiles : a.target) : 0;
+    // 256-lane workgroups: the grid's work items stay below 2^32
+    INTENT_REQUIRE((tiles + a.target) * a.HK < ((int64_t)1 << 24), INTENT_ERR_UNSUPPORTED,
+                   "%lld tiles of %d heads exceed the %lld workgroups that a launch covers", (long long)tiles, a.HK,
+                   (long long)((int64_t)1 << 24));
+    l.a = a;
+    l.items = (int)(tiles + a.target);
+    l.joins = (int)joins;
+    const int64_t mean = ((int64_t)a.T * a.group + a.S - 1) / a.S;
+    l.join_rows = (int)(mean < 16 ? mean : 16);
+    if (fp8) status = bf16 ? launch_attn_bf16_fp8(l, p.tiles, stream) : launch_attn_f16_fp8(l, p.tiles, stream);
+    else status = bf16 ? launch_attn_bf16(l, p.tiles, stream) : launch_attn_f16(l, p.tiles, stream);
+  }
+  return status;
+}
+
 }  // namespace
+
+extern "C" size_t intent_paged_attention_workspace_size(int64_t T, int64_t HQ, int64_t HK, int64_t D, int64_t S,
+                                                        int64_t table_width, int64_t page_size) {
+  if (T <= 0 || HQ <= 0 || HK <= 0 || S <= 0 || HQ % HK || table_width <= 0 || page_size <= 0 || !tiled(D) ||
+      table_width > kMostTokens / page_size || HQ > 65536 || T * HQ >= ((int64_t)1 << 26))
+    return 0;
+  const Plan plan = plan_of(T, S, HQ / HK);
+  size_t most = 0;
+  for (int i = 0; i < plan.parts; ++i) {
+    const size_t need = part_bytes(plan.part[i], T, S, HQ / HK, HK, D, table_width * page_size);
+    if (need > most) most = need;
+  }
+  return most;
+}
 
 extern "C" int intent_paged_attention(const void* q, int64_t T, int64_t HQ, int64_t q_ld, int is_bf16,
                                       int cache_is_fp8, const void* k_cache, int64_t k_page_ld, const void* v_cache,
@@ -148,7 +250,7 @@ extern "C" int intent_paged_attention(const void* q, int64_t T, int64_t HQ, int6
                                       int64_t page_size, int64_t D, const int32_t* page_table, int64_t S,
                                       int64_t table_width, int64_t table_ld, const int32_t* q_offsets,
                                       const int32_t* kv_lens, float scale, int causal, int64_t window, void* out,
-                                      int64_t out_ld, void* stream) {
+                                      int64_t out_ld, void* workspace, size_t workspace_bytes, void* stream) {
   clear_error();
   INTENT_REQUIRE(T >= 0 && HQ >= 0 && HK >= 0 && D >= 0 && S >= 0 && pages >= 0 && page_size >= 0 && table_width >= 0 &&
                      window >= 0 && T <= INT32_MAX && HQ <= 65536 && HK <= 65536 && S < INT32_MAX &&
@@ -164,8 +266,8 @@ extern "C" int intent_paged_attention(const void* q, int64_t T, int64_t HQ, int6
   const bool any = pages > 0 && page_size > 0 && table_width > 0;
   INTENT_REQUIRE(!any || (page_size & (page_size - 1)) == 0, INTENT_ERR_UNSUPPORTED,
                  "the page size must be a power of two, got %lld", (long long)page_size);
-  INTENT_REQUIRE(!any || table_width <= INT32_MAX / page_size, INTENT_ERR_UNSUPPORTED,
-                 "a table of %lld pages of %lld tokens exceeds 2^31 tokens", (long long)table_width,
+  INTENT_REQUIRE(!any || table_width <= kMostTokens / page_size, INTENT_ERR_UNSUPPORTED,
+                 "a table of %lld pages of %lld tokens exceeds 2^30 tokens", (long long)table_width,
                  (long long)page_size);
   // one wave for each row of a head: the grid's work items stay below 2^32
   INTENT_REQUIRE(T * HQ < ((int64_t)1 << 26), INTENT_ERR_UNSUPPORTED,
@@ -201,6 +303,10 @@ extern "C" int intent_paged_attention(const void* q, int64_t T, int64_t HQ, int6
   a.most_kv = any ? (int)(table_width * page_size) : 0;
   a.causal = causal != 0, a.window = (int)(window < INT32_MAX ? window : INT32_MAX);
   hipStream_t st = (hipStream_t)stream;
+  if (tiled(D)) {
+    const bool aligned = workspace != nullptr && intent::aligned16(workspace);
+    return launch_tiled(a, is_bf16 != 0, cache_is_fp8 != 0, aligned ? (float*)workspace : nullptr, workspace_bytes, st);
+  }
   if (cache_is_fp8) return is_bf16 ? launch_rows<true, true>(a, st) : launch_rows<false, true>(a, st);
   return is_bf16 ? launch_rows<true, false>(a, st) : launch_rows<false, false>(a, st);
 }

@@ -1,0 +1,792 @@
+// The tiled attention kernels (see paged_attn.h for the operator). Included by one source file for each
+// type of heads and cache.
+//
+// Both compute the transposed products, S^T = K Q^T and O^T = V^T P^T. An MFMA leaves four consecutive
+// rows of a column in a lane, so S^T puts the scores of one query row in one lane column: its softmax
+// needs no exchange but a maximum over two or four lane groups, and the weights are already where the
+// second product reads its right operand (its sum over tokens may go in any order: k index (g, j) of
+// lane group g is the token that the first product left there). The left operand V^T is read from
+// row-major values in LDS by the transposing read (ds_read_b64_tr_b16: of 16 lanes' 8 bytes, four rows
+// of 16 columns, each lane gets one column).
+//
+// Running softmax in base 2: weights w = exp2(t - M) with t the score times scale log2(e). M follows
+// the maximum only when that has risen by 8, so weights reach 2^8 at most and the sums are rescaled
+// rarely; in f32 and in 16-bit weights this costs no precision. With an 8-bit cache the value's scale
+// is part of the weight that is rounded: M follows the maximum of t + log2(scale), w = exp2(t - M) *
+// scale, and only the sum of weights takes exp2(t - M) by itself. The codes are exact in 16 bits.
+#pragma once
+
+#include "paged_attn.h"
+
+namespace intent {
+namespace attn {
+
+constexpr float kRise = 8.0f;
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
+
+// What tokens that no row of a tile sees are read from: pages behind a sequence's end hold anything.
+static __device__ __attribute__((aligned(16))) const uint32_t kZeroRow[128] = {};
+
+template <bool kBf16>
+INTENT_DEVICE f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (kBf16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(bit_cast<bf16x8>(a), bit_cast<bf16x8>(b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_f16(bit_cast<f16x8>(a), bit_cast<f16x8>(b), c, 0, 0, 0);
+}
+template <bool kBf16>
+INTENT_DEVICE f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (kBf16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(bit_cast<bf16x8>(a), bit_cast<bf16x8>(b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_f16(bit_cast<f16x8>(a), bit_cast<f16x8>(b), c, 0, 0, 0);
+}
+
+template <bool kBf16>
+INTENT_DEVICE uint32_t pack2(float lo, float hi) {
+  if constexpr (kBf16) return bf16x2_rne(lo, hi);
+  else return bit_cast<uint32_t>(__builtin_convertvector(f32x2{lo, hi}, f16x2));
+}
+
+// Eight E4M3FN codes as eight 16-bit floats (exact).
+template <bool kBf16>
+INTENT_DEVICE u32x4 widen_codes(uint32_t lo, uint32_t hi) {
+  u32x4 r;
+  if constexpr (kBf16) {
+    r[0] = bit_cast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false));
+    r[1] = bit_cast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true));
+    r[2] = bit_cast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false));
+    r[3] = bit_cast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true));
+  } else {
+    r[0] = bit_cast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false));
+    r[1] = bit_cast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true));
+    r[2] = bit_cast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false));
+    r[3] = bit_cast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true));
+  }
+  return r;
+}
+
+// 0x8000 in each half of a pair of 16-bit floats that is an infinity or NaN (all exponent bits set: one
+// more in the exponent's last place carries into the sign's, which the mask has cleared).
+template <bool kBf16>
+INTENT_DEVICE uint32_t not_finite(uint32_t pair) {
+  constexpr uint32_t kExponent = kBf16 ? 0x7f807f80u : 0x7c007c00u, kStep = kBf16 ? 0x00800080u : 0x04000400u;
+  return ((pair & kExponent) + kStep) & 0x80008000u;
+}
+
+INTENT_DEVICE u32x2 read_transposed(const char* lds) {
+  return bit_cast<u32x2>(__builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) s16x4*)(__attribute__((address_space(3))) char*)lds));
+}
+
+// Rows of LDS tiles are a power of two of bytes; the 16-byte chunk c of token t is kept at c ^ swizzle(t):
+// eight consecutive tokens have eight values (reads of one chunk down the tokens), and four
+// consecutive ones differ in the upper two bits (the transposing read takes 32 bytes of each).
+INTENT_DEVICE int swizzle(int t) { return (t & 3) << 1 | (t >> 2 & 1); }
+
+template <int D>
+constexpr int row_bytes() {
+  return D <= 64 ? 128 : D <= 128 ? 256 : 512;
+}
+
+// Orders a wave's LDS writes before its reads of other lanes' (the LDS itself takes them in order).
+INTENT_DEVICE void wave_lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// max(log2(scale), -100): the bound keeps exp2(t - M) finite beside tokens of zeros.
+INTENT_DEVICE float scale_exponent(float v) { return fmaxf(__builtin_amdgcn_logf(v), -100.0f); }
+
+// Where one query row of a tile (column r of S^T) stands: the tokens lo <= t < hi that it sees.
+struct RowView {
+  int lo, hi;
+};
+INTENT_DEVICE RowView row_view(const AttnArgs& a, const Span& w, int r) {
+  const int p = w.q.kv - w.q.count + (w.row0 + min(r, w.rows - 1)) / a.group;
+  return {first_seen(a, p), end_seen(a, p, w.q.kv)};
+}
+
+INTENT_DEVICE const uint16_t* q_row(const AttnArgs& a, const Span& w, int head, int r) {
+  const int row = w.row0 + min(r, w.rows - 1), token = row / a.group;
+  return a.q + (int64_t)(w.q.start + token) * a.q_ld + (int64_t)(head * a.group + row - token * a.group) * a.D;
+}
+INTENT_DEVICE uint16_t* out_row(const AttnArgs& a, const Span& w, int head, int r) {
+  const int row = w.row0 + r, token = row / a.group;
+  return a.out + (int64_t)(w.q.start + token) * a.out_ld + (int64_t)(head * a.group + row - token * a.group) * a.D;
+}
+
+// Queries with the sign of the scale, so that the kernels scale by its size and may take maxima first.
+INTENT_DEVICE u32x4 signed_query(const AttnArgs& a, u32x4 v) {
+  const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+  return u32x4{v[0] ^ flip, v[1] ^ flip, v[2] ^ flip, v[3] ^ flip};
+}
+
+INTENT_DEVICE float max_across16(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(bit_cast<uint32_t>(v), bit_cast<uint32_t>(v), false, false);
+  return fmaxf(bit_cast<float>(r[0]), bit_cast<float>(r[1]));
+}
+INTENT_DEVICE float max_across32(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(bit_cast<uint32_t>(v), bit_cast<uint32_t>(v), false, false);
+  return fmaxf(bit_cast<float>(r[0]), bit_cast<float>(r[1]));
+}
+INTENT_DEVICE float sum_across16(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(bit_cast<uint32_t>(v), bit_cast<uint32_t>(v), false, false);
+  return bit_cast<float>(r[0]) + bit_cast<float>(r[1]);
+}
+INTENT_DEVICE float sum_across32(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(bit_cast<uint32_t>(v), bit_cast<uint32_t>(v), false, false);
+  return bit_cast<float>(r[0]) + bit_cast<float>(r[1]);
+}
+
+// Keeps the halves of a pair of values whose tokens (the two of consecutive index from `t`) a row sees.
+INTENT_DEVICE uint32_t seen_pair(uint32_t pair, int t, int lo, int hi) {
+  const uint32_t keep = (t >= lo && t < hi ? 0xffffu : 0u) | (t + 1 >= lo && t + 1 < hi ? 0xffff0000u : 0u);
+  return pair & keep;
+}
+
+// ---- few rows: 16 * MT of them, the tokens over the waves -----------------------------------------
+
+// A wave takes 32 tokens at a time, four apart from its next: keys straight into the first product's
+// left operand (a lane holds 8 or 16 of a token's D), values through its own LDS rows; no barrier until
+// the four waves' results are joined. Keys and values of the next 32 tokens are under way during the
+// softmax and the second product, and the page ids of the ones after them.
+template <bool kBf16, bool kFp8, int D, int MT>
+__global__ __launch_bounds__(256, D <= 128 && MT <= 2 ? 2 : 1) void attn_rows_kernel(const AttnArgs a) {
+  constexpr int KS = D / 32, DT = D / 16, RB = row_bytes<D>();
+  constexpr bool kWide = !kFp8 || D % 64 == 0;         // 16 bytes a lane and load, else 8 codes
+  constexpr int LOADS = kFp8 && kWide ? D / 64 : KS;   // loads of a token's row
+  constexpr int ELEMS = kFp8 && kWide ? 16 : 8;        // elements of one
+  constexpr int OB = D + 4;                            // floats of a row in the joining buffer
+  constexpr int kLds = 4 * 32 * RB > 4 * 16 * OB * 4 ? 4 * 32 * RB : 4 * 16 * OB * 4;
+  __shared__ __attribute__((aligned(16))) char lds[kLds];
+  __shared__ __attribute__((aligned(16))) float scales[kFp8 ? 4 : 1][3][32];
+  __shared__ float stats[4][16][2];
+
+  const int head = blockIdx.x % a.HK;
+  Span w;
+  if (!find_span<16 * MT, 128>(a, blockIdx.x / a.HK, false, w)) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int col = lane & 15, g = lane >> 4;
+
+  // element index of load i of lane group g in a token's row
+  auto at = [&](int i) { return i * 4 * ELEMS + g * ELEMS; };
+  u32x4 q[MT][KS];
+  RowView view[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    view[m] = row_view(a, w, m * 16 + col);
+    const uint16_t* row = q_row(a, w, head, m * 16 + col);
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+      q[m][i] = signed_query(a, load16(row + (ELEMS == 16 ? at(i / 2) + (i & 1) * 8 : at(i))));
+  }
+  // the tokens that some row sees, and those that all rows see
+  const RowView top = row_view(a, w, 0), bottom = row_view(a, w, w.rows - 1);
+  const int some_lo = top.lo, some_hi = bottom.hi, all_lo = bottom.lo, all_hi = top.hi;
+  const float scale = fabsf(a.scale_log2);
+
+  f32x4 o[MT][DT];
+  float ref[MT], total[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    ref[m] = -INFINITY, total[m] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) o[m][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  char* mine = lds + wave * 32 * RB;
+  const int write_at = col * RB, swz = swizzle(col);
+  // transposing reads: tokens 4 g .. 4 g + 3 of each 16, columns 16 d ..
+  const int read_row = g * 4 + (col >> 2);
+  const int read_at = wave * 32 * RB + read_row * RB + (((col >> 1 & 1) ^ swizzle(read_row)) << 4) + (col & 1) * 8;
+
+  u32x4 kr[2][LOADS], vr[2][LOADS];
+  float ks[2], vs[2];
+  int ids[2];
+  auto token = [&](int t, int u) { return t + 16 * u + col; };
+  auto load_ids = [&](int t) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) ids[u] = page_of(a, w.s, min(max(token(t, u), some_lo), max(some_hi - 1, 0)));
+  };
+  auto load_rows = [&](int t) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int tk = token(t, u);
+      const bool live = tk >= some_lo && tk < some_hi;
+      constexpr int kBytes = kFp8 ? 1 : 2;
+      const char* k = (const char*)a.k_cache + row_in_cache(a, ids[u], a.k_page, head, tk, D) * kBytes;
+      const char* v = (const char*)a.v_cache + row_in_cache(a, ids[u], a.v_page, head, tk, D) * kBytes;
+      k = live ? k : (const char*)kZeroRow;
+      v = live ? v : (const char*)kZeroRow;
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        if constexpr (kWide) {
+          kr[u][i] = load16(k + at(i) * kBytes);
+          vr[u][i] = load16(v + at(i) * kBytes);
+        } else {
+          const u32x2 kc = *(const u32x2*)(k + at(i)), vc = *(const u32x2*)(v + at(i));
+          kr[u][i] = u32x4{kc[0], kc[1], 0u, 0u};
+          vr[u][i] = u32x4{vc[0], vc[1], 0u, 0u};
+        }
+      }
+      if constexpr (kFp8) {
+        const float* kp = a.k_scales + row_in_cache(a, ids[u], a.ks_page, head, tk, 1);
+        const float* vp = a.v_scales + row_in_cache(a, ids[u], a.vs_page, head, tk, 1);
+        ks[u] = *(live ? kp : (const float*)kZeroRow);
+        vs[u] = *(live ? vp : (const float*)kZeroRow);
+      }
+    }
+  };
+
+  int t = w.begin + wave * 32;
+  if (t < w.end) {
+    load_ids(t);
+    load_rows(t);
+    load_ids(t + 128);
+  }
+  for (; t < w.end; t += 128) {
+    // values and scales of these tokens to LDS, the scores' operands from the registers
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        char* row = mine + u * 16 * RB + write_at;
+        const int chunk = at(i) / 8;
+        if constexpr (kFp8) {
+          *(u32x4*)(row + ((chunk ^ swz) << 4)) = widen_codes<kBf16>(vr[u][i][0], vr[u][i][1]);
+          if constexpr (kWide) *(u32x4*)(row + (((chunk + 1) ^ swz) << 4)) = widen_codes<kBf16>(vr[u][i][2], vr[u][i][3]);
+        } else {
+          *(u32x4*)(row + ((chunk ^ swz) << 4)) = vr[u][i];
+        }
+      }
+      if constexpr (kFp8) {
+        if (g == 0) {
+          scales[wave][0][u * 16 + col] = ks[u] * scale;
+          scales[wave][1][u * 16 + col] = vs[u];
+          scales[wave][2][u * 16 + col] = scale_exponent(vs[u]);
+        }
+      }
+    }
+    wave_lds_order();
+    f32x4 s[MT][2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m) s[m][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        u32x4 k;
+        if constexpr (!kFp8) k = kr[u][i];
+        else if constexpr (kWide) k = widen_codes<kBf16>(kr[u][i / 2][(i & 1) * 2], kr[u][i / 2][(i & 1) * 2 + 1]);
+        else k = widen_codes<kBf16>(kr[u][i][0], kr[u][i][1]);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) s[m][u] = mfma16<kBf16>(k, q[m][i], s[m][u]);
+      }
+    }
+    const int now = t;
+    if (now + 128 < w.end) {
+      load_rows(now + 128);
+      load_ids(now + 256);
+    }
+    const bool masked = now < all_lo || now + 32 > all_hi;
+    u32x4 p[MT];
+    f32x4 k_mul[2], v_mul[2], v_exp[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if constexpr (kFp8) {
+        k_mul[u] = *(const f32x4*)&scales[wave][0][u * 16 + g * 4];
+        v_mul[u] = *(const f32x4*)&scales[wave][1][u * 16 + g * 4];
+        v_exp[u] = *(const f32x4*)&scales[wave][2][u * 16 + g * 4];
+      } else {
+        k_mul[u] = f32x4{scale, scale, scale, scale};
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      float x[2][4], high = -INFINITY;
+      bool seen[2][4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          x[u][r] = s[m][u][r] * k_mul[u][r];
+          float y = kFp8 ? x[u][r] + v_exp[u][r] : x[u][r];
+          seen[u][r] = true;
+          if (masked) {
+            const int tk = now + 16 * u + g * 4 + r;
+            seen[u][r] = tk >= view[m].lo && tk < view[m].hi;
+            x[u][r] = seen[u][r] ? x[u][r] : -INFINITY;
+            y = seen[u][r] ? y : -INFINITY;
+          }
+          high = fmaxf(high, y);
+        }
+      }
+      high = max_across32(max_across16(high));
+      if (__any(high > ref[m] + kRise)) {
+        const float next = fmaxf(ref[m], high);
+        const float keep = __builtin_amdgcn_exp2f(ref[m] - (next == -INFINITY ? 0.f : next));
+        ref[m] = next;
+        total[m] *= keep;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[m][d] *= keep;
+      }
+      const float base = ref[m] == -INFINITY ? 0.f : ref[m];
+      float wt[2][4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float e = __builtin_amdgcn_exp2f(x[u][r] - base);
+          total[m] += e;
+          wt[u][r] = kFp8 ? e * v_mul[u][r] : e;
+          if (kFp8 && masked) wt[u][r] = seen[u][r] ? wt[u][r] : 0.f;
+        }
+      }
+      p[m] = u32x4{pack2<kBf16>(wt[0][0], wt[0][1]), pack2<kBf16>(wt[0][2], wt[0][3]), pack2<kBf16>(wt[1][0], wt[1][1]),
+                   pack2<kBf16>(wt[1][2], wt[1][3])};
+    }
+    // V^T: tokens 4 g .. of the first 16, then of the second
+    u32x4 v[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      const char* from = lds + (read_at ^ (d * 32));
+      const u32x2 lo = read_transposed(from), hi = read_transposed(from + 16 * RB);
+      v[d] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+    }
+    bool apart = false;
+    if (masked && (some_lo != all_lo || some_hi != all_hi)) {
+      // rows of this tile see different tokens: 0 * NaN in one that does not see it must not reach it
+      uint32_t bad = 0;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bad |= not_finite<kBf16>(v[d][e]);
+      apart = __any(bad != 0);
+    }
+    if (apart) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        for (int c = 0; c < 16; ++c) {  // one row at a time, over the values that it sees
+          const int lo = lane_value(view[m].lo, c), hi = lane_value(view[m].hi, c);
+          const uint32_t only = col == c ? ~0u : 0u;
+          const u32x4 pc = u32x4{p[m][0] & only, p[m][1] & only, p[m][2] & only, p[m][3] & only};
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            u32x4 vc;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vc[e] = seen_pair(v[d][e], now + (e >> 1) * 16 + g * 4 + (e & 1) * 2, lo, hi);
+            const f32x4 add = mfma16<kBf16>(vc, pc, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[m][d][r] = col == c ? o[m][d][r] + add[r] : o[m][d][r];
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) o[m][d] = mfma16<kBf16>(v[d], p[m], o[m][d]);
+    }
+    wave_lds_order();
+  }
+
+  // join the four waves, 16 rows at a time
+  float* rows = (float*)lds;
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    if (m * 16 >= w.rows) break;
+    __syncthreads();
+    const float sum = sum_across32(sum_across16(total[m]));
+    if (g == 0) stats[wave][col][0] = ref[m], stats[wave][col][1] = sum;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) *(f32x4*)&rows[(wave * 16 + col) * OB + d * 16 + g * 4] = o[m][d];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * (D / 4); i += 256) {
+      const int r = i / (D / 4), d = i % (D / 4) * 4, row = m * 16 + r;
+      if (row >= w.rows) break;
+      float high = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) high = fmaxf(high, stats[k][r][0]);
+      const float base = high == -INFINITY ? 0.f : high;
+      f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+      float all = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float keep = __builtin_amdgcn_exp2f(stats[k][r][0] - base);
+        all += keep * stats[k][r][1];
+        acc += keep * *(const f32x4*)&rows[(k * 16 + r) * OB + d];
+      }
+      if (w.splits == 1) {
+        const RowView rv = row_view(a, w, row);
+        const float inv = rv.hi > rv.lo ? 1.0f / all : 0.f;
+        *(u32x2*)(out_row(a, w, head, row) + d) =
+            u32x2{pack2<kBf16>(acc[0] * inv, acc[1] * inv), pack2<kBf16>(acc[2] * inv, acc[3] * inv)};
+      } else {
+        const int64_t to = ((int64_t)w.slot * a.HK + head) * (16 * MT) + row;
+        *(f32x4*)(a.partial + to * D + d) = acc;
+        if (d == 0) *(f32x2*)(a.partial_stats + to * 2) = f32x2{high, all};
+      }
+    }
+  }
+}
+
+// ---- many rows: 128, 32 to a wave, all of them over the same tokens ----------------------------------
+
+// 64 tokens of keys and values in LDS at a time, in two buffers: the next ones are loaded into
+// registers while these are worked on and stored to the other buffer behind them, so one barrier for
+// each 64 tokens.
+template <bool kBf16, bool kFp8, int D>
+__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const AttnArgs a) {
+  constexpr int KS = D / 16, DT = D / 32, RB = row_bytes<D>();
+  constexpr int CHUNKS = kFp8 ? D / 16 : D / 8;       // 16-byte loads of a token's row
+  constexpr int SPREAD = kFp8 ? RB / 32 : RB / 16;    // lanes that take one (a power of two)
+  constexpr int STEP = 256 / SPREAD;                  // tokens that the workgroup loads at once
+  constexpr int LOADS = 64 / STEP;
+  constexpr int kTile = 64 * RB;
+  __shared__ __attribute__((aligned(16))) char lds[2][2][kTile];
+  __shared__ __attribute__((aligned(16))) float scales[kFp8 ? 2 : 1][3][64];
+
+  const int head = blockIdx.x % a.HK;
+  Span w;
+  if (!find_span<128, 64>(a, blockIdx.x / a.HK, false, w)) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int col = lane & 31, h = lane >> 5;
+  const int r0 = wave * 32;
+
+  u32x4 q[KS];
+  const RowView view = row_view(a, w, r0 + col);
+  {
+    const uint16_t* row = q_row(a, w, head, r0 + col);
+#pragma unroll
+    for (int i = 0; i < KS; ++i) q[i] = signed_query(a, load16(row + i * 16 + h * 8));
+  }
+  const int some_lo = row_view(a, w, 0).lo, some_hi = row_view(a, w, w.rows - 1).hi;
+  const RowView top = row_view(a, w, r0), bottom = row_view(a, w, r0 + 31);  // of this wave
+  const bool idle = r0 >= w.rows;
+  const float scale = fabsf(a.scale_log2);
+
+  f32x16 o[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+  float ref = -INFINITY, total = 0.f;
+
+  const int load_token = threadIdx.x / SPREAD, load_chunk = threadIdx.x % SPREAD;
+  const bool loads = load_chunk < CHUNKS;
+  u32x4 kr[LOADS], vr[LOADS];
+  float ks = 0.f, vs = 0.f;
+  int ids[LOADS], scale_id = 0;
+  auto clamped = [&](int t) { return min(max(t, some_lo), max(some_hi - 1, 0)); };
+  auto load_ids = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) ids[i] = page_of(a, w.s, clamped(t + load_token + i * STEP));
+    if constexpr (kFp8) scale_id = page_of(a, w.s, clamped(t + lane));
+  };
+  auto load_rows = [&](int t) {
+    constexpr int kBytes = kFp8 ? 1 : 2;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int tk = t + load_token + i * STEP;
+      const bool live = tk >= some_lo && tk < some_hi;
+      const char* k = (const char*)a.k_cache + row_in_cache(a, ids[i], a.k_page, head, tk, D) * kBytes;
+      const char* v = (const char*)a.v_cache + row_in_cache(a, ids[i], a.v_page, head, tk, D) * kBytes;
+      k = live ? k : (const char*)kZeroRow;
+      v = live ? v : (const char*)kZeroRow;
+      const int chunk = loads ? load_chunk : 0;
+      kr[i] = load16(k + chunk * 16);
+      vr[i] = load16(v + chunk * 16);
+    }
+    if constexpr (kFp8) {
+      const int tk = t + lane;
+      const bool live = tk >= some_lo && tk < some_hi;
+      const float* kp = a.k_scales + row_in_cache(a, scale_id, a.ks_page, head, tk, 1);
+      const float* vp = a.v_scales + row_in_cache(a, scale_id, a.vs_page, head, tk, 1);
+      ks = *(live ? kp : (const float*)kZeroRow);
+      vs = *(live ? vp : (const float*)kZeroRow);
+    }
+  };
+  auto store_rows = [&](int buffer) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int tk = load_token + i * STEP, swz = swizzle(tk);
+      if (loads) {
+        char* k = lds[buffer][0] + tk * RB;
+        char* v = lds[buffer][1] + tk * RB;
+        if constexpr (kFp8) {
+          const int c = load_chunk * 2;
+          *(u32x4*)(k + ((c ^ swz) << 4)) = widen_codes<kBf16>(kr[i][0], kr[i][1]);
+          *(u32x4*)(k + (((c + 1) ^ swz) << 4)) = widen_codes<kBf16>(kr[i][2], kr[i][3]);
+          *(u32x4*)(v + ((c ^ swz) << 4)) = widen_codes<kBf16>(vr[i][0], vr[i][1]);
+          *(u32x4*)(v + (((c + 1) ^ swz) << 4)) = widen_codes<kBf16>(vr[i][2], vr[i][3]);
+        } else {
+          *(u32x4*)(k + ((load_chunk ^ swz) << 4)) = kr[i];
+          *(u32x4*)(v + ((load_chunk ^ swz) << 4)) = vr[i];
+        }
+      }
+    }
+    if constexpr (kFp8) {
+      if (wave == 0) {
+        scales[buffer][0][lane] = ks * scale;
+        scales[buffer][1][lane] = vs;
+        scales[buffer][2][lane] = scale_exponent(vs);
+      }
+    }
+  };
+
+  const int k_at = col * RB + ((h ^ swizzle(col)) << 4);
+  const int i16 = lane & 15, read_row = h * 4 + (i16 >> 2);
+  const int v_at = read_row * RB + ((((lane >> 4 & 1) * 2 + (i16 >> 1 & 1)) ^ swizzle(read_row)) << 4) + (i16 & 1) * 8;
+
+  if (w.begin < w.end) {
+    load_ids(w.begin);
+    load_rows(w.begin);
+    load_ids(w.begin + 64);
+    store_rows(0);
+  }
+  __syncthreads();
+  int buffer = 0;
+  for (int t = w.begin; t < w.end; t += 64, buffer ^= 1) {
+    const bool more = t + 64 < w.end;
+    if (more) {
+      load_rows(t + 64);
+      load_ids(t + 128);
+    }
+    if (!idle && t < bottom.hi && t + 64 > top.lo) {  // some row of this wave sees some of these tokens
+      const char* keys = lds[buffer][0];
+      const char* values = lds[buffer][1];
+      f32x16 s[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
+#pragma unroll
+        for (int i = 0; i < KS; ++i)
+          s[u] = mfma32<kBf16>(*(const u32x4*)(keys + u * 32 * RB + (k_at ^ (i * 32))), q[i], s[u]);
+      }
+      const bool masked = t < bottom.lo || t + 64 > top.hi;
+      float high = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int t0 = u * 32 + i * 8 + h * 4;
+          f32x4 k_mul, v_exp;
+          if constexpr (kFp8) {
+            k_mul = *(const f32x4*)&scales[buffer][0][t0];
+            v_exp = *(const f32x4*)&scales[buffer][2][t0];
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float x = s[u][i * 4 + r] * (kFp8 ? k_mul[r] : scale);
+            float y = kFp8 ? x + v_exp[r] : x;
+            if (masked) {
+              const bool seen = t + t0 + r >= view.lo && t + t0 + r < view.hi;
+              x = seen ? x : -INFINITY;
+              y = seen ? y : -INFINITY;
+            }
+            s[u][i * 4 + r] = x;
+            high = fmaxf(high, y);
+          }
+        }
+      }
+      high = max_across32(high);
+      if (__any(high > ref + kRise)) {
+        const float next = fmaxf(ref, high);
+        const float keep = __builtin_amdgcn_exp2f(ref - (next == -INFINITY ? 0.f : next));
+        ref = next;
+        total *= keep;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[d][r] *= keep;
+      }
+      const float base = ref == -INFINITY ? 0.f : ref;
+      u32x4 p[4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int t0 = u * 32 + i * 8 + h * 4;
+          f32x4 v_mul;
+          if constexpr (kFp8) v_mul = *(const f32x4*)&scales[buffer][1][t0];
+          float wt[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float x = s[u][i * 4 + r], e = __builtin_amdgcn_exp2f(x - base);
+            total += e;
+            wt[r] = kFp8 ? e * v_mul[r] : e;
+            if (kFp8 && masked) wt[r] = t + t0 + r >= view.lo && t + t0 + r < view.hi ? wt[r] : 0.f;
+          }
+          p[u * 2 + i / 2][(i & 1) * 2] = pack2<kBf16>(wt[0], wt[1]);
+          p[u * 2 + i / 2][(i & 1) * 2 + 1] = pack2<kBf16>(wt[2], wt[3]);
+        }
+      }
+      auto value = [&](int d, int m) {
+        const char* from = values + (v_at ^ (d * 64)) + m * 16 * RB;
+        const u32x2 lo = read_transposed(from), hi = read_transposed(from + 8 * RB);
+        return u32x4{lo[0], lo[1], hi[0], hi[1]};
+      };
+      bool apart = false;
+      if (masked) {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            const u32x4 v = value(d, m);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bad |= not_finite<kBf16>(v[e]);
+          }
+        apart = __any(bad != 0);
+      }
+      if (apart) {
+        for (int c = 0; c < 32; ++c) {  // one row at a time, over the values that it sees
+          const int lo = lane_value(view.lo, c), hi = lane_value(view.hi, c);
+          const uint32_t only = col == c ? ~0u : 0u;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            f32x16 add;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) add[r] = 0.f;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+              u32x4 v = value(d, m), pc;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                v[e] = seen_pair(v[e], t + m * 16 + (e >> 1) * 8 + h * 4 + (e & 1) * 2, lo, hi);
+                pc[e] = p[m][e] & only;
+              }
+              add = mfma32<kBf16>(v, pc, add);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[d][r] = col == c ? o[d][r] + add[r] : o[d][r];
+          }
+        }
+      } else {
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int m = 0; m < 4; ++m) o[d] = mfma32<kBf16>(value(d, m), p[m], o[d]);
+      }
+    }
+    if (more) store_rows(buffer ^ 1);
+    __syncthreads();
+  }
+
+  const int r = r0 + col;
+  if (r >= w.rows) return;
+  const float all = sum_across32(total);
+  if (w.splits == 1) {
+    const float inv = view.hi > view.lo ? 1.0f / all : 0.f;
+    uint16_t* to = out_row(a, w, head, r);
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *(u32x2*)(to + d * 32 + i * 8 + h * 4) = u32x2{pack2<kBf16>(o[d][i * 4] * inv, o[d][i * 4 + 1] * inv),
+                                                       pack2<kBf16>(o[d][i * 4 + 2] * inv, o[d][i * 4 + 3] * inv)};
+  } else {
+    const int64_t to = ((int64_t)w.slot * a.HK + head) * 128 + r;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *(f32x4*)(a.partial + to * D + d * 32 + i * 8 + h * 4) =
+            f32x4{o[d][i * 4], o[d][i * 4 + 1], o[d][i * 4 + 2], o[d][i * 4 + 3]};
+    if (h == 0) *(f32x2*)(a.partial_stats + to * 2) = f32x2{ref, all};
+  }
+}
+
+// ---- the join of split tiles ---------------------------------------------------------------------
+
+// One workgroup for each row of a split tile (rows in turn where there are more): the waves take every
+// fourth split, in order, and are added in order.
+template <bool kBf16, int D, int ROWS, int UNIT>
+__global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
+  constexpr int E = (D + 63) / 64;  // columns of a lane
+  __shared__ float sums[4][64 * E];
+  __shared__ float all4[4];
+  const int head = blockIdx.x % a.HK;
+  Span w;
+  if (!find_span<ROWS, UNIT>(a, blockIdx.x / a.HK, true, w)) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  for (int r = blockIdx.y; r < w.rows; r += gridDim.y) {
+    auto at = [&](int j) { return ((int64_t)(w.slot + j) * a.HK + head) * ROWS + r; };
+    float high = -INFINITY;
+    for (int j = lane; j < w.splits; j += 64) high = fmaxf(high, a.partial_stats[at(j) * 2]);
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) high = fmaxf(high, __shfl_xor(high, off));
+    const float base = high == -INFINITY ? 0.f : high;
+    float acc[E], all = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll 4
+    for (int j = wave; j < w.splits; j += 4) {
+      const f32x2 st = *(const f32x2*)(a.partial_stats + at(j) * 2);
+      const float keep = __builtin_amdgcn_exp2f(st[0] - base);
+      all += keep * st[1];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int d = min(lane + 64 * e, D - 1);
+        acc[e] = __builtin_fmaf(keep, a.partial[at(j) * D + d], acc[e]);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e) sums[wave][lane + 64 * e] = acc[e];
+    if (lane == 0) all4[wave] = all;
+    __syncthreads();
+    const float total = all4[0] + all4[1] + all4[2] + all4[3];
+    const RowView rv = row_view(a, w, r);
+    const float inv = rv.hi > rv.lo ? 1.0f / total : 0.f;
+    uint16_t* to = out_row(a, w, head, r);
+    for (int d = threadIdx.x * 2; d < D; d += 512) {
+      const float x = sums[0][d] + sums[1][d] + sums[2][d] + sums[3][d];
+      const float y = sums[0][d + 1] + sums[1][d + 1] + sums[2][d + 1] + sums[3][d + 1];
+      *(uint32_t*)(to + d) = pack2<kBf16>(x * inv, y * inv);
+    }
+  }
+}
+
+template <bool kBf16, bool kFp8, int D, int MT>  // MT = 0: the 128-row tile
+int launch(const AttnLaunch& l, hipStream_t stream) {
+  const unsigned heads = (unsigned)l.a.HK;
+  constexpr int kRows = MT > 0 ? 16 * MT : 128, kUnit = MT > 0 ? 128 : 64;
+  if constexpr (MT > 0)
+    hipLaunchKernelGGL((attn_rows_kernel<kBf16, kFp8, D, MT>), dim3(l.items * heads), dim3(256), 0, stream, l.a);
+  else
+    hipLaunchKernelGGL((attn_tile_kernel<kBf16, kFp8, D>), dim3(l.items * heads), dim3(256), 0, stream, l.a);
+  const int status = launch_status_fmt("attn_%s_kernel<%s%s, D %d, %d rows%s>", MT > 0 ? "rows" : "tile",
+                                       kBf16 ? "bf16" : "f16", kFp8 ? ", fp8 cache" : "", D, kRows,
+                                       l.joins > 0 ? ", splits" : "");
+  if (status != INTENT_OK || l.joins == 0) return status;
+  hipLaunchKernelGGL((attn_join_kernel<kBf16, D, kRows, kUnit>), dim3(l.joins * heads, l.join_rows), dim3(256), 0, stream,
+                     l.a);
+  return launch_status_fmt("attn_%s_kernel<%s%s, D %d, %d rows, splits>", MT > 0 ? "rows" : "tile",
+                           kBf16 ? "bf16" : "f16", kFp8 ? ", fp8 cache" : "", D, kRows);
+}
+
+template <bool kBf16, bool kFp8, int D>
+int launch_d(const AttnLaunch& l, int tiles, hipStream_t stream) {
+  switch (tiles) {
+    case 1: return launch<kBf16, kFp8, D, 1>(l, stream);
+    case 2: return launch<kBf16, kFp8, D, 2>(l, stream);
+    case 4: return launch<kBf16, kFp8, D, 4>(l, stream);
+    default: return launch<kBf16, kFp8, D, 0>(l, stream);
+  }
+}
+
+template <bool kBf16, bool kFp8>
+int launch_any(const AttnLaunch& l, int tiles, hipStream_t stream) {
+  switch (l.a.D) {
+    case 64: return launch_d<kBf16, kFp8, 64>(l, tiles, stream);
+    case 96: return launch_d<kBf16, kFp8, 96>(l, tiles, stream);
+    case 128: return launch_d<kBf16, kFp8, 128>(l, tiles, stream);
+    case 256: return launch_d<kBf16, kFp8, 256>(l, tiles, stream);
+    default: return fail(INTENT_ERR_UNSUPPORTED, "no tiled attention kernel for heads of %d", l.a.D);
+  }
+}
+
+}  // namespace attn
+}  // namespace intent

@@ -1455,13 +1455,19 @@ def _attention_check(env: dict) -> None:
     _page_check(env)
 
 
+def _attention_scratch(env: dict) -> int:
+    return _native.library().intent_paged_attention_workspace_size(
+        env["T"], env["HQ"], env["HK"], env["D"], env["S"], env["MAX_PAGES"], env["PAGE"])
+
+
 def _attention_definition(dt: str, fp8: bool) -> KernelDefinition:
-    def launch(v: dict, env: dict, stream: int, workspace) -> str:
+    def launch(v: dict, env: dict, stream: int, scratch) -> str:
         q, out, table = v["q"], v["out"], v["page_table"]
         _native.call("intent_paged_attention", _ptr(q), env["T"], env["HQ"], _ld(q), int(dt == "bf16"), int(fp8),
                      *_cache_arguments(v, fp8), env["PAGES"], env["HK"], env["PAGE"], env["D"], _ptr(table), env["S"],
                      env["MAX_PAGES"], _ld(table), _ptr(v["q_offsets"]), _ptr(v["kv_lens"]), float(env["scale"]),
-                     int(bool(env["CAUSAL"])), int(env["WINDOW"]), _ptr(out), _ld(out), stream)
+                     int(bool(env["CAUSAL"])), int(env["WINDOW"]), _ptr(out), _ld(out),
+                     None if scratch is None else _ptr(scratch), 0 if scratch is None else scratch.numel(), stream)
         return "intent_paged_attention"
 
     return KernelDefinition(
@@ -1476,6 +1482,7 @@ def _attention_definition(dt: str, fp8: bool) -> KernelDefinition:
             Scalar("scale", "f32"),
         ),
         launch=launch,
+        scratch=_attention_scratch,
         constexprs={"CAUSAL": True, "WINDOW": 0},
         check=_attention_check,
         reference="no kernel of the reference's quantized path; I.matmul contractions over a paged operand",

@@ -762,7 +762,7 @@ def _append_args(**change):
 def _attention_args(**change):
     a = dict(q=FAKE, T=4, HQ=4, q_ld=256, bf16=0, fp8=1, kc=FAKE, kc_ld=2048, vc=FAKE, vc_ld=2048, ks=FAKE, ks_ld=32,
              vs=FAKE, vs_ld=32, pages=4, HK=2, page=16, D=64, table=FAKE, S=2, width=3, table_ld=3, offsets=FAKE,
-             kv=FAKE, scale=0.1, causal=1, window=0, out=FAKE, out_ld=256, stream=None)
+             kv=FAKE, scale=0.1, causal=1, window=0, out=FAKE, out_ld=256, ws=None, ws_bytes=0, stream=None)
     assert set(change) <= set(a)
     return list({**a, **change}.values())
 
