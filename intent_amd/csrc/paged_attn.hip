@@ -162,19 +162,22 @@ bool tiled(int64_t D) { return D == 64 || D == 96 || D == 128 || D == 256; }
 
 // The host knows the rows of all sequences together. Up to 64 for each on average, they go to the
 // kernel that spreads the tokens over the waves, with the tile that holds the average; beyond, each
-// sequence goes by its own: up to 32 rows there, more to the 128-row tile.
-Plan plan_of(int64_t T, int64_t S, int64_t group) {
+// sequence goes by its own: up to 32 rows there, more to the 128-row tile. Heads of 256 leave that
+// kernel registers for 16 rows only.
+Plan plan_of(int64_t T, int64_t S, int64_t group, int64_t D) {
   const int64_t rows = T * group, mean = (rows + S - 1) / S;
   Plan p{};
   p.parts = 1;
-  if (mean <= 64) {
+  const int most = D > 128 ? 16 : 64;
+  if (mean <= most) {
     p.part[0] = {mean <= 16 ? 1 : mean <= 32 ? 2 : 4, 0, INT32_MAX};
   } else if (S == 1) {
     p.part[0] = {0, 0, INT32_MAX};
   } else {
     p.parts = 2;
-    p.part[0] = {0, 32, INT32_MAX};
-    p.part[1] = {2, 0, 32};
+    const int few = D > 128 ? 16 : 32;
+    p.part[0] = {0, few, INT32_MAX};
+    p.part[1] = {few / 16, 0, few};
   }
   return p;
 }
@@ -199,7 +202,7 @@ size_t part_bytes(const Part& p, int64_t T, int64_t S, int64_t group, int64_t HK
 }
 
 int launch_tiled(AttnArgs a, bool bf16, bool fp8, float* workspace, size_t bytes, hipStream_t stream) {
-  const Plan plan = plan_of(a.T, a.S, a.group);
+  const Plan plan = plan_of(a.T, a.S, a.group, a.D);
   int status = INTENT_OK;
   for (int i = 0; i < plan.parts && status == INTENT_OK; ++i) {
     const Part& p = plan.part[i];
@@ -234,7 +237,7 @@ extern "C" size_t intent_paged_attention_workspace_size(int64_t T, int64_t HQ, i
   if (T <= 0 || HQ <= 0 || HK <= 0 || S <= 0 || HQ % HK || table_width <= 0 || page_size <= 0 || !tiled(D) ||
       table_width > kMostTokens / page_size || HQ > 65536 || T * HQ >= ((int64_t)1 << 26))
     return 0;
-  const Plan plan = plan_of(T, S, HQ / HK);
+  const Plan plan = plan_of(T, S, HQ / HK, D);
   size_t most = 0;
   for (int i = 0; i < plan.parts; ++i) {
     const size_t need = part_bytes(plan.part[i], T, S, HQ / HK, HK, D, table_width * page_size);

@@ -14,6 +14,11 @@
 // rarely; in f32 and in 16-bit weights this costs no precision. With an 8-bit cache the value's scale
 // is part of the weight that is rounded: M follows the maximum of t + log2(scale), w = exp2(t - M) *
 // scale, and only the sum of weights takes exp2(t - M) by itself. The codes are exact in 16 bits.
+//
+// A weight of zero does not keep an infinity or NaN out of a product. Tokens that no row of a tile sees
+// are read from a row of zeros; where rows of a tile see different tokens (the last of a chunk, the
+// first of a window), values that are not finite go into the product as zeros, and once the loop is
+// over they are added to the rows that see them (which has them infinite or NaN).
 #pragma once
 
 #include "paged_attn.h"
@@ -65,12 +70,28 @@ INTENT_DEVICE u32x4 widen_codes(uint32_t lo, uint32_t hi) {
   return r;
 }
 
-// 0x8000 in each half of a pair of 16-bit floats that is an infinity or NaN (all exponent bits set: one
-// more in the exponent's last place carries into the sign's, which the mask has cleared).
+// Eight 16-bit floats with zeros for infinities and NaN, which are noted in `found`. (All exponent bits
+// set: one more in the exponent's last place carries into the sign's place, which the mask has cleared.)
 template <bool kBf16>
-INTENT_DEVICE uint32_t not_finite(uint32_t pair) {
+INTENT_DEVICE u32x4 only_finite(u32x4 v, bool& found) {
   constexpr uint32_t kExponent = kBf16 ? 0x7f807f80u : 0x7c007c00u, kStep = kBf16 ? 0x00800080u : 0x04000400u;
-  return ((pair & kExponent) + kStep) & 0x80008000u;
+  uint32_t any = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t out = ((v[e] & kExponent) + kStep) & 0x80008000u;
+    any |= out;
+    v[e] &= ~((out >> 15) * 0xffffu);
+  }
+  found = found || any != 0;
+  return v;
+}
+
+// One cached value, its scale left out.
+template <bool kBf16, bool kFp8>
+INTENT_DEVICE float cached_value(const void* row, int d) {
+  if constexpr (kFp8) return __builtin_amdgcn_cvt_f32_fp8((int)((const uint8_t*)row)[d], 0);
+  else if constexpr (kBf16) return bit_cast<float>((uint32_t)((const uint16_t*)row)[d] << 16);
+  else return (float)((const f16*)row)[d];
 }
 
 INTENT_DEVICE u32x2 read_transposed(const char* lds) {
@@ -138,12 +159,6 @@ INTENT_DEVICE float sum_across32(float v) {
   return bit_cast<float>(r[0]) + bit_cast<float>(r[1]);
 }
 
-// Keeps the halves of a pair of values whose tokens (the two of consecutive index from `t`) a row sees.
-INTENT_DEVICE uint32_t seen_pair(uint32_t pair, int t, int lo, int hi) {
-  const uint32_t keep = (t >= lo && t < hi ? 0xffffu : 0u) | (t + 1 >= lo && t + 1 < hi ? 0xffff0000u : 0u);
-  return pair & keep;
-}
-
 // ---- few rows: 16 * MT of them, the tokens over the waves -----------------------------------------
 
 // A wave takes 32 tokens at a time, four apart from its next: keys straight into the first product's
@@ -183,7 +198,7 @@ __global__ __launch_bounds__(256, D <= 128 && MT <= 2 ? 2 : 1) void attn_rows_ke
   // the tokens that some row sees, and those that all rows see
   const RowView top = row_view(a, w, 0), bottom = row_view(a, w, w.rows - 1);
   const int some_lo = top.lo, some_hi = bottom.hi, all_lo = bottom.lo, all_hi = top.hi;
-  const float scale = fabsf(a.scale_log2);
+  const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);  // -inf stays what it is beside a scale of 0
 
   f32x4 o[MT][DT];
   float ref[MT], total[MT];
@@ -238,6 +253,9 @@ __global__ __launch_bounds__(256, D <= 128 && MT <= 2 ? 2 : 1) void attn_rows_ke
     }
   };
 
+  // whether rows of this tile see different ones of the tokens t ..
+  auto apart = [&](int t) { return (some_lo != all_lo || some_hi != all_hi) && (t < all_lo || t + 32 > all_hi); };
+  bool found = false;
   int t = w.begin + wave * 32;
   if (t < w.end) {
     load_ids(t);
@@ -246,17 +264,22 @@ __global__ __launch_bounds__(256, D <= 128 && MT <= 2 ? 2 : 1) void attn_rows_ke
   }
   for (; t < w.end; t += 128) {
     // values and scales of these tokens to LDS, the scores' operands from the registers
+    const bool masked = t < all_lo || t + 32 > all_hi;
+    const bool check = apart(t);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         char* row = mine + u * 16 * RB + write_at;
         const int chunk = at(i) / 8;
-        if constexpr (kFp8) {
-          *(u32x4*)(row + ((chunk ^ swz) << 4)) = widen_codes<kBf16>(vr[u][i][0], vr[u][i][1]);
-          if constexpr (kWide) *(u32x4*)(row + (((chunk + 1) ^ swz) << 4)) = widen_codes<kBf16>(vr[u][i][2], vr[u][i][3]);
-        } else {
-          *(u32x4*)(row + ((chunk ^ swz) << 4)) = vr[u][i];
+        u32x4 part = vr[u][i];
+        if constexpr (kFp8) part = widen_codes<kBf16>(vr[u][i][0], vr[u][i][1]);
+        if (check) part = only_finite<kBf16>(part, found);
+        *(u32x4*)(row + ((chunk ^ swz) << 4)) = part;
+        if constexpr (kFp8 && kWide) {
+          part = widen_codes<kBf16>(vr[u][i][2], vr[u][i][3]);
+          if (check) part = only_finite<kBf16>(part, found);
+          *(u32x4*)(row + (((chunk + 1) ^ swz) << 4)) = part;
         }
       }
       if constexpr (kFp8) {
@@ -288,40 +311,43 @@ __global__ __launch_bounds__(256, D <= 128 && MT <= 2 ? 2 : 1) void attn_rows_ke
       load_rows(now + 128);
       load_ids(now + 256);
     }
-    const bool masked = now < all_lo || now + 32 > all_hi;
     u32x4 p[MT];
-    f32x4 k_mul[2], v_mul[2], v_exp[2];
+    f32x4 v_mul[2], v_exp[2];
+    if constexpr (kFp8) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      if constexpr (kFp8) {
-        k_mul[u] = *(const f32x4*)&scales[wave][0][u * 16 + g * 4];
+      for (int u = 0; u < 2; ++u) {
+        const f32x4 k_mul = *(const f32x4*)&scales[wave][0][u * 16 + g * 4];
         v_mul[u] = *(const f32x4*)&scales[wave][1][u * 16 + g * 4];
         v_exp[u] = *(const f32x4*)&scales[wave][2][u * 16 + g * 4];
-      } else {
-        k_mul[u] = f32x4{scale, scale, scale, scale};
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[m][u][r] *= k_mul[r];
       }
     }
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      float x[2][4], high = -INFINITY;
-      bool seen[2][4];
+      // the highest score, times the value's scale; s is a score or, with an 8-bit cache, its t
+      float high = -INFINITY;
+      if (masked) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < 2; ++u) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          x[u][r] = s[m][u][r] * k_mul[u][r];
-          float y = kFp8 ? x[u][r] + v_exp[u][r] : x[u][r];
-          seen[u][r] = true;
-          if (masked) {
+          for (int r = 0; r < 4; ++r) {
             const int tk = now + 16 * u + g * 4 + r;
-            seen[u][r] = tk >= view[m].lo && tk < view[m].hi;
-            x[u][r] = seen[u][r] ? x[u][r] : -INFINITY;
-            y = seen[u][r] ? y : -INFINITY;
+            const bool seen = tk >= view[m].lo && tk < view[m].hi;
+            s[m][u][r] = seen ? s[m][u][r] : -INFINITY;
+            high = fmaxf(high, kFp8 && seen ? s[m][u][r] + v_exp[u][r] : s[m][u][r]);
           }
-          high = fmaxf(high, y);
         }
+      } else {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) high = fmaxf(high, kFp8 ? s[m][u][r] + v_exp[u][r] : s[m][u][r]);
       }
       high = max_across32(max_across16(high));
+      if constexpr (!kFp8) high *= scale;
       if (__any(high > ref[m] + kRise)) {
         const float next = fmaxf(ref[m], high);
         const float keep = __builtin_amdgcn_exp2f(ref[m] - (next == -INFINITY ? 0.f : next));
@@ -336,58 +362,49 @@ __global__ __launch_bounds__(256, D <= 128 && MT <= 2 ? 2 : 1) void attn_rows_ke
       for (int u = 0; u < 2; ++u) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float e = __builtin_amdgcn_exp2f(x[u][r] - base);
+          const float e = __builtin_amdgcn_exp2f(kFp8 ? s[m][u][r] - base : __builtin_fmaf(s[m][u][r], scale, -base));
           total[m] += e;
-          wt[u][r] = kFp8 ? e * v_mul[u][r] : e;
-          if (kFp8 && masked) wt[u][r] = seen[u][r] ? wt[u][r] : 0.f;
+          wt[u][r] = e;
+          if constexpr (kFp8) {
+            wt[u][r] = e * v_mul[u][r];
+            if (masked) wt[u][r] = s[m][u][r] == -INFINITY ? 0.f : wt[u][r];  // a scale that is not seen may be NaN
+          }
         }
       }
       p[m] = u32x4{pack2<kBf16>(wt[0][0], wt[0][1]), pack2<kBf16>(wt[0][2], wt[0][3]), pack2<kBf16>(wt[1][0], wt[1][1]),
                    pack2<kBf16>(wt[1][2], wt[1][3])};
     }
     // V^T: tokens 4 g .. of the first 16, then of the second
-    u32x4 v[DT];
-#pragma unroll
-    for (int d = 0; d < DT; ++d) {
+    auto value = [&](int d) {
       const char* from = lds + (read_at ^ (d * 32));
       const u32x2 lo = read_transposed(from), hi = read_transposed(from + 16 * RB);
-      v[d] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+      return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    };
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      const u32x4 v = value(d);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) o[m][d] = mfma16<kBf16>(v, p[m], o[m][d]);
     }
-    bool apart = false;
-    if (masked && (some_lo != all_lo || some_hi != all_hi)) {
-      // rows of this tile see different tokens: 0 * NaN in one that does not see it must not reach it
-      uint32_t bad = 0;
+    wave_lds_order();
+  }
+  if (__any(found)) {  // values left out of the products above
+    for (t = w.begin + wave * 32; t < w.end; t += 128) {
+      for (int tk = max(t, some_lo); apart(t) && tk < min(t + 32, some_hi); ++tk) {
+        const int page = page_of(a, w.s, tk);
+        const char* row = (const char*)a.v_cache + row_in_cache(a, page, a.v_page, head, tk, D) * (kFp8 ? 1 : 2);
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
+        for (int d = 0; d < DT; ++d) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) bad |= not_finite<kBf16>(v[d][e]);
-      apart = __any(bad != 0);
-    }
-    if (apart) {
+          for (int r = 0; r < 4; ++r) {
+            const float v = cached_value<kBf16, kFp8>(row, d * 16 + g * 4 + r);
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        for (int c = 0; c < 16; ++c) {  // one row at a time, over the values that it sees
-          const int lo = lane_value(view[m].lo, c), hi = lane_value(view[m].hi, c);
-          const uint32_t only = col == c ? ~0u : 0u;
-          const u32x4 pc = u32x4{p[m][0] & only, p[m][1] & only, p[m][2] & only, p[m][3] & only};
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            u32x4 vc;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) vc[e] = seen_pair(v[d][e], now + (e >> 1) * 16 + g * 4 + (e & 1) * 2, lo, hi);
-            const f32x4 add = mfma16<kBf16>(vc, pc, f32x4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[m][d][r] = col == c ? o[m][d][r] + add[r] : o[m][d][r];
+            for (int m = 0; m < MT; ++m)
+              if (tk >= view[m].lo && tk < view[m].hi && !(fabsf(v) < INFINITY)) o[m][d][r] += v;
           }
         }
       }
-    } else {
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int m = 0; m < MT; ++m) o[m][d] = mfma16<kBf16>(v[d], p[m], o[m][d]);
     }
-    wave_lds_order();
   }
 
   // join the four waves, 16 rows at a time
@@ -445,6 +462,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
   constexpr int kTile = 64 * RB;
   __shared__ __attribute__((aligned(16))) char lds[2][2][kTile];
   __shared__ __attribute__((aligned(16))) float scales[kFp8 ? 2 : 1][3][64];
+  __shared__ int left_out;  // values that are not finite were left out of a product
 
   const int head = blockIdx.x % a.HK;
   Span w;
@@ -460,10 +478,11 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
 #pragma unroll
     for (int i = 0; i < KS; ++i) q[i] = signed_query(a, load16(row + i * 16 + h * 8));
   }
-  const int some_lo = row_view(a, w, 0).lo, some_hi = row_view(a, w, w.rows - 1).hi;
+  const RowView first = row_view(a, w, 0), last = row_view(a, w, w.rows - 1);
+  const int some_lo = first.lo, some_hi = last.hi, all_lo = last.lo, all_hi = first.hi;
   const RowView top = row_view(a, w, r0), bottom = row_view(a, w, r0 + 31);  // of this wave
   const bool idle = r0 >= w.rows;
-  const float scale = fabsf(a.scale_log2);
+  const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);  // -inf stays what it is beside a scale of 0
 
   f32x16 o[DT];
 #pragma unroll
@@ -506,7 +525,11 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
       vs = *(live ? vp : (const float*)kZeroRow);
     }
   };
-  auto store_rows = [&](int buffer) {
+  // whether rows of this tile see different ones of the tokens t ..
+  auto apart = [&](int t) { return (some_lo != all_lo || some_hi != all_hi) && (t < all_lo || t + 64 > all_hi); };
+  auto store_rows = [&](int buffer, int t) {
+    const bool check = apart(t);
+    bool found = false;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int tk = load_token + i * STEP, swz = swizzle(tk);
@@ -517,14 +540,17 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
           const int c = load_chunk * 2;
           *(u32x4*)(k + ((c ^ swz) << 4)) = widen_codes<kBf16>(kr[i][0], kr[i][1]);
           *(u32x4*)(k + (((c + 1) ^ swz) << 4)) = widen_codes<kBf16>(kr[i][2], kr[i][3]);
-          *(u32x4*)(v + ((c ^ swz) << 4)) = widen_codes<kBf16>(vr[i][0], vr[i][1]);
-          *(u32x4*)(v + (((c + 1) ^ swz) << 4)) = widen_codes<kBf16>(vr[i][2], vr[i][3]);
+          u32x4 lo = widen_codes<kBf16>(vr[i][0], vr[i][1]), hi = widen_codes<kBf16>(vr[i][2], vr[i][3]);
+          if (check) lo = only_finite<kBf16>(lo, found), hi = only_finite<kBf16>(hi, found);
+          *(u32x4*)(v + ((c ^ swz) << 4)) = lo;
+          *(u32x4*)(v + (((c + 1) ^ swz) << 4)) = hi;
         } else {
           *(u32x4*)(k + ((load_chunk ^ swz) << 4)) = kr[i];
-          *(u32x4*)(v + ((load_chunk ^ swz) << 4)) = vr[i];
+          *(u32x4*)(v + ((load_chunk ^ swz) << 4)) = check ? only_finite<kBf16>(vr[i], found) : vr[i];
         }
       }
     }
+    if (found) left_out = 1;
     if constexpr (kFp8) {
       if (wave == 0) {
         scales[buffer][0][lane] = ks * scale;
@@ -538,11 +564,13 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
   const int i16 = lane & 15, read_row = h * 4 + (i16 >> 2);
   const int v_at = read_row * RB + ((((lane >> 4 & 1) * 2 + (i16 >> 1 & 1)) ^ swizzle(read_row)) << 4) + (i16 & 1) * 8;
 
+  if (threadIdx.x == 0) left_out = 0;
+  __syncthreads();
   if (w.begin < w.end) {
     load_ids(w.begin);
     load_rows(w.begin);
     load_ids(w.begin + 64);
-    store_rows(0);
+    store_rows(0, w.begin);
   }
   __syncthreads();
   int buffer = 0;
@@ -566,30 +594,39 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
       }
       const bool masked = t < bottom.lo || t + 64 > top.hi;
       float high = -INFINITY;
+      if constexpr (kFp8) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const f32x4 k_mul = *(const f32x4*)&scales[buffer][0][u * 32 + i * 8 + h * 4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[u][i * 4 + r] *= k_mul[r];
+          }
+      }
+      if (masked) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int tk = t + u * 32 + (r >> 2) * 8 + h * 4 + (r & 3);
+            s[u][r] = tk >= view.lo && tk < view.hi ? s[u][r] : -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int t0 = u * 32 + i * 8 + h * 4;
-          f32x4 k_mul, v_exp;
-          if constexpr (kFp8) {
-            k_mul = *(const f32x4*)&scales[buffer][0][t0];
-            v_exp = *(const f32x4*)&scales[buffer][2][t0];
-          }
+          f32x4 v_exp;
+          if constexpr (kFp8) v_exp = *(const f32x4*)&scales[buffer][2][u * 32 + i * 8 + h * 4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            float x = s[u][i * 4 + r] * (kFp8 ? k_mul[r] : scale);
-            float y = kFp8 ? x + v_exp[r] : x;
-            if (masked) {
-              const bool seen = t + t0 + r >= view.lo && t + t0 + r < view.hi;
-              x = seen ? x : -INFINITY;
-              y = seen ? y : -INFINITY;
-            }
-            s[u][i * 4 + r] = x;
+            float y = s[u][i * 4 + r];
+            if constexpr (kFp8) y = masked ? (y == -INFINITY ? y : y + v_exp[r]) : y + v_exp[r];
             high = fmaxf(high, y);
           }
         }
-      }
+      if constexpr (!kFp8) high *= scale;
       high = max_across32(high);
       if (__any(high > ref + kRise)) {
         const float next = fmaxf(ref, high);
@@ -613,10 +650,14 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
           float wt[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float x = s[u][i * 4 + r], e = __builtin_amdgcn_exp2f(x - base);
+            const float x = s[u][i * 4 + r];
+            const float e = __builtin_amdgcn_exp2f(kFp8 ? x - base : __builtin_fmaf(x, scale, -base));
             total += e;
-            wt[r] = kFp8 ? e * v_mul[r] : e;
-            if (kFp8 && masked) wt[r] = t + t0 + r >= view.lo && t + t0 + r < view.hi ? wt[r] : 0.f;
+            wt[r] = e;
+            if constexpr (kFp8) {
+              wt[r] = e * v_mul[r];
+              if (masked) wt[r] = x == -INFINITY ? 0.f : wt[r];  // a scale that is not seen may be NaN
+            }
           }
           p[u * 2 + i / 2][(i & 1) * 2] = pack2<kBf16>(wt[0], wt[1]);
           p[u * 2 + i / 2][(i & 1) * 2 + 1] = pack2<kBf16>(wt[2], wt[3]);
@@ -627,53 +668,32 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
         const u32x2 lo = read_transposed(from), hi = read_transposed(from + 8 * RB);
         return u32x4{lo[0], lo[1], hi[0], hi[1]};
       };
-      bool apart = false;
-      if (masked) {
-        uint32_t bad = 0;
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+      for (int d = 0; d < DT; ++d)
 #pragma unroll
-          for (int m = 0; m < 4; ++m) {
-            const u32x4 v = value(d, m);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) bad |= not_finite<kBf16>(v[e]);
-          }
-        apart = __any(bad != 0);
-      }
-      if (apart) {
-        for (int c = 0; c < 32; ++c) {  // one row at a time, over the values that it sees
-          const int lo = lane_value(view.lo, c), hi = lane_value(view.hi, c);
-          const uint32_t only = col == c ? ~0u : 0u;
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            f32x16 add;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) add[r] = 0.f;
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-              u32x4 v = value(d, m), pc;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                v[e] = seen_pair(v[e], t + m * 16 + (e >> 1) * 8 + h * 4 + (e & 1) * 2, lo, hi);
-                pc[e] = p[m][e] & only;
-              }
-              add = mfma32<kBf16>(v, pc, add);
-            }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[d][r] = col == c ? o[d][r] + add[r] : o[d][r];
-          }
-        }
-      } else {
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int m = 0; m < 4; ++m) o[d] = mfma32<kBf16>(value(d, m), p[m], o[d]);
-      }
+        for (int m = 0; m < 4; ++m) o[d] = mfma32<kBf16>(value(d, m), p[m], o[d]);
     }
-    if (more) store_rows(buffer ^ 1);
+    if (more) store_rows(buffer ^ 1, t + 64);
     __syncthreads();
   }
 
+  if (left_out != 0) {
+    for (int t = w.begin; t < w.end; t += 64) {
+      for (int tk = max(t, some_lo); apart(t) && tk < min(t + 64, some_hi); ++tk) {
+        const int page = page_of(a, w.s, tk);
+        const char* row = (const char*)a.v_cache + row_in_cache(a, page, a.v_page, head, tk, D) * (kFp8 ? 1 : 2);
+        const bool seen = tk >= view.lo && tk < view.hi;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float v = cached_value<kBf16, kFp8>(row, d * 32 + (r >> 2) * 8 + h * 4 + (r & 3));
+            if (seen && !(fabsf(v) < INFINITY)) o[d][r] += v;
+          }
+        }
+      }
+    }
+  }
   const int r = r0 + col;
   if (r >= w.rows) return;
   const float all = sum_across32(total);
@@ -769,12 +789,12 @@ int launch(const AttnLaunch& l, hipStream_t stream) {
 
 template <bool kBf16, bool kFp8, int D>
 int launch_d(const AttnLaunch& l, int tiles, hipStream_t stream) {
-  switch (tiles) {
-    case 1: return launch<kBf16, kFp8, D, 1>(l, stream);
-    case 2: return launch<kBf16, kFp8, D, 2>(l, stream);
-    case 4: return launch<kBf16, kFp8, D, 4>(l, stream);
-    default: return launch<kBf16, kFp8, D, 0>(l, stream);
+  if (tiles == 1) return launch<kBf16, kFp8, D, 1>(l, stream);
+  if constexpr (D <= 128) {
+    if (tiles == 2) return launch<kBf16, kFp8, D, 2>(l, stream);
+    if (tiles == 4) return launch<kBf16, kFp8, D, 4>(l, stream);
   }
+  return launch<kBf16, kFp8, D, 0>(l, stream);
 }
 
 template <bool kBf16, bool kFp8>
