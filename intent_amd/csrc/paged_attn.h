@@ -28,6 +28,8 @@ struct AttnArgs {
   int64_t out_ld;
   float scale_log2;  // scale * log2(e): the kernels work with exp2
   int T, S, HQ, HK, group, D, pages, page_shift, most_kv, causal, window;
+  // the page strides again for the tiled kernels: in 16 bytes, and in scales
+  uint32_t k_step, v_step, ks_step, vs_step;
   // work list of the tiled kernels (find_span)
   int min_rows, max_rows;  // sequences with more rows (new tokens times group) than min, up to max
   int target;              // workgroups for each cached head that tiles are split for; 0: none
@@ -164,6 +166,12 @@ INTENT_DEVICE bool find_span(const AttnArgs& a, int item, bool joins, Span& r) {
 INTENT_DEVICE int page_of(const AttnArgs& a, int s, int t) {
   return (int)min((uint32_t)a.page_table[(int64_t)s * a.table_ld + (t >> a.page_shift)], (uint32_t)a.pages - 1u);
 }
+
+// The table's entry of token t as it is, and the page that it names.
+INTENT_DEVICE uint32_t table_entry(const AttnArgs& a, int s, int t) {
+  return (uint32_t)a.page_table[(int64_t)s * a.table_ld + (t >> a.page_shift)];
+}
+INTENT_DEVICE uint32_t page_named(const AttnArgs& a, uint32_t entry) { return min(entry, (uint32_t)a.pages - 1u); }
 
 // Row of token t of a page and head in a cache with `row` elements for each token.
 INTENT_DEVICE int64_t row_in_cache(const AttnArgs& a, int page, int64_t page_ld, int head, int t, int row) {

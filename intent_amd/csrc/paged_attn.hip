@@ -6,6 +6,7 @@ namespace {
 using namespace intent;
 
 constexpr int64_t kMostTokens = (int64_t)1 << 30;  // of a sequence: positions stay far inside 32 bits
+constexpr int64_t kMostStride = UINT32_MAX;
 
 template <bool kBf16>
 INTENT_DEVICE float widen1(uint16_t v) {
@@ -222,8 +223,10 @@ int launch_tiled(AttnArgs a, bool bf16, bool fp8, float* workspace, size_t bytes
     l.a = a;
     l.items = (int)(tiles + a.target);
     l.joins = (int)joins;
-    const int64_t mean = ((int64_t)a.T * a.group + a.S - 1) / a.S;
-    l.join_rows = (int)(mean < 16 ? mean : 16);
+    // rows of a split tile side by side: at most those of a mean sequence, and 2048 workgroups in all
+    const int64_t mean = ((int64_t)a.T * a.group + a.S - 1) / a.S, room = joins > 0 ? 2048 / (joins * a.HK) : 0;
+    const int64_t side = mean < p.rows() ? mean : p.rows();
+    l.join_rows = (int)(room < 1 ? 1 : room < side ? room : side);
     if (fp8) status = bf16 ? launch_attn_bf16_fp8(l, p.tiles, stream) : launch_attn_f16_fp8(l, p.tiles, stream);
     else status = bf16 ? launch_attn_bf16(l, p.tiles, stream) : launch_attn_f16(l, p.tiles, stream);
   }
@@ -293,10 +296,16 @@ extern "C" int intent_paged_attention(const void* q, int64_t T, int64_t HQ, int6
                        (!cache_is_fp8 || (intent::aligned4(k_scales) && intent::aligned4(v_scales))),
                    INTENT_ERR_ALIGNMENT, "the cache must be 16-byte aligned with page strides of whole 16 bytes");
   }
+  INTENT_REQUIRE(!any || pages == 1 || (k_page_ld <= kMostStride && v_page_ld <= kMostStride &&
+                                        k_scales_ld <= kMostStride && v_scales_ld <= kMostStride),
+                 INTENT_ERR_UNSUPPORTED, "page stride past 2^32 elements");
   AttnArgs a{};
   a.q = (const uint16_t*)q, a.q_ld = q_ld;
   a.k_cache = k_cache, a.v_cache = v_cache, a.k_page = k_page_ld, a.v_page = v_page_ld;
   a.k_scales = k_scales, a.v_scales = v_scales, a.ks_page = k_scales_ld, a.vs_page = v_scales_ld;
+  const int64_t units = cache_is_fp8 ? 16 : 8;
+  a.k_step = (uint32_t)(k_page_ld / units), a.v_step = (uint32_t)(v_page_ld / units);
+  a.ks_step = (uint32_t)k_scales_ld, a.vs_step = (uint32_t)v_scales_ld;
   a.page_table = page_table, a.table_ld = table_ld;
   a.q_offsets = q_offsets, a.kv_lens = kv_lens;
   a.out = (uint16_t*)out, a.out_ld = out_ld;

@@ -26,6 +26,8 @@
 namespace intent {
 namespace attn {
 
+using ::load16;
+
 constexpr float kRise = 8.0f;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -34,6 +36,29 @@ typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
 
 // What tokens that no row of a tile sees are read from: pages behind a sequence's end hold anything.
 static __device__ __attribute__((aligned(16))) const uint32_t kZeroRow[128] = {};
+
+// A cached token's row (or scale) of a page, or the row of zeros: global addresses throughout, so that
+// the loads count on vmcnt alone.
+typedef const __attribute__((address_space(1))) char* global_bytes;
+INTENT_DEVICE global_bytes as_global(const void* p) { return (global_bytes)p; }
+// Rows (of kRowBytes) of a head from token t on, t and the page uniform or not.
+template <int kRowBytes>
+INTENT_DEVICE global_bytes cached_rows(const AttnArgs& a, const void* base, uint32_t page, uint32_t step, int head, int t) {
+  const uint32_t row = (uint32_t)((head << a.page_shift) + (t & ((1 << a.page_shift) - 1)));
+  return as_global(base) + ((uint64_t)page * step + (uint64_t)row * (kRowBytes / 16)) * 16;
+}
+INTENT_DEVICE global_bytes cached_scales(const AttnArgs& a, const float* base, uint32_t page, uint32_t step, int head, int t) {
+  const uint32_t row = (uint32_t)((head << a.page_shift) + (t & ((1 << a.page_shift) - 1)));
+  return as_global(base) + ((uint64_t)page * step + row) * 4;
+}
+INTENT_DEVICE float load_float(global_bytes p) { return *(const __attribute__((address_space(1))) float*)p; }
+// The table's entry of a token that is the same in all lanes: a scalar load.
+INTENT_DEVICE uint32_t uniform_entry(const AttnArgs& a, int s, int t) {
+  const int64_t at = (int64_t)s * a.table_ld + (t >> a.page_shift);
+  return *(const __attribute__((address_space(4))) uint32_t*)(a.page_table + at);
+}
+INTENT_DEVICE u32x4 load16(global_bytes p) { return *(const __attribute__((address_space(1))) u32x4*)p; }
+INTENT_DEVICE u32x2 load8(global_bytes p) { return *(const __attribute__((address_space(1))) u32x2*)p; }
 
 template <bool kBf16>
 INTENT_DEVICE f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
@@ -99,10 +124,16 @@ INTENT_DEVICE u32x2 read_transposed(const char* lds) {
       (__attribute__((address_space(3))) s16x4*)(__attribute__((address_space(3))) char*)lds));
 }
 
-// Rows of LDS tiles are a power of two of bytes; the 16-byte chunk c of token t is kept at c ^ swizzle(t):
-// eight consecutive tokens have eight values (reads of one chunk down the tokens), and four
-// consecutive ones differ in the upper two bits (the transposing read takes 32 bytes of each).
-INTENT_DEVICE int swizzle(int t) { return (t & 3) << 1 | (t >> 2 & 1); }
+// Rows of LDS tiles are a power of two of bytes (RB); the 16-byte chunk c of token t is kept at
+// c ^ swizzle(t). LDS has 64 banks of 4 bytes, so that 16 lanes of a 16-byte access and 32 of an 8-byte
+// one have to lie apart in 256 bytes: one chunk of 16 consecutive tokens (16 bytes each), and what a
+// transposing read takes of 4 tokens (64 bytes each, the 128-row kernel) or of 8 (32 bytes each, the
+// other). Rows of 128 bytes alternate between the halves of the banks by themselves.
+template <int RB, bool kTileKernel>
+INTENT_DEVICE int swizzle(int t) {
+  if constexpr (kTileKernel) return RB == 128 ? (t >> 1 & 1) << 2 | (t >> 2 & 3) : (t & 3) << 2 | (t >> 2 & 3);
+  else return RB == 128 ? (t >> 1 & 3) << 1 | (t >> 3 & 1) : (t & 7) << 1 | (t >> 3 & 1);
+}
 
 template <int D>
 constexpr int row_bytes() {
@@ -210,46 +241,66 @@ __global__ __launch_bounds__(256, D <= 128 && MT <= 2 ? 2 : 1) void attn_rows_ke
   }
 
   char* mine = lds + wave * 32 * RB;
-  const int write_at = col * RB, swz = swizzle(col);
+  const int write_at = col * RB, swz = swizzle<RB, false>(col);
   // transposing reads: tokens 4 g .. 4 g + 3 of each 16, columns 16 d ..
   const int read_row = g * 4 + (col >> 2);
-  const int read_at = wave * 32 * RB + read_row * RB + (((col >> 1 & 1) ^ swizzle(read_row)) << 4) + (col & 1) * 8;
+  const int read_at = wave * 32 * RB + read_row * RB + (((col >> 1 & 1) ^ swizzle<RB, false>(read_row)) << 4) + (col & 1) * 8;
 
   u32x4 kr[2][LOADS], vr[2][LOADS];
   float ks[2], vs[2];
-  int ids[2];
-  auto token = [&](int t, int u) { return t + 16 * u + col; };
+  // Pages of 16 tokens and more: each 16 tokens lie in one, whose id is a scalar (loaded ahead, clamped
+  // where it is used, so that the wait for it is there). Smaller ones: each lane looks up its token's.
+  constexpr int kBytes = kFp8 ? 1 : 2;
+  const bool paged = a.page_shift >= 4;
+  const uint32_t lane_at = col * (D * kBytes) + g * ELEMS * kBytes;
+  uint32_t ids[2];
+  auto clamped = [&](int t) { return min(max(t, some_lo), max(some_hi - 1, 0)); };
   auto load_ids = [&](int t) {
+    if (paged)
 #pragma unroll
-    for (int u = 0; u < 2; ++u) ids[u] = page_of(a, w.s, min(max(token(t, u), some_lo), max(some_hi - 1, 0)));
+      for (int u = 0; u < 2; ++u) ids[u] = uniform_entry(a, w.s, clamped(t + 16 * u));
   };
   auto load_rows = [&](int t) {
+    const bool whole = t >= some_lo && t + 32 <= some_hi;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int tk = token(t, u);
-      const bool live = tk >= some_lo && tk < some_hi;
-      constexpr int kBytes = kFp8 ? 1 : 2;
-      const char* k = (const char*)a.k_cache + row_in_cache(a, ids[u], a.k_page, head, tk, D) * kBytes;
-      const char* v = (const char*)a.v_cache + row_in_cache(a, ids[u], a.v_page, head, tk, D) * kBytes;
-      k = live ? k : (const char*)kZeroRow;
-      v = live ? v : (const char*)kZeroRow;
+      const int t16 = t + 16 * u, tk = t16 + col;
+      global_bytes k, v, kp{}, vp{};
+      if (paged) {
+        const uint32_t page = page_named(a, ids[u]);
+        k = cached_rows<D * kBytes>(a, a.k_cache, page, a.k_step, head, t16) + lane_at;
+        v = cached_rows<D * kBytes>(a, a.v_cache, page, a.v_step, head, t16) + lane_at;
+        if constexpr (kFp8) {
+          kp = cached_scales(a, a.k_scales, page, a.ks_step, head, t16) + col * 4;
+          vp = cached_scales(a, a.v_scales, page, a.vs_step, head, t16) + col * 4;
+        }
+      } else {
+        const uint32_t page = page_named(a, table_entry(a, w.s, clamped(tk)));
+        k = cached_rows<D * kBytes>(a, a.k_cache, page, a.k_step, head, tk) + g * ELEMS * kBytes;
+        v = cached_rows<D * kBytes>(a, a.v_cache, page, a.v_step, head, tk) + g * ELEMS * kBytes;
+        if constexpr (kFp8) {
+          kp = cached_scales(a, a.k_scales, page, a.ks_step, head, tk);
+          vp = cached_scales(a, a.v_scales, page, a.vs_step, head, tk);
+        }
+      }
+      if (!whole) {
+        const bool live = tk >= some_lo && tk < some_hi;
+        const global_bytes zero = as_global(kZeroRow);
+        k = live ? k : zero, v = live ? v : zero, kp = live ? kp : zero, vp = live ? vp : zero;
+      }
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
+        constexpr int kStep = 4 * ELEMS * kBytes;
         if constexpr (kWide) {
-          kr[u][i] = load16(k + at(i) * kBytes);
-          vr[u][i] = load16(v + at(i) * kBytes);
+          kr[u][i] = load16(k + i * kStep);
+          vr[u][i] = load16(v + i * kStep);
         } else {
-          const u32x2 kc = *(const u32x2*)(k + at(i)), vc = *(const u32x2*)(v + at(i));
+          const u32x2 kc = load8(k + i * kStep), vc = load8(v + i * kStep);
           kr[u][i] = u32x4{kc[0], kc[1], 0u, 0u};
           vr[u][i] = u32x4{vc[0], vc[1], 0u, 0u};
         }
       }
-      if constexpr (kFp8) {
-        const float* kp = a.k_scales + row_in_cache(a, ids[u], a.ks_page, head, tk, 1);
-        const float* vp = a.v_scales + row_in_cache(a, ids[u], a.vs_page, head, tk, 1);
-        ks[u] = *(live ? kp : (const float*)kZeroRow);
-        vs[u] = *(live ? vp : (const float*)kZeroRow);
-      }
+      if constexpr (kFp8) ks[u] = load_float(kp), vs[u] = load_float(vp);
     }
   };
 
@@ -495,34 +546,50 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
   const bool loads = load_chunk < CHUNKS;
   u32x4 kr[LOADS], vr[LOADS];
   float ks = 0.f, vs = 0.f;
-  int ids[LOADS], scale_id = 0;
+  // Pages of STEP tokens and more: each load's tokens lie in one, whose id is a scalar (as above).
+  constexpr int kBytes = kFp8 ? 1 : 2;
+  const bool paged = (1 << a.page_shift) >= STEP;
+  const int chunk = loads ? load_chunk : 0;
+  const uint32_t lane_at = load_token * (D * kBytes) + chunk * 16;
+  uint32_t ids[LOADS];
   auto clamped = [&](int t) { return min(max(t, some_lo), max(some_hi - 1, 0)); };
   auto load_ids = [&](int t) {
+    if (paged)
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) ids[i] = page_of(a, w.s, clamped(t + load_token + i * STEP));
-    if constexpr (kFp8) scale_id = page_of(a, w.s, clamped(t + lane));
+      for (int i = 0; i < LOADS; ++i) ids[i] = uniform_entry(a, w.s, clamped(t + i * STEP));
   };
   auto load_rows = [&](int t) {
-    constexpr int kBytes = kFp8 ? 1 : 2;
+    const bool whole = t >= some_lo && t + 64 <= some_hi;
+    const global_bytes zero = as_global(kZeroRow);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int tk = t + load_token + i * STEP;
-      const bool live = tk >= some_lo && tk < some_hi;
-      const char* k = (const char*)a.k_cache + row_in_cache(a, ids[i], a.k_page, head, tk, D) * kBytes;
-      const char* v = (const char*)a.v_cache + row_in_cache(a, ids[i], a.v_page, head, tk, D) * kBytes;
-      k = live ? k : (const char*)kZeroRow;
-      v = live ? v : (const char*)kZeroRow;
-      const int chunk = loads ? load_chunk : 0;
-      kr[i] = load16(k + chunk * 16);
-      vr[i] = load16(v + chunk * 16);
+      const int first_token = t + i * STEP, tk = first_token + load_token;
+      global_bytes k, v;
+      if (paged) {
+        const uint32_t page = page_named(a, ids[i]);
+        k = cached_rows<D * kBytes>(a, a.k_cache, page, a.k_step, head, first_token) + lane_at;
+        v = cached_rows<D * kBytes>(a, a.v_cache, page, a.v_step, head, first_token) + lane_at;
+      } else {
+        const uint32_t page = page_named(a, table_entry(a, w.s, clamped(tk)));
+        k = cached_rows<D * kBytes>(a, a.k_cache, page, a.k_step, head, tk) + chunk * 16;
+        v = cached_rows<D * kBytes>(a, a.v_cache, page, a.v_step, head, tk) + chunk * 16;
+      }
+      if (!whole) {
+        const bool live = tk >= some_lo && tk < some_hi;
+        k = live ? k : zero, v = live ? v : zero;
+      }
+      kr[i] = load16(k);
+      vr[i] = load16(v);
     }
     if constexpr (kFp8) {
-      const int tk = t + lane;
-      const bool live = tk >= some_lo && tk < some_hi;
-      const float* kp = a.k_scales + row_in_cache(a, scale_id, a.ks_page, head, tk, 1);
-      const float* vp = a.v_scales + row_in_cache(a, scale_id, a.vs_page, head, tk, 1);
-      ks = *(live ? kp : (const float*)kZeroRow);
-      vs = *(live ? vp : (const float*)kZeroRow);
+      if (wave == 0) {
+        const int tk = t + lane;
+        const bool live = tk >= some_lo && tk < some_hi;
+        const uint32_t page = page_named(a, table_entry(a, w.s, clamped(tk)));
+        const global_bytes kp = cached_scales(a, a.k_scales, page, a.ks_step, head, tk);
+        const global_bytes vp = cached_scales(a, a.v_scales, page, a.vs_step, head, tk);
+        ks = load_float(live ? kp : zero), vs = load_float(live ? vp : zero);
+      }
     }
   };
   // whether rows of this tile see different ones of the tokens t ..
@@ -532,7 +599,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
     bool found = false;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int tk = load_token + i * STEP, swz = swizzle(tk);
+      const int tk = load_token + i * STEP, swz = swizzle<RB, true>(tk);
       if (loads) {
         char* k = lds[buffer][0] + tk * RB;
         char* v = lds[buffer][1] + tk * RB;
@@ -560,9 +627,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
     }
   };
 
-  const int k_at = col * RB + ((h ^ swizzle(col)) << 4);
+  const int k_at = col * RB + ((h ^ swizzle<RB, true>(col)) << 4);
   const int i16 = lane & 15, read_row = h * 4 + (i16 >> 2);
-  const int v_at = read_row * RB + ((((lane >> 4 & 1) * 2 + (i16 >> 1 & 1)) ^ swizzle(read_row)) << 4) + (i16 & 1) * 8;
+  const int v_at = read_row * RB + ((((lane >> 4 & 1) * 2 + (i16 >> 1 & 1)) ^ swizzle<RB, true>(read_row)) << 4) + (i16 & 1) * 8;
 
   if (threadIdx.x == 0) left_out = 0;
   __syncthreads();
@@ -664,8 +731,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
         }
       }
       auto value = [&](int d, int m) {
-        const char* from = values + (v_at ^ (d * 64)) + m * 16 * RB;
-        const u32x2 lo = read_transposed(from), hi = read_transposed(from + 8 * RB);
+        // tokens 8 further: their swizzle differs in one bit
+        const u32x2 lo = read_transposed(values + (v_at ^ (d * 64)) + m * 16 * RB);
+        const u32x2 hi = read_transposed(values + (v_at ^ (d * 64) ^ 32) + (m * 16 + 8) * RB);
         return u32x4{lo[0], lo[1], hi[0], hi[1]};
       };
 #pragma unroll
