@@ -17,7 +17,7 @@
 //
 // A weight of zero does not keep an infinity or NaN out of a product. Tokens that no row of a tile sees
 // are read from a row of zeros; where rows of a tile see different tokens (the last of a chunk, the
-// first of a window), values that are not finite go into the product as zeros, and once the loop is
+// first of a window), values (and scales) that are not finite go into the product as zeros, and once the loop is
 // over they are added to the rows that see them (which has them infinite or NaN).
 #pragma once
 
@@ -71,6 +71,9 @@ INTENT_DEVICE f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
   else return __builtin_amdgcn_mfma_f32_32x32x16_f16(bit_cast<f16x8>(a), bit_cast<f16x8>(b), c, 0, 0, 0);
 }
 
+// Keeps the compiler from turning a rarely taken uniform branch into selects on the common path.
+INTENT_DEVICE void rarely() { asm volatile(""); }
+
 template <bool kBf16>
 INTENT_DEVICE uint32_t pack2(float lo, float hi) {
   if constexpr (kBf16) return bf16x2_rne(lo, hi);
@@ -95,17 +98,20 @@ INTENT_DEVICE u32x4 widen_codes(uint32_t lo, uint32_t hi) {
   return r;
 }
 
-// Eight 16-bit floats with zeros for infinities and NaN, which are noted in `found`. (All exponent bits
-// set: one more in the exponent's last place carries into the sign's place, which the mask has cleared.)
-template <bool kBf16>
+// 16 bytes of cached values with zeros for infinities and NaN, which are noted in `found`. (All exponent
+// bits of a 16-bit float set: one more in the exponent's last place carries into the sign's place, which
+// the mask has cleared. E4M3FN: all bits but the sign's, and there are no infinities.)
+template <bool kBf16, bool kFp8>
 INTENT_DEVICE u32x4 only_finite(u32x4 v, bool& found) {
-  constexpr uint32_t kExponent = kBf16 ? 0x7f807f80u : 0x7c007c00u, kStep = kBf16 ? 0x00800080u : 0x04000400u;
+  constexpr uint32_t kExponent = kFp8 ? 0x7f7f7f7fu : kBf16 ? 0x7f807f80u : 0x7c007c00u;
+  constexpr uint32_t kStep = kFp8 ? 0x01010101u : kBf16 ? 0x00800080u : 0x04000400u;
+  constexpr uint32_t kSigns = kFp8 ? 0x80808080u : 0x80008000u;
   uint32_t any = 0;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const uint32_t out = ((v[e] & kExponent) + kStep) & 0x80008000u;
+    const uint32_t out = ((v[e] & kExponent) + kStep) & kSigns;
     any |= out;
-    v[e] &= ~((out >> 15) * 0xffffu);
+    v[e] &= ~((out >> (kFp8 ? 7 : 15)) * (kFp8 ? 0xffu : 0xffffu));
   }
   found = found || any != 0;
   return v;
@@ -260,47 +266,46 @@ __global__ __launch_bounds__(256, D <= 128 && MT <= 2 ? 2 : 1) void attn_rows_ke
 #pragma unroll
       for (int u = 0; u < 2; ++u) ids[u] = uniform_entry(a, w.s, clamped(t + 16 * u));
   };
-  auto load_rows = [&](int t) {
-    const bool whole = t >= some_lo && t + 32 <= some_hi;
+  auto issue = [&](int u, global_bytes k, global_bytes v, global_bytes kp, global_bytes vp) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int t16 = t + 16 * u, tk = t16 + col;
-      global_bytes k, v, kp{}, vp{};
-      if (paged) {
-        const uint32_t page = page_named(a, ids[u]);
-        k = cached_rows<D * kBytes>(a, a.k_cache, page, a.k_step, head, t16) + lane_at;
-        v = cached_rows<D * kBytes>(a, a.v_cache, page, a.v_step, head, t16) + lane_at;
-        if constexpr (kFp8) {
-          kp = cached_scales(a, a.k_scales, page, a.ks_step, head, t16) + col * 4;
-          vp = cached_scales(a, a.v_scales, page, a.vs_step, head, t16) + col * 4;
-        }
+    for (int i = 0; i < LOADS; ++i) {
+      constexpr int kStep = 4 * ELEMS * kBytes;
+      if constexpr (kWide) {
+        kr[u][i] = load16(k + i * kStep);
+        vr[u][i] = load16(v + i * kStep);
       } else {
-        const uint32_t page = page_named(a, table_entry(a, w.s, clamped(tk)));
-        k = cached_rows<D * kBytes>(a, a.k_cache, page, a.k_step, head, tk) + g * ELEMS * kBytes;
-        v = cached_rows<D * kBytes>(a, a.v_cache, page, a.v_step, head, tk) + g * ELEMS * kBytes;
-        if constexpr (kFp8) {
-          kp = cached_scales(a, a.k_scales, page, a.ks_step, head, tk);
-          vp = cached_scales(a, a.v_scales, page, a.vs_step, head, tk);
-        }
+        const u32x2 kc = load8(k + i * kStep), vc = load8(v + i * kStep);
+        kr[u][i] = u32x4{kc[0], kc[1], 0u, 0u};
+        vr[u][i] = u32x4{vc[0], vc[1], 0u, 0u};
       }
-      if (!whole) {
-        const bool live = tk >= some_lo && tk < some_hi;
-        const global_bytes zero = as_global(kZeroRow);
-        k = live ? k : zero, v = live ? v : zero, kp = live ? kp : zero, vp = live ? vp : zero;
-      }
+    }
+    if constexpr (kFp8) ks[u] = load_float(kp), vs[u] = load_float(vp);
+  };
+  auto load_rows = [&](int t) {
+    const global_bytes zero = as_global(kZeroRow);
+    if (paged && t >= some_lo && t + 32 <= some_hi) {
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        constexpr int kStep = 4 * ELEMS * kBytes;
-        if constexpr (kWide) {
-          kr[u][i] = load16(k + i * kStep);
-          vr[u][i] = load16(v + i * kStep);
-        } else {
-          const u32x2 kc = load8(k + i * kStep), vc = load8(v + i * kStep);
-          kr[u][i] = u32x4{kc[0], kc[1], 0u, 0u};
-          vr[u][i] = u32x4{vc[0], vc[1], 0u, 0u};
-        }
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t page = page_named(a, ids[u]);
+        const int t16 = t + 16 * u;
+        issue(u, cached_rows<D * kBytes>(a, a.k_cache, page, a.k_step, head, t16) + lane_at,
+              cached_rows<D * kBytes>(a, a.v_cache, page, a.v_step, head, t16) + lane_at,
+              cached_scales(a, a.k_scales, page, a.ks_step, head, t16) + col * 4,
+              cached_scales(a, a.v_scales, page, a.vs_step, head, t16) + col * 4);
       }
-      if constexpr (kFp8) ks[u] = load_float(kp), vs[u] = load_float(vp);
+    } else {
+      rarely();
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int tk = t + 16 * u + col;
+        const bool live = tk >= some_lo && tk < some_hi;
+        const uint32_t page = page_named(a, paged ? ids[u] : table_entry(a, w.s, clamped(tk)));
+        const global_bytes k = cached_rows<D * kBytes>(a, a.k_cache, page, a.k_step, head, tk) + g * ELEMS * kBytes;
+        const global_bytes v = cached_rows<D * kBytes>(a, a.v_cache, page, a.v_step, head, tk) + g * ELEMS * kBytes;
+        const global_bytes kp = cached_scales(a, a.k_scales, page, a.ks_step, head, tk);
+        const global_bytes vp = cached_scales(a, a.v_scales, page, a.vs_step, head, tk);
+        issue(u, live ? k : zero, live ? v : zero, live ? kp : zero, live ? vp : zero);
+      }
     }
   };
 
@@ -316,21 +321,32 @@ __global__ __launch_bounds__(256, D <= 128 && MT <= 2 ? 2 : 1) void attn_rows_ke
   for (; t < w.end; t += 128) {
     // values and scales of these tokens to LDS, the scores' operands from the registers
     const bool masked = t < all_lo || t + 32 > all_hi;
-    const bool check = apart(t);
+    if (apart(t)) {
+      rarely();
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) vr[u][i] = only_finite<kBf16, kFp8>(vr[u][i], found);
+      if constexpr (kFp8) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const bool good = fabsf(vs[u]) < INFINITY;
+          found = found || !good;
+          vs[u] = good ? vs[u] : 0.f;
+        }
+      }
+    }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         char* row = mine + u * 16 * RB + write_at;
         const int chunk = at(i) / 8;
-        u32x4 part = vr[u][i];
-        if constexpr (kFp8) part = widen_codes<kBf16>(vr[u][i][0], vr[u][i][1]);
-        if (check) part = only_finite<kBf16>(part, found);
-        *(u32x4*)(row + ((chunk ^ swz) << 4)) = part;
-        if constexpr (kFp8 && kWide) {
-          part = widen_codes<kBf16>(vr[u][i][2], vr[u][i][3]);
-          if (check) part = only_finite<kBf16>(part, found);
-          *(u32x4*)(row + (((chunk + 1) ^ swz) << 4)) = part;
+        if constexpr (kFp8) {
+          *(u32x4*)(row + ((chunk ^ swz) << 4)) = widen_codes<kBf16>(vr[u][i][0], vr[u][i][1]);
+          if constexpr (kWide) *(u32x4*)(row + (((chunk + 1) ^ swz) << 4)) = widen_codes<kBf16>(vr[u][i][2], vr[u][i][3]);
+        } else {
+          *(u32x4*)(row + ((chunk ^ swz) << 4)) = vr[u][i];
         }
       }
       if constexpr (kFp8) {
@@ -381,22 +397,21 @@ __global__ __launch_bounds__(256, D <= 128 && MT <= 2 ? 2 : 1) void attn_rows_ke
       // the highest score, times the value's scale; s is a score or, with an 8-bit cache, its t
       float high = -INFINITY;
       if (masked) {
+        rarely();
+        const int lo = view[m].lo - now - g * 4, hi = view[m].hi - now - g * 4;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int tk = now + 16 * u + g * 4 + r;
-            const bool seen = tk >= view[m].lo && tk < view[m].hi;
+            const bool seen = 16 * u + r >= lo && 16 * u + r < hi;
             s[m][u][r] = seen ? s[m][u][r] : -INFINITY;
-            high = fmaxf(high, kFp8 && seen ? s[m][u][r] + v_exp[u][r] : s[m][u][r]);
           }
         }
-      } else {
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) high = fmaxf(high, kFp8 ? s[m][u][r] + v_exp[u][r] : s[m][u][r]);
       }
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) high = fmaxf(high, kFp8 ? s[m][u][r] + v_exp[u][r] : s[m][u][r]);
       high = max_across32(max_across16(high));
       if constexpr (!kFp8) high *= scale;
       if (__any(high > ref[m] + kRise)) {
@@ -418,7 +433,6 @@ __global__ __launch_bounds__(256, D <= 128 && MT <= 2 ? 2 : 1) void attn_rows_ke
           wt[u][r] = e;
           if constexpr (kFp8) {
             wt[u][r] = e * v_mul[u][r];
-            if (masked) wt[u][r] = s[m][u][r] == -INFINITY ? 0.f : wt[u][r];  // a scale that is not seen may be NaN
           }
         }
       }
@@ -443,12 +457,13 @@ __global__ __launch_bounds__(256, D <= 128 && MT <= 2 ? 2 : 1) void attn_rows_ke
     for (t = w.begin + wave * 32; t < w.end; t += 128) {
       for (int tk = max(t, some_lo); apart(t) && tk < min(t + 32, some_hi); ++tk) {
         const int page = page_of(a, w.s, tk);
-        const char* row = (const char*)a.v_cache + row_in_cache(a, page, a.v_page, head, tk, D) * (kFp8 ? 1 : 2);
+        const char* row = (const char*)a.v_cache + row_in_cache(a, page, a.v_page, head, tk, D) * kBytes;
+        const float times = kFp8 ? a.v_scales[row_in_cache(a, page, a.vs_page, head, tk, 1)] : 1.f;
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float v = cached_value<kBf16, kFp8>(row, d * 16 + g * 4 + r);
+            const float v = cached_value<kBf16, kFp8>(row, d * 16 + g * 4 + r) * times;
 #pragma unroll
             for (int m = 0; m < MT; ++m)
               if (tk >= view[m].lo && tk < view[m].hi && !(fabsf(v) < INFINITY)) o[m][d][r] += v;
@@ -559,27 +574,27 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
       for (int i = 0; i < LOADS; ++i) ids[i] = uniform_entry(a, w.s, clamped(t + i * STEP));
   };
   auto load_rows = [&](int t) {
-    const bool whole = t >= some_lo && t + 64 <= some_hi;
     const global_bytes zero = as_global(kZeroRow);
+    if (paged && t >= some_lo && t + 64 <= some_hi) {
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int first_token = t + i * STEP, tk = first_token + load_token;
-      global_bytes k, v;
-      if (paged) {
+      for (int i = 0; i < LOADS; ++i) {
         const uint32_t page = page_named(a, ids[i]);
-        k = cached_rows<D * kBytes>(a, a.k_cache, page, a.k_step, head, first_token) + lane_at;
-        v = cached_rows<D * kBytes>(a, a.v_cache, page, a.v_step, head, first_token) + lane_at;
-      } else {
-        const uint32_t page = page_named(a, table_entry(a, w.s, clamped(tk)));
-        k = cached_rows<D * kBytes>(a, a.k_cache, page, a.k_step, head, tk) + chunk * 16;
-        v = cached_rows<D * kBytes>(a, a.v_cache, page, a.v_step, head, tk) + chunk * 16;
+        const int from = t + i * STEP;
+        kr[i] = load16(cached_rows<D * kBytes>(a, a.k_cache, page, a.k_step, head, from) + lane_at);
+        vr[i] = load16(cached_rows<D * kBytes>(a, a.v_cache, page, a.v_step, head, from) + lane_at);
       }
-      if (!whole) {
+    } else {
+      rarely();
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int tk = t + i * STEP + load_token;
         const bool live = tk >= some_lo && tk < some_hi;
-        k = live ? k : zero, v = live ? v : zero;
+        const uint32_t page = page_named(a, paged ? ids[i] : table_entry(a, w.s, clamped(tk)));
+        const global_bytes k = cached_rows<D * kBytes>(a, a.k_cache, page, a.k_step, head, tk) + chunk * 16;
+        const global_bytes v = cached_rows<D * kBytes>(a, a.v_cache, page, a.v_step, head, tk) + chunk * 16;
+        kr[i] = load16(live ? k : zero);
+        vr[i] = load16(live ? v : zero);
       }
-      kr[i] = load16(k);
-      vr[i] = load16(v);
     }
     if constexpr (kFp8) {
       if (wave == 0) {
@@ -595,8 +610,18 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
   // whether rows of this tile see different ones of the tokens t ..
   auto apart = [&](int t) { return (some_lo != all_lo || some_hi != all_hi) && (t < all_lo || t + 64 > all_hi); };
   auto store_rows = [&](int buffer, int t) {
-    const bool check = apart(t);
-    bool found = false;
+    if (apart(t)) {
+      rarely();
+      bool found = false;
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) vr[i] = only_finite<kBf16, kFp8>(vr[i], found);
+      if constexpr (kFp8) {
+        const bool good = fabsf(vs) < INFINITY;
+        found = found || !good;
+        vs = good ? vs : 0.f;
+      }
+      if (found) left_out = 1;
+    }
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int tk = load_token + i * STEP, swz = swizzle<RB, true>(tk);
@@ -607,17 +632,14 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
           const int c = load_chunk * 2;
           *(u32x4*)(k + ((c ^ swz) << 4)) = widen_codes<kBf16>(kr[i][0], kr[i][1]);
           *(u32x4*)(k + (((c + 1) ^ swz) << 4)) = widen_codes<kBf16>(kr[i][2], kr[i][3]);
-          u32x4 lo = widen_codes<kBf16>(vr[i][0], vr[i][1]), hi = widen_codes<kBf16>(vr[i][2], vr[i][3]);
-          if (check) lo = only_finite<kBf16>(lo, found), hi = only_finite<kBf16>(hi, found);
-          *(u32x4*)(v + ((c ^ swz) << 4)) = lo;
-          *(u32x4*)(v + (((c + 1) ^ swz) << 4)) = hi;
+          *(u32x4*)(v + ((c ^ swz) << 4)) = widen_codes<kBf16>(vr[i][0], vr[i][1]);
+          *(u32x4*)(v + (((c + 1) ^ swz) << 4)) = widen_codes<kBf16>(vr[i][2], vr[i][3]);
         } else {
           *(u32x4*)(k + ((load_chunk ^ swz) << 4)) = kr[i];
-          *(u32x4*)(v + ((load_chunk ^ swz) << 4)) = check ? only_finite<kBf16>(vr[i], found) : vr[i];
+          *(u32x4*)(v + ((load_chunk ^ swz) << 4)) = vr[i];
         }
       }
     }
-    if (found) left_out = 1;
     if constexpr (kFp8) {
       if (wave == 0) {
         scales[buffer][0][lane] = ks * scale;
@@ -672,12 +694,14 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
           }
       }
       if (masked) {
+        rarely();
+        const int lo = view.lo - t - h * 4, hi = view.hi - t - h * 4;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const int tk = t + u * 32 + (r >> 2) * 8 + h * 4 + (r & 3);
-            s[u][r] = tk >= view.lo && tk < view.hi ? s[u][r] : -INFINITY;
+            const int tk = u * 32 + (r >> 2) * 8 + (r & 3);
+            s[u][r] = tk >= lo && tk < hi ? s[u][r] : -INFINITY;
           }
       }
 #pragma unroll
@@ -687,11 +711,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
           f32x4 v_exp;
           if constexpr (kFp8) v_exp = *(const f32x4*)&scales[buffer][2][u * 32 + i * 8 + h * 4];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float y = s[u][i * 4 + r];
-            if constexpr (kFp8) y = masked ? (y == -INFINITY ? y : y + v_exp[r]) : y + v_exp[r];
-            high = fmaxf(high, y);
-          }
+          for (int r = 0; r < 4; ++r) high = fmaxf(high, kFp8 ? s[u][i * 4 + r] + v_exp[r] : s[u][i * 4 + r]);
         }
       if constexpr (!kFp8) high *= scale;
       high = max_across32(high);
@@ -721,10 +741,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
             const float e = __builtin_amdgcn_exp2f(kFp8 ? x - base : __builtin_fmaf(x, scale, -base));
             total += e;
             wt[r] = e;
-            if constexpr (kFp8) {
-              wt[r] = e * v_mul[r];
-              if (masked) wt[r] = x == -INFINITY ? 0.f : wt[r];  // a scale that is not seen may be NaN
-            }
+            if constexpr (kFp8) wt[r] = e * v_mul[r];
           }
           p[u * 2 + i / 2][(i & 1) * 2] = pack2<kBf16>(wt[0], wt[1]);
           p[u * 2 + i / 2][(i & 1) * 2 + 1] = pack2<kBf16>(wt[2], wt[3]);
@@ -749,13 +766,14 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
     for (int t = w.begin; t < w.end; t += 64) {
       for (int tk = max(t, some_lo); apart(t) && tk < min(t + 64, some_hi); ++tk) {
         const int page = page_of(a, w.s, tk);
-        const char* row = (const char*)a.v_cache + row_in_cache(a, page, a.v_page, head, tk, D) * (kFp8 ? 1 : 2);
+        const char* row = (const char*)a.v_cache + row_in_cache(a, page, a.v_page, head, tk, D) * kBytes;
+        const float times = kFp8 ? a.v_scales[row_in_cache(a, page, a.vs_page, head, tk, 1)] : 1.f;
         const bool seen = tk >= view.lo && tk < view.hi;
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const float v = cached_value<kBf16, kFp8>(row, d * 32 + (r >> 2) * 8 + h * 4 + (r & 3));
+            const float v = cached_value<kBf16, kFp8>(row, d * 32 + (r >> 2) * 8 + h * 4 + (r & 3)) * times;
             if (seen && !(fabsf(v) < INFINITY)) o[d][r] += v;
           }
         }
