@@ -753,6 +753,17 @@ int intent_paged_attention(const void* q, int64_t T, int64_t HQ, int64_t q_ld,
 size_t intent_paged_attention_workspace_size(int64_t T, int64_t HQ, int64_t HK, int64_t D, int64_t S,
                                              int64_t table_width, int64_t page_size);
 
+/*
+ * Repeats a call that the caller keeps as slots: one int64 for each argument
+ * before the stream, in the entry's order (pointers and integers as they are, a
+ * float by its bits in the low half). The entry checks them as in any call; the
+ * only saving is the caller's own cost of handing over some 30 arguments.
+ */
+#define INTENT_RECORD_QK_NORM_ROPE 0
+#define INTENT_RECORD_PAGED_KV_APPEND 1
+#define INTENT_RECORD_PAGED_ATTENTION 2
+int intent_amd_replay(int record, const int64_t* slots, int64_t count, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

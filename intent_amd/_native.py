@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -94,6 +95,7 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "intent_paged_attention": ([P, I64, I64, I64, INT, INT, P, I64, P, I64, P, I64, P, I64, I64, I64, I64, I64, P, I64,
                                 I64, I64, P, P, F32, INT, I64, P, I64, P, SIZE, P], INT),
     "intent_paged_attention_workspace_size": ([I64, I64, I64, I64, I64, I64, I64], SIZE),
+    "intent_amd_replay": ([INT, P, I64, P], INT),
     "intent_hbm_read_probe": ([P, I64, INT, INT, P, I64, P], INT),
     "intent_mfma_peak_probe": ([INT, I64, I64, P, P], INT),
 }
@@ -145,6 +147,30 @@ def call(entry: str, *arguments) -> None:
     status = getattr(library(), entry)(*arguments)
     if status != INTENT_OK:
         raise status_error(status, entry, last_error())
+
+
+RECORDS = {"intent_qk_norm_rope": 0, "intent_paged_kv_append": 1, "intent_paged_attention": 2}
+
+
+class Record:
+    """A call of an entry kept as slots (intent_amd_replay): repeated for a stream without its arguments
+    being converted again."""
+
+    def __init__(self, entry: str, arguments: tuple):
+        types = SIGNATURES[entry][0][:-1]
+        if len(arguments) != len(types):
+            raise TypeError(f"{entry} takes {len(types)} arguments before the stream, got {len(arguments)}")
+        self.entry = entry
+        self._number = RECORDS[entry]
+        self._count = len(types)
+        self._slots = (I64 * len(types))(*(
+            int.from_bytes(struct.pack("<f", a), "little") if t is F32 else a or 0 for t, a in zip(types, arguments)))
+        self._replay = library().intent_amd_replay
+
+    def __call__(self, stream: int) -> None:
+        status = self._replay(self._number, self._slots, self._count, stream)
+        if status != INTENT_OK:
+            raise status_error(status, self.entry, last_error())
 
 
 def device_arch(device: int) -> str:

@@ -223,7 +223,7 @@ int launch_tiled(AttnArgs a, bool bf16, bool fp8, float* workspace, size_t bytes
     l.a = a;
     l.items = (int)(tiles + a.target);
     l.joins = (int)joins;
-    // rows of a split tile side by side: at most those of a mean sequence, and 2048 workgroups in all
+    // workgroups for the rows of a split tile: one for each of a mean sequence, up to 2048 in all
     const int64_t mean = ((int64_t)a.T * a.group + a.S - 1) / a.S, room = joins > 0 ? 2048 / (joins * a.HK) : 0;
     const int64_t side = mean < p.rows() ? mean : p.rows();
     l.join_rows = (int)(room < 1 ? 1 : room < side ? room : side);

@@ -806,52 +806,78 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
 
 // ---- the join of split tiles ---------------------------------------------------------------------
 
-// One workgroup for each row of a split tile (rows in turn where there are more): the waves take every
-// fourth split, in order, and are added in order.
+// out = sum_j w_j O_j / sum_j w_j l_j, w_j = exp2(M_j - max M), over the parts of a tile in a fixed order.
+// A lane holds D / 64 columns of a row (two of 96). Up to 16 parts a wave takes a row by itself; more are
+// dealt to the four waves of a workgroup, whose sums are added in order. Each wave works out the weights
+// of 64 parts at a time, one in each lane, while its first parts are on their way.
 template <bool kBf16, int D, int ROWS, int UNIT>
 __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
-  constexpr int E = (D + 63) / 64;  // columns of a lane
-  __shared__ float sums[4][64 * E];
-  __shared__ float all4[4];
+  constexpr int E = (D + 63) / 64, AHEAD = 8;
+  typedef float part __attribute__((ext_vector_type(E)));
+  __shared__ part sums[4][64];
   const int head = blockIdx.x % a.HK;
   Span w;
   if (!find_span<ROWS, UNIT>(a, blockIdx.x / a.HK, true, w)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  for (int r = blockIdx.y; r < w.rows; r += gridDim.y) {
+  const bool mine = lane * E < D;
+  const int d0 = mine ? lane * E : 0;
+  const bool alone = w.splits <= 16;
+  const int ways = alone ? 1 : 4, way = alone ? 0 : wave;  // waves of a row, and this one's place
+  for (int r = alone ? blockIdx.y * 4 + wave : blockIdx.y; r < w.rows; r += alone ? gridDim.y * 4 : gridDim.y) {
     auto at = [&](int j) { return ((int64_t)(w.slot + j) * a.HK + head) * ROWS + r; };
-    float high = -INFINITY;
-    for (int j = lane; j < w.splits; j += 64) high = fmaxf(high, a.partial_stats[at(j) * 2]);
+    auto load = [&](int j) { return *(const part*)(a.partial + at(min(j, w.splits - 1)) * D + d0); };
+    part ahead[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) ahead[i] = load(way + i * ways);
+    f32x2 st = f32x2{-INFINITY, 0.f};
+    if (lane < w.splits) st = *(const f32x2*)(a.partial_stats + at(lane) * 2);
+    float high = st[0];
+    for (int j = lane + 64; j < w.splits; j += 64) high = fmaxf(high, a.partial_stats[at(j) * 2]);
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) high = fmaxf(high, __shfl_xor(high, off));
     const float base = high == -INFINITY ? 0.f : high;
-    float acc[E], all = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
-#pragma unroll 4
-    for (int j = wave; j < w.splits; j += 4) {
-      const f32x2 st = *(const f32x2*)(a.partial_stats + at(j) * 2);
-      const float keep = __builtin_amdgcn_exp2f(st[0] - base);
-      all += keep * st[1];
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int d = min(lane + 64 * e, D - 1);
-        acc[e] = __builtin_fmaf(keep, a.partial[at(j) * D + d], acc[e]);
+    part acc{};
+    float total = 0.f;
+    for (int j0 = 0; j0 < w.splits; j0 += 64) {
+      if (j0 > 0) {
+        st = f32x2{-INFINITY, 0.f};
+        if (j0 + lane < w.splits) st = *(const f32x2*)(a.partial_stats + at(j0 + lane) * 2);
       }
-    }
-    __syncthreads();
+      const float keep = __builtin_amdgcn_exp2f(st[0] - base);
+      float all = keep * st[1];
 #pragma unroll
-    for (int e = 0; e < E; ++e) sums[wave][lane + 64 * e] = acc[e];
-    if (lane == 0) all4[wave] = all;
-    __syncthreads();
-    const float total = all4[0] + all4[1] + all4[2] + all4[3];
+      for (int off = 32; off >= 1; off >>= 1) all += __shfl_xor(all, off);
+      total += all;
+      const int n = min(w.splits - j0, 64);
+      auto add = [&](part v, int i) {
+        const float k = bit_cast<float>(__builtin_amdgcn_readlane(bit_cast<int>(keep), i));
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = __builtin_fmaf(k, v[e], acc[e]);
+      };
+      int i = way;
+      if (j0 == 0) {
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+          if (way + k * ways < n) add(ahead[k], way + k * ways);
+        i += AHEAD * ways;
+      }
+#pragma unroll 4
+      for (; i < n; i += ways) add(load(j0 + i), i);
+    }
+    if (!alone) {
+      __syncthreads();
+      sums[wave][lane] = acc;
+      __syncthreads();
+      if (wave != 0) continue;
+      acc = sums[0][lane] + sums[1][lane] + sums[2][lane] + sums[3][lane];
+    }
     const RowView rv = row_view(a, w, r);
     const float inv = rv.hi > rv.lo ? 1.0f / total : 0.f;
-    uint16_t* to = out_row(a, w, head, r);
-    for (int d = threadIdx.x * 2; d < D; d += 512) {
-      const float x = sums[0][d] + sums[1][d] + sums[2][d] + sums[3][d];
-      const float y = sums[0][d + 1] + sums[1][d + 1] + sums[2][d + 1] + sums[3][d + 1];
-      *(uint32_t*)(to + d) = pack2<kBf16>(x * inv, y * inv);
-    }
+    uint16_t* to = out_row(a, w, head, r) + d0;
+    if (!mine) continue;
+    if constexpr (E == 1) *to = (uint16_t)(pack2<kBf16>(acc[0] * inv, 0.f) & 0xffffu);
+    else if constexpr (E == 2) *(uint32_t*)to = pack2<kBf16>(acc[0] * inv, acc[1] * inv);
+    else *(u32x2*)to = u32x2{pack2<kBf16>(acc[0] * inv, acc[1] * inv), pack2<kBf16>(acc[2] * inv, acc[3] * inv)};
   }
 }
 

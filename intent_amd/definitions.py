@@ -54,6 +54,9 @@ class KernelDefinition:
     # launch calls, from its extents and whether it has scratch.
     entries: tuple = ()
     entry: Callable[[dict, bool], str] | None = None
+    # (entry, its arguments before the stream) of a launch, where it is one call of one entry: a
+    # prepared call then keeps them converted.
+    call: Callable[[dict, dict, Any], tuple] | None = None
 
     @property
     def __name__(self) -> str:  # the reference uses definition.__name__ as the entry name
@@ -1316,6 +1319,15 @@ def _prefix(dt: str) -> str:
     return "" if dt == "f16" else dt + "_"
 
 
+def _one_call(call: Callable[[dict, dict, Any], tuple]) -> dict:
+    """The launch of a definition that is one call of one entry."""
+    def launch(v: dict, env: dict, stream: int, scratch) -> str:
+        entry, arguments = call(v, env, scratch)
+        _native.call(entry, *arguments, stream)
+        return entry
+    return {"launch": launch, "call": call}
+
+
 def _heads_check(env: dict) -> None:
     for name, extent in (("q_weight", env["WQ"]), ("k_weight", env["WK"])):
         if extent not in (0, env["D"]):
@@ -1343,12 +1355,10 @@ _HEADS_CONSTEXPRS = {"EPS": 1e-6, "INTERLEAVED": False}
 
 
 def _norm_rope_definition(dt: str) -> KernelDefinition:
-    def launch(v: dict, env: dict, stream: int, workspace) -> str:
+    def call(v: dict, env: dict, scratch) -> tuple:
         first, rest = _heads_arguments(v, env)
         q_out, k_out = v["q_out"], v["k_out"]
-        _native.call("intent_qk_norm_rope", *first, *rest, int(dt == "bf16"), _ptr(q_out), _ld(q_out), _ptr(k_out),
-                     _ld(k_out), stream)
-        return "intent_qk_norm_rope"
+        return "intent_qk_norm_rope", (*first, *rest, int(dt == "bf16"), _ptr(q_out), _ld(q_out), _ptr(k_out), _ld(k_out))
 
     return KernelDefinition(
         name=_prefix(dt) + "qk_norm_rope",
@@ -1362,7 +1372,7 @@ def _norm_rope_definition(dt: str) -> KernelDefinition:
             Param("q_out", dt, ("T", "HQ", "D"), OUT, leading_stride=True),
             Param("k_out", dt, ("T", "HK", "D"), OUT, leading_stride=True),
         ),
-        launch=launch,
+        **_one_call(call),
         constexprs=dict(_HEADS_CONSTEXPRS),
         check=_heads_check,
         reference="no kernel of the reference's quantized path; the pass between its projections and the attention",
@@ -1405,13 +1415,12 @@ _CACHE_DOC = "E4M3FN codes with a scale per token and head, max(absmax, 1e-12) /
 
 
 def _append_definition(dt: str, fp8: bool) -> KernelDefinition:
-    def launch(v: dict, env: dict, stream: int, workspace) -> str:
+    def call(v: dict, env: dict, scratch) -> tuple:
         first, rest = _heads_arguments(v, env)
         value, q_out = v["v"], v["q_out"]
-        _native.call("intent_paged_kv_append", *first, _ptr(value), _ld(value), *rest, _ptr(v["slots"]),
-                     int(dt == "bf16"), int(fp8), *_cache_arguments(v, fp8), env["PAGES"], env["PAGE"], _ptr(q_out),
-                     _ld(q_out), stream)
-        return "intent_paged_kv_append"
+        return "intent_paged_kv_append", (
+            *first, _ptr(value), _ld(value), *rest, _ptr(v["slots"]), int(dt == "bf16"), int(fp8),
+            *_cache_arguments(v, fp8), env["PAGES"], env["PAGE"], _ptr(q_out), _ld(q_out))
 
     return KernelDefinition(
         name=_prefix(dt) + "paged_kv_append" + ("_fp8" if fp8 else ""),
@@ -1427,7 +1436,7 @@ def _append_definition(dt: str, fp8: bool) -> KernelDefinition:
             *_cache_params(dt, fp8, INOUT),
             Param("q_out", dt, ("T", "HQ", "D"), OUT, leading_stride=True),
         ),
-        launch=launch,
+        **_one_call(call),
         constexprs=dict(_HEADS_CONSTEXPRS),
         check=_append_check,
         reference="examples/kernels/quantization/fp8.py:11-39 (the quantizer's rule, one group for each head)" if fp8 else
@@ -1461,14 +1470,13 @@ def _attention_scratch(env: dict) -> int:
 
 
 def _attention_definition(dt: str, fp8: bool) -> KernelDefinition:
-    def launch(v: dict, env: dict, stream: int, scratch) -> str:
+    def call(v: dict, env: dict, scratch) -> tuple:
         q, out, table = v["q"], v["out"], v["page_table"]
-        _native.call("intent_paged_attention", _ptr(q), env["T"], env["HQ"], _ld(q), int(dt == "bf16"), int(fp8),
-                     *_cache_arguments(v, fp8), env["PAGES"], env["HK"], env["PAGE"], env["D"], _ptr(table), env["S"],
-                     env["MAX_PAGES"], _ld(table), _ptr(v["q_offsets"]), _ptr(v["kv_lens"]), float(env["scale"]),
-                     int(bool(env["CAUSAL"])), int(env["WINDOW"]), _ptr(out), _ld(out),
-                     None if scratch is None else _ptr(scratch), 0 if scratch is None else scratch.numel(), stream)
-        return "intent_paged_attention"
+        return "intent_paged_attention", (
+            _ptr(q), env["T"], env["HQ"], _ld(q), int(dt == "bf16"), int(fp8), *_cache_arguments(v, fp8), env["PAGES"],
+            env["HK"], env["PAGE"], env["D"], _ptr(table), env["S"], env["MAX_PAGES"], _ld(table), _ptr(v["q_offsets"]),
+            _ptr(v["kv_lens"]), float(env["scale"]), int(bool(env["CAUSAL"])), int(env["WINDOW"]), _ptr(out), _ld(out),
+            None if scratch is None else _ptr(scratch), 0 if scratch is None else scratch.numel())
 
     return KernelDefinition(
         name=_prefix(dt) + "paged_attention" + ("_fp8" if fp8 else ""),
@@ -1481,7 +1489,7 @@ def _attention_definition(dt: str, fp8: bool) -> KernelDefinition:
             Param("out", dt, ("T", "HQ", "D"), OUT, leading_stride=True),
             Scalar("scale", "f32"),
         ),
-        launch=launch,
+        **_one_call(call),
         scratch=_attention_scratch,
         constexprs={"CAUSAL": True, "WINDOW": 0},
         check=_attention_check,

@@ -327,6 +327,10 @@ class HIPRuntime:
         entry = self.definition.launch(binding.views, binding.env, _current_stream(self.device), binding.workspace)
         self._latest = (entry, _native.library().intent_amd_last_kernel())
 
+    def _replay(self, record) -> None:
+        record(_current_stream(self.device))
+        self._latest = (record.entry, _native.library().intent_amd_last_kernel())
+
     # ---- provider surface -------------------------------------------------------
     def launch_bound(self, binding: Binding):
         self._launch(binding)
@@ -393,6 +397,8 @@ class HIPPreparedCall:
         self._binding = binding
         # the stream whose order the allocator follows when the scratch is given back
         self._stream = _current_stream(runtime.device) if owns_scratch and binding.workspace is not None else None
+        call = runtime.definition.call
+        self._record = None if call is None else _native.Record(*call(binding.views, binding.env, binding.workspace))
 
     def compile(self) -> None:
         _native.library()  # the code objects are prebuilt; this validates the library and ABI
@@ -402,7 +408,10 @@ class HIPPreparedCall:
             import torch
 
             self._binding.workspace.record_stream(torch.cuda.current_stream(self._runtime.device))
-        self._runtime._launch(self._binding)
+        if self._record is not None:
+            self._runtime._replay(self._record)
+        else:
+            self._runtime._launch(self._binding)
 
     def result(self):
         return _result(self._binding.outputs)

@@ -818,3 +818,20 @@ def test_empty_calls_are_no_ops():
     assert status("intent_paged_attention", *_attention_args(T=0)) == 0
     assert status("intent_paged_attention", *_attention_args(S=0)) == 0
     assert ctypes.sizeof(ctypes.c_void_p) == 8
+
+
+def test_replayed_calls_are_checked():
+    """A call kept as slots goes through its entry's own checks; a wrong record is refused."""
+    with pytest.raises(ValueError, match="multiple of the HK"):
+        _native.Record("intent_paged_attention", tuple(_attention_args(HK=3)[:-1]))(0)
+    _native.Record("intent_paged_attention", tuple(_attention_args(T=0)[:-1]))(0)
+    with pytest.raises(NotImplementedError, match="power of two"):
+        _native.Record("intent_paged_kv_append", tuple(_append_args(page=12)[:-1]))(0)
+    with pytest.raises(ValueError, match="16-byte"):
+        _native.Record("intent_qk_norm_rope", tuple(_norm_args(q=FAKE + 8)[:-1]))(0)
+    with pytest.raises(TypeError, match="takes"):
+        _native.Record("intent_qk_norm_rope", tuple(_norm_args()))
+    slots = (ctypes.c_int64 * 4)()
+    assert status("intent_amd_replay", 0, slots, 4, None) == INVALID and "slots" in _native.last_error()
+    assert status("intent_amd_replay", 9, slots, 4, None) == INVALID
+    assert status("intent_amd_replay", 0, None, 22, None) == INVALID
