@@ -98,66 +98,77 @@ INTENT_DEVICE Extent extent_of(const AttnArgs& a, int s) {
 
 INTENT_DEVICE int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 
+// Sum over the wave, and sum of the lanes up to this one (DPP: shifts in rows of 16, then each row's
+// last value to the rows behind it).
+template <int CTRL, int ROWS>
+INTENT_DEVICE int dpp_add(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+INTENT_DEVICE int wave_prefix(int v) {
+  v = dpp_add<0x111, 0xf>(v);
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  v = dpp_add<0x118, 0xf>(v);
+  v = dpp_add<0x142, 0xa>(v);
+  return dpp_add<0x143, 0xc>(v);
+}
+INTENT_DEVICE float wave_total(float v) {
+  const float in[1] = {v};
+  float out[1];
+  WaveReduce<1>::run(in, out);
+  return out[0];
+}
+
 // Finds share `item` of one head's list: the sequences in order, each with its row tiles from the last
 // (which sees most) to the first, each tile in `splits` parts of its tokens. The parts are sized so
 // that all sequences together give about a.target of them: units / chunk of each, chunk = the units
-// that a workgroup would get of an even share. With `joins`, the list of the tiles that are split.
-// Every wave does it by itself: no plan is kept, so a captured call follows lengths that change.
+// that a workgroup would get of an even share (rounded up, so never less than that: the workspace is
+// sized by it). With `joins`, the list of the tiles that are split. Every wave does it by itself: no
+// plan is kept, so a captured call follows lengths that change. The counts of one list fit 32 bits (the
+// host bounds the grid).
 template <int ROWS, int UNIT>
 INTENT_DEVICE bool find_span(const AttnArgs& a, int item, bool joins, Span& r) {
   const int lane = threadIdx.x & 63;
   const Extent first = extent_of<ROWS, UNIT>(a, lane);
-  int64_t chunk = INT32_MAX;
+  int chunk = INT32_MAX;
   if (a.target > 0) {
-    int64_t all = (int64_t)first.tiles * first.units;
+    float all = (float)first.tiles * (float)first.units;
     for (int s0 = 64; s0 < a.S; s0 += 64) {
       const Extent e = extent_of<ROWS, UNIT>(a, s0 + lane);
-      all += (int64_t)e.tiles * e.units;
+      all += (float)e.tiles * (float)e.units;
     }
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) all += __shfl_xor(all, off);
-    chunk = (all + a.target - 1) / a.target;
-    if (chunk < 1) chunk = 1;
+    chunk = (int)fminf(wave_total(all) * (1.0f + 0x1p-12f) / (float)a.target, 1.0e9f) + 1;
   }
-  int64_t base = 0;  // shares (low half) and slots of split tiles (high half) before sequence s0
+  int base = 0, slots = 0;  // shares, and slots of split tiles, before sequence s0
   for (int s0 = 0; s0 < a.S; s0 += 64) {
     const Extent e = s0 == 0 ? first : extent_of<ROWS, UNIT>(a, s0 + lane);
-    int splits = 1;
-    if (e.units > chunk) {
-      splits = (int)((e.units + chunk - 1) / chunk);
-      if (splits > kMostSplits) splits = kMostSplits;
-    }
-    const int parts = e.tiles * splits;
-    const int64_t mine = (int64_t)(splits > 1 ? parts : 0) << 32 | (uint32_t)(joins ? (splits > 1 ? e.tiles : 0) : parts);
-    int64_t up = mine;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int64_t v = __shfl_up(up, off);
-      if (lane >= off) up += v;
-    }
-    up += base;
-    const uint64_t past = __ballot((int)(uint32_t)up > item);
+    const int splits = e.units > chunk ? min((int)(((uint32_t)e.units + (uint32_t)chunk - 1u) / (uint32_t)chunk), kMostSplits) : 1;
+    const int parts = e.tiles * splits, kept = splits > 1 ? parts : 0;
+    const int mine = joins ? (splits > 1 ? e.tiles : 0) : parts;
+    const int up = wave_prefix(mine) + base, kept_up = wave_prefix(kept) + slots;
+    const uint64_t past = __ballot(up > item);
     if (past) {
       const int at = __builtin_ctzll(past);
-      const int64_t before = up - mine;
       r.s = s0 + at;
       r.q.start = lane_value(e.q.start, at), r.q.count = lane_value(e.q.count, at), r.q.kv = lane_value(e.q.kv, at);
       r.splits = lane_value(splits, at);
       const int tiles = lane_value(e.tiles, at);
-      const int local = item - lane_value((int)(uint32_t)before, at);
-      r.slot = lane_value((int)(before >> 32), at) + (joins ? local * r.splits : local);
-      const int turn = joins ? local : local / r.splits, split = joins ? 0 : local - turn * r.splits;
+      const int local = item - lane_value(up - mine, at);
+      r.slot = lane_value(kept_up - kept, at) + (joins ? local * r.splits : local);
+      const int turn = joins ? local : (int)((uint32_t)local / (uint32_t)r.splits), split = joins ? 0 : local - turn * r.splits;
       r.row0 = (tiles - 1 - turn) * ROWS;
       r.rows = min(ROWS, r.q.count * a.group - r.row0);
-      const int p0 = r.q.kv - r.q.count + r.row0 / a.group;
-      const int p1 = r.q.kv - r.q.count + (r.row0 + r.rows - 1) / a.group;
+      const int p0 = r.q.kv - r.q.count + (int)((uint32_t)r.row0 / (uint32_t)a.group);
+      const int p1 = r.q.kv - r.q.count + (int)((uint32_t)(r.row0 + r.rows - 1) / (uint32_t)a.group);
       const int lo = first_seen(a, p0) & ~63, hi = end_seen(a, p1, r.q.kv);
-      const int64_t units = hi > lo ? (hi - lo + UNIT - 1) / UNIT : 0;
-      r.begin = lo + (int)(units * split / r.splits) * UNIT;
-      r.end = min(hi, lo + (int)(units * (split + 1) / r.splits) * UNIT);
+      const uint32_t units = hi > lo ? (uint32_t)(hi - lo + UNIT - 1) / UNIT : 0u;
+      const uint32_t each = units / (uint32_t)r.splits, more = units - each * (uint32_t)r.splits;
+      const uint32_t from = each * split + min((uint32_t)split, more), to = from + each + ((uint32_t)split < more ? 1u : 0u);
+      r.begin = lo + (int)from * UNIT;
+      r.end = min(hi, lo + (int)to * UNIT);
       return true;
     }
-    base = __shfl(up, 63);
+    base = lane_value(up, 63), slots = lane_value(kept_up, 63);
   }
   return false;
 }

@@ -144,14 +144,20 @@ int launch_rows(const AttnArgs& a, hipStream_t stream) {
 
 // ---- which kernel, and into how many parts --------------------------------------------
 
-// Workgroups that the tiles are split for: two for each of the 256 CUs.
-constexpr int kFill = 512;
-
 struct Part {
   int tiles;  // 16-row tiles of the kernel with the tokens over the waves; 0: 128 rows
   int min_rows, max_rows;
   int rows() const { return tiles > 0 ? 16 * tiles : 128; }
   int unit() const { return tiles > 0 ? 128 : 64; }
+  // Workgroups that the tiles are split for: what the 256 CUs hold at one time (by the kernels' registers),
+  // and twice that where a CU holds three, which evens out sequences of different lengths and costs
+  // little (four sequences of 60000 to 131000 tokens: 300 us at 512, 235 at 768, 239 at 1536; 64 of 300
+  // to 8191 126, 128 and 119 us). One workgroup to a CU loses by a second round (16 sequences of five
+  // drafted tokens: 28 us at 256, 34 at 512).
+  int fill(int64_t D) const {
+    if (tiles == 0) return 512;
+    return D > 128 ? 256 : tiles * D <= 128 ? 1536 : tiles * D <= 256 ? 512 : 256;
+  }
 };
 
 struct Plan {
@@ -171,7 +177,7 @@ Plan plan_of(int64_t T, int64_t S, int64_t group, int64_t D) {
   p.parts = 1;
   const int most = D > 128 ? 16 : 64;
   if (mean <= most) {
-    p.part[0] = {mean <= 16 ? 1 : mean <= 32 ? 2 : 4, 0, INT32_MAX};
+    p.part[0] = {mean > 16 ? (int)((mean + 15) / 16) : 1, 0, INT32_MAX};
   } else if (S == 1) {
     p.part[0] = {0, 0, INT32_MAX};
   } else {
@@ -189,8 +195,8 @@ int64_t tiles_bound(const Part& p, int64_t T, int64_t S, int64_t group) {
 
 // Parts of all split tiles of one head: fewer than twice the target (each of two parts at least has
 // more than half its share), and at most every tile's most.
-int64_t slots_bound(const Part& p, int64_t T, int64_t S, int64_t group, int64_t HK, int64_t most_kv) {
-  const int64_t target = (kFill + HK - 1) / HK;
+int64_t slots_bound(const Part& p, int64_t T, int64_t S, int64_t group, int64_t HK, int64_t D, int64_t most_kv) {
+  const int64_t target = (p.fill(D) + HK - 1) / HK;
   int64_t splits = (most_kv + p.unit() - 1) / p.unit();
   if (splits > kMostSplits) splits = kMostSplits;
   if (splits < 2) return 0;
@@ -199,7 +205,7 @@ int64_t slots_bound(const Part& p, int64_t T, int64_t S, int64_t group, int64_t 
 }
 
 size_t part_bytes(const Part& p, int64_t T, int64_t S, int64_t group, int64_t HK, int64_t D, int64_t most_kv) {
-  return (size_t)(slots_bound(p, T, S, group, HK, most_kv) * HK * p.rows() * (D + 2) * 4);
+  return (size_t)(slots_bound(p, T, S, group, HK, D, most_kv) * HK * p.rows() * (D + 2) * 4);
 }
 
 int launch_tiled(AttnArgs a, bool bf16, bool fp8, float* workspace, size_t bytes, hipStream_t stream) {
@@ -211,9 +217,9 @@ int launch_tiled(AttnArgs a, bool bf16, bool fp8, float* workspace, size_t bytes
     const bool split = need > 0 && workspace != nullptr && bytes >= need;
     AttnLaunch l{};
     a.min_rows = p.min_rows, a.max_rows = p.max_rows;
-    a.target = split ? (kFill + a.HK - 1) / a.HK : 0;
+    a.target = split ? (p.fill(a.D) + a.HK - 1) / a.HK : 0;
     a.partial = workspace;
-    a.partial_stats = split ? workspace + slots_bound(p, a.T, a.S, a.group, a.HK, a.most_kv) * a.HK * p.rows() * a.D : nullptr;
+    a.partial_stats = split ? workspace + slots_bound(p, a.T, a.S, a.group, a.HK, a.D, a.most_kv) * a.HK * p.rows() * a.D : nullptr;
     const int64_t tiles = tiles_bound(p, a.T, a.S, a.group);
     const int64_t joins = split ? (tiles < a.target ? tiles : a.target) : 0;
     // 256-lane workgroups: the grid's work items stay below 2^32

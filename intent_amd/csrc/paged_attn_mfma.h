@@ -160,16 +160,16 @@ struct RowView {
   int lo, hi;
 };
 INTENT_DEVICE RowView row_view(const AttnArgs& a, const Span& w, int r) {
-  const int p = w.q.kv - w.q.count + (w.row0 + min(r, w.rows - 1)) / a.group;
+  const int p = w.q.kv - w.q.count + (int)((uint32_t)(w.row0 + min(r, w.rows - 1)) / (uint32_t)a.group);
   return {first_seen(a, p), end_seen(a, p, w.q.kv)};
 }
 
 INTENT_DEVICE const uint16_t* q_row(const AttnArgs& a, const Span& w, int head, int r) {
-  const int row = w.row0 + min(r, w.rows - 1), token = row / a.group;
+  const int row = w.row0 + min(r, w.rows - 1), token = (int)((uint32_t)row / (uint32_t)a.group);
   return a.q + (int64_t)(w.q.start + token) * a.q_ld + (int64_t)(head * a.group + row - token * a.group) * a.D;
 }
 INTENT_DEVICE uint16_t* out_row(const AttnArgs& a, const Span& w, int head, int r) {
-  const int row = w.row0 + r, token = row / a.group;
+  const int row = w.row0 + r, token = (int)((uint32_t)row / (uint32_t)a.group);
   return a.out + (int64_t)(w.q.start + token) * a.out_ld + (int64_t)(head * a.group + row - token * a.group) * a.D;
 }
 
@@ -203,7 +203,7 @@ INTENT_DEVICE float sum_across32(float v) {
 // the four waves' results are joined. Keys and values of the next 32 tokens are under way during the
 // softmax and the second product, and the page ids of the ones after them.
 template <bool kBf16, bool kFp8, int D, int MT>
-__global__ __launch_bounds__(256, D <= 128 && MT <= 2 ? 2 : 1) void attn_rows_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 256 ? 2 : 1) void attn_rows_kernel(const AttnArgs a) {
   constexpr int KS = D / 32, DT = D / 16, RB = row_bytes<D>();
   constexpr bool kWide = !kFp8 || D % 64 == 0;         // 16 bytes a lane and load, else 8 codes
   constexpr int LOADS = kFp8 && kWide ? D / 64 : KS;   // loads of a token's row
@@ -674,13 +674,14 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
       const char* values = lds[buffer][1];
       f32x16 s[2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
 #pragma unroll
-        for (int i = 0; i < KS; ++i)
+      for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
           s[u] = mfma32<kBf16>(*(const u32x4*)(keys + u * 32 * RB + (k_at ^ (i * 32))), q[i], s[u]);
-      }
       const bool masked = t < bottom.lo || t + 64 > top.hi;
       float high = -INFINITY;
       if constexpr (kFp8) {
@@ -754,9 +755,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
         return u32x4{lo[0], lo[1], hi[0], hi[1]};
       };
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
+      for (int m = 0; m < 4; ++m)
 #pragma unroll
-        for (int m = 0; m < 4; ++m) o[d] = mfma32<kBf16>(value(d, m), p[m], o[d]);
+        for (int d = 0; d < DT; ++d) o[d] = mfma32<kBf16>(value(d, m), p[m], o[d]);
     }
     if (more) store_rows(buffer ^ 1, t + 64);
     __syncthreads();
@@ -904,6 +905,7 @@ int launch_d(const AttnLaunch& l, int tiles, hipStream_t stream) {
   if (tiles == 1) return launch<kBf16, kFp8, D, 1>(l, stream);
   if constexpr (D <= 128) {
     if (tiles == 2) return launch<kBf16, kFp8, D, 2>(l, stream);
+    if (tiles == 3) return launch<kBf16, kFp8, D, 3>(l, stream);
     if (tiles == 4) return launch<kBf16, kFp8, D, 4>(l, stream);
   }
   return launch<kBf16, kFp8, D, 0>(l, stream);
