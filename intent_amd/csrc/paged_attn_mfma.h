@@ -566,50 +566,70 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
   const bool paged = (1 << a.page_shift) >= STEP;
   const int chunk = loads ? load_chunk : 0;
   const uint32_t lane_at = load_token * (D * kBytes) + chunk * 16;
-  uint32_t ids[LOADS];
-  auto clamped = [&](int t) { return min(max(t, some_lo), max(some_hi - 1, 0)); };
-  auto load_ids = [&](int t) {
-    if (paged)
+  typedef uint32_t Ids __attribute__((ext_vector_type(LOADS)));
+  Ids ids{}, next_ids{};  // of the values' and the keys' tokens to load next
+  auto clamped = [&](int t) __attribute__((always_inline)) { return min(max(t, some_lo), max(some_hi - 1, 0)); };
+  const bool one_page = a.page_shift >= 6;  // the 64 tokens in one page
+  auto load_ids = [&](int t) __attribute__((always_inline)) {
+    if (one_page) {
+      next_ids[0] = uniform_entry(a, w.s, clamped(t));
+    } else if (paged) {
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i) ids[i] = uniform_entry(a, w.s, clamped(t + i * STEP));
+      for (int i = 0; i < LOADS; ++i) next_ids[i] = uniform_entry(a, w.s, clamped(t + i * STEP));
+    }
   };
-  auto load_rows = [&](int t) {
-    const global_bytes zero = as_global(kZeroRow);
-    if (paged && t >= some_lo && t + 64 <= some_hi) {
+  auto load = [&](u32x4(&to)[LOADS], Ids id, const void* cache, uint32_t step, int t) __attribute__((always_inline)) {
+    const bool whole = t >= some_lo && t + 64 <= some_hi;
+    if (whole && one_page) {
+      const global_bytes from = cached_rows<D * kBytes>(a, cache, page_named(a, id[0]), step, head, t);
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const uint32_t page = page_named(a, ids[i]);
-        const int from = t + i * STEP;
-        kr[i] = load16(cached_rows<D * kBytes>(a, a.k_cache, page, a.k_step, head, from) + lane_at);
-        vr[i] = load16(cached_rows<D * kBytes>(a, a.v_cache, page, a.v_step, head, from) + lane_at);
-      }
+      for (int i = 0; i < LOADS; ++i) to[i] = load16(from + i * (STEP * D * kBytes) + lane_at);
+    } else if (whole && paged) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i)
+        to[i] = load16(cached_rows<D * kBytes>(a, cache, page_named(a, id[i]), step, head, t + i * STEP) + lane_at);
     } else {
       rarely();
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         const int tk = t + i * STEP + load_token;
-        const bool live = tk >= some_lo && tk < some_hi;
-        const uint32_t page = page_named(a, paged ? ids[i] : table_entry(a, w.s, clamped(tk)));
-        const global_bytes k = cached_rows<D * kBytes>(a, a.k_cache, page, a.k_step, head, tk) + chunk * 16;
-        const global_bytes v = cached_rows<D * kBytes>(a, a.v_cache, page, a.v_step, head, tk) + chunk * 16;
-        kr[i] = load16(live ? k : zero);
-        vr[i] = load16(live ? v : zero);
+        const uint32_t page = page_named(a, one_page ? id[0] : paged ? id[i] : table_entry(a, w.s, clamped(tk)));
+        const global_bytes from = cached_rows<D * kBytes>(a, cache, page, step, head, tk) + chunk * 16;
+        to[i] = load16(tk >= some_lo && tk < some_hi ? from : as_global(kZeroRow));
       }
     }
+  };
+  auto load_keys = [&](int t) __attribute__((always_inline)) { load(kr, next_ids, a.k_cache, a.k_step, t); };
+  auto load_values = [&](int t) __attribute__((always_inline)) {
+    load(vr, ids, a.v_cache, a.v_step, t);
     if constexpr (kFp8) {
       if (wave == 0) {
         const int tk = t + lane;
         const bool live = tk >= some_lo && tk < some_hi;
         const uint32_t page = page_named(a, table_entry(a, w.s, clamped(tk)));
-        const global_bytes kp = cached_scales(a, a.k_scales, page, a.ks_step, head, tk);
+        const global_bytes kp = cached_scales(a, a.k_scales, page, a.ks_step, head, tk), zero = as_global(kZeroRow);
         const global_bytes vp = cached_scales(a, a.v_scales, page, a.vs_step, head, tk);
         ks = load_float(live ? kp : zero), vs = load_float(live ? vp : zero);
       }
     }
   };
+  auto store = [&](char* to, const u32x4(&from)[LOADS]) __attribute__((always_inline)) {
+    if (!loads) return;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int tk = load_token + i * STEP, swz = swizzle<RB, true>(tk);
+      char* row = to + tk * RB;
+      if constexpr (kFp8) {
+        *(u32x4*)(row + ((load_chunk * 2 ^ swz) << 4)) = widen_codes<kBf16>(from[i][0], from[i][1]);
+        *(u32x4*)(row + (((load_chunk * 2 + 1) ^ swz) << 4)) = widen_codes<kBf16>(from[i][2], from[i][3]);
+      } else {
+        *(u32x4*)(row + ((load_chunk ^ swz) << 4)) = from[i];
+      }
+    }
+  };
   // whether rows of this tile see different ones of the tokens t ..
-  auto apart = [&](int t) { return (some_lo != all_lo || some_hi != all_hi) && (t < all_lo || t + 64 > all_hi); };
-  auto store_rows = [&](int buffer, int t) {
+  auto apart = [&](int t) __attribute__((always_inline)) { return (some_lo != all_lo || some_hi != all_hi) && (t < all_lo || t + 64 > all_hi); };
+  auto store_values = [&](int buffer, int t) __attribute__((always_inline)) {
     if (apart(t)) {
       rarely();
       bool found = false;
@@ -622,24 +642,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
       }
       if (found) left_out = 1;
     }
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int tk = load_token + i * STEP, swz = swizzle<RB, true>(tk);
-      if (loads) {
-        char* k = lds[buffer][0] + tk * RB;
-        char* v = lds[buffer][1] + tk * RB;
-        if constexpr (kFp8) {
-          const int c = load_chunk * 2;
-          *(u32x4*)(k + ((c ^ swz) << 4)) = widen_codes<kBf16>(kr[i][0], kr[i][1]);
-          *(u32x4*)(k + (((c + 1) ^ swz) << 4)) = widen_codes<kBf16>(kr[i][2], kr[i][3]);
-          *(u32x4*)(v + ((c ^ swz) << 4)) = widen_codes<kBf16>(vr[i][0], vr[i][1]);
-          *(u32x4*)(v + (((c + 1) ^ swz) << 4)) = widen_codes<kBf16>(vr[i][2], vr[i][3]);
-        } else {
-          *(u32x4*)(k + ((load_chunk ^ swz) << 4)) = kr[i];
-          *(u32x4*)(v + ((load_chunk ^ swz) << 4)) = vr[i];
-        }
-      }
-    }
+    store(lds[buffer][1], vr);
     if constexpr (kFp8) {
       if (wave == 0) {
         scales[buffer][0][lane] = ks * scale;
@@ -653,35 +656,51 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
   const int i16 = lane & 15, read_row = h * 4 + (i16 >> 2);
   const int v_at = read_row * RB + ((((lane >> 4 & 1) * 2 + (i16 >> 1 & 1)) ^ swizzle<RB, true>(read_row)) << 4) + (i16 & 1) * 8;
 
-  if (threadIdx.x == 0) left_out = 0;
-  __syncthreads();
-  if (w.begin < w.end) {
-    load_ids(w.begin);
-    load_rows(w.begin);
-    load_ids(w.begin + 64);
-    store_rows(0, w.begin);
-  }
-  __syncthreads();
-  int buffer = 0;
-  for (int t = w.begin; t < w.end; t += 64, buffer ^= 1) {
-    const bool more = t + 64 < w.end;
-    if (more) {
-      load_rows(t + 64);
-      load_ids(t + 128);
-    }
-    if (!idle && t < bottom.hi && t + 64 > top.lo) {  // some row of this wave sees some of these tokens
-      const char* keys = lds[buffer][0];
-      const char* values = lds[buffer][1];
-      f32x16 s[2];
+  auto scores = [&](int buffer, f32x16(&s)[2]) __attribute__((always_inline)) {
+    const char* keys = lds[buffer][0];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
 #pragma unroll
       for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
-#pragma unroll
-      for (int i = 0; i < KS; ++i)
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-          s[u] = mfma32<kBf16>(*(const u32x4*)(keys + u * 32 * RB + (k_at ^ (i * 32))), q[i], s[u]);
+        s[u] = mfma32<kBf16>(*(const u32x4*)(keys + u * 32 * RB + (k_at ^ (i * 32))), q[i], s[u]);
+  };
+
+  // Tokens t: values (and scales) in buffer j, their scores in registers; tokens t + 64: keys in buffer
+  // j ^ 1. Keys of t + 128 and values of t + 64 are under way.
+  if (threadIdx.x == 0) left_out = 0;
+  __syncthreads();
+  f32x16 s[2];
+  if (w.begin < w.end) {
+    load_ids(w.begin);
+    load_keys(w.begin);
+    ids = next_ids;
+    load_values(w.begin);
+    load_ids(w.begin + 64);
+    store(lds[0][0], kr);
+    load_keys(w.begin + 64);
+    ids = next_ids;
+    load_ids(w.begin + 128);
+    store_values(0, w.begin);
+    store(lds[1][0], kr);
+  }
+  __syncthreads();
+  if (w.begin < w.end) scores(0, s);
+  __syncthreads();  // the first keys are read: their buffer may be written
+  int j = 0;
+  for (int t = w.begin; t < w.end; t += 64, j ^= 1) {
+    const bool more = t + 64 < w.end;
+    if (more) {
+      load_values(t + 64);
+      load_keys(t + 128);
+      ids = next_ids;
+      load_ids(t + 192);
+    }
+    if (!idle) {
+      const char* values = lds[j][1];
       const bool masked = t < bottom.lo || t + 64 > top.hi;
       float high = -INFINITY;
       if constexpr (kFp8) {
@@ -689,7 +708,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const f32x4 k_mul = *(const f32x4*)&scales[buffer][0][u * 32 + i * 8 + h * 4];
+            const f32x4 k_mul = *(const f32x4*)&scales[j][0][u * 32 + i * 8 + h * 4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) s[u][i * 4 + r] *= k_mul[r];
           }
@@ -710,13 +729,14 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           f32x4 v_exp;
-          if constexpr (kFp8) v_exp = *(const f32x4*)&scales[buffer][2][u * 32 + i * 8 + h * 4];
+          if constexpr (kFp8) v_exp = *(const f32x4*)&scales[j][2][u * 32 + i * 8 + h * 4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) high = fmaxf(high, kFp8 ? s[u][i * 4 + r] + v_exp[r] : s[u][i * 4 + r]);
         }
       if constexpr (!kFp8) high *= scale;
       high = max_across32(high);
       if (__any(high > ref + kRise)) {
+        rarely();
         const float next = fmaxf(ref, high);
         const float keep = __builtin_amdgcn_exp2f(ref - (next == -INFINITY ? 0.f : next));
         ref = next;
@@ -727,39 +747,72 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
           for (int r = 0; r < 16; ++r) o[d][r] *= keep;
       }
       const float base = ref == -INFINITY ? 0.f : ref;
-      u32x4 p[4];
+      // Sixteen steps, each with the weights of two tokens, its part of the next tokens' products with the
+      // queries (of what lies in that buffer behind the last tokens, too: not used then) and, four steps
+      // behind, of the products with these values, so that the matrix unit works through all of them.
+      constexpr int S_ALL = 2 * KS, V_ALL = 4 * DT, K_AHEAD = 4, V_AHEAD = 2;
+      f32x16 after[2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int t0 = u * 32 + i * 8 + h * 4;
-          f32x4 v_mul;
-          if constexpr (kFp8) v_mul = *(const f32x4*)&scales[buffer][1][t0];
-          float wt[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float x = s[u][i * 4 + r];
-            const float e = __builtin_amdgcn_exp2f(kFp8 ? x - base : __builtin_fmaf(x, scale, -base));
-            total += e;
-            wt[r] = e;
-            if constexpr (kFp8) wt[r] = e * v_mul[r];
-          }
-          p[u * 2 + i / 2][(i & 1) * 2] = pack2<kBf16>(wt[0], wt[1]);
-          p[u * 2 + i / 2][(i & 1) * 2 + 1] = pack2<kBf16>(wt[2], wt[3]);
-        }
-      }
-      auto value = [&](int d, int m) {
+        for (int r = 0; r < 16; ++r) after[u][r] = 0.f;
+      const char* keys = lds[j ^ 1][0];
+      auto key = [&](int n) __attribute__((always_inline)) {
+        return *(const u32x4*)(keys + (n & 1) * 32 * RB + (k_at ^ ((n >> 1) * 32)));
+      };
+      auto value = [&](int n) __attribute__((always_inline)) {
+        const int m = n / DT, d = n % DT;
         // tokens 8 further: their swizzle differs in one bit
         const u32x2 lo = read_transposed(values + (v_at ^ (d * 64)) + m * 16 * RB);
         const u32x2 hi = read_transposed(values + (v_at ^ (d * 64) ^ 32) + (m * 16 + 8) * RB);
         return u32x4{lo[0], lo[1], hi[0], hi[1]};
       };
+      u32x4 p[4], kf[S_ALL], vf[V_ALL];
 #pragma unroll
-      for (int m = 0; m < 4; ++m)
+      for (int n = 0; n < K_AHEAD; ++n) kf[n] = key(n);
+      auto products = [&](int from, int to) __attribute__((always_inline)) {
 #pragma unroll
-        for (int d = 0; d < DT; ++d) o[d] = mfma32<kBf16>(value(d, m), p[m], o[d]);
+        for (int n = 0; n < V_ALL; ++n) {
+          if (n < from || n >= to) continue;
+          if (n + V_AHEAD < V_ALL) vf[n + V_AHEAD] = value(n + V_AHEAD);
+          o[n % DT] = mfma32<kBf16>(vf[n], p[n / DT], o[n % DT]);
+        }
+      };
+      float sums[2] = {0.f, 0.f};
+      f32x4 v_mul;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+#pragma unroll
+        for (int n = i * S_ALL / 16; n < (i + 1) * S_ALL / 16; ++n) {
+          if (n + K_AHEAD < S_ALL) kf[n + K_AHEAD] = key(n + K_AHEAD);
+          after[n & 1] = mfma32<kBf16>(kf[n], q[n >> 1], after[n & 1]);
+        }
+        if (i == 3) {
+#pragma unroll
+          for (int n = 0; n < V_AHEAD; ++n) vf[n] = value(n);
+        }
+        if (i >= 4) products((i - 4) * DT / 4, (i - 3) * DT / 4);
+        if constexpr (kFp8)
+          if (i % 2 == 0) v_mul = *(const f32x4*)&scales[j][1][(i / 2 / 4) * 32 + (i / 2 % 4) * 8 + h * 4];
+        float wt[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float x = s[i / 8][i % 8 * 2 + e];
+          const float y = __builtin_amdgcn_exp2f(kFp8 ? x - base : __builtin_fmaf(x, scale, -base));
+          sums[e] += y;
+          wt[e] = kFp8 ? y * v_mul[i % 2 * 2 + e] : y;
+        }
+        p[i / 4][i % 4] = pack2<kBf16>(wt[0], wt[1]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      products(3 * DT, V_ALL);
+      total += sums[0] + sums[1];
+      s[0] = after[0], s[1] = after[1];
     }
-    if (more) store_rows(buffer ^ 1, t + 64);
+    if (more) {
+      store_values(j ^ 1, t + 64);
+      store(lds[j][0], kr);
+    }
     __syncthreads();
   }
 
@@ -825,8 +878,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
   const bool alone = w.splits <= 16;
   const int ways = alone ? 1 : 4, way = alone ? 0 : wave;  // waves of a row, and this one's place
   for (int r = alone ? blockIdx.y * 4 + wave : blockIdx.y; r < w.rows; r += alone ? gridDim.y * 4 : gridDim.y) {
-    auto at = [&](int j) { return ((int64_t)(w.slot + j) * a.HK + head) * ROWS + r; };
-    auto load = [&](int j) { return *(const part*)(a.partial + at(min(j, w.splits - 1)) * D + d0); };
+    auto at = [&](int j) __attribute__((always_inline)) { return ((int64_t)(w.slot + j) * a.HK + head) * ROWS + r; };
+    auto load = [&](int j) __attribute__((always_inline)) { return *(const part*)(a.partial + at(min(j, w.splits - 1)) * D + d0); };
     part ahead[AHEAD];
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) ahead[i] = load(way + i * ways);
@@ -850,7 +903,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
       for (int off = 32; off >= 1; off >>= 1) all += __shfl_xor(all, off);
       total += all;
       const int n = min(w.splits - j0, 64);
-      auto add = [&](part v, int i) {
+      auto add = [&](part v, int i) __attribute__((always_inline)) {
         const float k = bit_cast<float>(__builtin_amdgcn_readlane(bit_cast<int>(keep), i));
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = __builtin_fmaf(k, v[e], acc[e]);
