@@ -44,12 +44,12 @@ struct AttnLaunch {
   int items, joins, join_rows;
 };
 
-// The tiled kernels for one type and cache (paged_attn_*.hip): 16 * tiles rows over one workgroup's
-// four waves, which split the tokens ("rows" kernel, tiles 1, 2 or 4), or 128 rows, 32 to a wave.
-int launch_attn_f16(const AttnLaunch& l, int tiles, hipStream_t stream);
-int launch_attn_bf16(const AttnLaunch& l, int tiles, hipStream_t stream);
-int launch_attn_f16_fp8(const AttnLaunch& l, int tiles, hipStream_t stream);
-int launch_attn_bf16_fp8(const AttnLaunch& l, int tiles, hipStream_t stream);
+// The tiled kernels for one type and cache (paged_attn_*.hip), by the rows of a tile: 16 to 64, whose
+// tokens are spread over a workgroup's four waves, or 128 or 256, 32 to a wave.
+int launch_attn_f16(const AttnLaunch& l, int rows, hipStream_t stream);
+int launch_attn_bf16(const AttnLaunch& l, int rows, hipStream_t stream);
+int launch_attn_f16_fp8(const AttnLaunch& l, int rows, hipStream_t stream);
+int launch_attn_bf16_fp8(const AttnLaunch& l, int rows, hipStream_t stream);
 
 // Query rows [start, start + count) and cached tokens of sequence s.
 struct Sequence {

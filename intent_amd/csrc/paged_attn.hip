@@ -145,18 +145,17 @@ int launch_rows(const AttnArgs& a, hipStream_t stream) {
 // ---- which kernel, and into how many parts --------------------------------------------
 
 struct Part {
-  int tiles;  // 16-row tiles of the kernel with the tokens over the waves; 0: 128 rows
+  int rows;  // of a tile
   int min_rows, max_rows;
-  int rows() const { return tiles > 0 ? 16 * tiles : 128; }
-  int unit() const { return tiles > 0 ? 128 : 64; }
+  int unit() const { return rows <= 64 ? 128 : 64; }
   // Workgroups that the tiles are split for: what the 256 CUs hold at one time (by the kernels' registers),
   // and twice that where a CU holds three, which evens out sequences of different lengths and costs
   // little (four sequences of 60000 to 131000 tokens: 300 us at 512, 235 at 768, 239 at 1536; 64 of 300
   // to 8191 126, 128 and 119 us). One workgroup to a CU loses by a second round (16 sequences of five
   // drafted tokens: 28 us at 256, 34 at 512).
   int fill(int64_t D) const {
-    if (tiles == 0) return 512;
-    return D > 128 ? 256 : tiles * D <= 128 ? 1536 : tiles * D <= 256 ? 512 : 256;
+    if (rows > 64) return rows == 256 ? 256 : 512;
+    return D > 128 ? 256 : rows * D <= 2048 ? 1536 : rows * D <= 4096 ? 512 : 256;
   }
 };
 
@@ -176,21 +175,22 @@ Plan plan_of(int64_t T, int64_t S, int64_t group, int64_t D) {
   Plan p{};
   p.parts = 1;
   const int most = D > 128 ? 16 : 64;
+  const int BIG = D <= 128 && mean >= 512 ? 256 : 128;
   if (mean <= most) {
-    p.part[0] = {mean > 16 ? (int)((mean + 15) / 16) : 1, 0, INT32_MAX};
+    p.part[0] = {mean > 16 ? (int)((mean + 15) / 16) * 16 : 16, 0, INT32_MAX};
   } else if (S == 1) {
-    p.part[0] = {0, 0, INT32_MAX};
+    p.part[0] = {BIG, 0, INT32_MAX};
   } else {
     p.parts = 2;
     const int few = D > 128 ? 16 : 32;
-    p.part[0] = {0, few, INT32_MAX};
-    p.part[1] = {few / 16, 0, few};
+    p.part[0] = {BIG, few, INT32_MAX};
+    p.part[1] = {few, 0, few};
   }
   return p;
 }
 
 int64_t tiles_bound(const Part& p, int64_t T, int64_t S, int64_t group) {
-  return T * group / p.rows() + (S < T ? S : T);
+  return T * group / p.rows + (S < T ? S : T);
 }
 
 // Parts of all split tiles of one head: fewer than twice the target (each of two parts at least has
@@ -205,7 +205,7 @@ int64_t slots_bound(const Part& p, int64_t T, int64_t S, int64_t group, int64_t 
 }
 
 size_t part_bytes(const Part& p, int64_t T, int64_t S, int64_t group, int64_t HK, int64_t D, int64_t most_kv) {
-  return (size_t)(slots_bound(p, T, S, group, HK, D, most_kv) * HK * p.rows() * (D + 2) * 4);
+  return (size_t)(slots_bound(p, T, S, group, HK, D, most_kv) * HK * p.rows * (D + 2) * 4);
 }
 
 int launch_tiled(AttnArgs a, bool bf16, bool fp8, float* workspace, size_t bytes, hipStream_t stream) {
@@ -219,7 +219,7 @@ int launch_tiled(AttnArgs a, bool bf16, bool fp8, float* workspace, size_t bytes
     a.min_rows = p.min_rows, a.max_rows = p.max_rows;
     a.target = split ? (p.fill(a.D) + a.HK - 1) / a.HK : 0;
     a.partial = workspace;
-    a.partial_stats = split ? workspace + slots_bound(p, a.T, a.S, a.group, a.HK, a.D, a.most_kv) * a.HK * p.rows() * a.D : nullptr;
+    a.partial_stats = split ? workspace + slots_bound(p, a.T, a.S, a.group, a.HK, a.D, a.most_kv) * a.HK * p.rows * a.D : nullptr;
     const int64_t tiles = tiles_bound(p, a.T, a.S, a.group);
     const int64_t joins = split ? (tiles < a.target ? tiles : a.target) : 0;
     // 256-lane workgroups: the grid's work items stay below 2^32
@@ -231,10 +231,10 @@ int launch_tiled(AttnArgs a, bool bf16, bool fp8, float* workspace, size_t bytes
     l.joins = (int)joins;
     // workgroups for the rows of a split tile: one for each of a mean sequence, up to 2048 in all
     const int64_t mean = ((int64_t)a.T * a.group + a.S - 1) / a.S, room = joins > 0 ? 2048 / (joins * a.HK) : 0;
-    const int64_t side = mean < p.rows() ? mean : p.rows();
+    const int64_t side = mean < p.rows ? mean : p.rows;
     l.join_rows = (int)(room < 1 ? 1 : room < side ? room : side);
-    if (fp8) status = bf16 ? launch_attn_bf16_fp8(l, p.tiles, stream) : launch_attn_f16_fp8(l, p.tiles, stream);
-    else status = bf16 ? launch_attn_bf16(l, p.tiles, stream) : launch_attn_f16(l, p.tiles, stream);
+    if (fp8) status = bf16 ? launch_attn_bf16_fp8(l, p.rows, stream) : launch_attn_f16_fp8(l, p.rows, stream);
+    else status = bf16 ? launch_attn_bf16(l, p.rows, stream) : launch_attn_f16(l, p.rows, stream);
   }
   return status;
 }

@@ -15,8 +15,8 @@
 // is part of the weight that is rounded: M follows the maximum of t + log2(scale), w = exp2(t - M) *
 // scale, and only the sum of weights takes exp2(t - M) by itself. The codes are exact in 16 bits.
 //
-// A weight of zero does not keep an infinity or NaN out of a product. Tokens that no row of a tile sees
-// are read from a row of zeros; where rows of a tile see different tokens (the last of a chunk, the
+// A weight of zero does not keep an infinity or NaN out of a product. Values of tokens that no row of a
+// tile sees (pages behind a sequence's end hold anything) are set to zero; where rows of a tile see different tokens (the last of a chunk, the
 // first of a window), values (and scales) that are not finite go into the product as zeros, and once the loop is
 // over they are added to the rows that see them (which has them infinite or NaN).
 #pragma once
@@ -34,11 +34,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
 
-// What tokens that no row of a tile sees are read from: pages behind a sequence's end hold anything.
-static __device__ __attribute__((aligned(16))) const uint32_t kZeroRow[128] = {};
-
-// A cached token's row (or scale) of a page, or the row of zeros: global addresses throughout, so that
-// the loads count on vmcnt alone.
+// A cached token's row or scale: global addresses, so that the loads count on vmcnt alone.
 typedef const __attribute__((address_space(1))) char* global_bytes;
 INTENT_DEVICE global_bytes as_global(const void* p) { return (global_bytes)p; }
 // Rows (of kRowBytes) of a head from token t on, t and the page uniform or not.
@@ -52,11 +48,6 @@ INTENT_DEVICE global_bytes cached_scales(const AttnArgs& a, const float* base, u
   return as_global(base) + ((uint64_t)page * step + row) * 4;
 }
 INTENT_DEVICE float load_float(global_bytes p) { return *(const __attribute__((address_space(1))) float*)p; }
-// The table's entry of a token that is the same in all lanes: a scalar load.
-INTENT_DEVICE uint32_t uniform_entry(const AttnArgs& a, int s, int t) {
-  const int64_t at = (int64_t)s * a.table_ld + (t >> a.page_shift);
-  return *(const __attribute__((address_space(4))) uint32_t*)(a.page_table + at);
-}
 INTENT_DEVICE u32x4 load16(global_bytes p) { return *(const __attribute__((address_space(1))) u32x4*)p; }
 INTENT_DEVICE u32x2 load8(global_bytes p) { return *(const __attribute__((address_space(1))) u32x2*)p; }
 
@@ -254,18 +245,16 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
 
   u32x4 kr[2][LOADS], vr[2][LOADS];
   float ks[2], vs[2];
-  // Pages of 16 tokens and more: each 16 tokens lie in one, whose id is a scalar (loaded ahead, clamped
-  // where it is used, so that the wait for it is there). Smaller ones: each lane looks up its token's.
+  // Pages of 16 tokens and more: each 16 tokens lie in one. The table's entries of this wave's next 32
+  // times 32 tokens are kept one in each lane (a vector load every 32 times: scalar loads would make
+  // every wait for LDS a wait for them) and clamped where they are used. Smaller pages: each lane looks
+  // up its token's.
   constexpr int kBytes = kFp8 ? 1 : 2;
   const bool paged = a.page_shift >= 4;
   const uint32_t lane_at = col * (D * kBytes) + g * ELEMS * kBytes;
-  uint32_t ids[2];
   auto clamped = [&](int t) { return min(max(t, some_lo), max(some_hi - 1, 0)); };
-  auto load_ids = [&](int t) {
-    if (paged)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) ids[u] = uniform_entry(a, w.s, clamped(t + 16 * u));
-  };
+  uint32_t entries = 0, next_entries = 0;
+  auto batch = [&](int t) { return table_entry(a, w.s, clamped(t + (lane >> 1) * 128 + (lane & 1) * 16)); };
   auto issue = [&](int u, global_bytes k, global_bytes v, global_bytes kp, global_bytes vp) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
@@ -281,30 +270,32 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
     }
     if constexpr (kFp8) ks[u] = load_float(kp), vs[u] = load_float(vp);
   };
+  int place = 0;  // of the entries of the tokens to load next
+  // Tokens that no row sees are loaded too (a page that is there, whatever it holds): their scores are
+  // masked, their values set to zero when they are stored.
   auto load_rows = [&](int t) {
-    const global_bytes zero = as_global(kZeroRow);
-    if (paged && t >= some_lo && t + 32 <= some_hi) {
+    if (paged) {
+      if (place == 64) entries = next_entries, next_entries = batch(t + 32 * 128), place = 0;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const uint32_t page = page_named(a, ids[u]);
+        const uint32_t page = page_named(a, (uint32_t)lane_value((int)entries, place + u));
         const int t16 = t + 16 * u;
         issue(u, cached_rows<D * kBytes>(a, a.k_cache, page, a.k_step, head, t16) + lane_at,
               cached_rows<D * kBytes>(a, a.v_cache, page, a.v_step, head, t16) + lane_at,
               cached_scales(a, a.k_scales, page, a.ks_step, head, t16) + col * 4,
               cached_scales(a, a.v_scales, page, a.vs_step, head, t16) + col * 4);
       }
+      place += 2;
     } else {
       rarely();
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int tk = t + 16 * u + col;
-        const bool live = tk >= some_lo && tk < some_hi;
-        const uint32_t page = page_named(a, paged ? ids[u] : table_entry(a, w.s, clamped(tk)));
-        const global_bytes k = cached_rows<D * kBytes>(a, a.k_cache, page, a.k_step, head, tk) + g * ELEMS * kBytes;
-        const global_bytes v = cached_rows<D * kBytes>(a, a.v_cache, page, a.v_step, head, tk) + g * ELEMS * kBytes;
-        const global_bytes kp = cached_scales(a, a.k_scales, page, a.ks_step, head, tk);
-        const global_bytes vp = cached_scales(a, a.v_scales, page, a.vs_step, head, tk);
-        issue(u, live ? k : zero, live ? v : zero, live ? kp : zero, live ? vp : zero);
+        const uint32_t page = page_named(a, table_entry(a, w.s, clamped(tk)));
+        issue(u, cached_rows<D * kBytes>(a, a.k_cache, page, a.k_step, head, tk) + g * ELEMS * kBytes,
+              cached_rows<D * kBytes>(a, a.v_cache, page, a.v_step, head, tk) + g * ELEMS * kBytes,
+              cached_scales(a, a.k_scales, page, a.ks_step, head, tk),
+              cached_scales(a, a.v_scales, page, a.vs_step, head, tk));
       }
     }
   };
@@ -314,13 +305,24 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
   bool found = false;
   int t = w.begin + wave * 32;
   if (t < w.end) {
-    load_ids(t);
+    if (paged) entries = batch(t), next_entries = batch(t + 32 * 128);
     load_rows(t);
-    load_ids(t + 128);
   }
   for (; t < w.end; t += 128) {
     // values and scales of these tokens to LDS, the scores' operands from the registers
     const bool masked = t < all_lo || t + 32 > all_hi;
+    if (t < some_lo || t + 32 > some_hi) {
+      rarely();
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int tk = t + 16 * u + col;
+        if (tk < some_lo || tk >= some_hi) {
+          vs[u] = 0.f;
+#pragma unroll
+          for (int i = 0; i < LOADS; ++i) vr[u][i] = u32x4{0u, 0u, 0u, 0u};
+        }
+      }
+    }
     if (apart(t)) {
       rarely();
 #pragma unroll
@@ -374,10 +376,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
       }
     }
     const int now = t;
-    if (now + 128 < w.end) {
-      load_rows(now + 128);
-      load_ids(now + 256);
-    }
+    if (now + 128 < w.end) load_rows(now + 128);
     u32x4 p[MT];
     f32x4 v_mul[2], v_exp[2];
     if constexpr (kFp8) {
@@ -518,13 +517,14 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
 // 64 tokens of keys and values in LDS at a time, in two buffers: the next ones are loaded into
 // registers while these are worked on and stored to the other buffer behind them, so one barrier for
 // each 64 tokens.
-template <bool kBf16, bool kFp8, int D>
-__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const AttnArgs a) {
+template <bool kBf16, bool kFp8, int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void attn_tile_kernel(const AttnArgs a) {
   constexpr int KS = D / 16, DT = D / 32, RB = row_bytes<D>();
   constexpr int CHUNKS = kFp8 ? D / 16 : D / 8;       // 16-byte loads of a token's row
   constexpr int SPREAD = kFp8 ? RB / 32 : RB / 16;    // lanes that take one (a power of two)
-  constexpr int STEP = 256 / SPREAD;                  // tokens that the workgroup loads at once
-  constexpr int LOADS = 64 / STEP;
+  constexpr int EACH = 64 / SPREAD;                   // tokens that a wave loads at once
+  constexpr int STEP = EACH * WAVES;                  // and the workgroup
+  constexpr int LOADS = STEP >= 64 ? 1 : 64 / STEP, ROWS = 32 * WAVES;
   constexpr int kTile = 64 * RB;
   __shared__ __attribute__((aligned(16))) char lds[2][2][kTile];
   __shared__ __attribute__((aligned(16))) float scales[kFp8 ? 2 : 1][3][64];
@@ -532,7 +532,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
 
   const int head = blockIdx.x % a.HK;
   Span w;
-  if (!find_span<128, 64>(a, blockIdx.x / a.HK, false, w)) return;
+  if (!find_span<ROWS, 64>(a, blockIdx.x / a.HK, false, w)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int col = lane & 31, h = lane >> 5;
   const int r0 = wave * 32;
@@ -557,59 +557,63 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
     for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
   float ref = -INFINITY, total = 0.f;
 
-  const int load_token = threadIdx.x / SPREAD, load_chunk = threadIdx.x % SPREAD;
-  const bool loads = load_chunk < CHUNKS;
+  const int wave_token = wave * EACH & 63;  // where there are more waves than tokens, those behind idle
+  const int load_token = wave_token + lane / SPREAD, load_chunk = lane % SPREAD;
+  const bool loads = load_chunk < CHUNKS && wave * EACH < 64;
   u32x4 kr[LOADS], vr[LOADS];
   float ks = 0.f, vs = 0.f;
-  // Pages of STEP tokens and more: each load's tokens lie in one, whose id is a scalar (as above).
+  // Pages of EACH tokens and more (16 at most): each load's tokens lie in one, whose id is a scalar.
   constexpr int kBytes = kFp8 ? 1 : 2;
-  const bool paged = (1 << a.page_shift) >= STEP;
-  const int chunk = loads ? load_chunk : 0;
-  const uint32_t lane_at = load_token * (D * kBytes) + chunk * 16;
-  typedef uint32_t Ids __attribute__((ext_vector_type(LOADS)));
-  Ids ids{}, next_ids{};  // of the values' and the keys' tokens to load next
-  auto clamped = [&](int t) __attribute__((always_inline)) { return min(max(t, some_lo), max(some_hi - 1, 0)); };
+  const bool paged = (1 << a.page_shift) >= EACH;
+  const int chunk = load_chunk < CHUNKS ? load_chunk : 0;
+  const uint32_t lane_at = (lane / SPREAD) * (D * kBytes) + chunk * 16;
+  // The table's entries of the next `span` times 64 tokens, one in each lane, in two batches (a vector
+  // load for each: scalar loads would make every wait for LDS a wait for them).
   const bool one_page = a.page_shift >= 6;  // the 64 tokens in one page
-  auto load_ids = [&](int t) __attribute__((always_inline)) {
+  constexpr int kLoadsLog = LOADS == 1 ? 0 : LOADS == 2 ? 1 : LOADS == 4 ? 2 : 3;
+  const int pieces_log = one_page ? 0 : kLoadsLog, span_log = 6 - pieces_log, span = 1 << span_log;
+  auto clamped = [&](int t) __attribute__((always_inline)) { return min(max(t, some_lo), max(some_hi - 1, 0)); };
+  auto batch = [&](int t) __attribute__((always_inline)) {
+    return table_entry(a, w.s, clamped(t + (lane >> pieces_log) * 64 + (lane & ((1 << pieces_log) - 1)) * STEP + wave_token));
+  };
+  uint32_t entries[2] = {0, 0};
+  // of the i-th load of the tokens n * 64 behind w.begin
+  auto entry = [&](int n, int i) __attribute__((always_inline)) {
+    return (uint32_t)lane_value((int)(n >> span_log & 1 ? entries[1] : entries[0]),
+                                ((n & (span - 1)) << pieces_log) + (one_page ? 0 : i));
+  };
+  // Tokens that no row sees are loaded too (a page that is there, whatever it holds): their scores are
+  // masked, their values set to zero when they are stored.
+  auto load = [&](u32x4(&fetched)[LOADS], const void* cache, uint32_t step, int t) __attribute__((always_inline)) {
+    const int n = (t - w.begin) >> 6;
     if (one_page) {
-      next_ids[0] = uniform_entry(a, w.s, clamped(t));
+      const global_bytes from = cached_rows<D * kBytes>(a, cache, page_named(a, entry(n, 0)), step, head, t + wave_token);
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) fetched[i] = load16(from + i * (STEP * D * kBytes) + lane_at);
     } else if (paged) {
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i) next_ids[i] = uniform_entry(a, w.s, clamped(t + i * STEP));
-    }
-  };
-  auto load = [&](u32x4(&to)[LOADS], Ids id, const void* cache, uint32_t step, int t) __attribute__((always_inline)) {
-    const bool whole = t >= some_lo && t + 64 <= some_hi;
-    if (whole && one_page) {
-      const global_bytes from = cached_rows<D * kBytes>(a, cache, page_named(a, id[0]), step, head, t);
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) to[i] = load16(from + i * (STEP * D * kBytes) + lane_at);
-    } else if (whole && paged) {
-#pragma unroll
       for (int i = 0; i < LOADS; ++i)
-        to[i] = load16(cached_rows<D * kBytes>(a, cache, page_named(a, id[i]), step, head, t + i * STEP) + lane_at);
+        fetched[i] = load16(cached_rows<D * kBytes>(a, cache, page_named(a, entry(n, i)), step, head, t + i * STEP + wave_token) +
+                            lane_at);
     } else {
       rarely();
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         const int tk = t + i * STEP + load_token;
-        const uint32_t page = page_named(a, one_page ? id[0] : paged ? id[i] : table_entry(a, w.s, clamped(tk)));
-        const global_bytes from = cached_rows<D * kBytes>(a, cache, page, step, head, tk) + chunk * 16;
-        to[i] = load16(tk >= some_lo && tk < some_hi ? from : as_global(kZeroRow));
+        const uint32_t page = page_named(a, table_entry(a, w.s, clamped(tk)));
+        fetched[i] = load16(cached_rows<D * kBytes>(a, cache, page, step, head, tk) + chunk * 16);
       }
     }
   };
-  auto load_keys = [&](int t) __attribute__((always_inline)) { load(kr, next_ids, a.k_cache, a.k_step, t); };
+  auto load_keys = [&](int t) __attribute__((always_inline)) { load(kr, a.k_cache, a.k_step, t); };
   auto load_values = [&](int t) __attribute__((always_inline)) {
-    load(vr, ids, a.v_cache, a.v_step, t);
+    load(vr, a.v_cache, a.v_step, t);
     if constexpr (kFp8) {
       if (wave == 0) {
         const int tk = t + lane;
-        const bool live = tk >= some_lo && tk < some_hi;
         const uint32_t page = page_named(a, table_entry(a, w.s, clamped(tk)));
-        const global_bytes kp = cached_scales(a, a.k_scales, page, a.ks_step, head, tk), zero = as_global(kZeroRow);
-        const global_bytes vp = cached_scales(a, a.v_scales, page, a.vs_step, head, tk);
-        ks = load_float(live ? kp : zero), vs = load_float(live ? vp : zero);
+        ks = load_float(cached_scales(a, a.k_scales, page, a.ks_step, head, tk));
+        vs = load_float(cached_scales(a, a.v_scales, page, a.vs_step, head, tk));
       }
     }
   };
@@ -630,6 +634,15 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
   // whether rows of this tile see different ones of the tokens t ..
   auto apart = [&](int t) __attribute__((always_inline)) { return (some_lo != all_lo || some_hi != all_hi) && (t < all_lo || t + 64 > all_hi); };
   auto store_values = [&](int buffer, int t) __attribute__((always_inline)) {
+    if (t < some_lo || t + 64 > some_hi) {
+      rarely();
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int tk = t + i * STEP + load_token;
+        if (tk < some_lo || tk >= some_hi) vr[i] = u32x4{0u, 0u, 0u, 0u};
+      }
+      if (t + lane < some_lo || t + lane >= some_hi) vs = 0.f;
+    }
     if (apart(t)) {
       rarely();
       bool found = false;
@@ -675,15 +688,11 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
   __syncthreads();
   f32x16 s[2];
   if (w.begin < w.end) {
-    load_ids(w.begin);
+    if (paged) entries[0] = batch(w.begin), entries[1] = batch(w.begin + span * 64);
     load_keys(w.begin);
-    ids = next_ids;
     load_values(w.begin);
-    load_ids(w.begin + 64);
     store(lds[0][0], kr);
     load_keys(w.begin + 64);
-    ids = next_ids;
-    load_ids(w.begin + 128);
     store_values(0, w.begin);
     store(lds[1][0], kr);
   }
@@ -696,8 +705,13 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
     if (more) {
       load_values(t + 64);
       load_keys(t + 128);
-      ids = next_ids;
-      load_ids(t + 192);
+      const int n = (t + 64 - w.begin) >> 6;
+      if (paged && (n & (span - 1)) == span - 1) {  // past a batch: the one behind the other takes its place
+        rarely();
+        const uint32_t later = batch(t + 64 + (span + 1) * 64);
+        if (n >> span_log & 1) entries[1] = later;
+        else entries[0] = later;
+      }
     }
     if (!idle) {
       const char* values = lds[j][1];
@@ -780,8 +794,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
       };
       float sums[2] = {0.f, 0.f};
       f32x4 v_mul;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
+      auto step = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
         for (int n = i * S_ALL / 16; n < (i + 1) * S_ALL / 16; ++n) {
           if (n + K_AHEAD < S_ALL) kf[n + K_AHEAD] = key(n + K_AHEAD);
@@ -804,7 +817,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
         }
         p[i / 4][i % 4] = pack2<kBf16>(wt[0], wt[1]);
         __builtin_amdgcn_sched_barrier(0);
-      }
+      };
+#pragma unroll
+      for (int i = 0; i < 16; ++i) step(i);
       products(3 * DT, V_ALL);
       total += sums[0] + sums[1];
       s[0] = after[0], s[1] = after[1];
@@ -847,7 +862,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile_kernel(const 
         *(u32x2*)(to + d * 32 + i * 8 + h * 4) = u32x2{pack2<kBf16>(o[d][i * 4] * inv, o[d][i * 4 + 1] * inv),
                                                        pack2<kBf16>(o[d][i * 4 + 2] * inv, o[d][i * 4 + 3] * inv)};
   } else {
-    const int64_t to = ((int64_t)w.slot * a.HK + head) * 128 + r;
+    const int64_t to = ((int64_t)w.slot * a.HK + head) * ROWS + r;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -935,42 +950,46 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
   }
 }
 
-template <bool kBf16, bool kFp8, int D, int MT>  // MT = 0: the 128-row tile
+// The kernel, and the join of its split tiles. ROWS up to 64: rows of the first kernel; 128 or 256: of
+// the second's four or eight waves.
+template <bool kBf16, bool kFp8, int D, int ROWS>
 int launch(const AttnLaunch& l, hipStream_t stream) {
   const unsigned heads = (unsigned)l.a.HK;
-  constexpr int kRows = MT > 0 ? 16 * MT : 128, kUnit = MT > 0 ? 128 : 64;
-  if constexpr (MT > 0)
-    hipLaunchKernelGGL((attn_rows_kernel<kBf16, kFp8, D, MT>), dim3(l.items * heads), dim3(256), 0, stream, l.a);
+  constexpr bool kFew = ROWS <= 64;
+  if constexpr (kFew)
+    hipLaunchKernelGGL((attn_rows_kernel<kBf16, kFp8, D, ROWS / 16>), dim3(l.items * heads), dim3(256), 0, stream, l.a);
   else
-    hipLaunchKernelGGL((attn_tile_kernel<kBf16, kFp8, D>), dim3(l.items * heads), dim3(256), 0, stream, l.a);
-  const int status = launch_status_fmt("attn_%s_kernel<%s%s, D %d, %d rows%s>", MT > 0 ? "rows" : "tile",
-                                       kBf16 ? "bf16" : "f16", kFp8 ? ", fp8 cache" : "", D, kRows,
+    hipLaunchKernelGGL((attn_tile_kernel<kBf16, kFp8, D, ROWS / 32>), dim3(l.items * heads), dim3(ROWS * 2), 0, stream,
+                       l.a);
+  const int status = launch_status_fmt("attn_%s_kernel<%s%s, D %d, %d rows%s>", kFew ? "rows" : "tile",
+                                       kBf16 ? "bf16" : "f16", kFp8 ? ", fp8 cache" : "", D, ROWS,
                                        l.joins > 0 ? ", splits" : "");
   if (status != INTENT_OK || l.joins == 0) return status;
-  hipLaunchKernelGGL((attn_join_kernel<kBf16, D, kRows, kUnit>), dim3(l.joins * heads, l.join_rows), dim3(256), 0, stream,
-                     l.a);
-  return launch_status_fmt("attn_%s_kernel<%s%s, D %d, %d rows, splits>", MT > 0 ? "rows" : "tile",
-                           kBf16 ? "bf16" : "f16", kFp8 ? ", fp8 cache" : "", D, kRows);
+  hipLaunchKernelGGL((attn_join_kernel<kBf16, D, ROWS, kFew ? 128 : 64>), dim3(l.joins * heads, l.join_rows), dim3(256),
+                     0, stream, l.a);
+  return launch_status_fmt("attn_%s_kernel<%s%s, D %d, %d rows, splits>", kFew ? "rows" : "tile", kBf16 ? "bf16" : "f16",
+                           kFp8 ? ", fp8 cache" : "", D, ROWS);
 }
 
 template <bool kBf16, bool kFp8, int D>
-int launch_d(const AttnLaunch& l, int tiles, hipStream_t stream) {
-  if (tiles == 1) return launch<kBf16, kFp8, D, 1>(l, stream);
+int launch_d(const AttnLaunch& l, int rows, hipStream_t stream) {
+  if (rows == 16) return launch<kBf16, kFp8, D, 16>(l, stream);
   if constexpr (D <= 128) {
-    if (tiles == 2) return launch<kBf16, kFp8, D, 2>(l, stream);
-    if (tiles == 3) return launch<kBf16, kFp8, D, 3>(l, stream);
-    if (tiles == 4) return launch<kBf16, kFp8, D, 4>(l, stream);
+    if (rows == 32) return launch<kBf16, kFp8, D, 32>(l, stream);
+    if (rows == 48) return launch<kBf16, kFp8, D, 48>(l, stream);
+    if (rows == 64) return launch<kBf16, kFp8, D, 64>(l, stream);
+    if (rows == 256) return launch<kBf16, kFp8, D, 256>(l, stream);
   }
-  return launch<kBf16, kFp8, D, 0>(l, stream);
+  return launch<kBf16, kFp8, D, 128>(l, stream);
 }
 
 template <bool kBf16, bool kFp8>
-int launch_any(const AttnLaunch& l, int tiles, hipStream_t stream) {
+int launch_any(const AttnLaunch& l, int rows, hipStream_t stream) {
   switch (l.a.D) {
-    case 64: return launch_d<kBf16, kFp8, 64>(l, tiles, stream);
-    case 96: return launch_d<kBf16, kFp8, 96>(l, tiles, stream);
-    case 128: return launch_d<kBf16, kFp8, 128>(l, tiles, stream);
-    case 256: return launch_d<kBf16, kFp8, 256>(l, tiles, stream);
+    case 64: return launch_d<kBf16, kFp8, 64>(l, rows, stream);
+    case 96: return launch_d<kBf16, kFp8, 96>(l, rows, stream);
+    case 128: return launch_d<kBf16, kFp8, 128>(l, rows, stream);
+    case 256: return launch_d<kBf16, kFp8, 256>(l, rows, stream);
     default: return fail(INTENT_ERR_UNSUPPORTED, "no tiled attention kernel for heads of %d", l.a.D);
   }
 }
