@@ -123,7 +123,7 @@ INTENT_DEVICE float wave_total(float v) {
 // (which sees most) to the first, each tile in `splits` parts of its tokens. The parts are sized so
 // that all sequences together give about a.target of them: units / chunk of each, chunk = the units
 // that a workgroup would get of an even share (rounded up, so never less than that: the workspace is
-// sized by it). With `joins`, the list of the tiles that are split. Every wave does it by itself: no
+// sized by it), but for 64 and more new rows no fewer than 8 units (a join costs as many). With `joins`, the list of the tiles that are split. Every wave does it by itself: no
 // plan is kept, so a captured call follows lengths that change. The counts of one list fit 32 bits (the
 // host bounds the grid).
 template <int ROWS, int UNIT>
@@ -138,11 +138,13 @@ INTENT_DEVICE bool find_span(const AttnArgs& a, int item, bool joins, Span& r) {
       all += (float)e.tiles * (float)e.units;
     }
     chunk = (int)fminf(wave_total(all) * (1.0f + 0x1p-12f) / (float)a.target, 1.0e9f) + 1;
+    if (ROWS > 64) chunk = max(chunk, 8);
   }
   int base = 0, slots = 0;  // shares, and slots of split tiles, before sequence s0
   for (int s0 = 0; s0 < a.S; s0 += 64) {
     const Extent e = s0 == 0 ? first : extent_of<ROWS, UNIT>(a, s0 + lane);
-    const int splits = e.units > chunk ? min((int)(((uint32_t)e.units + (uint32_t)chunk - 1u) / (uint32_t)chunk), kMostSplits) : 1;
+    const uint32_t near = ((uint32_t)e.units + (uint32_t)chunk / 2u) / (uint32_t)chunk;  // to the nearest
+    const int splits = near > 1u ? min((int)near, kMostSplits) : 1;
     const int parts = e.tiles * splits, kept = splits > 1 ? parts : 0;
     const int mine = joins ? (splits > 1 ? e.tiles : 0) : parts;
     const int up = wave_prefix(mine) + base, kept_up = wave_prefix(kept) + slots;

@@ -175,7 +175,7 @@ Plan plan_of(int64_t T, int64_t S, int64_t group, int64_t D) {
   Plan p{};
   p.parts = 1;
   const int most = D > 128 ? 16 : 64;
-  const int BIG = D <= 128 && mean >= 512 ? 256 : 128;
+  const int BIG = D <= 128 && mean >= 2048 ? 256 : 128;
   if (mean <= most) {
     p.part[0] = {mean > 16 ? (int)((mean + 15) / 16) * 16 : 16, 0, INT32_MAX};
   } else if (S == 1) {
@@ -193,8 +193,8 @@ int64_t tiles_bound(const Part& p, int64_t T, int64_t S, int64_t group) {
   return T * group / p.rows + (S < T ? S : T);
 }
 
-// Parts of all split tiles of one head: fewer than twice the target (each of two parts at least has
-// more than half its share), and at most every tile's most.
+// Parts of all split tiles of one head: fewer than twice the target (a tile of one and a half shares and
+// more is cut to the nearest number of them), and at most every tile's most.
 int64_t slots_bound(const Part& p, int64_t T, int64_t S, int64_t group, int64_t HK, int64_t D, int64_t most_kv) {
   const int64_t target = (p.fill(D) + HK - 1) / HK;
   int64_t splits = (most_kv + p.unit() - 1) / p.unit();
@@ -214,7 +214,9 @@ int launch_tiled(AttnArgs a, bool bf16, bool fp8, float* workspace, size_t bytes
   for (int i = 0; i < plan.parts && status == INTENT_OK; ++i) {
     const Part& p = plan.part[i];
     const size_t need = part_bytes(p, a.T, a.S, a.group, a.HK, a.D, a.most_kv);
-    const bool split = need > 0 && workspace != nullptr && bytes >= need;
+    // one sequence's tiles all attend the same tokens: enough of them even out by themselves
+    const bool many = a.S == 1 && (int64_t)a.T * a.group / p.rows * a.HK >= 2 * p.fill(a.D);
+    const bool split = need > 0 && workspace != nullptr && bytes >= need && !many;
     AttnLaunch l{};
     a.min_rows = p.min_rows, a.max_rows = p.max_rows;
     a.target = split ? (p.fill(a.D) + a.HK - 1) / a.HK : 0;
@@ -229,8 +231,8 @@ int launch_tiled(AttnArgs a, bool bf16, bool fp8, float* workspace, size_t bytes
     l.a = a;
     l.items = (int)(tiles + a.target);
     l.joins = (int)joins;
-    // workgroups for the rows of a split tile: one for each of a mean sequence, up to 2048 in all
-    const int64_t mean = ((int64_t)a.T * a.group + a.S - 1) / a.S, room = joins > 0 ? 2048 / (joins * a.HK) : 0;
+    // workgroups for the rows of a split tile: one for each of a mean sequence, up to 1024 in all
+    const int64_t mean = ((int64_t)a.T * a.group + a.S - 1) / a.S, room = joins > 0 ? 1024 / (joins * a.HK) : 0;
     const int64_t side = mean < p.rows ? mean : p.rows;
     l.join_rows = (int)(room < 1 ? 1 : room < side ? room : side);
     if (fp8) status = bf16 ? launch_attn_bf16_fp8(l, p.rows, stream) : launch_attn_f16_fp8(l, p.rows, stream);

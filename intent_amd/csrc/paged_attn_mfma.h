@@ -518,7 +518,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
 // registers while these are worked on and stored to the other buffer behind them, so one barrier for
 // each 64 tokens.
 template <bool kBf16, bool kFp8, int D, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void attn_tile_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1) void attn_tile_kernel(const AttnArgs a) {
   constexpr int KS = D / 16, DT = D / 32, RB = row_bytes<D>();
   constexpr int CHUNKS = kFp8 ? D / 16 : D / 8;       // 16-byte loads of a token's row
   constexpr int SPREAD = kFp8 ? RB / 32 : RB / 16;    // lanes that take one (a power of two)
@@ -526,6 +526,8 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void attn_tile_kernel
   constexpr int STEP = EACH * WAVES;                  // and the workgroup
   constexpr int LOADS = STEP >= 64 ? 1 : 64 / STEP, ROWS = 32 * WAVES;
   constexpr int kTile = 64 * RB;
+  // Whether the scores of the next 64 tokens are computed during the softmax of these.
+  constexpr bool kAhead = D > 64;
   __shared__ __attribute__((aligned(16))) char lds[2][2][kTile];
   __shared__ __attribute__((aligned(16))) float scales[kFp8 ? 2 : 1][3][64];
   __shared__ int left_out;  // values that are not finite were left out of a product
@@ -682,8 +684,9 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void attn_tile_kernel
         s[u] = mfma32<kBf16>(*(const u32x4*)(keys + u * 32 * RB + (k_at ^ (i * 32))), q[i], s[u]);
   };
 
-  // Tokens t: values (and scales) in buffer j, their scores in registers; tokens t + 64: keys in buffer
-  // j ^ 1. Keys of t + 128 and values of t + 64 are under way.
+  // kAhead: of tokens t, values (and scales) in buffer j, their scores in registers; of t + 64, keys in
+  // buffer j ^ 1; values of t + 64 and keys of t + 128 under way. Else keys and values of t in buffer j,
+  // those of t + 64 under way.
   if (threadIdx.x == 0) left_out = 0;
   __syncthreads();
   f32x16 s[2];
@@ -691,20 +694,28 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void attn_tile_kernel
     if (paged) entries[0] = batch(w.begin), entries[1] = batch(w.begin + span * 64);
     load_keys(w.begin);
     load_values(w.begin);
-    store(lds[0][0], kr);
-    load_keys(w.begin + 64);
-    store_values(0, w.begin);
-    store(lds[1][0], kr);
+    if constexpr (kAhead) {
+      u32x4 second[LOADS];
+      load(second, a.k_cache, a.k_step, w.begin + 64);
+      store(lds[0][0], kr);
+      store_values(0, w.begin);
+      store(lds[1][0], second);
+    } else {
+      store(lds[0][0], kr);
+      store_values(0, w.begin);
+    }
   }
   __syncthreads();
-  if (w.begin < w.end) scores(0, s);
-  __syncthreads();  // the first keys are read: their buffer may be written
+  if constexpr (kAhead) {
+    if (w.begin < w.end) scores(0, s);
+    __syncthreads();  // the first keys are read: their buffer may be written
+  }
   int j = 0;
   for (int t = w.begin; t < w.end; t += 64, j ^= 1) {
     const bool more = t + 64 < w.end;
     if (more) {
       load_values(t + 64);
-      load_keys(t + 128);
+      load_keys(t + (kAhead ? 128 : 64));
       const int n = (t + 64 - w.begin) >> 6;
       if (paged && (n & (span - 1)) == span - 1) {  // past a batch: the one behind the other takes its place
         rarely();
@@ -714,6 +725,7 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void attn_tile_kernel
       }
     }
     if (!idle) {
+      if constexpr (!kAhead) scores(j, s);
       const char* values = lds[j][1];
       const bool masked = t < bottom.lo || t + 64 > top.hi;
       float high = -INFINITY;
@@ -762,8 +774,8 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void attn_tile_kernel
       }
       const float base = ref == -INFINITY ? 0.f : ref;
       // Sixteen steps, each with the weights of two tokens, its part of the next tokens' products with the
-      // queries (of what lies in that buffer behind the last tokens, too: not used then) and, four steps
-      // behind, of the products with these values, so that the matrix unit works through all of them.
+      // queries (kAhead; of what lies in that buffer behind the last tokens, too: not used then) and, four
+      // steps behind, of the products with these values, so that the matrix unit works through all of them.
       constexpr int S_ALL = 2 * KS, V_ALL = 4 * DT, K_AHEAD = 4, V_AHEAD = 2;
       f32x16 after[2];
 #pragma unroll
@@ -782,8 +794,10 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void attn_tile_kernel
         return u32x4{lo[0], lo[1], hi[0], hi[1]};
       };
       u32x4 p[4], kf[S_ALL], vf[V_ALL];
+      if constexpr (kAhead) {
 #pragma unroll
-      for (int n = 0; n < K_AHEAD; ++n) kf[n] = key(n);
+        for (int n = 0; n < K_AHEAD; ++n) kf[n] = key(n);
+      }
       auto products = [&](int from, int to) __attribute__((always_inline)) {
 #pragma unroll
         for (int n = 0; n < V_ALL; ++n) {
@@ -795,10 +809,12 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void attn_tile_kernel
       float sums[2] = {0.f, 0.f};
       f32x4 v_mul;
       auto step = [&](int i) __attribute__((always_inline)) {
+        if constexpr (kAhead) {
 #pragma unroll
-        for (int n = i * S_ALL / 16; n < (i + 1) * S_ALL / 16; ++n) {
-          if (n + K_AHEAD < S_ALL) kf[n + K_AHEAD] = key(n + K_AHEAD);
-          after[n & 1] = mfma32<kBf16>(kf[n], q[n >> 1], after[n & 1]);
+          for (int n = i * S_ALL / 16; n < (i + 1) * S_ALL / 16; ++n) {
+            if (n + K_AHEAD < S_ALL) kf[n + K_AHEAD] = key(n + K_AHEAD);
+            after[n & 1] = mfma32<kBf16>(kf[n], q[n >> 1], after[n & 1]);
+          }
         }
         if (i == 3) {
 #pragma unroll
@@ -822,11 +838,11 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void attn_tile_kernel
       for (int i = 0; i < 16; ++i) step(i);
       products(3 * DT, V_ALL);
       total += sums[0] + sums[1];
-      s[0] = after[0], s[1] = after[1];
+      if constexpr (kAhead) s[0] = after[0], s[1] = after[1];
     }
     if (more) {
       store_values(j ^ 1, t + 64);
-      store(lds[j][0], kr);
+      store(lds[kAhead ? j : j ^ 1][0], kr);
     }
     __syncthreads();
   }
@@ -876,28 +892,68 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void attn_tile_kernel
 // ---- the join of split tiles ---------------------------------------------------------------------
 
 // out = sum_j w_j O_j / sum_j w_j l_j, w_j = exp2(M_j - max M), over the parts of a tile in a fixed order.
-// A lane holds D / 64 columns of a row (two of 96). Up to 16 parts a wave takes a row by itself; more are
-// dealt to the four waves of a workgroup, whose sums are added in order. Each wave works out the weights
-// of 64 parts at a time, one in each lane, while its first parts are on their way.
+// Up to 16 parts, a row is D / 4 lanes of four columns, and a wave takes as many rows as it holds. More
+// parts are dealt to the four waves of a workgroup (D / 64 columns a lane), whose sums are added in
+// order; each works out the weights of 64 parts at a time, one in each lane, while its first parts are on
+// their way.
 template <bool kBf16, int D, int ROWS, int UNIT>
 __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
-  constexpr int E = (D + 63) / 64, AHEAD = 8;
+  constexpr int E = (D + 63) / 64, AHEAD = 8, FEW = 16;
+  constexpr int LANES = D == 96 ? 32 : D / 4, TOGETHER = 64 / LANES;  // lanes of a row, rows of a wave
   typedef float part __attribute__((ext_vector_type(E)));
   __shared__ part sums[4][64];
   const int head = blockIdx.x % a.HK;
   Span w;
   if (!find_span<ROWS, UNIT>(a, blockIdx.x / a.HK, true, w)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (w.splits <= FEW) {
+    const int c = lane % LANES * 4 < D ? lane % LANES * 4 : 0;
+    for (int first = (blockIdx.y * 4 + wave) * TOGETHER; first < w.rows; first += gridDim.y * 4 * TOGETHER) {
+      const int r = first + lane / LANES, row = min(r, w.rows - 1);
+      auto at = [&](int j) { return ((int64_t)(w.slot + j) * a.HK + head) * ROWS + row; };
+      f32x2 st[FEW];
+      float high = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < FEW; ++j) {
+        st[j] = f32x2{-INFINITY, 0.f};
+        if (j < w.splits) st[j] = *(const f32x2*)(a.partial_stats + at(j) * 2);
+      }
+#pragma unroll
+      for (int j = 0; j < FEW; ++j) high = fmaxf(high, st[j][0]);
+      const float base = high == -INFINITY ? 0.f : high;
+      f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+      float total = 0.f;
+#pragma unroll
+      for (int j0 = 0; j0 < FEW; j0 += 4) {
+        if (j0 < w.splits) {
+          f32x4 v[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = *(const f32x4*)(a.partial + at(min(j0 + j, w.splits - 1)) * D + c);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float keep = __builtin_amdgcn_exp2f(st[j0 + j][0] - base);
+            total += keep * st[j0 + j][1];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(keep, j0 + j < w.splits ? v[j][e] : 0.f, acc[e]);
+          }
+        }
+      }
+      const RowView rv = row_view(a, w, row);
+      const float inv = rv.hi > rv.lo ? 1.0f / total : 0.f;
+      if (r < w.rows && lane % LANES * 4 < D)
+        *(u32x2*)(out_row(a, w, head, row) + c) =
+            u32x2{pack2<kBf16>(acc[0] * inv, acc[1] * inv), pack2<kBf16>(acc[2] * inv, acc[3] * inv)};
+    }
+    return;
+  }
   const bool mine = lane * E < D;
   const int d0 = mine ? lane * E : 0;
-  const bool alone = w.splits <= 16;
-  const int ways = alone ? 1 : 4, way = alone ? 0 : wave;  // waves of a row, and this one's place
-  for (int r = alone ? blockIdx.y * 4 + wave : blockIdx.y; r < w.rows; r += alone ? gridDim.y * 4 : gridDim.y) {
-    auto at = [&](int j) __attribute__((always_inline)) { return ((int64_t)(w.slot + j) * a.HK + head) * ROWS + r; };
-    auto load = [&](int j) __attribute__((always_inline)) { return *(const part*)(a.partial + at(min(j, w.splits - 1)) * D + d0); };
+  for (int r = blockIdx.y; r < w.rows; r += gridDim.y) {
+    auto at = [&](int j) { return ((int64_t)(w.slot + j) * a.HK + head) * ROWS + r; };
+    auto load = [&](int j) { return *(const part*)(a.partial + at(min(j, w.splits - 1)) * D + d0); };
     part ahead[AHEAD];
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) ahead[i] = load(way + i * ways);
+    for (int i = 0; i < AHEAD; ++i) ahead[i] = load(wave + i * 4);
     f32x2 st = f32x2{-INFINITY, 0.f};
     if (lane < w.splits) st = *(const f32x2*)(a.partial_stats + at(lane) * 2);
     float high = st[0];
@@ -918,32 +974,29 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
       for (int off = 32; off >= 1; off >>= 1) all += __shfl_xor(all, off);
       total += all;
       const int n = min(w.splits - j0, 64);
-      auto add = [&](part v, int i) __attribute__((always_inline)) {
+      auto add = [&](part v, int i) {
         const float k = bit_cast<float>(__builtin_amdgcn_readlane(bit_cast<int>(keep), i));
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = __builtin_fmaf(k, v[e], acc[e]);
       };
-      int i = way;
+      int i = wave;
       if (j0 == 0) {
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k)
-          if (way + k * ways < n) add(ahead[k], way + k * ways);
-        i += AHEAD * ways;
+          if (wave + k * 4 < n) add(ahead[k], wave + k * 4);
+        i += AHEAD * 4;
       }
 #pragma unroll 4
-      for (; i < n; i += ways) add(load(j0 + i), i);
+      for (; i < n; i += 4) add(load(j0 + i), i);
     }
-    if (!alone) {
-      __syncthreads();
-      sums[wave][lane] = acc;
-      __syncthreads();
-      if (wave != 0) continue;
-      acc = sums[0][lane] + sums[1][lane] + sums[2][lane] + sums[3][lane];
-    }
+    __syncthreads();
+    sums[wave][lane] = acc;
+    __syncthreads();
+    if (wave != 0 || !mine) continue;
+    acc = sums[0][lane] + sums[1][lane] + sums[2][lane] + sums[3][lane];
     const RowView rv = row_view(a, w, r);
     const float inv = rv.hi > rv.lo ? 1.0f / total : 0.f;
     uint16_t* to = out_row(a, w, head, r) + d0;
-    if (!mine) continue;
     if constexpr (E == 1) *to = (uint16_t)(pack2<kBf16>(acc[0] * inv, 0.f) & 0xffffu);
     else if constexpr (E == 2) *(uint32_t*)to = pack2<kBf16>(acc[0] * inv, acc[1] * inv);
     else *(u32x2*)to = u32x2{pack2<kBf16>(acc[0] * inv, acc[1] * inv), pack2<kBf16>(acc[2] * inv, acc[3] * inv)};
