@@ -218,17 +218,28 @@ int launch(PrepArgs a, int64_t T, hipStream_t stream) {
   a.items = T * a.items_per_token;
   const int64_t blocks = (a.items + 256 / LPR - 1) / (256 / LPR);
   hipLaunchKernelGGL((attn_prep_kernel<kBf16, MODE, LPR, RPG>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
-  return intent::launch_status_fmt("attn_prep_kernel<%s%s, %d lanes, %d heads>", kBf16 ? "bf16" : "f16",
-                                   MODE == kCacheFp8 ? ", fp8 cache" : MODE == kCacheSame ? ", cache" : "", LPR, RPG);
+  static const intent::KernelName name("attn_prep_kernel<%s%s, %d lanes, %d heads>", kBf16 ? "bf16" : "f16",
+                                       MODE == kCacheFp8 ? ", fp8 cache" : MODE == kCacheSame ? ", cache" : "", LPR, RPG);
+  return intent::launch_status(name.text);
+}
+
+// Two heads to a group once one each is more lanes than twice what the GPU holds (2^19): they share the
+// table's row (8192 tokens of 32 + 8 heads of 128: 39.4 us with one, 36.7 with two, 36.5 with four; with
+// values into an f16 cache 42.9, 40.1, 42.6). Fewer tokens are a matter of latency (64 tokens into an
+// 8-bit cache: 4.0, 4.9 and 6.9 us).
+template <bool kBf16, int MODE, int LPR>
+int launch_heads(const PrepArgs& a, int64_t T, hipStream_t stream) {
+  return T * a.heads * LPR >= (int64_t)1 << 20 ? launch<kBf16, MODE, LPR, 2>(a, T, stream)
+                                               : launch<kBf16, MODE, LPR, 1>(a, T, stream);
 }
 
 template <bool kBf16, int MODE>
 int launch_lanes(const PrepArgs& a, int64_t T, hipStream_t stream) {
   const int chunks = a.D / 8;
-  if (chunks <= 8) return launch<kBf16, MODE, 8, 1>(a, T, stream);
-  if (chunks <= 16) return launch<kBf16, MODE, 16, 1>(a, T, stream);
-  if (chunks <= 32) return launch<kBf16, MODE, 32, 1>(a, T, stream);
-  return launch<kBf16, MODE, 64, 1>(a, T, stream);
+  if (chunks <= 8) return launch_heads<kBf16, MODE, 8>(a, T, stream);
+  if (chunks <= 16) return launch_heads<kBf16, MODE, 16>(a, T, stream);
+  if (chunks <= 32) return launch_heads<kBf16, MODE, 32>(a, T, stream);
+  return launch_heads<kBf16, MODE, 64>(a, T, stream);
 }
 
 // The checks that both entries share; fills the arguments they share.

@@ -30,6 +30,13 @@ int launch_status(const char* kernel);
 // Same, with a printf-formatted kernel name (template parameters).
 int launch_status_fmt(const char* fmt, ...) __attribute__((format(printf, 1, 2)));
 
+// A kernel's name, formatted once (a static of the launch): launches of a few microseconds do not format it
+// each time.
+struct KernelName {
+  char text[128];
+  explicit KernelName(const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+};
+
 // Writes `bits` (the low elem_bytes = 1, 2 or 4 bytes) to every element of a
 // rows x cols matrix with a leading stride of ld elements: the output of a
 // contraction over an empty K, which is its epilogue applied to zero.

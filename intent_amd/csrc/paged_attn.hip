@@ -139,7 +139,8 @@ template <bool kBf16, bool kFp8>
 int launch_rows(const AttnArgs& a, hipStream_t stream) {
   const int64_t blocks = ((int64_t)a.T * a.HQ + 3) / 4;
   hipLaunchKernelGGL((paged_attn_row_kernel<kBf16, kFp8>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
-  return launch_status_fmt("paged_attn_row_kernel<%s%s>", kBf16 ? "bf16" : "f16", kFp8 ? ", fp8 cache" : "");
+  static const KernelName name("paged_attn_row_kernel<%s%s>", kBf16 ? "bf16" : "f16", kFp8 ? ", fp8 cache" : "");
+  return launch_status(name.text);
 }
 
 // ---- which kernel, and into how many parts --------------------------------------------
@@ -154,7 +155,7 @@ struct Part {
   // to 8191 126, 128 and 119 us). One workgroup to a CU loses by a second round (16 sequences of five
   // drafted tokens: 28 us at 256, 34 at 512).
   int fill(int64_t D) const {
-    if (rows > 64) return rows == 256 ? 256 : 512;
+    if (rows > 64) return rows == 256 || D > 128 ? 256 : 512;
     return D > 128 ? 256 : rows * D <= 2048 ? 1536 : rows * D <= 4096 ? 512 : 256;
   }
 };
@@ -166,25 +167,31 @@ struct Plan {
 
 bool tiled(int64_t D) { return D == 64 || D == 96 || D == 128 || D == 256; }
 
-// The host knows the rows of all sequences together. Up to 64 for each on average, they go to the
-// kernel that spreads the tokens over the waves, with the tile that holds the average; beyond, each
-// sequence goes by its own: up to 32 rows there, more to the 128-row tile. Heads of 256 leave that
-// kernel registers for 16 rows only.
-Plan plan_of(int64_t T, int64_t S, int64_t group, int64_t D) {
-  const int64_t rows = T * group, mean = (rows + S - 1) / S;
+// The host knows the extents only. Sequences of one new token each, one sequence, or as many new tokens as
+// equal chunks make: all alike, and the kernel that spreads the tokens over the waves takes up to 64 rows
+// of them in the tile that holds one (heads of 256 leave it registers for 16), the other kernel more. Any
+// other batch may mix decoding sequences with chunks: beyond 2048 rows in all, each sequence goes by its
+// own rows to one of the two, which a chunk of 900 tokens among 63 decoding sequences repays several
+// times; fewer rows do not repay the launches (12 sequences of 1 to 24 tokens, 460 rows: 19 us in one, 32
+// in two).
+//
+// More than 64 rows: with fewer than 22 tiles of 128 the other kernel's 64 rows, whose waves share the tokens,
+// still fill more of the GPU (397 rows of two heads over 594 tokens: 17 us, 29 in tiles of 128; 758 x 4 of one
+// head over 917 21 and 21; 512 x 4 of eight over 512 22 and 20). Tiles of 256 halve what is loaded for a row
+// but need one and a half rounds of them to even out (4096 x 4 rows of eight heads over 4096: 157 us, 163 in
+// tiles of 128; 2048 x 4 over 2048: 71 and 59).
+Plan plan_of(int64_t T, int64_t S, int64_t HK, int64_t group, int64_t D) {
+  const int64_t mean = (T * group + S - 1) / S;
+  const int most = D > 128 ? 16 : 64, few = D > 128 || group <= 16 ? 16 : 32;
+  const int tile = D > 128 || T * group * HK < 384 * 256 ? (D > 128 || T * group * HK >= 22 * 128 ? 128 : 64) : 256;
   Plan p{};
-  p.parts = 1;
-  const int most = D > 128 ? 16 : 64;
-  const int BIG = D <= 128 && mean >= 2048 ? 256 : 128;
-  if (mean <= most) {
-    p.part[0] = {mean > 16 ? (int)((mean + 15) / 16) * 16 : 16, 0, INT32_MAX};
-  } else if (S == 1) {
-    p.part[0] = {BIG, 0, INT32_MAX};
-  } else {
+  if (T > S && T % S != 0 && T * group > 2048) {
     p.parts = 2;
-    const int few = D > 128 ? 16 : 32;
-    p.part[0] = {BIG, few, INT32_MAX};
+    p.part[0] = {tile, few, INT32_MAX};
     p.part[1] = {few, 0, few};
+  } else {
+    p.parts = 1;
+    p.part[0] = {mean <= 16 ? 16 : mean <= most ? (int)((mean + 15) / 16) * 16 : tile, 0, INT32_MAX};
   }
   return p;
 }
@@ -209,7 +216,7 @@ size_t part_bytes(const Part& p, int64_t T, int64_t S, int64_t group, int64_t HK
 }
 
 int launch_tiled(AttnArgs a, bool bf16, bool fp8, float* workspace, size_t bytes, hipStream_t stream) {
-  const Plan plan = plan_of(a.T, a.S, a.group, a.D);
+  const Plan plan = plan_of(a.T, a.S, a.HK, a.group, a.D);
   int status = INTENT_OK;
   for (int i = 0; i < plan.parts && status == INTENT_OK; ++i) {
     const Part& p = plan.part[i];
@@ -248,7 +255,7 @@ extern "C" size_t intent_paged_attention_workspace_size(int64_t T, int64_t HQ, i
   if (T <= 0 || HQ <= 0 || HK <= 0 || S <= 0 || HQ % HK || table_width <= 0 || page_size <= 0 || !tiled(D) ||
       table_width > kMostTokens / page_size || HQ > 65536 || T * HQ >= ((int64_t)1 << 26))
     return 0;
-  const Plan plan = plan_of(T, S, HQ / HK, D);
+  const Plan plan = plan_of(T, S, HK, HQ / HK, D);
   size_t most = 0;
   for (int i = 0; i < plan.parts; ++i) {
     const size_t need = part_bytes(plan.part[i], T, S, HQ / HK, HK, D, table_width * page_size);

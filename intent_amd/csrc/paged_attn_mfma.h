@@ -1014,14 +1014,15 @@ int launch(const AttnLaunch& l, hipStream_t stream) {
   else
     hipLaunchKernelGGL((attn_tile_kernel<kBf16, kFp8, D, ROWS / 32>), dim3(l.items * heads), dim3(ROWS * 2), 0, stream,
                        l.a);
-  const int status = launch_status_fmt("attn_%s_kernel<%s%s, D %d, %d rows%s>", kFew ? "rows" : "tile",
-                                       kBf16 ? "bf16" : "f16", kFp8 ? ", fp8 cache" : "", D, ROWS,
-                                       l.joins > 0 ? ", splits" : "");
+  static const KernelName name("attn_%s_kernel<%s%s, D %d, %d rows>", kFew ? "rows" : "tile", kBf16 ? "bf16" : "f16",
+                               kFp8 ? ", fp8 cache" : "", D, ROWS);
+  const int status = launch_status(name.text);
   if (status != INTENT_OK || l.joins == 0) return status;
   hipLaunchKernelGGL((attn_join_kernel<kBf16, D, ROWS, kFew ? 128 : 64>), dim3(l.joins * heads, l.join_rows), dim3(256),
                      0, stream, l.a);
-  return launch_status_fmt("attn_%s_kernel<%s%s, D %d, %d rows, splits>", kFew ? "rows" : "tile", kBf16 ? "bf16" : "f16",
-                           kFp8 ? ", fp8 cache" : "", D, ROWS);
+  static const KernelName joined("attn_%s_kernel<%s%s, D %d, %d rows, splits>", kFew ? "rows" : "tile",
+                                 kBf16 ? "bf16" : "f16", kFp8 ? ", fp8 cache" : "", D, ROWS);
+  return launch_status(joined.text);
 }
 
 template <bool kBf16, bool kFp8, int D>

@@ -36,6 +36,13 @@ int launch_status_fmt(const char* fmt, ...) {
   return launch_status(name);
 }
 
+KernelName::KernelName(const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(text, sizeof(text), fmt, ap);
+  va_end(ap);
+}
+
 }  // namespace intent
 
 extern "C" int intent_amd_abi_version(void) { return INTENT_AMD_ABI_VERSION; }

@@ -104,10 +104,12 @@ def ref_attention(q, k_cache, v_cache, k_scales, v_scales, table, q_offsets, kv_
             qh, k, v = q[start:start + n, h].double(), rows[0][:, h // (HQ // HK)], rows[1][:, h // (HQ // HK)]
             logit = (qh @ k.T * scale).masked_fill(~seen, -math.inf)
             w = torch.softmax(logit, -1).masked_fill(~seen, 0.0)  # no seen token: a row of NaN, masked to zeros
-            # what a row does not see does not reach it, whatever it holds
-            o = torch.stack([w[i, seen[i]] @ v[seen[i]] for i in range(n)])
-            size = torch.stack([w[i, seen[i]] @ v[seen[i]].abs() for i in range(n)])
-            big = torch.stack([v[seen[i]].abs().amax(0) if seen[i].any() else v.new_zeros(D) for i in range(n)])
+            if v.isfinite().all():
+                o, size, big = w @ v, w @ v.abs(), v.abs().amax(0)
+            else:  # what a row does not see does not reach it, whatever it holds
+                o = torch.stack([w[i, seen[i]] @ v[seen[i]] for i in range(n)])
+                size = torch.stack([w[i, seen[i]] @ v[seen[i]].abs() for i in range(n)])
+                big = torch.stack([v[seen[i]].abs().amax(0) if seen[i].any() else v.new_zeros(D) for i in range(n)])
             off = (qh.abs() @ k.abs().nan_to_num(0, 0, 0).T * abs(scale)).masked_fill(~seen, 0).amax(-1, keepdim=True)
             many = seen.sum(-1, keepdim=True).double()
             out[start:start + n, h] = o
@@ -332,6 +334,19 @@ ATTENTION_CASES = [
     ("f16", False, [(3, 90), (1, 150)], 2, 1, 512, 4, True, 0),
     ("bf16", False, [(1, 3000), (1, 2500)], 8, 1, 128, 16, True, 0),
     ("f16", False, [(300, 1200)], 8, 1, 128, 16, True, 0),
+    # equal chunks of 48 and 64 rows, pages smaller than a load, and chunks of eight waves
+    ("bf16", False, [(6, 300), (6, 70)], 28, 4, 128, 16, True, 0),
+    ("f16", True, [(8, 100), (8, 900)], 16, 2, 64, 2, True, 0),
+    ("f16", True, [(7, 450), (9, 66)], 14, 2, 96, 32, True, 0),
+    ("bf16", False, [(70, 700)], 4, 2, 128, 2, True, 0),
+    ("f16", True, [(100, 1000)], 4, 2, 128, 4, True, 60),
+    ("f16", True, [(600, 700)], 8, 2, 64, 16, True, 0),
+    ("bf16", True, [(260, 900)], 16, 2, 128, 64, True, 0),
+    ("f16", False, [(800, 900)], 128, 1, 64, 16, True, 0),
+    ("bf16", True, [(800, 860)], 128, 1, 96, 32, True, 300),
+    ("f16", True, [(1100, 1130), (1, 400)], 96, 1, 128, 16, True, 0),
+    ("bf16", False, [(300, 500), (400, 420)], 8, 1, 96, 16, True, 0),
+    ("f16", False, [(40, 300), (1, 500), (2, 30), (90, 90)], 4, 2, 256, 32, True, 0),
     ("bf16", False, [(1, 40 + 13 * i) for i in range(70)] + [(0, 5)] * 60 + [(2, 30)], 4, 2, 64, 16, True, 0),
 ]
 
@@ -523,6 +538,28 @@ def test_paged_attention_repeats_bit_for_bit(gpu, lens):
     first = _run_attention(inputs, "bf16", False, 0.0884, True, 0)
     for _ in range(3):
         assert torch.equal(first, _run_attention(inputs, "bf16", False, 0.0884, True, 0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,HQ,kv,PAGE,D,fp8", [(1, 4, 20000, 16, 64, False), (1, 2, 17000, 64, 128, True),
+                                                  (70, 2, 9500, 64, 64, False), (40, 4, 13000, 16, 128, True),
+                                                  (130, 1, 5000, 16, 256, False)])
+def test_paged_attention_without_a_workspace(gpu, new, HQ, kv, PAGE, D, fp8):
+    """The entry with no workspace runs unsplit, over tables longer than what a wave keeps of one; and the
+    split call agrees with it."""
+    inputs = _attention_inputs(31, "f16", fp8, [(new, kv)], HQ, 1, D, PAGE, poison=False)
+    q, k, v, ks, vs, table, offsets, lens = _cuda(*inputs)
+    out = torch.full_like(q, float("nan"))
+    scales = (ks.data_ptr(), ks.stride(0), vs.data_ptr(), vs.stride(0)) if fp8 else (None, 0, None, 0)
+    _native.call("intent_paged_attention", q.data_ptr(), new, HQ, q.stride(0), 0, int(fp8), k.data_ptr(), k.stride(0),
+                 v.data_ptr(), v.stride(0), *scales, k.shape[0], 1, PAGE, D, table.data_ptr(), 1, table.shape[1],
+                 table.stride(0), offsets.data_ptr(), lens.data_ptr(), D ** -0.5, 1, 0, out.data_ptr(), out.stride(0),
+                 None, 0, torch.cuda.current_stream().cuda_stream)
+    want, tol = ref_attention(*inputs, D ** -0.5, True, 0)
+    _close(out, want, tol)
+    assert "splits" not in _native.last_kernel()
+    _close(_run_attention(inputs, "f16", fp8, D ** -0.5, True, 0), want, tol)
+    assert "splits" in _native.last_kernel()
 
 
 # ---- together --------------------------------------------------------------------------
