@@ -16,6 +16,10 @@
 // hold one chunk each, so a row's sums stay inside a DPP row or a half-wave and a rotation
 // partner is a lane of the same group. A group takes RPG heads of one token, which share its
 // cosines and sines and whose loads are all issued before the first is used.
+//
+// Bound by memory for many tokens: 8192 of 32 + 8 heads of 128 (172 MB) take 36.7 us, 4.7 TB/s, with values
+// into an f16 cache (206 MB) 40.1 us, 5.1 TB/s, the rate of a large copy; 64 tokens 4 us, a chain of
+// latencies (position, table row, store).
 #include "common.h"
 #include "internal.h"
 
@@ -255,9 +259,9 @@ int check_heads(PrepArgs& a, const void* q, int64_t T, int64_t HQ, int64_t q_ld,
   INTENT_REQUIRE(D % 8 == 0 && D <= 512 && R % 16 == 0, INTENT_ERR_UNSUPPORTED,
                  "D=%lld must be a multiple of 8 up to 512 and R=%lld a multiple of 16", (long long)D, (long long)R);
   // a lane group of at most 64 for each head: the grid's work items stay below 2^32
-  INTENT_REQUIRE(T * (HQ + 2 * HK) < ((int64_t)1 << 26), INTENT_ERR_UNSUPPORTED,
+  INTENT_REQUIRE(T * (HQ + 2 * HK) < ((int64_t)1 << 25), INTENT_ERR_UNSUPPORTED,
                  "T * (HQ + 2 HK) = %lld heads exceed the %lld a launch covers", (long long)(T * (HQ + 2 * HK)),
-                 (long long)((int64_t)1 << 26));
+                 (long long)((int64_t)1 << 25));
   if (T == 0 || D == 0) return INTENT_OK;
   INTENT_REQUIRE((HQ == 0 || (q && q_out)) && (HK == 0 || k), INTENT_ERR_INVALID_ARGUMENT, "null pointer argument");
   INTENT_REQUIRE((HQ == 0 || ((T == 1 || (q_ld >= HQ * D && q_out_ld >= HQ * D)))) && (HK == 0 || T == 1 || k_ld >= HK * D),

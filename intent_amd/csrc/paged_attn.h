@@ -33,6 +33,7 @@ struct AttnArgs {
   // work list of the tiled kernels (find_span)
   int min_rows, max_rows;  // sequences with more rows (new tokens times group) than min, up to max
   int target;              // workgroups for each cached head that tiles are split for; 0: none
+  int slots;               // parts of split tiles of one head that the workspace holds
   float* partial;          // [slot][HK][tile rows][D] unnormalised sums, then [slot][HK][tile rows][2]
   float* partial_stats;
 };
@@ -85,14 +86,13 @@ struct Extent {
 
 template <int ROWS, int UNIT>
 INTENT_DEVICE Extent extent_of(const AttnArgs& a, int s) {
-  Extent e{};
-  if (s >= a.S) return e;
-  e.q = sequence_of(a, s);
+  Extent e;
+  e.q = sequence_of(a, min(s, a.S - 1));
   const int64_t rows = (int64_t)e.q.count * a.group;
-  if (rows <= a.min_rows || rows > a.max_rows) return e;
-  e.tiles = (int)((rows + ROWS - 1) / ROWS);
+  const bool listed = s < a.S && rows > a.min_rows && rows <= a.max_rows;
   const int lo = first_seen(a, e.q.kv - e.q.count) & ~63;
-  e.units = (e.q.kv - lo + UNIT - 1) / UNIT;
+  e.tiles = listed ? (int)((rows + ROWS - 1) / ROWS) : 0;
+  e.units = listed ? (e.q.kv - lo + UNIT - 1) / UNIT : 0;
   return e;
 }
 
@@ -119,6 +119,30 @@ INTENT_DEVICE float wave_total(float v) {
   return out[0];
 }
 
+// Rows and tokens of share `local` of a sequence's (r.s, r.q and r.splits are set; with `joins`, of its
+// tiles), whose parts begin at `slot`.
+template <int ROWS, int UNIT>
+INTENT_DEVICE bool span_of(const AttnArgs& a, int tiles, int local, int slot, bool joins, Span& r) {
+  r.slot = slot + (joins ? local * r.splits : local);
+  const int turn = joins ? local : (int)((uint32_t)local / (uint32_t)r.splits);
+  const int split = joins ? 0 : local - turn * r.splits;
+  // offsets that overlap may count up to anything: nothing outside the rows and the workspace then
+  if (local < 0 || turn >= tiles || (r.splits > 1 && (r.slot < 0 || r.slot >= a.slots))) return false;
+  if (joins && r.slot + r.splits > a.slots) return false;
+  r.row0 = (tiles - 1 - turn) * ROWS;
+  r.rows = min(ROWS, r.q.count * a.group - r.row0);
+  const int before = r.q.kv - r.q.count;
+  const int p0 = before + (int)((uint32_t)r.row0 / (uint32_t)a.group);
+  const int p1 = before + (int)((uint32_t)(r.row0 + r.rows - 1) / (uint32_t)a.group);
+  const int lo = first_seen(a, p0) & ~63, hi = end_seen(a, p1, r.q.kv);
+  const uint32_t units = hi > lo ? (uint32_t)(hi - lo + UNIT - 1) / UNIT : 0u;
+  const uint32_t each = units / (uint32_t)r.splits, more = units - each * (uint32_t)r.splits;
+  const uint32_t from = each * split + min((uint32_t)split, more), to = from + each + ((uint32_t)split < more ? 1u : 0u);
+  r.begin = lo + (int)from * UNIT;
+  r.end = min(hi, lo + (int)to * UNIT);
+  return true;
+}
+
 // Finds share `item` of one head's list: the sequences in order, each with its row tiles from the last
 // (which sees most) to the first, each tile in `splits` parts of its tokens. The parts are sized so
 // that all sequences together give about a.target of them: units / chunk of each, chunk = the units
@@ -126,53 +150,62 @@ INTENT_DEVICE float wave_total(float v) {
 // sized by it), but for 64 and more new rows no fewer than 8 units (a join costs as many). With `joins`, the list of the tiles that are split. Every wave does it by itself: no
 // plan is kept, so a captured call follows lengths that change. The counts of one list fit 32 bits (the
 // host bounds the grid).
-template <int ROWS, int UNIT>
-INTENT_DEVICE bool find_span(const AttnArgs& a, int item, bool joins, Span& r) {
+//
+// Lanes take a sequence each of 64, or of AT times 64 whose extents are all loaded before the first is
+// used: 2048 sequences of 512 tokens take 1245 us with 64 at a time, 935 with 256; one sequence takes 7.1
+// us with 64 and would wait for three useless loads with 256.
+template <int ROWS, int UNIT, int AT>
+INTENT_DEVICE bool find_span_by(const AttnArgs& a, int item, bool joins, Span& r) {
   const int lane = threadIdx.x & 63;
-  const Extent first = extent_of<ROWS, UNIT>(a, lane);
+  Extent e[AT];
+#pragma unroll
+  for (int i = 0; i < AT; ++i) e[i] = extent_of<ROWS, UNIT>(a, i * 64 + lane);
   int chunk = INT32_MAX;
   if (a.target > 0) {
-    float all = (float)first.tiles * (float)first.units;
-    for (int s0 = 64; s0 < a.S; s0 += 64) {
-      const Extent e = extent_of<ROWS, UNIT>(a, s0 + lane);
-      all += (float)e.tiles * (float)e.units;
+    float all = 0.f;
+#pragma unroll
+    for (int i = 0; i < AT; ++i) all += (float)e[i].tiles * (float)e[i].units;
+    for (int s0 = AT * 64; s0 < a.S; s0 += AT * 64) {
+      Extent f[AT];
+#pragma unroll
+      for (int i = 0; i < AT; ++i) f[i] = extent_of<ROWS, UNIT>(a, s0 + i * 64 + lane);
+#pragma unroll
+      for (int i = 0; i < AT; ++i) all += (float)f[i].tiles * (float)f[i].units;
     }
     chunk = (int)fminf(wave_total(all) * (1.0f + 0x1p-12f) / (float)a.target, 1.0e9f) + 1;
     if (ROWS > 64) chunk = max(chunk, 8);
   }
   int base = 0, slots = 0;  // shares, and slots of split tiles, before sequence s0
-  for (int s0 = 0; s0 < a.S; s0 += 64) {
-    const Extent e = s0 == 0 ? first : extent_of<ROWS, UNIT>(a, s0 + lane);
-    const uint32_t near = ((uint32_t)e.units + (uint32_t)chunk / 2u) / (uint32_t)chunk;  // to the nearest
-    const int splits = near > 1u ? min((int)near, kMostSplits) : 1;
-    const int parts = e.tiles * splits, kept = splits > 1 ? parts : 0;
-    const int mine = joins ? (splits > 1 ? e.tiles : 0) : parts;
-    const int up = wave_prefix(mine) + base, kept_up = wave_prefix(kept) + slots;
-    const uint64_t past = __ballot(up > item);
-    if (past) {
-      const int at = __builtin_ctzll(past);
-      r.s = s0 + at;
-      r.q.start = lane_value(e.q.start, at), r.q.count = lane_value(e.q.count, at), r.q.kv = lane_value(e.q.kv, at);
-      r.splits = lane_value(splits, at);
-      const int tiles = lane_value(e.tiles, at);
-      const int local = item - lane_value(up - mine, at);
-      r.slot = lane_value(kept_up - kept, at) + (joins ? local * r.splits : local);
-      const int turn = joins ? local : (int)((uint32_t)local / (uint32_t)r.splits), split = joins ? 0 : local - turn * r.splits;
-      r.row0 = (tiles - 1 - turn) * ROWS;
-      r.rows = min(ROWS, r.q.count * a.group - r.row0);
-      const int p0 = r.q.kv - r.q.count + (int)((uint32_t)r.row0 / (uint32_t)a.group);
-      const int p1 = r.q.kv - r.q.count + (int)((uint32_t)(r.row0 + r.rows - 1) / (uint32_t)a.group);
-      const int lo = first_seen(a, p0) & ~63, hi = end_seen(a, p1, r.q.kv);
-      const uint32_t units = hi > lo ? (uint32_t)(hi - lo + UNIT - 1) / UNIT : 0u;
-      const uint32_t each = units / (uint32_t)r.splits, more = units - each * (uint32_t)r.splits;
-      const uint32_t from = each * split + min((uint32_t)split, more), to = from + each + ((uint32_t)split < more ? 1u : 0u);
-      r.begin = lo + (int)from * UNIT;
-      r.end = min(hi, lo + (int)to * UNIT);
-      return true;
+  for (int s0 = 0;;) {
+#pragma unroll
+    for (int i = 0; i < AT; ++i) {
+      const uint32_t near = ((uint32_t)e[i].units + (uint32_t)chunk / 2u) / (uint32_t)chunk;  // to the nearest
+      const int splits = near > 1u ? min((int)near, kMostSplits) : 1;
+      const int parts = e[i].tiles * splits, kept = splits > 1 ? parts : 0;
+      const int mine = joins ? (splits > 1 ? e[i].tiles : 0) : parts;
+      const int up = wave_prefix(mine) + base, kept_up = wave_prefix(kept) + slots;
+      const uint64_t past = __ballot(up > item);
+      if (past) {
+        const int at = __builtin_ctzll(past);
+        r.s = s0 + i * 64 + at;
+        r.q.start = lane_value(e[i].q.start, at), r.q.count = lane_value(e[i].q.count, at);
+        r.q.kv = lane_value(e[i].q.kv, at);
+        r.splits = lane_value(splits, at);
+        const int local = item - lane_value(up - mine, at), slot = lane_value(kept_up - kept, at);
+        return span_of<ROWS, UNIT>(a, lane_value(e[i].tiles, at), local, slot, joins, r);
+      }
+      base = lane_value(up, 63), slots = lane_value(kept_up, 63);
     }
-    base = lane_value(up, 63), slots = lane_value(kept_up, 63);
+    s0 += AT * 64;
+    if (s0 >= a.S) return false;
+#pragma unroll
+    for (int i = 0; i < AT; ++i) e[i] = extent_of<ROWS, UNIT>(a, s0 + i * 64 + lane);
   }
-  return false;
+}
+template <int ROWS, int UNIT>
+INTENT_DEVICE bool find_span(const AttnArgs& a, int item, bool joins, Span& r) {
+  if (a.S <= 64) return find_span_by<ROWS, UNIT, 1>(a, item, joins, r);
+  return find_span_by<ROWS, UNIT, 4>(a, item, joins, r);
 }
 
 // Page of token t (t < most_kv) of sequence s.

@@ -227,14 +227,15 @@ int launch_tiled(AttnArgs a, bool bf16, bool fp8, float* workspace, size_t bytes
     AttnLaunch l{};
     a.min_rows = p.min_rows, a.max_rows = p.max_rows;
     a.target = split ? (p.fill(a.D) + a.HK - 1) / a.HK : 0;
+    a.slots = split ? (int)slots_bound(p, a.T, a.S, a.group, a.HK, a.D, a.most_kv) : 0;
     a.partial = workspace;
-    a.partial_stats = split ? workspace + slots_bound(p, a.T, a.S, a.group, a.HK, a.D, a.most_kv) * a.HK * p.rows * a.D : nullptr;
+    a.partial_stats = split ? workspace + (int64_t)a.slots * a.HK * p.rows * a.D : nullptr;
     const int64_t tiles = tiles_bound(p, a.T, a.S, a.group);
     const int64_t joins = split ? (tiles < a.target ? tiles : a.target) : 0;
-    // 256-lane workgroups: the grid's work items stay below 2^32
-    INTENT_REQUIRE((tiles + a.target) * a.HK < ((int64_t)1 << 24), INTENT_ERR_UNSUPPORTED,
+    // workgroups of 256 or 512 lanes: the grid's work items stay below 2^32
+    INTENT_REQUIRE((tiles + a.target) * a.HK < ((int64_t)1 << 23), INTENT_ERR_UNSUPPORTED,
                    "%lld tiles of %d heads exceed the %lld workgroups that a launch covers", (long long)tiles, a.HK,
-                   (long long)((int64_t)1 << 24));
+                   (long long)((int64_t)1 << 23));
     l.a = a;
     l.items = (int)(tiles + a.target);
     l.joins = (int)joins;
@@ -253,7 +254,7 @@ int launch_tiled(AttnArgs a, bool bf16, bool fp8, float* workspace, size_t bytes
 extern "C" size_t intent_paged_attention_workspace_size(int64_t T, int64_t HQ, int64_t HK, int64_t D, int64_t S,
                                                         int64_t table_width, int64_t page_size) {
   if (T <= 0 || HQ <= 0 || HK <= 0 || S <= 0 || HQ % HK || table_width <= 0 || page_size <= 0 || !tiled(D) ||
-      table_width > kMostTokens / page_size || HQ > 65536 || T * HQ >= ((int64_t)1 << 26))
+      table_width > kMostTokens / page_size || HQ > 65536 || T * HQ >= ((int64_t)1 << 25))
     return 0;
   const Plan plan = plan_of(T, S, HK, HQ / HK, D);
   size_t most = 0;
@@ -290,9 +291,11 @@ extern "C" int intent_paged_attention(const void* q, int64_t T, int64_t HQ, int6
   INTENT_REQUIRE(!any || table_width <= kMostTokens / page_size, INTENT_ERR_UNSUPPORTED,
                  "a table of %lld pages of %lld tokens exceeds 2^30 tokens", (long long)table_width,
                  (long long)page_size);
-  // one wave for each row of a head: the grid's work items stay below 2^32
-  INTENT_REQUIRE(T * HQ < ((int64_t)1 << 26), INTENT_ERR_UNSUPPORTED,
-                 "T * HQ = %lld rows exceed the %lld a launch covers", (long long)(T * HQ), (long long)((int64_t)1 << 26));
+  INTENT_REQUIRE(!any || HK <= UINT32_MAX / page_size, INTENT_ERR_UNSUPPORTED, "pages of %lld tokens of %lld heads",
+                 (long long)page_size, (long long)HK);
+  // at most a wave for each row of a head: the grid's work items stay below 2^32
+  INTENT_REQUIRE(T * HQ < ((int64_t)1 << 25), INTENT_ERR_UNSUPPORTED,
+                 "T * HQ = %lld rows exceed the %lld a launch covers", (long long)(T * HQ), (long long)((int64_t)1 << 25));
   INTENT_REQUIRE(q && out && q_offsets && kv_lens && (!any || (k_cache && v_cache && page_table)) &&
                      (!any || !cache_is_fp8 || (k_scales && v_scales)),
                  INTENT_ERR_INVALID_ARGUMENT, "null pointer argument");

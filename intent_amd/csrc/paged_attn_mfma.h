@@ -16,9 +16,10 @@
 // scale, and only the sum of weights takes exp2(t - M) by itself. The codes are exact in 16 bits.
 //
 // A weight of zero does not keep an infinity or NaN out of a product. Values of tokens that no row of a
-// tile sees (pages behind a sequence's end hold anything) are set to zero; where rows of a tile see different tokens (the last of a chunk, the
-// first of a window), values (and scales) that are not finite go into the product as zeros, and once the loop is
-// over they are added to the rows that see them (which has them infinite or NaN).
+// tile sees (pages behind a sequence's end hold anything) are set to zero; where rows of a tile see
+// different tokens (the last of a chunk, the first of a window), values and scales that are not finite
+// go into the product as zeros, and once the loop is over they are added to the rows that see them, which
+// makes those infinite or NaN.
 #pragma once
 
 #include "paged_attn.h"
@@ -32,7 +33,6 @@ constexpr float kRise = 8.0f;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
 
 // A cached token's row or scale: global addresses, so that the loads count on vmcnt alone.
 typedef const __attribute__((address_space(1))) char* global_bytes;
@@ -40,11 +40,11 @@ INTENT_DEVICE global_bytes as_global(const void* p) { return (global_bytes)p; }
 // Rows (of kRowBytes) of a head from token t on, t and the page uniform or not.
 template <int kRowBytes>
 INTENT_DEVICE global_bytes cached_rows(const AttnArgs& a, const void* base, uint32_t page, uint32_t step, int head, int t) {
-  const uint32_t row = (uint32_t)((head << a.page_shift) + (t & ((1 << a.page_shift) - 1)));
+  const uint32_t row = ((uint32_t)head << a.page_shift) + ((uint32_t)t & ((1u << a.page_shift) - 1u));
   return as_global(base) + ((uint64_t)page * step + (uint64_t)row * (kRowBytes / 16)) * 16;
 }
 INTENT_DEVICE global_bytes cached_scales(const AttnArgs& a, const float* base, uint32_t page, uint32_t step, int head, int t) {
-  const uint32_t row = (uint32_t)((head << a.page_shift) + (t & ((1 << a.page_shift) - 1)));
+  const uint32_t row = ((uint32_t)head << a.page_shift) + ((uint32_t)t & ((1u << a.page_shift) - 1u));
   return as_global(base) + ((uint64_t)page * step + row) * 4;
 }
 INTENT_DEVICE float load_float(global_bytes p) { return *(const __attribute__((address_space(1))) float*)p; }
@@ -124,7 +124,7 @@ INTENT_DEVICE u32x2 read_transposed(const char* lds) {
 // Rows of LDS tiles are a power of two of bytes (RB); the 16-byte chunk c of token t is kept at
 // c ^ swizzle(t). LDS has 64 banks of 4 bytes, so that 16 lanes of a 16-byte access and 32 of an 8-byte
 // one have to lie apart in 256 bytes: one chunk of 16 consecutive tokens (16 bytes each), and what a
-// transposing read takes of 4 tokens (64 bytes each, the 128-row kernel) or of 8 (32 bytes each, the
+// transposing read takes of 4 tokens (64 bytes each, the kernel of many rows) or of 8 (32 bytes each, the
 // other). Rows of 128 bytes alternate between the halves of the banks by themselves.
 template <int RB, bool kTileKernel>
 INTENT_DEVICE int swizzle(int t) {
@@ -143,8 +143,8 @@ INTENT_DEVICE void wave_lds_order() {
   __builtin_amdgcn_wave_barrier();
 }
 
-// max(log2(scale), -100): the bound keeps exp2(t - M) finite beside tokens of zeros.
-INTENT_DEVICE float scale_exponent(float v) { return fmaxf(__builtin_amdgcn_logf(v), -100.0f); }
+// max(log2|scale|, -100): the bound keeps exp2(t - M) finite beside tokens of zeros.
+INTENT_DEVICE float scale_exponent(float v) { return fmaxf(__builtin_amdgcn_logf(fabsf(v)), -100.0f); }
 
 // Where one query row of a tile (column r of S^T) stands: the tokens lo <= t < hi that it sees.
 struct RowView {
@@ -189,12 +189,18 @@ INTENT_DEVICE float sum_across32(float v) {
 
 // ---- few rows: 16 * MT of them, the tokens over the waves -----------------------------------------
 
-// A wave takes 32 tokens at a time, four apart from its next: keys straight into the first product's
-// left operand (a lane holds 8 or 16 of a token's D), values through its own LDS rows; no barrier until
-// the four waves' results are joined. Keys and values of the next 32 tokens are under way during the
-// softmax and the second product, and the page ids of the ones after them.
+// A wave takes 32 tokens of each 128: keys straight into the first product's left operand (a lane holds 8
+// or 16 of a token's D), values through its own LDS rows; no barrier until the four waves' results are
+// joined. Keys and values of its next 32 tokens are under way during the softmax and the second product.
+//
+// Bound by the reads of the cache: with 16 rows of heads of 128 three workgroups to a CU keep 12 waves of
+// 16 KB (8 KB of 8-bit) under way. Four sequences of 60000 to 131000 tokens, 32 heads sharing 8 (1.42 GB):
+// 242 us, 5.9 TB/s, where a large copy moves 5.1; 64 of 300 to 8191 tokens in 8 bits (645 MB): 124 us, 5.2
+// TB/s, the lengths being uneven. One sequence of 4096 tokens (17 MB) is a chain of latencies, 7 us and 4
+// for the join.
 template <bool kBf16, bool kFp8, int D, int MT>
-__global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 256 ? 2 : 1) void attn_rows_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 256 ? 2 : 1)
+    void attn_rows_kernel(const AttnArgs a) {
   constexpr int KS = D / 32, DT = D / 16, RB = row_bytes<D>();
   constexpr bool kWide = !kFp8 || D % 64 == 0;         // 16 bytes a lane and load, else 8 codes
   constexpr int LOADS = kFp8 && kWide ? D / 64 : KS;   // loads of a token's row
@@ -429,10 +435,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
         for (int r = 0; r < 4; ++r) {
           const float e = __builtin_amdgcn_exp2f(kFp8 ? s[m][u][r] - base : __builtin_fmaf(s[m][u][r], scale, -base));
           total[m] += e;
-          wt[u][r] = e;
-          if constexpr (kFp8) {
-            wt[u][r] = e * v_mul[u][r];
-          }
+          wt[u][r] = kFp8 ? e * v_mul[u][r] : e;
         }
       }
       p[m] = u32x4{pack2<kBf16>(wt[0][0], wt[0][1]), pack2<kBf16>(wt[0][2], wt[0][3]), pack2<kBf16>(wt[1][0], wt[1][1]),
@@ -512,13 +515,24 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
   }
 }
 
-// ---- many rows: 128, 32 to a wave, all of them over the same tokens ----------------------------------
+// ---- many rows: 128 or 256, 32 to a wave, all of them over the same tokens ----------------------------
 
 // 64 tokens of keys and values in LDS at a time, in two buffers: the next ones are loaded into
 // registers while these are worked on and stored to the other buffer behind them, so one barrier for
 // each 64 tokens.
+//
+// The matrix unit and the softmax have about the same to do for 32 rows and 64 tokens of heads of 128: 32
+// MFMAs of 32 cycles, and 180 vector instructions, of which 32 exponentials at a quarter of the rate. So the
+// next tokens' products with the queries are issued between the exponentials of these, which needs the
+// scores of both: heads of 64, whose products are half as long, do better with three waves to a SIMD and
+// without (1925 tokens in 24 sequences over a window of 1000: 24 us against 29). Prefill of 4096 tokens,
+// 32 heads sharing 8 (137 GFLOP): 152 to 161 us, 850 to 900 TFLOP/s, where the library's product of
+// 8192^3 reaches 1200; 3696 tokens in two chunks over 10000 to 18000 in 8 bits 1115 to 1170 us, 780 to 820
+// TFLOP/s. What is left: with the loads of the cache taken away it takes 140 us, with the vector work
+// 117, with the products 111; each wave's own chain, not one unit, sets the time.
 template <bool kBf16, bool kFp8, int D, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1) void attn_tile_kernel(const AttnArgs a) {
+__global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
+    void attn_tile_kernel(const AttnArgs a) {
   constexpr int KS = D / 16, DT = D / 32, RB = row_bytes<D>();
   constexpr int CHUNKS = kFp8 ? D / 16 : D / 8;       // 16-byte loads of a token's row
   constexpr int SPREAD = kFp8 ? RB / 32 : RB / 16;    // lanes that take one (a power of two)
@@ -569,8 +583,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1) void at
   const bool paged = (1 << a.page_shift) >= EACH;
   const int chunk = load_chunk < CHUNKS ? load_chunk : 0;
   const uint32_t lane_at = (lane / SPREAD) * (D * kBytes) + chunk * 16;
-  // The table's entries of the next `span` times 64 tokens, one in each lane, in two batches (a vector
-  // load for each: scalar loads would make every wait for LDS a wait for them).
+  // The table's entries of the next `span` times 64 tokens, one in each lane, in two batches (as above).
   const bool one_page = a.page_shift >= 6;  // the 64 tokens in one page
   constexpr int kLoadsLog = LOADS == 1 ? 0 : LOADS == 2 ? 1 : LOADS == 4 ? 2 : 3;
   const int pieces_log = one_page ? 0 : kLoadsLog, span_log = 6 - pieces_log, span = 1 << span_log;
@@ -986,7 +999,6 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
           if (wave + k * 4 < n) add(ahead[k], wave + k * 4);
         i += AHEAD * 4;
       }
-#pragma unroll 4
       for (; i < n; i += 4) add(load(j0 + i), i);
     }
     __syncthreads();

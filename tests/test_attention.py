@@ -348,6 +348,9 @@ ATTENTION_CASES = [
     ("bf16", False, [(300, 500), (400, 420)], 8, 1, 96, 16, True, 0),
     ("f16", False, [(40, 300), (1, 500), (2, 30), (90, 90)], 4, 2, 256, 32, True, 0),
     ("bf16", False, [(1, 40 + 13 * i) for i in range(70)] + [(0, 5)] * 60 + [(2, 30)], 4, 2, 64, 16, True, 0),
+    # more sequences than a wave takes at once, one of them split
+    ("f16", False, [(1, 1 + 7 * i % 40) for i in range(555)] + [(1, 9000), (1, 0)] + [(1, 33)] * 60, 2, 1, 64, 16, True, 0),
+    ("bf16", True, [(4, 4 + i % 30) for i in range(300)] + [(700, 900)] + [(1, 50)] * 5, 4, 1, 64, 16, True, 0),
 ]
 
 
@@ -478,6 +481,15 @@ def test_paged_attention_scales(gpu, lens, scale):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("lens", [[(1, 500)], [(90, 300)]], ids=str)
+def test_paged_attention_fp8_scales_below_zero(gpu, lens):
+    inputs = list(_attention_inputs(32, "f16", True, lens, 8, 2, 64, 16, poison=False))
+    inputs[3], inputs[4] = -inputs[3], -300 * inputs[4]
+    want, tol = ref_attention(*inputs, 0.1, True, 0)
+    _close(_run_attention(inputs, "f16", True, 0.1, True, 0), want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens", [[(1, 500)], [(90, 300)]], ids=str)
 def test_paged_attention_fp8_scales_of_many_sizes(gpu, lens):
     """Tokens whose values differ by orders of magnitude, and tokens of zeros."""
     for dt in ("f16", "bf16"):
@@ -538,6 +550,26 @@ def test_paged_attention_repeats_bit_for_bit(gpu, lens):
     first = _run_attention(inputs, "bf16", False, 0.0884, True, 0)
     for _ in range(3):
         assert torch.equal(first, _run_attention(inputs, "bf16", False, 0.0884, True, 0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("offsets", [[0, 40, 0, 40, 0, 40], [40, 0, 40, 0, 40, 0], [-9, 40, 7, 99, -1, 3], [50, 50, 50, 0, 0, 50]])
+@pytest.mark.parametrize("D", [64, 80])
+def test_paged_attention_offsets_that_overlap(gpu, offsets, D):
+    """Sequences whose rows overlap (no valid batch) end with rows of either; no row outside the tensor and
+    nothing behind the workspace is written."""
+    lens = [(8, 700)] * 5
+    q, k, v, _, _, table, _, kv = _cuda(*_attention_inputs(32, "f16", False, lens, 4, 2, D, 16, poison=False))
+    T = q.shape[0]
+    need = _native.library().intent_paged_attention_workspace_size(T, 4, 2, D, 5, table.shape[1], 16)
+    guard = torch.full((need + 4096,), 0x5a, dtype=torch.uint8, device="cuda")
+    wide = torch.full((T + 8, 4, D), 7.0, dtype=torch.float16, device="cuda")
+    offs = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    _native.call("intent_paged_attention", q.data_ptr(), T, 4, q.stride(0), 0, 0, k.data_ptr(), k.stride(0), v.data_ptr(),
+                 v.stride(0), None, 0, None, 0, k.shape[0], 2, 16, D, table.data_ptr(), 5, table.shape[1], table.stride(0),
+                 offs.data_ptr(), kv.data_ptr(), 0.125, 1, 0, wide.data_ptr(), wide.stride(0), guard.data_ptr(), need,
+                 torch.cuda.current_stream().cuda_stream)
+    assert bool((guard[need:] == 0x5a).all()) and bool((wide[T:] == 7).all())
 
 
 @pytest.mark.gpu
