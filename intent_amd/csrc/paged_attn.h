@@ -38,19 +38,26 @@ struct AttnArgs {
   float* partial_stats;
 };
 
-// A launch of the tiled kernels: the arguments, workgroups for each cached head, of the kernel and of
-// the join of its splits (0: none).
-struct AttnLaunch {
-  AttnArgs a;
-  int items, joins, join_rows;
-};
-
 // The tiled kernels for one type and cache (paged_attn_*.hip), by the rows of a tile: 16 to 64, whose
-// tokens are spread over a workgroup's four waves, or 128 or 256, 32 to a wave.
-int launch_attn_f16(const AttnLaunch& l, int rows, hipStream_t stream);
-int launch_attn_bf16(const AttnLaunch& l, int rows, hipStream_t stream);
-int launch_attn_f16_fp8(const AttnLaunch& l, int rows, hipStream_t stream);
-int launch_attn_bf16_fp8(const AttnLaunch& l, int rows, hipStream_t stream);
+// tokens are spread over a workgroup's four waves, or 128 or 256, 32 to a wave. `items` workgroups for
+// each cached head.
+int launch_attn_f16(const AttnArgs& a, int items, int rows, hipStream_t stream);
+int launch_attn_bf16(const AttnArgs& a, int items, int rows, hipStream_t stream);
+int launch_attn_f16_fp8(const AttnArgs& a, int items, int rows, hipStream_t stream);
+int launch_attn_bf16_fp8(const AttnArgs& a, int items, int rows, hipStream_t stream);
+
+// One launch for the joins of the split tiles of up to two lists: the rows of each one's tiles, its units of
+// tokens (their logarithm) and workgroups for each cached head (0: no list), and the second list's own
+// arguments where they differ.
+struct AttnJoin {
+  int items[2], tile[2], unit_log[2];
+  int min_rows, max_rows, target, slots;
+  float *partial, *partial_stats;
+  AttnArgs a;
+};
+// with `side` workgroups for the rows of a tile
+int launch_join_f16(const AttnJoin& j, int side, hipStream_t stream);
+int launch_join_bf16(const AttnJoin& j, int side, hipStream_t stream);
 
 // Query rows [start, start + count) and cached tokens of sequence s.
 struct Sequence {
@@ -84,15 +91,14 @@ struct Extent {
   int tiles, units;
 };
 
-template <int ROWS, int UNIT>
-INTENT_DEVICE Extent extent_of(const AttnArgs& a, int s) {
+INTENT_DEVICE Extent extent_of(const AttnArgs& a, int tile, int unit_log, int s) {
   Extent e;
   e.q = sequence_of(a, min(s, a.S - 1));
-  const int64_t rows = (int64_t)e.q.count * a.group;
+  const int rows = e.q.count * a.group;
   const bool listed = s < a.S && rows > a.min_rows && rows <= a.max_rows;
   const int lo = first_seen(a, e.q.kv - e.q.count) & ~63;
-  e.tiles = listed ? (int)((rows + ROWS - 1) / ROWS) : 0;
-  e.units = listed ? (e.q.kv - lo + UNIT - 1) / UNIT : 0;
+  e.tiles = listed ? (int)(((uint32_t)rows + (uint32_t)tile - 1u) / (uint32_t)tile) : 0;
+  e.units = listed ? (e.q.kv - lo + (1 << unit_log) - 1) >> unit_log : 0;
   return e;
 }
 
@@ -121,29 +127,28 @@ INTENT_DEVICE float wave_total(float v) {
 
 // Rows and tokens of share `local` of a sequence's (r.s, r.q and r.splits are set; with `joins`, of its
 // tiles), whose parts begin at `slot`.
-template <int ROWS, int UNIT>
-INTENT_DEVICE bool span_of(const AttnArgs& a, int tiles, int local, int slot, bool joins, Span& r) {
+INTENT_DEVICE bool span_of(const AttnArgs& a, int tile, int unit_log, int tiles, int local, int slot, bool joins, Span& r) {
   r.slot = slot + (joins ? local * r.splits : local);
   const int turn = joins ? local : (int)((uint32_t)local / (uint32_t)r.splits);
   const int split = joins ? 0 : local - turn * r.splits;
   // offsets that overlap may count up to anything: nothing outside the rows and the workspace then
   if (local < 0 || turn >= tiles || (r.splits > 1 && (r.slot < 0 || r.slot >= a.slots))) return false;
   if (joins && r.slot + r.splits > a.slots) return false;
-  r.row0 = (tiles - 1 - turn) * ROWS;
-  r.rows = min(ROWS, r.q.count * a.group - r.row0);
+  r.row0 = (tiles - 1 - turn) * tile;
+  r.rows = min(tile, r.q.count * a.group - r.row0);
   const int before = r.q.kv - r.q.count;
   const int p0 = before + (int)((uint32_t)r.row0 / (uint32_t)a.group);
   const int p1 = before + (int)((uint32_t)(r.row0 + r.rows - 1) / (uint32_t)a.group);
   const int lo = first_seen(a, p0) & ~63, hi = end_seen(a, p1, r.q.kv);
-  const uint32_t units = hi > lo ? (uint32_t)(hi - lo + UNIT - 1) / UNIT : 0u;
+  const uint32_t units = hi > lo ? (uint32_t)(hi - lo + (1 << unit_log) - 1) >> unit_log : 0u;
   const uint32_t each = units / (uint32_t)r.splits, more = units - each * (uint32_t)r.splits;
   const uint32_t from = each * split + min((uint32_t)split, more), to = from + each + ((uint32_t)split < more ? 1u : 0u);
-  r.begin = lo + (int)from * UNIT;
-  r.end = min(hi, lo + (int)to * UNIT);
+  r.begin = lo + ((int)from << unit_log);
+  r.end = min(hi, lo + ((int)to << unit_log));
   return true;
 }
 
-// Finds share `item` of one head's list: the sequences in order, each with its row tiles from the last
+// Finds share `item` of one head's list of tiles of `tile` rows, tokens in units of 1 << unit_log: the sequences in order, each with its row tiles from the last
 // (which sees most) to the first, each tile in `splits` parts of its tokens. The parts are sized so
 // that all sequences together give about a.target of them: units / chunk of each, chunk = the units
 // that a workgroup would get of an even share (rounded up, so never less than that: the workspace is
@@ -154,12 +159,12 @@ INTENT_DEVICE bool span_of(const AttnArgs& a, int tiles, int local, int slot, bo
 // Lanes take a sequence each of 64, or of AT times 64 whose extents are all loaded before the first is
 // used: 2048 sequences of 512 tokens take 1245 us with 64 at a time, 935 with 256; one sequence takes 7.1
 // us with 64 and would wait for three useless loads with 256.
-template <int ROWS, int UNIT, int AT>
-INTENT_DEVICE bool find_span_by(const AttnArgs& a, int item, bool joins, Span& r) {
+template <int AT>
+INTENT_DEVICE bool find_span_by(const AttnArgs& a, int tile, int unit_log, int item, bool joins, Span& r) {
   const int lane = threadIdx.x & 63;
   Extent e[AT];
 #pragma unroll
-  for (int i = 0; i < AT; ++i) e[i] = extent_of<ROWS, UNIT>(a, i * 64 + lane);
+  for (int i = 0; i < AT; ++i) e[i] = extent_of(a, tile, unit_log, i * 64 + lane);
   int chunk = INT32_MAX;
   if (a.target > 0) {
     float all = 0.f;
@@ -168,12 +173,12 @@ INTENT_DEVICE bool find_span_by(const AttnArgs& a, int item, bool joins, Span& r
     for (int s0 = AT * 64; s0 < a.S; s0 += AT * 64) {
       Extent f[AT];
 #pragma unroll
-      for (int i = 0; i < AT; ++i) f[i] = extent_of<ROWS, UNIT>(a, s0 + i * 64 + lane);
+      for (int i = 0; i < AT; ++i) f[i] = extent_of(a, tile, unit_log, s0 + i * 64 + lane);
 #pragma unroll
       for (int i = 0; i < AT; ++i) all += (float)f[i].tiles * (float)f[i].units;
     }
     chunk = (int)fminf(wave_total(all) * (1.0f + 0x1p-12f) / (float)a.target, 1.0e9f) + 1;
-    if (ROWS > 64) chunk = max(chunk, 8);
+    if (tile > 64) chunk = max(chunk, 8);
   }
   int base = 0, slots = 0;  // shares, and slots of split tiles, before sequence s0
   for (int s0 = 0;;) {
@@ -192,20 +197,19 @@ INTENT_DEVICE bool find_span_by(const AttnArgs& a, int item, bool joins, Span& r
         r.q.kv = lane_value(e[i].q.kv, at);
         r.splits = lane_value(splits, at);
         const int local = item - lane_value(up - mine, at), slot = lane_value(kept_up - kept, at);
-        return span_of<ROWS, UNIT>(a, lane_value(e[i].tiles, at), local, slot, joins, r);
+        return span_of(a, tile, unit_log, lane_value(e[i].tiles, at), local, slot, joins, r);
       }
       base = lane_value(up, 63), slots = lane_value(kept_up, 63);
     }
     s0 += AT * 64;
     if (s0 >= a.S) return false;
 #pragma unroll
-    for (int i = 0; i < AT; ++i) e[i] = extent_of<ROWS, UNIT>(a, s0 + i * 64 + lane);
+    for (int i = 0; i < AT; ++i) e[i] = extent_of(a, tile, unit_log, s0 + i * 64 + lane);
   }
 }
-template <int ROWS, int UNIT>
-INTENT_DEVICE bool find_span(const AttnArgs& a, int item, bool joins, Span& r) {
-  if (a.S <= 64) return find_span_by<ROWS, UNIT, 1>(a, item, joins, r);
-  return find_span_by<ROWS, UNIT, 4>(a, item, joins, r);
+INTENT_DEVICE bool find_span(const AttnArgs& a, int tile, int unit_log, int item, bool joins, Span& r) {
+  if (a.S <= 64) return find_span_by<1>(a, tile, unit_log, item, joins, r);
+  return find_span_by<4>(a, tile, unit_log, item, joins, r);
 }
 
 // Page of token t (t < most_kv) of sequence s.

@@ -148,7 +148,7 @@ int launch_rows(const AttnArgs& a, hipStream_t stream) {
 struct Part {
   int rows;  // of a tile
   int min_rows, max_rows;
-  int unit() const { return rows <= 64 ? 128 : 64; }
+  int unit_log() const { return rows <= 64 ? 7 : 6; }  // of the tokens that a share is a multiple of
   // Workgroups that the tiles are split for: what the 256 CUs hold at one time (by the kernels' registers),
   // and twice that where a CU holds three, which evens out sequences of different lengths and costs
   // little (four sequences of 60000 to 131000 tokens: 300 us at 512, 235 at 768, 239 at 1536; 64 of 300
@@ -196,15 +196,17 @@ Plan plan_of(int64_t T, int64_t S, int64_t HK, int64_t group, int64_t D) {
   return p;
 }
 
+// Tiles of one head: every sequence's last one may be partly filled, and sequences of at most a tile have one.
 int64_t tiles_bound(const Part& p, int64_t T, int64_t S, int64_t group) {
-  return T * group / p.rows + (S < T ? S : T);
+  const int64_t some = S < T ? S : T;
+  return p.max_rows <= p.rows ? some : T * group / p.rows + some;
 }
 
 // Parts of all split tiles of one head: fewer than twice the target (a tile of one and a half shares and
 // more is cut to the nearest number of them), and at most every tile's most.
 int64_t slots_bound(const Part& p, int64_t T, int64_t S, int64_t group, int64_t HK, int64_t D, int64_t most_kv) {
   const int64_t target = (p.fill(D) + HK - 1) / HK;
-  int64_t splits = (most_kv + p.unit() - 1) / p.unit();
+  int64_t splits = (most_kv + (1 << p.unit_log()) - 1) >> p.unit_log();
   if (splits > kMostSplits) splits = kMostSplits;
   if (splits < 2) return 0;
   const int64_t all = tiles_bound(p, T, S, group) * splits;
@@ -217,36 +219,50 @@ size_t part_bytes(const Part& p, int64_t T, int64_t S, int64_t group, int64_t HK
 
 int launch_tiled(AttnArgs a, bool bf16, bool fp8, float* workspace, size_t bytes, hipStream_t stream) {
   const Plan plan = plan_of(a.T, a.S, a.HK, a.group, a.D);
-  int status = INTENT_OK;
-  for (int i = 0; i < plan.parts && status == INTENT_OK; ++i) {
+  size_t need = 0;
+  for (int i = 0; i < plan.parts; ++i) need += part_bytes(plan.part[i], a.T, a.S, a.group, a.HK, a.D, a.most_kv);
+  AttnJoin join{};
+  int lists = 0;
+  for (int i = 0; i < plan.parts; ++i) {
     const Part& p = plan.part[i];
-    const size_t need = part_bytes(p, a.T, a.S, a.group, a.HK, a.D, a.most_kv);
+    const int64_t slots = slots_bound(p, a.T, a.S, a.group, a.HK, a.D, a.most_kv);
     // one sequence's tiles all attend the same tokens: enough of them even out by themselves
     const bool many = a.S == 1 && (int64_t)a.T * a.group / p.rows * a.HK >= 2 * p.fill(a.D);
-    const bool split = need > 0 && workspace != nullptr && bytes >= need && !many;
-    AttnLaunch l{};
+    const bool split = slots > 0 && workspace != nullptr && bytes >= need && !many;
     a.min_rows = p.min_rows, a.max_rows = p.max_rows;
     a.target = split ? (p.fill(a.D) + a.HK - 1) / a.HK : 0;
-    a.slots = split ? (int)slots_bound(p, a.T, a.S, a.group, a.HK, a.D, a.most_kv) : 0;
+    a.slots = split ? (int)slots : 0;
     a.partial = workspace;
-    a.partial_stats = split ? workspace + (int64_t)a.slots * a.HK * p.rows * a.D : nullptr;
+    a.partial_stats = split ? workspace + slots * a.HK * p.rows * a.D : nullptr;
     const int64_t tiles = tiles_bound(p, a.T, a.S, a.group);
-    const int64_t joins = split ? (tiles < a.target ? tiles : a.target) : 0;
     // workgroups of 256 or 512 lanes: the grid's work items stay below 2^32
     INTENT_REQUIRE((tiles + a.target) * a.HK < ((int64_t)1 << 23), INTENT_ERR_UNSUPPORTED,
                    "%lld tiles of %d heads exceed the %lld workgroups that a launch covers", (long long)tiles, a.HK,
                    (long long)((int64_t)1 << 23));
-    l.a = a;
-    l.items = (int)(tiles + a.target);
-    l.joins = (int)joins;
-    // workgroups for the rows of a split tile: one for each of a mean sequence, up to 1024 in all
-    const int64_t mean = ((int64_t)a.T * a.group + a.S - 1) / a.S, room = joins > 0 ? 1024 / (joins * a.HK) : 0;
-    const int64_t side = mean < p.rows ? mean : p.rows;
-    l.join_rows = (int)(room < 1 ? 1 : room < side ? room : side);
-    if (fp8) status = bf16 ? launch_attn_bf16_fp8(l, p.rows, stream) : launch_attn_f16_fp8(l, p.rows, stream);
-    else status = bf16 ? launch_attn_bf16(l, p.rows, stream) : launch_attn_f16(l, p.rows, stream);
+    const int items = (int)(tiles + a.target);
+    const int status = fp8 ? (bf16 ? launch_attn_bf16_fp8(a, items, p.rows, stream) : launch_attn_f16_fp8(a, items, p.rows, stream))
+                           : (bf16 ? launch_attn_bf16(a, items, p.rows, stream) : launch_attn_f16(a, items, p.rows, stream));
+    if (status != INTENT_OK) return status;
+    if (!split) continue;
+    // a tile is split from one and a half shares on
+    const int64_t most = a.target * 2 / 3 + 1;
+    if (lists == 0) {
+      join.a = a;
+    } else {
+      join.min_rows = a.min_rows, join.max_rows = a.max_rows, join.target = a.target, join.slots = a.slots;
+      join.partial = a.partial, join.partial_stats = a.partial_stats;
+    }
+    join.tile[lists] = p.rows, join.unit_log[lists] = p.unit_log();
+    join.items[lists++] = (int)(tiles < most ? tiles : most);
+    workspace += part_bytes(p, a.T, a.S, a.group, a.HK, a.D, a.most_kv) / 4;
   }
-  return status;
+  if (lists == 0) return INTENT_OK;
+  // workgroups for the rows of a split tile: one for each of a mean sequence, up to 1024 in all
+  const int64_t mean = ((int64_t)a.T * a.group + a.S - 1) / a.S;
+  const int64_t room = 1024 / ((int64_t)(join.items[0] + join.items[1]) * a.HK), rows = plan.part[0].rows;
+  const int64_t side = mean < rows ? mean : rows;
+  const int sides = (int)(room < 1 ? 1 : room < side ? room : side);
+  return bf16 ? launch_join_bf16(join, sides, stream) : launch_join_f16(join, sides, stream);
 }
 
 }  // namespace
@@ -257,12 +273,10 @@ extern "C" size_t intent_paged_attention_workspace_size(int64_t T, int64_t HQ, i
       table_width > kMostTokens / page_size || HQ > 65536 || T * HQ >= ((int64_t)1 << 25))
     return 0;
   const Plan plan = plan_of(T, S, HK, HQ / HK, D);
-  size_t most = 0;
-  for (int i = 0; i < plan.parts; ++i) {
-    const size_t need = part_bytes(plan.part[i], T, S, HQ / HK, HK, D, table_width * page_size);
-    if (need > most) most = need;
-  }
-  return most;
+  size_t need = 0;
+  for (int i = 0; i < plan.parts; ++i)
+    need += part_bytes(plan.part[i], T, S, HQ / HK, HK, D, table_width * page_size);
+  return need;
 }
 
 extern "C" int intent_paged_attention(const void* q, int64_t T, int64_t HQ, int64_t q_ld, int is_bf16,

@@ -213,7 +213,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
 
   const int head = blockIdx.x % a.HK;
   Span w;
-  if (!find_span<16 * MT, 128>(a, blockIdx.x / a.HK, false, w)) return;
+  if (!find_span(a, 16 * MT, 7, blockIdx.x / a.HK, false, w)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int col = lane & 15, g = lane >> 4;
 
@@ -548,7 +548,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
 
   const int head = blockIdx.x % a.HK;
   Span w;
-  if (!find_span<ROWS, 64>(a, blockIdx.x / a.HK, false, w)) return;
+  if (!find_span(a, ROWS, 6, blockIdx.x / a.HK, false, w)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int col = lane & 31, h = lane >> 5;
   const int r0 = wave * 32;
@@ -909,21 +909,28 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
 // parts are dealt to the four waves of a workgroup (D / 64 columns a lane), whose sums are added in
 // order; each works out the weights of 64 parts at a time, one in each lane, while its first parts are on
 // their way.
-template <bool kBf16, int D, int ROWS, int UNIT>
-__global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
+template <bool kBf16, int D>
+__global__ __launch_bounds__(256) void attn_join_kernel(int items, int tile, int unit_log, const AttnJoin j) {
   constexpr int E = (D + 63) / 64, AHEAD = 8, FEW = 16;
   constexpr int LANES = D == 96 ? 32 : D / 4, TOGETHER = 64 / LANES;  // lanes of a row, rows of a wave
   typedef float part __attribute__((ext_vector_type(E)));
   __shared__ part sums[4][64];
+  AttnArgs a = j.a;
   const int head = blockIdx.x % a.HK;
+  int item = blockIdx.x / a.HK;
+  if (item >= items) {
+    item -= items, tile = j.tile[1], unit_log = j.unit_log[1];
+    a.min_rows = j.min_rows, a.max_rows = j.max_rows, a.target = j.target, a.slots = j.slots;
+    a.partial = j.partial, a.partial_stats = j.partial_stats;
+  }
   Span w;
-  if (!find_span<ROWS, UNIT>(a, blockIdx.x / a.HK, true, w)) return;
+  if (!find_span(a, tile, unit_log, item, true, w)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (w.splits <= FEW) {
     const int c = lane % LANES * 4 < D ? lane % LANES * 4 : 0;
     for (int first = (blockIdx.y * 4 + wave) * TOGETHER; first < w.rows; first += gridDim.y * 4 * TOGETHER) {
       const int r = first + lane / LANES, row = min(r, w.rows - 1);
-      auto at = [&](int j) { return ((int64_t)(w.slot + j) * a.HK + head) * ROWS + row; };
+      auto at = [&](int j) { return ((int64_t)(w.slot + j) * a.HK + head) * tile + row; };
       f32x2 st[FEW];
       float high = -INFINITY;
 #pragma unroll
@@ -962,7 +969,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
   const bool mine = lane * E < D;
   const int d0 = mine ? lane * E : 0;
   for (int r = blockIdx.y; r < w.rows; r += gridDim.y) {
-    auto at = [&](int j) { return ((int64_t)(w.slot + j) * a.HK + head) * ROWS + r; };
+    auto at = [&](int j) { return ((int64_t)(w.slot + j) * a.HK + head) * tile + r; };
     auto load = [&](int j) { return *(const part*)(a.partial + at(min(j, w.splits - 1)) * D + d0); };
     part ahead[AHEAD];
 #pragma unroll
@@ -1015,48 +1022,60 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const AttnArgs a) {
   }
 }
 
-// The kernel, and the join of its split tiles. ROWS up to 64: rows of the first kernel; 128 or 256: of
-// the second's four or eight waves.
+// ROWS up to 64: rows of the first kernel; 128 or 256: of the second's four or eight waves.
 template <bool kBf16, bool kFp8, int D, int ROWS>
-int launch(const AttnLaunch& l, hipStream_t stream) {
-  const unsigned heads = (unsigned)l.a.HK;
+int launch(const AttnArgs& a, int items, hipStream_t stream) {
+  const unsigned groups = (unsigned)items * (unsigned)a.HK;
   constexpr bool kFew = ROWS <= 64;
   if constexpr (kFew)
-    hipLaunchKernelGGL((attn_rows_kernel<kBf16, kFp8, D, ROWS / 16>), dim3(l.items * heads), dim3(256), 0, stream, l.a);
+    hipLaunchKernelGGL((attn_rows_kernel<kBf16, kFp8, D, ROWS / 16>), dim3(groups), dim3(256), 0, stream, a);
   else
-    hipLaunchKernelGGL((attn_tile_kernel<kBf16, kFp8, D, ROWS / 32>), dim3(l.items * heads), dim3(ROWS * 2), 0, stream,
-                       l.a);
+    hipLaunchKernelGGL((attn_tile_kernel<kBf16, kFp8, D, ROWS / 32>), dim3(groups), dim3(ROWS * 2), 0, stream, a);
   static const KernelName name("attn_%s_kernel<%s%s, D %d, %d rows>", kFew ? "rows" : "tile", kBf16 ? "bf16" : "f16",
                                kFp8 ? ", fp8 cache" : "", D, ROWS);
-  const int status = launch_status(name.text);
-  if (status != INTENT_OK || l.joins == 0) return status;
-  hipLaunchKernelGGL((attn_join_kernel<kBf16, D, ROWS, kFew ? 128 : 64>), dim3(l.joins * heads, l.join_rows), dim3(256),
-                     0, stream, l.a);
-  static const KernelName joined("attn_%s_kernel<%s%s, D %d, %d rows, splits>", kFew ? "rows" : "tile",
-                                 kBf16 ? "bf16" : "f16", kFp8 ? ", fp8 cache" : "", D, ROWS);
-  return launch_status(joined.text);
+  return launch_status(name.text);
 }
 
 template <bool kBf16, bool kFp8, int D>
-int launch_d(const AttnLaunch& l, int rows, hipStream_t stream) {
-  if (rows == 16) return launch<kBf16, kFp8, D, 16>(l, stream);
+int launch_d(const AttnArgs& a, int items, int rows, hipStream_t stream) {
+  if (rows == 16) return launch<kBf16, kFp8, D, 16>(a, items, stream);
   if constexpr (D <= 128) {
-    if (rows == 32) return launch<kBf16, kFp8, D, 32>(l, stream);
-    if (rows == 48) return launch<kBf16, kFp8, D, 48>(l, stream);
-    if (rows == 64) return launch<kBf16, kFp8, D, 64>(l, stream);
-    if (rows == 256) return launch<kBf16, kFp8, D, 256>(l, stream);
+    if (rows == 32) return launch<kBf16, kFp8, D, 32>(a, items, stream);
+    if (rows == 48) return launch<kBf16, kFp8, D, 48>(a, items, stream);
+    if (rows == 64) return launch<kBf16, kFp8, D, 64>(a, items, stream);
+    if (rows == 256) return launch<kBf16, kFp8, D, 256>(a, items, stream);
   }
-  return launch<kBf16, kFp8, D, 128>(l, stream);
+  return launch<kBf16, kFp8, D, 128>(a, items, stream);
 }
 
 template <bool kBf16, bool kFp8>
-int launch_any(const AttnLaunch& l, int rows, hipStream_t stream) {
-  switch (l.a.D) {
-    case 64: return launch_d<kBf16, kFp8, 64>(l, rows, stream);
-    case 96: return launch_d<kBf16, kFp8, 96>(l, rows, stream);
-    case 128: return launch_d<kBf16, kFp8, 128>(l, rows, stream);
-    case 256: return launch_d<kBf16, kFp8, 256>(l, rows, stream);
-    default: return fail(INTENT_ERR_UNSUPPORTED, "no tiled attention kernel for heads of %d", l.a.D);
+int launch_any(const AttnArgs& a, int items, int rows, hipStream_t stream) {
+  switch (a.D) {
+    case 64: return launch_d<kBf16, kFp8, 64>(a, items, rows, stream);
+    case 96: return launch_d<kBf16, kFp8, 96>(a, items, rows, stream);
+    case 128: return launch_d<kBf16, kFp8, 128>(a, items, rows, stream);
+    case 256: return launch_d<kBf16, kFp8, 256>(a, items, rows, stream);
+    default: return fail(INTENT_ERR_UNSUPPORTED, "no tiled attention kernel for heads of %d", a.D);
+  }
+}
+
+template <bool kBf16, int D>
+int launch_join_d(const AttnJoin& j, int side, hipStream_t stream) {
+  const unsigned groups = (unsigned)(j.items[0] + j.items[1]) * (unsigned)j.a.HK;
+  hipLaunchKernelGGL((attn_join_kernel<kBf16, D>), dim3(groups, side), dim3(256), 0, stream, j.items[0], j.tile[0],
+                     j.unit_log[0], j);
+  static const KernelName name("attn_join_kernel<%s, D %d> of splits", kBf16 ? "bf16" : "f16", D);
+  return launch_status(name.text);
+}
+
+template <bool kBf16>
+int launch_join(const AttnJoin& j, int side, hipStream_t stream) {
+  switch (j.a.D) {
+    case 64: return launch_join_d<kBf16, 64>(j, side, stream);
+    case 96: return launch_join_d<kBf16, 96>(j, side, stream);
+    case 128: return launch_join_d<kBf16, 128>(j, side, stream);
+    case 256: return launch_join_d<kBf16, 256>(j, side, stream);
+    default: return fail(INTENT_ERR_UNSUPPORTED, "no tiled attention kernel for heads of %d", j.a.D);
   }
 }
 
