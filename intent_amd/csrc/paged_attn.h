@@ -127,7 +127,8 @@ INTENT_DEVICE float wave_total(float v) {
 
 // Rows and tokens of share `local` of a sequence's (r.s, r.q and r.splits are set; with `joins`, of its
 // tiles), whose parts begin at `slot`.
-INTENT_DEVICE bool span_of(const AttnArgs& a, int tile, int unit_log, int tiles, int local, int slot, bool joins, Span& r) {
+INTENT_DEVICE bool span_of(const AttnArgs& a, int tile, int unit_log, int tiles, int local, int slot, bool joins,
+                           Span& r) {
   r.slot = slot + (joins ? local * r.splits : local);
   const int turn = joins ? local : (int)((uint32_t)local / (uint32_t)r.splits);
   const int split = joins ? 0 : local - turn * r.splits;
@@ -142,19 +143,21 @@ INTENT_DEVICE bool span_of(const AttnArgs& a, int tile, int unit_log, int tiles,
   const int lo = first_seen(a, p0) & ~63, hi = end_seen(a, p1, r.q.kv);
   const uint32_t units = hi > lo ? (uint32_t)(hi - lo + (1 << unit_log) - 1) >> unit_log : 0u;
   const uint32_t each = units / (uint32_t)r.splits, more = units - each * (uint32_t)r.splits;
-  const uint32_t from = each * split + min((uint32_t)split, more), to = from + each + ((uint32_t)split < more ? 1u : 0u);
+  const uint32_t from = each * split + min((uint32_t)split, more);
+  const uint32_t to = from + each + ((uint32_t)split < more ? 1u : 0u);
   r.begin = lo + ((int)from << unit_log);
   r.end = min(hi, lo + ((int)to << unit_log));
   return true;
 }
 
-// Finds share `item` of one head's list of tiles of `tile` rows, tokens in units of 1 << unit_log: the sequences in order, each with its row tiles from the last
-// (which sees most) to the first, each tile in `splits` parts of its tokens. The parts are sized so
-// that all sequences together give about a.target of them: units / chunk of each, chunk = the units
-// that a workgroup would get of an even share (rounded up, so never less than that: the workspace is
-// sized by it), but for 64 and more new rows no fewer than 8 units (a join costs as many). With `joins`, the list of the tiles that are split. Every wave does it by itself: no
-// plan is kept, so a captured call follows lengths that change. The counts of one list fit 32 bits (the
-// host bounds the grid).
+// Finds share `item` of one head's list of tiles of `tile` rows, tokens in units of 1 << unit_log: the
+// sequences in order, each with its row tiles from the last (which sees most) to the first, each tile in
+// `splits` parts of its tokens. The parts are sized so that all sequences together give about a.target of
+// them: units / chunk of each, to the nearest number, chunk = the units that a workgroup would get of an
+// even share (rounded up, so never less than that: the workspace is sized by it), but for tiles of more
+// than 64 rows no fewer than 8 units (a join costs as many). With `joins`, the list of the tiles that are
+// split. Every wave does it by itself: no plan is kept, so a captured call follows lengths that change. The
+// counts of one list fit 32 bits (the host bounds the grid).
 //
 // Lanes take a sequence each of 64, or of AT times 64 whose extents are all loaded before the first is
 // used: 2048 sequences of 512 tokens take 1245 us with 64 at a time, 935 with 256; one sequence takes 7.1

@@ -240,8 +240,8 @@ int launch_tiled(AttnArgs a, bool bf16, bool fp8, float* workspace, size_t bytes
                    "%lld tiles of %d heads exceed the %lld workgroups that a launch covers", (long long)tiles, a.HK,
                    (long long)((int64_t)1 << 23));
     const int items = (int)(tiles + a.target);
-    const int status = fp8 ? (bf16 ? launch_attn_bf16_fp8(a, items, p.rows, stream) : launch_attn_f16_fp8(a, items, p.rows, stream))
-                           : (bf16 ? launch_attn_bf16(a, items, p.rows, stream) : launch_attn_f16(a, items, p.rows, stream));
+    const auto go = fp8 ? (bf16 ? launch_attn_bf16_fp8 : launch_attn_f16_fp8) : (bf16 ? launch_attn_bf16 : launch_attn_f16);
+    const int status = go(a, items, p.rows, stream);
     if (status != INTENT_OK) return status;
     if (!split) continue;
     // a tile is split from one and a half shares on
@@ -296,7 +296,8 @@ extern "C" int intent_paged_attention(const void* q, int64_t T, int64_t HQ, int6
                  (long long)page_size);
   if (T == 0 || HQ == 0 || D == 0 || S == 0) return INTENT_OK;
   INTENT_REQUIRE(HK > 0 && HQ % HK == 0, INTENT_ERR_INVALID_ARGUMENT,
-                 "HQ=%lld query heads must be a multiple of the HK=%lld heads of the cache", (long long)HQ, (long long)HK);
+                 "HQ=%lld query heads must be a multiple of the HK=%lld heads of the cache", (long long)HQ,
+                 (long long)HK);
   INTENT_REQUIRE(D % 8 == 0 && D <= 512, INTENT_ERR_UNSUPPORTED, "D must be a multiple of 8 up to 512, got %lld",
                  (long long)D);
   const bool any = pages > 0 && page_size > 0 && table_width > 0;
@@ -309,7 +310,8 @@ extern "C" int intent_paged_attention(const void* q, int64_t T, int64_t HQ, int6
                  (long long)page_size, (long long)HK);
   // at most a wave for each row of a head: the grid's work items stay below 2^32
   INTENT_REQUIRE(T * HQ < ((int64_t)1 << 25), INTENT_ERR_UNSUPPORTED,
-                 "T * HQ = %lld rows exceed the %lld a launch covers", (long long)(T * HQ), (long long)((int64_t)1 << 25));
+                 "T * HQ = %lld rows exceed the %lld a launch covers", (long long)(T * HQ),
+                 (long long)((int64_t)1 << 25));
   INTENT_REQUIRE(q && out && q_offsets && kv_lens && (!any || (k_cache && v_cache && page_table)) &&
                      (!any || !cache_is_fp8 || (k_scales && v_scales)),
                  INTENT_ERR_INVALID_ARGUMENT, "null pointer argument");

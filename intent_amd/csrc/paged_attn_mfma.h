@@ -39,11 +39,13 @@ typedef const __attribute__((address_space(1))) char* global_bytes;
 INTENT_DEVICE global_bytes as_global(const void* p) { return (global_bytes)p; }
 // Rows (of kRowBytes) of a head from token t on, t and the page uniform or not.
 template <int kRowBytes>
-INTENT_DEVICE global_bytes cached_rows(const AttnArgs& a, const void* base, uint32_t page, uint32_t step, int head, int t) {
+INTENT_DEVICE global_bytes cached_rows(const AttnArgs& a, const void* base, uint32_t page, uint32_t step, int head,
+                                       int t) {
   const uint32_t row = ((uint32_t)head << a.page_shift) + ((uint32_t)t & ((1u << a.page_shift) - 1u));
   return as_global(base) + ((uint64_t)page * step + (uint64_t)row * (kRowBytes / 16)) * 16;
 }
-INTENT_DEVICE global_bytes cached_scales(const AttnArgs& a, const float* base, uint32_t page, uint32_t step, int head, int t) {
+INTENT_DEVICE global_bytes cached_scales(const AttnArgs& a, const float* base, uint32_t page, uint32_t step, int head,
+                                         int t) {
   const uint32_t row = ((uint32_t)head << a.page_shift) + ((uint32_t)t & ((1u << a.page_shift) - 1u));
   return as_global(base) + ((uint64_t)page * step + row) * 4;
 }
@@ -53,12 +55,14 @@ INTENT_DEVICE u32x2 load8(global_bytes p) { return *(const __attribute__((addres
 
 template <bool kBf16>
 INTENT_DEVICE f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
-  if constexpr (kBf16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(bit_cast<bf16x8>(a), bit_cast<bf16x8>(b), c, 0, 0, 0);
+  if constexpr (kBf16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(bit_cast<bf16x8>(a), bit_cast<bf16x8>(b), c, 0, 0, 0);
   else return __builtin_amdgcn_mfma_f32_16x16x32_f16(bit_cast<f16x8>(a), bit_cast<f16x8>(b), c, 0, 0, 0);
 }
 template <bool kBf16>
 INTENT_DEVICE f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
-  if constexpr (kBf16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(bit_cast<bf16x8>(a), bit_cast<bf16x8>(b), c, 0, 0, 0);
+  if constexpr (kBf16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(bit_cast<bf16x8>(a), bit_cast<bf16x8>(b), c, 0, 0, 0);
   else return __builtin_amdgcn_mfma_f32_32x32x16_f16(bit_cast<f16x8>(a), bit_cast<f16x8>(b), c, 0, 0, 0);
 }
 
@@ -247,7 +251,8 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
   const int write_at = col * RB, swz = swizzle<RB, false>(col);
   // transposing reads: tokens 4 g .. 4 g + 3 of each 16, columns 16 d ..
   const int read_row = g * 4 + (col >> 2);
-  const int read_at = wave * 32 * RB + read_row * RB + (((col >> 1 & 1) ^ swizzle<RB, false>(read_row)) << 4) + (col & 1) * 8;
+  const int read_at =
+      wave * 32 * RB + read_row * RB + (((col >> 1 & 1) ^ swizzle<RB, false>(read_row)) << 4) + (col & 1) * 8;
 
   u32x4 kr[2][LOADS], vr[2][LOADS];
   float ks[2], vs[2];
@@ -352,7 +357,8 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
         const int chunk = at(i) / 8;
         if constexpr (kFp8) {
           *(u32x4*)(row + ((chunk ^ swz) << 4)) = widen_codes<kBf16>(vr[u][i][0], vr[u][i][1]);
-          if constexpr (kWide) *(u32x4*)(row + (((chunk + 1) ^ swz) << 4)) = widen_codes<kBf16>(vr[u][i][2], vr[u][i][3]);
+          if constexpr (kWide)
+            *(u32x4*)(row + (((chunk + 1) ^ swz) << 4)) = widen_codes<kBf16>(vr[u][i][2], vr[u][i][3]);
         } else {
           *(u32x4*)(row + ((chunk ^ swz) << 4)) = vr[u][i];
         }
@@ -529,7 +535,8 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
 // 32 heads sharing 8 (137 GFLOP): 152 to 161 us, 850 to 900 TFLOP/s, where the library's product of
 // 8192^3 reaches 1200; 3696 tokens in two chunks over 10000 to 18000 in 8 bits 1115 to 1170 us, 780 to 820
 // TFLOP/s. What is left: with the loads of the cache taken away it takes 140 us, with the vector work
-// 117, with the products 111; each wave's own chain, not one unit, sets the time.
+// 117, with the products 111; each wave's own chain, not one unit, sets the time. 64 rows to a wave read LDS
+// half as often, but one wave to a SIMD and 1500 copies between the two halves of its registers take 215 us.
 template <bool kBf16, bool kFp8, int D, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
     void attn_tile_kernel(const AttnArgs a) {
@@ -589,7 +596,8 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
   const int pieces_log = one_page ? 0 : kLoadsLog, span_log = 6 - pieces_log, span = 1 << span_log;
   auto clamped = [&](int t) __attribute__((always_inline)) { return min(max(t, some_lo), max(some_hi - 1, 0)); };
   auto batch = [&](int t) __attribute__((always_inline)) {
-    return table_entry(a, w.s, clamped(t + (lane >> pieces_log) * 64 + (lane & ((1 << pieces_log) - 1)) * STEP + wave_token));
+    const int piece = lane & ((1 << pieces_log) - 1);
+    return table_entry(a, w.s, clamped(t + (lane >> pieces_log) * 64 + piece * STEP + wave_token));
   };
   uint32_t entries[2] = {0, 0};
   // of the i-th load of the tokens n * 64 behind w.begin
@@ -602,14 +610,16 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
   auto load = [&](u32x4(&fetched)[LOADS], const void* cache, uint32_t step, int t) __attribute__((always_inline)) {
     const int n = (t - w.begin) >> 6;
     if (one_page) {
-      const global_bytes from = cached_rows<D * kBytes>(a, cache, page_named(a, entry(n, 0)), step, head, t + wave_token);
+      const uint32_t page = page_named(a, entry(n, 0));
+      const global_bytes from = cached_rows<D * kBytes>(a, cache, page, step, head, t + wave_token);
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) fetched[i] = load16(from + i * (STEP * D * kBytes) + lane_at);
     } else if (paged) {
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i)
-        fetched[i] = load16(cached_rows<D * kBytes>(a, cache, page_named(a, entry(n, i)), step, head, t + i * STEP + wave_token) +
-                            lane_at);
+      for (int i = 0; i < LOADS; ++i) {
+        const uint32_t page = page_named(a, entry(n, i));
+        fetched[i] = load16(cached_rows<D * kBytes>(a, cache, page, step, head, t + i * STEP + wave_token) + lane_at);
+      }
     } else {
       rarely();
 #pragma unroll
@@ -647,7 +657,9 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
     }
   };
   // whether rows of this tile see different ones of the tokens t ..
-  auto apart = [&](int t) __attribute__((always_inline)) { return (some_lo != all_lo || some_hi != all_hi) && (t < all_lo || t + 64 > all_hi); };
+  auto apart = [&](int t) __attribute__((always_inline)) {
+    return (some_lo != all_lo || some_hi != all_hi) && (t < all_lo || t + 64 > all_hi);
+  };
   auto store_values = [&](int buffer, int t) __attribute__((always_inline)) {
     if (t < some_lo || t + 64 > some_hi) {
       rarely();
@@ -682,7 +694,8 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
 
   const int k_at = col * RB + ((h ^ swizzle<RB, true>(col)) << 4);
   const int i16 = lane & 15, read_row = h * 4 + (i16 >> 2);
-  const int v_at = read_row * RB + ((((lane >> 4 & 1) * 2 + (i16 >> 1 & 1)) ^ swizzle<RB, true>(read_row)) << 4) + (i16 & 1) * 8;
+  const int v_chunk = (lane >> 4 & 1) * 2 + (i16 >> 1 & 1);
+  const int v_at = read_row * RB + ((v_chunk ^ swizzle<RB, true>(read_row)) << 4) + (i16 & 1) * 8;
 
   auto scores = [&](int buffer, f32x16(&s)[2]) __attribute__((always_inline)) {
     const char* keys = lds[buffer][0];
@@ -908,7 +921,9 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
 // Up to 16 parts, a row is D / 4 lanes of four columns, and a wave takes as many rows as it holds. More
 // parts are dealt to the four waves of a workgroup (D / 64 columns a lane), whose sums are added in
 // order; each works out the weights of 64 parts at a time, one in each lane, while its first parts are on
-// their way.
+// their way. What the first list needs to be found comes before the struct, where the kernel has it in
+// registers when it starts. A launch and a chain of four latencies: 4.2 to 4.8 us for one tile of 32 parts;
+// one launch for the tiles of a mixture's two lists 7.2 us, where two took 11.4.
 template <bool kBf16, int D>
 __global__ __launch_bounds__(256) void attn_join_kernel(int items, int tile, int unit_log, const AttnJoin j) {
   constexpr int E = (D + 63) / 64, AHEAD = 8, FEW = 16;
