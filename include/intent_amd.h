@@ -732,7 +732,8 @@ int intent_paged_kv_append(const void* q, int64_t T, int64_t HQ, int64_t q_ld,
  * does not reach it, whatever it holds. f32 scores, softmax and sums; the
  * weights are rounded to q's type for the product with the values.
  * Lengths, offsets and page ids are clamped to the tensors, never followed out
- * of them. D % 8 == 0, D <= 512 (heads of 64, 96, 128 and 256 run the MFMA
+ * of them; offsets rise, and sequences whose rows overlap leave those rows
+ * undefined. D % 8 == 0, D <= 512 (heads of 64, 96, 128 and 256 run the MFMA
  * kernels, others one wave for each row). No reference counterpart.
  * workspace: where few rows attend many tokens, their tokens are split over
  * workgroups, whose f32 sums pass through it; _workspace_size gives the bytes
