@@ -698,12 +698,14 @@ int intent_qk_norm_rope(const void* q, int64_t T, int64_t HQ, int64_t q_ld,
  * elements from a page to the next; page_size a power of two): token t goes to
  * slot slots[t] = page * page_size + place. A negative slot (a padded row) or
  * one past the cache is skipped; its q_out row is written all the same. Slots
- * of one call are distinct: one given twice ends with rows of either token.
+ * of one call are distinct: one given twice ends with elements of either token
+ * (in 8 bits, with the scale of either).
  * The cache holds the heads' type, or E4M3FN codes (cache_is_fp8) with scales
  * f32 [pages][HK][page_size] (k_scales_ld, v_scales_ld from a page to the next):
  * scale = max(absmax, 1e-12) / 448 of a token's head, code = e4m3fn(clamp(y /
  * scale, +-448)), the rule of intent_fp8_groupwise_quantize for bf16 with one
- * group for each head. Everything else in the cache stays as it is.
+ * group for each head; a head that holds an infinity or NaN reads as NaN.
+ * Everything else in the cache stays as it is.
  * No reference counterpart.
  */
 int intent_paged_kv_append(const void* q, int64_t T, int64_t HQ, int64_t q_ld,
@@ -730,7 +732,8 @@ int intent_paged_kv_append(const void* q, int64_t T, int64_t HQ, int64_t q_ld,
  * a row that sees nothing (an empty cache, more new tokens than cached ones)
  * is zero, rows of no sequence are not written, and what a row does not see
  * does not reach it, whatever it holds. f32 scores, softmax and sums; the
- * weights are rounded to q's type for the product with the values.
+ * weights are rounded to q's type for the product with the values. The scale is
+ * finite.
  * Lengths, offsets and page ids are clamped to the tensors, never followed out
  * of them; offsets rise, and sequences whose rows overlap leave those rows
  * undefined. D % 8 == 0, D <= 512 (heads of 64, 96, 128 and 256 run the MFMA

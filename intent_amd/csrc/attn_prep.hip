@@ -47,10 +47,15 @@ struct PrepArgs {
 
 enum Mode { kKeysOut = 0, kCacheSame = 1, kCacheFp8 = 2 };
 
+// The larger of two floats without a sign, by their bits: NaN is the largest.
+INTENT_DEVICE float magnitude_max(float a, float b) {
+  return bit_cast<float>(max(bit_cast<uint32_t>(a), bit_cast<uint32_t>(b)));
+}
+
 // Sum or maximum over the LPR lanes of a group.
 template <int LPR, bool kMax>
 INTENT_DEVICE float group_reduce(float v) {
-  auto join = [](float a, float b) { return kMax ? fmaxf(a, b) : a + b; };
+  auto join = [](float a, float b) { return kMax ? magnitude_max(a, b) : a + b; };
   v = join(v, dpp_f32<0xB1>(v));             // quad_perm [1,0,3,2]
   v = join(v, dpp_f32<0x4E>(v));             // quad_perm [2,3,0,1]
   v = join(v, dpp_f32<0x141>(v));            // mirrored in halves of a row: 8 lanes
@@ -195,14 +200,19 @@ __global__ __launch_bounds__(256) void attn_prep_kernel(const PrepArgs a) {
       } else {
         float amax = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[j]));
-        const float scale = __fdiv_rn(fmaxf(group_reduce<LPR, true>(amax), 1.0e-12f), 448.0f);
+        for (int j = 0; j < 8; ++j) amax = magnitude_max(amax, fabsf(x[j]));
+        // a head that holds an infinity or NaN reads as NaN throughout: its scale is infinite or NaN, and
+        // the clamp lets NaN pass
+        const float scale = __fdiv_rn(magnitude_max(group_reduce<LPR, true>(amax), 1.0e-12f), 448.0f);
         uint32_t code[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           float t[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) t[e] = fminf(fmaxf(__fdiv_rn(x[4 * j + e], scale), -448.0f), 448.0f);
+          for (int e = 0; e < 4; ++e) {
+            t[e] = __fdiv_rn(x[4 * j + e], scale);
+            t[e] = t[e] < -448.0f ? -448.0f : t[e] > 448.0f ? 448.0f : t[e];
+          }
           int word = __builtin_amdgcn_cvt_pk_fp8_f32(t[0], t[1], 0, false);
           code[j] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(t[2], t[3], word, true);
         }

@@ -295,6 +295,9 @@ extern "C" int intent_paged_attention(const void* q, int64_t T, int64_t HQ, int6
                  (long long)T, (long long)HQ, (long long)HK, (long long)D, (long long)S, (long long)pages,
                  (long long)page_size);
   if (T == 0 || HQ == 0 || D == 0 || S == 0) return INTENT_OK;
+  const float scale_log2 = scale * 1.44269504088896340736f;
+  INTENT_REQUIRE(__builtin_isfinite(scale_log2), INTENT_ERR_INVALID_ARGUMENT, "scale * log2(e) must be finite, got %g",
+                 (double)scale_log2);
   INTENT_REQUIRE(HK > 0 && HQ % HK == 0, INTENT_ERR_INVALID_ARGUMENT,
                  "HQ=%lld query heads must be a multiple of the HK=%lld heads of the cache", (long long)HQ,
                  (long long)HK);
@@ -343,7 +346,7 @@ extern "C" int intent_paged_attention(const void* q, int64_t T, int64_t HQ, int6
   a.page_table = page_table, a.table_ld = table_ld;
   a.q_offsets = q_offsets, a.kv_lens = kv_lens;
   a.out = (uint16_t*)out, a.out_ld = out_ld;
-  a.scale_log2 = scale * 1.44269504088896340736f;
+  a.scale_log2 = scale_log2;
   a.T = (int)T, a.S = (int)S, a.HQ = (int)HQ, a.HK = (int)HK, a.group = (int)(HQ / HK), a.D = (int)D;
   a.pages = any ? (int)pages : 0, a.page_shift = any ? __builtin_ctzll((unsigned long long)page_size) : 0;
   a.most_kv = any ? (int)(table_width * page_size) : 0;

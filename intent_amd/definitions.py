@@ -1475,7 +1475,8 @@ def _attention_definition(dt: str, fp8: bool) -> KernelDefinition:
         return "intent_paged_attention", (
             _ptr(q), env["T"], env["HQ"], _ld(q), int(dt == "bf16"), int(fp8), *_cache_arguments(v, fp8), env["PAGES"],
             env["HK"], env["PAGE"], env["D"], _ptr(table), env["S"], env["MAX_PAGES"], _ld(table), _ptr(v["q_offsets"]),
-            _ptr(v["kv_lens"]), float(env["scale"]), int(bool(env["CAUSAL"])), int(env["WINDOW"]), _ptr(out), _ld(out),
+            _ptr(v["kv_lens"]), float(env["scale"]), int(bool(env["CAUSAL"])), min(int(env["WINDOW"]), 2 ** 31),
+            _ptr(out), _ld(out),
             None if scratch is None else _ptr(scratch), 0 if scratch is None else scratch.numel())
 
     return KernelDefinition(

@@ -304,6 +304,27 @@ def test_paged_kv_append_zero_rows_and_large_values(gpu):
     assert bool((v[0, :, 1].float().abs() == 448).all()) and bool(torch.isfinite(vs).all())
 
 
+@pytest.mark.gpu
+def test_paged_kv_append_values_that_are_not_finite(gpu):
+    """fp8: a head that holds an infinity or NaN reads as NaN, its neighbours as without it."""
+    heads = list(_heads(7, "bf16", 6, 2, 2, 64, 0, "k", strided=False))
+    clean = [h.clone() for h in heads]
+    heads[1], heads[2] = heads[1].clone(), heads[2].clone()
+    heads[1][3, 0, 1] = float("nan")
+    heads[2][1, 0, 3], heads[2][2, 1, 63], heads[2][4, 1, 0] = float("nan"), float("inf"), float("-inf")
+    results = []
+    for h in (heads, clean):
+        caches = _cuda(*_caches(_gen(1), "bf16", True, 1, 2, 8, 64))
+        _compile("paged_kv_append", "bf16", True).run(*_cuda(*h, torch.arange(6, dtype=torch.int32)), *caches)
+        k, v, ks, vs = (c.cpu() for c in caches)
+        results.append((k[0, :, :6].float() * ks[0, :, :6, None], v[0, :, :6].float() * vs[0, :, :6, None]))
+    for got, want, bad in zip(*results, ([(0, 3)], [(0, 1), (1, 2), (1, 4)])):
+        held = torch.zeros(2, 6, dtype=torch.bool)
+        for head, token in bad:
+            held[head, token] = True
+        assert bool(got[held].isnan().all()) and torch.equal(got[~held], want[~held])
+
+
 # ---- attention -------------------------------------------------------------------------
 
 ATTENTION_CASES = [
@@ -862,6 +883,9 @@ INVALID, ALIGN, UNSUPPORTED = errors.INTENT_ERR_INVALID_ARGUMENT, errors.INTENT_
     ("intent_paged_attention", _attention_args, INVALID, dict(HK=0)),
     ("intent_paged_attention", _attention_args, INVALID, dict(window=-1)),
     ("intent_paged_attention", _attention_args, INVALID, dict(kv=None)),
+    ("intent_paged_attention", _attention_args, INVALID, dict(scale=float("nan"))),
+    ("intent_paged_attention", _attention_args, INVALID, dict(scale=float("-inf"))),
+    ("intent_paged_attention", _attention_args, INVALID, dict(scale=3e38)),
     ("intent_paged_attention", _attention_args, INVALID, dict(vs=None)),
     ("intent_paged_attention", _attention_args, INVALID, dict(out_ld=128)),
     ("intent_paged_attention", _attention_args, INVALID, dict(table_ld=2)),
