@@ -722,6 +722,56 @@ def test_captured_and_replayed(gpu, new):
 
 
 @pytest.mark.gpu
+def test_two_graphs_of_unprepared_calls(gpu):
+    """run() captured twice (decoding and a chunk, both split), the graphs replayed in turn and at once on two
+    streams, over lengths that change in place, with eager calls between."""
+    art = _compile("paged_attention", "bf16")
+    sets = [_attention_inputs(70 + i, "bf16", False, lens, 8, 2, 128, 16, poison=False)
+            for i, lens in enumerate(([(1, 3000), (1, 900)], [(60, 2500)]))]
+    device = [[t for t in _cuda(*s) if t is not None] for s in sets]
+    for d in device:
+        art.run(*d, 0.0884)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for d in device:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(art.run(*d, 0.0884))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for cut in (0, 700, 1300, 0):
+        eager = []
+        for d, s in zip(device, sets):
+            d[5].copy_((s[7] - cut).clamp(min=0).to(torch.int32))
+            eager.append(art.run(*d, 0.0884))
+        torch.cuda.synchronize()
+        for stream, graph in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for i, graph in enumerate(graphs):
+            assert torch.equal(outs[i], eager[i]), (cut, i)
+            outs[i].fill_(float("nan"))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(outs[i], eager[i]), (cut, i)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 80, 256])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_paged_attention_without_a_cache(gpu, D, fp8):
+    """A table of no pages, and a cache of none: nothing is seen, every row is zero."""
+    for new in (1, 5, 90):
+        inputs = list(_attention_inputs(33, "f16", fp8, [(new, 40)], 4, 2, D, 16, poison=False))
+        inputs[5] = inputs[5][:, :0]
+        assert bool((_run_attention(inputs, "f16", fp8, 0.1, True, 0) == 0).all())
+        inputs[5] = torch.zeros(1, 3, dtype=torch.int32)
+        inputs[1:5] = [None if c is None else c[:0] for c in inputs[1:5]]
+        assert bool((_run_attention(inputs, "f16", fp8, 0.1, True, 0) == 0).all())
+
+
+@pytest.mark.gpu
 def test_two_streams_at_once(gpu):
     """Calls of one artifact on two streams, in flight together, share nothing."""
     art = _compile("paged_attention", "f16")
