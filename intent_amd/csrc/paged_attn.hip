@@ -169,7 +169,10 @@ bool tiled(int64_t D) { return D == 64 || D == 96 || D == 128 || D == 256; }
 
 // The host knows the extents only. Sequences of one new token each, one sequence, or as many new tokens as
 // equal chunks make: all alike, and the kernel that spreads the tokens over the waves takes up to 64 rows
-// of them in the tile that holds one (heads of 256 leave it registers for 16), the other kernel more. Any
+// of them in the tile that holds one, the other kernel more. Heads of 256 leave it registers for 16 rows:
+// up to 32 rows still do better in two of those tiles than in half of a tile of 128 (24 rows of 16 sequences
+// over 5000 tokens: 51 and 57 us, in 8 bits 32 and 48; 40 rows 125 and 59), and so do fewer than 512 rows in
+// all (400 of one head over 4000: 26 and 37; 312 of 13 sequences 129 and 47). Any
 // other batch may mix decoding sequences with chunks: beyond 2048 rows in all, each sequence goes by its
 // own rows to one of the two, which a chunk of 900 tokens among 63 decoding sequences repays several
 // times; fewer rows do not repay the launches (12 sequences of 1 to 24 tokens, 460 rows: 19 us in one, 32
@@ -182,8 +185,9 @@ bool tiled(int64_t D) { return D == 64 || D == 96 || D == 128 || D == 256; }
 // tiles of 128; 2048 x 4 over 2048: 71 and 59).
 Plan plan_of(int64_t T, int64_t S, int64_t HK, int64_t group, int64_t D) {
   const int64_t mean = (T * group + S - 1) / S;
-  const int most = D > 128 ? 16 : 64, few = D > 128 || group <= 16 ? 16 : 32;
-  const int tile = D > 128 || T * group * HK < 384 * 256 ? (D > 128 || T * group * HK >= 22 * 128 ? 128 : 64) : 256;
+  const int most = D > 128 ? 32 : 64, few = D > 128 || group <= 16 ? 16 : 32;
+  const int64_t all = T * group * HK;
+  const int tile = D > 128 ? (all < 4 * 128 ? 16 : 128) : all < 22 * 128 ? 64 : all < 384 * 256 ? 128 : 256;
   Plan p{};
   if (T > S && T % S != 0 && T * group > 2048) {
     p.parts = 2;
@@ -191,7 +195,8 @@ Plan plan_of(int64_t T, int64_t S, int64_t HK, int64_t group, int64_t D) {
     p.part[1] = {few, 0, few};
   } else {
     p.parts = 1;
-    p.part[0] = {mean <= 16 ? 16 : mean <= most ? (int)((mean + 15) / 16) * 16 : tile, 0, INT32_MAX};
+    const int few_rows = D > 128 ? 16 : (int)((mean + 15) / 16) * 16;
+    p.part[0] = {mean <= 16 ? 16 : mean <= most ? few_rows : tile, 0, INT32_MAX};
   }
   return p;
 }
@@ -202,10 +207,21 @@ int64_t tiles_bound(const Part& p, int64_t T, int64_t S, int64_t group) {
   return p.max_rows <= p.rows ? some : T * group / p.rows + some;
 }
 
+// Shares of one head that its tiles are split for. Sequences of a tile each that take half the GPU and more
+// as they are: with heads of 256, whose tiles have a CU to themselves, lengths that differ leave a second
+// round of a few long shares, so twice as many (111 sequences of 2600 to 7500 tokens on two heads: 612 us
+// with 256 shares, 401 with 512; 128 of them 570 and 434; all of 5000 332 and 360). More tiles to a sequence
+// even out by themselves.
+int64_t target_of(const Part& p, int64_t T, int64_t S, int64_t group, int64_t HK, int64_t D) {
+  const int64_t fill = p.fill(D);
+  const bool uneven = D > 128 && p.rows == 128 && T * group <= S * p.rows && S * HK * 2 > fill;
+  return (fill * (uneven ? 2 : 1) + HK - 1) / HK;
+}
+
 // Parts of all split tiles of one head: fewer than twice the target (a tile of one and a half shares and
 // more is cut to the nearest number of them), and at most every tile's most.
 int64_t slots_bound(const Part& p, int64_t T, int64_t S, int64_t group, int64_t HK, int64_t D, int64_t most_kv) {
-  const int64_t target = (p.fill(D) + HK - 1) / HK;
+  const int64_t target = target_of(p, T, S, group, HK, D);
   int64_t splits = (most_kv + (1 << p.unit_log()) - 1) >> p.unit_log();
   if (splits > kMostSplits) splits = kMostSplits;
   if (splits < 2) return 0;
@@ -230,7 +246,7 @@ int launch_tiled(AttnArgs a, bool bf16, bool fp8, float* workspace, size_t bytes
     const bool many = a.S == 1 && (int64_t)a.T * a.group / p.rows * a.HK >= 2 * p.fill(a.D);
     const bool split = slots > 0 && workspace != nullptr && bytes >= need && !many;
     a.min_rows = p.min_rows, a.max_rows = p.max_rows;
-    a.target = split ? (p.fill(a.D) + a.HK - 1) / a.HK : 0;
+    a.target = split ? (int)target_of(p, a.T, a.S, a.group, a.HK, a.D) : 0;
     a.slots = split ? (int)slots : 0;
     a.partial = workspace;
     a.partial_stats = split ? workspace + slots * a.HK * p.rows * a.D : nullptr;

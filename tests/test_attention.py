@@ -369,6 +369,10 @@ ATTENTION_CASES = [
     ("bf16", False, [(300, 500), (400, 420)], 8, 1, 96, 16, True, 0),
     ("f16", False, [(40, 300), (1, 500), (2, 30), (90, 90)], 4, 2, 256, 32, True, 0),
     ("bf16", False, [(1, 40 + 13 * i) for i in range(70)] + [(0, 5)] * 60 + [(2, 30)], 4, 2, 64, 16, True, 0),
+    # heads of 256: two tiles of 16 rows, fewer than 512 rows, and a round of uneven sequences
+    ("f16", True, [(3, 300), (3, 90)], 16, 2, 256, 16, True, 0),
+    ("bf16", False, [(60, 200), (60, 400)], 3, 1, 256, 32, True, 50),
+    ("bf16", True, [(7, 60 + 900 * (i % 17 == 3)) for i in range(70)], 16, 2, 256, 16, True, 0),
     # more sequences than a wave takes at once, one of them split
     ("f16", False, [(1, 1 + 7 * i % 40) for i in range(555)] + [(1, 9000), (1, 0)] + [(1, 33)] * 60, 2, 1, 64, 16, True, 0),
     ("bf16", True, [(4, 4 + i % 30) for i in range(300)] + [(700, 900)] + [(1, 50)] * 5, 4, 1, 64, 16, True, 0),
