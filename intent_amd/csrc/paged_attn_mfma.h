@@ -11,9 +11,15 @@
 //
 // Running softmax in base 2: weights w = exp2(t - M) with t the score times scale log2(e). M follows
 // the maximum only when that has risen by 8, so weights reach 2^8 at most and the sums are rescaled
-// rarely; in f32 and in 16-bit weights this costs no precision. With an 8-bit cache the value's scale
-// is part of the weight that is rounded: M follows the maximum of t + log2(scale), w = exp2(t - M) *
-// scale, and only the sum of weights takes exp2(t - M) by itself. The codes are exact in 16 bits.
+// rarely. With an 8-bit cache the value's scale is part of the weight that is rounded: M follows the
+// maximum of t + log2(scale), w = exp2(t - M) * scale, and only the sum of weights takes exp2(t - M) by
+// itself. The codes are exact in 16 bits.
+//
+// The product with the values takes the weights rounded to the heads' type, half a step of it each, like
+// the values beside them; the sums of weights are those before the rounding. bf16 has the exponents of
+// f32. f16 ends at 2^-24, and a long flat tail behind one token that outweighs it may lie below: there all
+// weights are 2^kLift higher (2^15 at most), so each is off by half a step or by 2^-32 of the highest, and
+// numerators, sums and parts alike carry the factor, which their quotient drops.
 //
 // A weight of zero does not keep an infinity or NaN out of a product. Values of tokens that no row of a
 // tile sees (pages behind a sequence's end hold anything) are set to zero; where rows of a tile see
@@ -30,6 +36,8 @@ namespace attn {
 using ::load16;
 
 constexpr float kRise = 8.0f;
+template <bool kBf16>
+constexpr float kLift = kBf16 ? 0.f : 7.f;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -147,8 +155,11 @@ INTENT_DEVICE void wave_lds_order() {
   __builtin_amdgcn_wave_barrier();
 }
 
-// max(log2|scale|, -100): the bound keeps exp2(t - M) finite beside tokens of zeros.
-INTENT_DEVICE float scale_exponent(float v) { return fmaxf(__builtin_amdgcn_logf(fabsf(v)), -100.0f); }
+// log2|scale|, bounded so that sums of exp2(t - M), 2^(100 + kRise) at most, stay finite beside tokens of zeros.
+template <bool kBf16>
+INTENT_DEVICE float scale_exponent(float v) {
+  return fmaxf(__builtin_amdgcn_logf(fabsf(v)), kLift<kBf16> - 100.0f);
+}
 
 // Where one query row of a tile (column r of S^T) stands: the tokens lo <= t < hi that it sees.
 struct RowView {
@@ -367,7 +378,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
         if (g == 0) {
           scales[wave][0][u * 16 + col] = ks[u] * scale;
           scales[wave][1][u * 16 + col] = vs[u];
-          scales[wave][2][u * 16 + col] = scale_exponent(vs[u]);
+          scales[wave][2][u * 16 + col] = scale_exponent<kBf16>(vs[u]);
         }
       }
     }
@@ -433,7 +444,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[m][d] *= keep;
       }
-      const float base = ref[m] == -INFINITY ? 0.f : ref[m];
+      const float base = (ref[m] == -INFINITY ? 0.f : ref[m]) - kLift<kBf16>;
       float wt[2][4];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -687,7 +698,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
       if (wave == 0) {
         scales[buffer][0][lane] = ks * scale;
         scales[buffer][1][lane] = vs;
-        scales[buffer][2][lane] = scale_exponent(vs);
+        scales[buffer][2][lane] = scale_exponent<kBf16>(vs);
       }
     }
   };
@@ -798,7 +809,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[d][r] *= keep;
       }
-      const float base = ref == -INFINITY ? 0.f : ref;
+      const float base = (ref == -INFINITY ? 0.f : ref) - kLift<kBf16>;
       // Sixteen steps, each with the weights of two tokens, its part of the next tokens' products with the
       // queries (kAhead; of what lies in that buffer behind the last tokens, too: not used then) and, four
       // steps behind, of the products with these values, so that the matrix unit works through all of them.

@@ -619,6 +619,65 @@ def test_paged_attention_without_a_workspace(gpu, new, HQ, kv, PAGE, D, fp8):
     assert "splits" in _native.last_kernel()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,HQ,D,n", [(1, 4, 64, 30000), (7, 8, 96, 20000), (1, 1, 256, 20000), (352, 8, 64, 9000),
+                                         (352, 8, 128, 9000), (64, 8, 256, 9000)])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_paged_attention_one_token_over_a_flat_tail(gpu, new, HQ, D, n, fp8):
+    """f16: the first token outweighs each of the others by about 2^26.5 and its value is zero, so the output is
+    what the others' weights leave. A weight is off by half a step of the type, or by 2^-32 of the highest (2^-25
+    where that is 2^7), not by 2^-25 of it."""
+    inputs = list(_attention_inputs(34, "f16", fp8, [(new, n)], HQ, 1, D, 16, poison=False, q_std=0.3))
+    q, k, v, ks, vs, table = inputs[:6]
+    gen, scale = _gen(2), D ** -0.5
+    q[..., 0] = 4.0
+    high = 26.5 * math.log(2) / (4.0 * scale)
+    tail = (64 + _randn(gen, *v.shape, std=16)).clamp(8, 128)
+    page = int(table[0, 0])
+    if fp8:
+        ks.fill_(0.01), vs.copy_(0.9 + 0.2 * torch.rand(vs.shape, generator=gen))
+        v.copy_(tail.to(F8))
+        k[..., 0], k[page, 0, 0] = 0, 0
+        k[page, 0, 0, 0] = 448
+        ks[page, 0, 0] = high / 448
+    else:
+        v.copy_(tail.half())
+        k[..., 0], k[page, 0, 0] = 0, 0
+        k[page, 0, 0, 0] = high
+    v[page, 0, 0] = 0
+    want, _ = ref_attention(*inputs, scale, True, 0)
+    big = 128 * (1.1 if fp8 else 1.0)
+    keys = k.double() if ks is None else k.double() * ks.double()[..., None]
+    off = scale * (keys.abs() @ q.double().abs().amax((0, 1))).amax()
+    # the values are positive, so size = |out|: weights and output by 2^-11, scores (twice), exponentials, sums
+    tol = want * (2 * 2.0 ** -11 + 2 * (D + 4) * 2.0 ** -24 * off + 2.0 ** -21 + 2 * n * 2.0 ** -24) + 2.0 ** -25
+    tol += n * 2.0 ** -32 * big
+    assert 0.002 < float(want.min()) and float((tol / want).max()) < 0.06
+    _close(_run_attention(inputs, "f16", fp8, scale, True, 0), want, tol)
+    dq, dk, dv, dks, dvs, dtable, offsets, lens = _cuda(*inputs)
+    out = torch.full_like(dq, float("nan"))
+    scales = (dks.data_ptr(), dks.stride(0), dvs.data_ptr(), dvs.stride(0)) if fp8 else (None, 0, None, 0)
+    _native.call("intent_paged_attention", dq.data_ptr(), new, HQ, dq.stride(0), 0, int(fp8), dk.data_ptr(), dk.stride(0),
+                 dv.data_ptr(), dv.stride(0), *scales, dk.shape[0], 1, 16, D, dtable.data_ptr(), 1, dtable.shape[1],
+                 dtable.stride(0), offsets.data_ptr(), lens.data_ptr(), scale, 1, 0, out.data_ptr(), out.stride(0),
+                 None, 0, torch.cuda.current_stream().cuda_stream)
+    _close(out, want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,n", [(1, 20000), (352, 5000)])
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+def test_paged_attention_fp8_values_of_zero(gpu, new, n, dt):
+    """Value scales of zero throughout, and scores that rise: the sums of weights stay finite, every row is zero."""
+    inputs = list(_attention_inputs(35, dt, True, [(new, n)], 8, 1, 64, 16, poison=False))
+    q, k, ks, table = inputs[0], inputs[1], inputs[3], inputs[5]
+    q[..., 0], k[..., 0] = 4.0, 64.0
+    t = torch.arange(n)
+    ks[table[0, t // 16].long(), 0, t % 16] = t / n
+    inputs[4].zero_()
+    assert bool((_run_attention(inputs, dt, True, 0.5, True, 0) == 0).all())
+
+
 # ---- together --------------------------------------------------------------------------
 
 @pytest.mark.gpu
