@@ -185,6 +185,10 @@ INTENT_DEVICE u32x4 signed_query(const AttnArgs& a, u32x4 v) {
   return u32x4{v[0] ^ flip, v[1] ^ flip, v[2] ^ flip, v[3] ^ flip};
 }
 
+// The size of the scale; instead of zero the smallest f32, which moves no finite score by more than 2^-20 and
+// leaves a masked one at -inf.
+INTENT_DEVICE float scale_of(const AttnArgs& a) { return fmaxf(fabsf(a.scale_log2), 0x1p-149f); }
+
 INTENT_DEVICE float max_across16(float v) {
   const auto r = __builtin_amdgcn_permlane16_swap(bit_cast<uint32_t>(v), bit_cast<uint32_t>(v), false, false);
   return fmaxf(bit_cast<float>(r[0]), bit_cast<float>(r[1]));
@@ -247,7 +251,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
   // the tokens that some row sees, and those that all rows see
   const RowView top = row_view(a, w, 0), bottom = row_view(a, w, w.rows - 1);
   const int some_lo = top.lo, some_hi = bottom.hi, all_lo = bottom.lo, all_hi = top.hi;
-  const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);  // -inf stays what it is beside a scale of 0
+  const float scale = scale_of(a);
 
   f32x4 o[MT][DT];
   float ref[MT], total[MT];
@@ -582,7 +586,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
   const int some_lo = first.lo, some_hi = last.hi, all_lo = last.lo, all_hi = first.hi;
   const RowView top = row_view(a, w, r0), bottom = row_view(a, w, r0 + 31);  // of this wave
   const bool idle = r0 >= w.rows;
-  const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);  // -inf stays what it is beside a scale of 0
+  const float scale = scale_of(a);
 
   f32x16 o[DT];
 #pragma unroll

@@ -678,6 +678,21 @@ def test_paged_attention_fp8_values_of_zero(gpu, new, n, dt):
     assert bool((_run_attention(inputs, dt, True, 0.5, True, 0) == 0).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [0.0, 3e-36, -3e-36])
+@pytest.mark.parametrize("new,D", [(1, 64), (100, 128), (3, 80)])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_paged_attention_scales_beside_large_scores(gpu, new, D, fp8, scale):
+    """A scale far below one is taken as it is where q.k is as large as bf16 heads make it, zero as zero."""
+    inputs = list(_attention_inputs(36, "bf16", fp8, [(new, 300)], 8, 2, D, 16, poison=False, q_std=1e17))
+    if fp8:
+        inputs[3].mul_(1e17)
+    else:
+        inputs[1].mul_(1e17)
+    want, tol = ref_attention(*inputs, scale, True, 0)
+    _close(_run_attention(inputs, "bf16", fp8, scale, True, 0), want, tol)
+
+
 # ---- together --------------------------------------------------------------------------
 
 @pytest.mark.gpu
