@@ -50,7 +50,7 @@ class _Layout:
 
     Everything the checks of ``_bind`` derive from those alone: a call with the same
     combination needs only its addresses compared (``pairs``: the views of which one is
-    writable, spans in bytes)."""
+    writable, and how their rows may lie between one another's; spans in bytes)."""
 
     env: dict
     names: tuple        # the supplied views, in argument order
@@ -143,8 +143,9 @@ class HIPRuntime:
             tensors = arguments
         if known.pairs:
             starts = [t.data_ptr() for t in tensors]
-            for i, j in known.pairs:
-                if starts[i] < starts[j] + known.spans[j] and starts[j] < starts[i] + known.spans[i]:
+            for i, j, rows in known.pairs:
+                if (starts[i] < starts[j] + known.spans[j] and starts[j] < starts[i] + known.spans[i]
+                        and not _rows_apart(rows, starts[i], starts[j])):
                     return None  # _bind names the overlap
         views = dict(zip(known.names, tensors))
         if known.outputs:
@@ -168,7 +169,8 @@ class HIPRuntime:
             return
         views = [(p, a) for p, a in zip(params, arguments) if p.name not in self._scalars]
         spans = tuple(_span_bytes(t) for _, t in views)
-        pairs = tuple((i, j) for i in range(len(views)) for j in range(i + 1, len(views))
+        pairs = tuple((i, j, _row_pair(views[i][1], views[j][1]))
+                      for i in range(len(views)) for j in range(i + 1, len(views))
                       if spans[i] and spans[j]
                       and (views[i][0].name in self._writable or views[j][0].name in self._writable))
         made = () if supplied_outputs else tuple((p.name, tuple(binding.views[p.name].shape), binding.views[p.name].dtype)
@@ -278,7 +280,8 @@ class HIPRuntime:
             raise ValueError(f"{p.name} must be contiguous")
 
     def _check_aliases(self, views: dict) -> None:
-        """Writable views may not overlap any other view (noalias contract)."""
+        """Writable views may not share an element with any other view (noalias contract). Views whose rows
+        lie between one another's (keys and values of one allocation, slices of one row) share none."""
         writable = self._writable
         spans = {}
         for name, t in views.items():
@@ -292,7 +295,7 @@ class HIPRuntime:
                 if a not in writable and b not in writable:
                     continue
                 (s0, e0), (s1, e1) = spans[a], spans[b]
-                if s0 < e1 and s1 < e0:
+                if s0 < e1 and s1 < e0 and not _rows_apart(_row_pair(views[a], views[b]), s0, s1):
                     raise ValueError(f"{self.definition.name}: {a} and {b} overlap; writable views must not alias")
 
     def _needs(self, env: dict) -> tuple[int, int]:
@@ -378,6 +381,25 @@ def _span_bytes(t) -> int:
     if t.numel() == 0:
         return 0
     return (sum((extent - 1) * stride for extent, stride in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _row_pair(a, b) -> tuple | None:
+    """(bytes from a row to the next, bytes of a row of `a`, of `b`) where the first axes of two views of at
+    least one element step alike (a view of one row steps like any), else None."""
+    steps = {t.stride(0) * t.element_size() for t in (a, b) if t.dim() and t.shape[0] > 1}
+    if len(steps) != 1 or 0 in steps:
+        return None
+    return steps.pop(), _span_bytes(a[0] if a.dim() else a), _span_bytes(b[0] if b.dim() else b)
+
+
+def _rows_apart(pair: tuple | None, a: int, b: int) -> bool:
+    """Whether no row of the view that starts at address `a` meets one of the view at `b`: modulo the step, the
+    second's rows begin behind the first's and end before the first's next."""
+    if pair is None:
+        return False
+    step, a_row, b_row = pair
+    behind = (b - a) % step
+    return behind >= a_row and step - behind >= b_row
 
 
 def _result(outputs: tuple):

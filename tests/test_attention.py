@@ -16,6 +16,7 @@ import torch
 
 import intent_amd as intent
 from intent_amd import _native, errors
+from intent_amd import runtime as runtime_module
 from intent_amd.runtime import HIPRuntime
 
 TYPES = {"f16": torch.float16, "bf16": torch.bfloat16}
@@ -835,6 +836,46 @@ def test_two_graphs_of_unprepared_calls(gpu):
             assert torch.equal(outs[i], eager[i]), (cut, i)
 
 
+def _combined(gen, dt, fp8, pages, HK, PAGE, D):
+    """One allocation of keys and values side by side in each page [pages, 2, HK, PAGE, D] (and their scales)."""
+    x = _randn(gen, pages, 2, HK, PAGE, D)
+    kv = (x * 100).clamp(-448, 448).to(F8) if fp8 else x.to(TYPES[dt])
+    return (kv, torch.rand(pages, 2, HK, PAGE, generator=gen) * 0.01 + 0.002) if fp8 else (kv,)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [7, 900])
+@pytest.mark.parametrize("dt,fp8", [("f16", False), ("bf16", True)])
+def test_keys_and_values_of_one_allocation(gpu, dt, fp8, T):
+    """Append and attention over kv[:, 0] and kv[:, 1]: both halves get their own rows, all others stay."""
+    HQ, HK, D, PAGE, pages = 8, 2, 64, 16, 70
+    gen = _gen(45)
+    heads = _heads(46, dt, T, HQ, HK, D, 0, "")
+    slots = torch.randperm(pages * PAGE, generator=gen)[:T].to(torch.int32)
+    tensors = _combined(gen, dt, fp8, pages, HK, PAGE, D)
+    apart = [t[:, i].clone().contiguous() for t in tensors for i in (0, 1)]
+    device, alone = _cuda(*tensors), _cuda(*apart)
+    views = [t[:, i] for t in device for i in (0, 1)]
+    append = _compile("paged_kv_append", dt, fp8)
+    args = _cuda(*heads, slots)
+    for _ in range(2):  # bound, and known
+        q_out = append.run(*args, *views)
+    assert torch.equal(q_out, append.run(*args, *alone))
+    for got, want in zip(views, alone):
+        assert torch.equal(got.contiguous().view(torch.uint8), want.view(torch.uint8))
+    table = torch.randperm(pages, generator=gen).to(torch.int32)[None]
+    rest = _cuda(table, torch.tensor([0, T], dtype=torch.int32), torch.tensor([pages * PAGE - 3], dtype=torch.int32))
+    attend = _compile("paged_attention", dt, fp8)
+    out = attend.run(q_out, *views, *rest, 0.125)
+    assert torch.equal(out, attend.run(q_out, *alone, *rest, 0.125))
+    # and an output between the queries of one buffer
+    wide = torch.zeros(T, 2, HQ, D, dtype=TYPES[dt], device="cuda")
+    wide[:, 0] = q_out
+    for _ in range(2):
+        attend(wide[:, 0], *views, *rest, wide[:, 1], 0.125)
+    assert torch.equal(wide[:, 0], q_out) and torch.equal(wide[:, 1], out)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("D", [64, 80, 256])
 @pytest.mark.parametrize("fp8", [False, True])
@@ -953,6 +994,52 @@ def test_layouts_are_checked(monkeypatch):
         rt._check_layout(param["k_cache"], cache[:, :, 0, :])
     with pytest.raises(ValueError, match="smaller than the row"):
         rt._check_layout(param["q"], q[:1].expand(5, 6, 64))
+
+
+def test_views_between_one_another_are_taken(monkeypatch):
+    """Keys and values of one allocation, and outputs of one row, share no element; views that do are refused
+    on the first call and on a known layout."""
+    rt = runtime_for("paged_kv_append_fp8")
+    rt._home = torch.device("cpu")
+    monkeypatch.setattr(rt, "_launch", lambda binding: None)
+    q, k, v, qw, kw, table, positions = _heads(1, "f16", 5, 6, 2, 64, 32, "qk")
+    kv, scales = _combined(_gen(1), "f16", True, 4, 2, 8, 64)
+    slots = torch.zeros(5, dtype=torch.int32)
+    args = (q, k, v, qw, kw, table, positions, slots, kv[:, 0], kv[:, 1], scales[:, 0], scales[:, 1])
+    assert rt.rebind(args, False) is None
+    rt.run(*args)
+    assert rt.rebind(args, False) is not None
+    swapped = args[:8] + (kv[:, 1], kv[:, 0], scales[:, 1], scales[:, 0])
+    assert rt.rebind(swapped, False) is not None
+    row = kv.stride(0)
+
+    def refused(a, b):
+        for _ in range(2):
+            change = args[:8] + (a, b) + args[10:]
+            assert rt.rebind(change, False) is None
+            with pytest.raises(ValueError, match="k_cache and v_cache overlap"):
+                rt.run(*change)
+
+    flat = torch.zeros(5 * row, dtype=torch.uint8).view(F8)
+    part = [flat[at:at + 4 * row].view(4, 2, 2, 8, 64)[:, 0] for at in (0, row // 2, row // 2 - 16, row // 2 + 16, 16)]
+    rt.run(*args[:8], part[0], part[1], *args[10:])  # the rows fill the step exactly
+    for other in (part[0], part[2], part[3], part[4]):
+        refused(part[0], other)
+    attend = runtime_for("paged_attention")
+    attend._home = torch.device("cpu")
+    monkeypatch.setattr(attend, "_launch", lambda binding: None)
+    inputs = [t for t in _attention_inputs(1, "f16", False, [(2, 9), (1, 3)], 4, 2, 64, 4) if t is not None]
+    rows = torch.zeros(3, 2, 4, 64, dtype=torch.float16)
+    attend.launch(rows[:, 0], *inputs[1:], rows[:, 1], 0.1)
+    assert attend.rebind((rows[:, 0], *inputs[1:], rows[:, 1], 0.1), True) is not None
+    with pytest.raises(ValueError, match="overlap"):
+        attend.launch(rows[:, 0], *inputs[1:], rows[:, 0], 0.1)
+    with pytest.raises(ValueError, match="overlap"):  # steps that differ: rows meet further on
+        attend.launch(rows[:, 0], *inputs[1:], rows.view(-1)[256:256 + 768].view(3, 4, 64), 0.1)
+    single = rows[1:2, 1]  # a view of one row, between or within the rows of the other
+    assert runtime_module._rows_apart(runtime_module._row_pair(rows[:, 0], single), rows.data_ptr(), single.data_ptr())
+    assert not runtime_module._rows_apart(runtime_module._row_pair(rows[:, 1], single), rows[:, 1].data_ptr(),
+                                          single.data_ptr())
 
 
 FAKE = 0x1000
