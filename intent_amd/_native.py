@@ -157,7 +157,14 @@ class _Slots:
         types = SIGNATURES[entry][0][:-1]
         self.number = number
         self.count = len(types)
-        self.pack = struct.Struct("<" + "".join("f4x" if t is F32 else "q" for t in types)).pack
+        self.entry = entry
+        self._pack = struct.Struct("<" + "".join("f4x" if t is F32 else "q" for t in types)).pack
+
+    def pack(self, arguments) -> bytes:
+        try:
+            return self._pack(*arguments)
+        except OverflowError as error:  # no f32 holds the scalar
+            raise ValueError(f"{self.entry}: {error}") from None
 
 
 RECORDS = {entry: _Slots(number, entry)
@@ -167,7 +174,7 @@ RECORDS = {entry: _Slots(number, entry)
 def call_packed(entry: str, arguments: tuple, stream: int) -> None:
     """``call`` of one of the entries in RECORDS; null pointers are 0."""
     slots = RECORDS[entry]
-    status = library().intent_amd_replay(slots.number, slots.pack(*arguments), slots.count, stream)
+    status = library().intent_amd_replay(slots.number, slots.pack(arguments), slots.count, stream)
     if status != INTENT_OK:
         raise status_error(status, entry, last_error())
 
@@ -182,7 +189,7 @@ class Record:
         self.entry = entry
         self._number = slots.number
         self._count = slots.count
-        self._slots = slots.pack(*(0 if a is None else a for a in arguments))
+        self._slots = slots.pack(0 if a is None else a for a in arguments)
         self._replay = library().intent_amd_replay
 
     def __call__(self, stream: int) -> None:

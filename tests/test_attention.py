@@ -1143,3 +1143,14 @@ def test_replayed_calls_are_checked():
     assert status("intent_amd_replay", 0, slots, 4, None) == INVALID and "slots" in _native.last_error()
     assert status("intent_amd_replay", 9, slots, 4, None) == INVALID
     assert status("intent_amd_replay", 0, None, 22, None) == INVALID
+
+
+def test_scalars_past_32_bits_are_refused():
+    """A scale or epsilon that no f32 holds is refused like one that is not finite."""
+    for scale in (1e39, -1e300):
+        with pytest.raises(ValueError, match="intent_paged_attention"):
+            _native.Record("intent_paged_attention", tuple(_attention_args(scale=scale)[:-1]))(0)
+        with pytest.raises(ValueError, match="intent_paged_attention"):
+            _native.call_packed("intent_paged_attention", tuple(a or 0 for a in _attention_args(scale=scale)[:-1]), 0)
+    with pytest.raises(ValueError, match="intent_qk_norm_rope"):
+        _native.Record("intent_qk_norm_rope", tuple(_norm_args(eps=1e40)[:-1]))
