@@ -292,6 +292,29 @@ def test_paged_kv_append(gpu, case):
         assert torch.equal(_slot_rows(after[1], slots).view(torch.uint8), codes.view(torch.uint8))
 
 
+# Prompts: two heads to a lane group (2^20 lanes and more), of one kind or at the seams between queries, keys and
+# values, and an odd one left over.
+PROMPT_CASES = [
+    # dtype, fp8, T, HQ, HK, D, R, interleaved, norms, page size, pages
+    ("f16", False, 18733, 3, 2, 64, 64, False, "qk", 16, 1175), ("bf16", True, 18733, 3, 2, 64, 32, True, "q", 64, 300),
+    ("bf16", False, 6561, 4, 3, 96, 96, False, "k", 32, 206), ("f16", True, 13109, 3, 1, 128, 128, False, "qk", 128, 104),
+    ("bf16", False, 3641, 5, 2, 192, 64, True, "qk", 256, 15), ("bf16", True, 6560, 1, 2, 256, 128, False, "", 16, 411),
+    ("f16", True, 1827, 7, 1, 512, 512, False, "qk", 8, 240), ("f16", False, 65537, 0, 1, 64, 0, False, "", 2, 32800),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", PROMPT_CASES, ids=lambda c: "-".join(map(str, c)))
+def test_prompts(gpu, case):
+    dt, fp8, T, HQ, HK, D, R, interleaved, norms, _, _ = case
+    test_paged_kv_append(gpu, case)
+    assert "2 heads" in _native.last_kernel()
+    lanes = 8 if D <= 64 else 16 if D <= 128 else 32 if D <= 256 else 64
+    more = -(-2 ** 20 // (lanes * (HQ + HK)))  # without the values
+    test_qk_norm_rope(gpu, (dt, more + 5, HQ, HK, D, R, interleaved, norms))
+    assert "2 heads" in _native.last_kernel()
+
+
 @pytest.mark.gpu
 def test_paged_kv_append_zero_rows_and_large_values(gpu):
     """fp8: a zero head gets the smallest scale and zero codes; the largest values stay finite."""
@@ -694,6 +717,32 @@ def test_paged_attention_scales_beside_large_scores(gpu, new, D, fp8, scale):
     _close(_run_attention(inputs, "bf16", fp8, scale, True, 0), want, tol)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,D,fp8", [(50003, 64, False), (131000, 128, True)])
+def test_paged_attention_most_parts(gpu, n, D, fp8):
+    """One sequence over more units of tokens than a tile is cut into parts (256)."""
+    inputs = _attention_inputs(37, "bf16", fp8, [(1, n)], 4, 1, D, 64, poison=False)
+    want, tol = ref_attention(*inputs, D ** -0.5, True, 0)
+    _close(_run_attention(inputs, "bf16", fp8, D ** -0.5, True, 0), want, tol)
+    assert "splits" in _native.last_kernel()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+@pytest.mark.parametrize("chunk,spare", [(138, 0), (137, 0), (130, 7), (129, 7)])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_paged_attention_decoding_beside_a_chunk(gpu, chunk, spare, D, fp8):
+    """Seven decoding sequences and a chunk, whose tokens (and padded rows) are a multiple of the sequences or not:
+    one list of tiles or two."""
+    lens = [(1, 60 + 97 * i) for i in range(4)] + [(chunk, chunk + 300)] + [(1, 1200), (1, 1), (1, 333)]
+    for window in (0, 200):
+        inputs = _attention_inputs(38, "f16", fp8, lens, 16, 1, D, 16, spare=spare)
+        want, tol = ref_attention(*inputs, D ** -0.5, True, window)
+        got = _run_attention(inputs, "f16", fp8, D ** -0.5, True, window)
+        rows = sum(n for n, _ in lens)
+        _close(got[:rows], want[:rows], tol[:rows])
+
+
 # ---- together --------------------------------------------------------------------------
 
 @pytest.mark.gpu
@@ -915,6 +964,22 @@ def test_as_torch_op(gpu):
     art = _compile("paged_attention", "f16")
     op = art.as_torch_op("intent_amd_attention_test::paged_attention")
     assert torch.equal(op(*inputs, 0.125), art.run(*inputs, 0.125))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,fp8", [("f16", False), ("bf16", True)])
+def test_append_as_torch_op(gpu, dt, fp8):
+    """Caches and scales written in place; views of one storage are the artifact's, not the operator's."""
+    heads, slots = _cuda(*_heads(61, dt, 9, 4, 2, 64, 64, "qk")), torch.arange(3, 12, dtype=torch.int32, device="cuda")
+    first, second = (_cuda(*_caches(_gen(3), dt, fp8, 3, 2, 8, 64)) for _ in range(2))
+    art = _compile("paged_kv_append", dt, fp8)
+    op = art.as_torch_op(f"intent_amd_attention_test::{dt}_append_{int(fp8)}")
+    assert torch.equal(op(*heads, slots, *first), art.run(*heads, slots, *second))
+    for got, want in zip(first, second):
+        assert torch.equal(got.view(torch.uint8), want.view(torch.uint8))
+    kv = _cuda(*_combined(_gen(4), dt, fp8, 3, 2, 8, 64))
+    with pytest.raises(NotImplementedError, match="shares storage"):
+        op(*heads, slots, *(t[:, i] for t in kv for i in (0, 1)))
 
 
 # ---- refusals (CPU) --------------------------------------------------------------------
