@@ -76,6 +76,9 @@ INTENT_DEVICE Sequence sequence_of(const AttnArgs& a, int s) {
 INTENT_DEVICE int first_seen(const AttnArgs& a, int p) { return a.window > 0 && p >= a.window ? p - a.window + 1 : 0; }
 INTENT_DEVICE int end_seen(const AttnArgs& a, int p, int kv) { return a.causal ? min(max(p + 1, 0), kv) : kv; }
 
+// Parts of a tile. One sequence on one cached head would be cut further to fill the GPU, but its join goes through
+// the parts of a row in one workgroup: 131000 tokens take 40 us in 256 parts and 111 in 1024; on two heads 47 and
+// 68, on eight (fewer parts by themselves) 117 and 117.
 constexpr int kMostSplits = 256;
 
 // A workgroup's share: rows row0 .. row0 + rows of a sequence (row = new token * group + head of the
