@@ -705,8 +705,9 @@ int intent_qk_norm_rope(const void* q, int64_t T, int64_t HQ, int64_t q_ld,
  * scale = max(absmax, 1e-12) / 448 of a token's head, code = e4m3fn(clamp(y /
  * scale, +-448)), the rule of intent_fp8_groupwise_quantize for bf16 with one
  * group for each head; a head that holds an infinity or NaN reads as NaN.
- * Everything else in the cache stays as it is.
- * No reference counterpart.
+ * Everything else in the cache stays as it is. Page strides are whole 16 bytes
+ * (so pages of one token in 8 bits hold an even number of heads where D % 16 is
+ * 8); caches may lie between one another's pages. No reference counterpart.
  */
 int intent_paged_kv_append(const void* q, int64_t T, int64_t HQ, int64_t q_ld,
                            const void* k, int64_t HK, int64_t k_ld,
@@ -732,8 +733,9 @@ int intent_paged_kv_append(const void* q, int64_t T, int64_t HQ, int64_t q_ld,
  * a row that sees nothing (an empty cache, more new tokens than cached ones)
  * is zero, rows of no sequence are not written, and what a row does not see
  * does not reach it, whatever it holds. f32 scores, softmax and sums; the
- * weights are rounded to q's type for the product with the values. The scale is
- * finite.
+ * weights are rounded to q's type for the product with the values (in f16 to
+ * half a step or 2^-32 of the highest; heads off the MFMA kernels keep f32).
+ * The scale is finite.
  * Lengths, offsets and page ids are clamped to the tensors, never followed out
  * of them; offsets rise, and sequences whose rows overlap leave those rows
  * undefined. D % 8 == 0, D <= 512 (heads of 64, 96, 128 and 256 run the MFMA
