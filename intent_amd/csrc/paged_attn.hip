@@ -167,17 +167,17 @@ struct Plan {
 
 bool tiled(int64_t D) { return D == 64 || D == 96 || D == 128 || D == 256; }
 
-// The host knows the extents only. Sequences of one new token each, and one sequence, are all alike, and as
-// many new tokens as equal chunks make are taken to be: the kernel that spreads the tokens over the waves takes
-// up to 64 rows of them in the tile that holds one, the other kernel more. Heads of 256 leave it registers for 16 rows:
-// up to 32 rows still do better in two of those tiles than in half of a tile of 128 (24 rows of 16 sequences
-// over 5000 tokens: 51 and 57 us, in 8 bits 32 and 48; 40 rows 125 and 59), and so do fewer than 512 rows in
-// all (400 of one head over 4000: 26 and 37; 312 of 13 sequences 129 and 47). Any
-// other batch may mix decoding sequences with chunks: beyond 2048 rows in all, each sequence goes by its
-// own rows to one of the two; fewer rows do not repay the launches (12 sequences of 1 to 24 tokens, 460 rows:
-// 19 us in one, 32 in two). Short sequences are those of up to 16 rows, or up to 32 where more than 16 heads
-// share a cached one, so that decoding stays among them (15 decoding sequences and a chunk of 403, groups of
-// 24: 87 us, 92 with up to 16 rows; it loses with 63 of them, 120 and 112, and in groups of 32, 83 and 67).
+// The host knows the extents only. Sequences of one new token each, and one sequence, are all alike, and as many
+// new tokens as equal chunks make are taken to be: the kernel that spreads the tokens over the waves takes up to
+// 64 rows of them in the tile that holds one, the other kernel more. Heads of 256 leave it registers for 16
+// rows: up to 32 rows still do better in two of those tiles than in half of a tile of 128 (24 rows of 16
+// sequences over 5000 tokens: 51 and 57 us, in 8 bits 32 and 48; 40 rows 125 and 59), and so do fewer than 512
+// rows in all (400 of one head over 4000: 26 and 37; 312 of 13 sequences 129 and 47). Any other batch may mix
+// decoding sequences with chunks: beyond 2048 rows in all, each sequence goes by its own rows to one of the two;
+// fewer rows do not repay the launches (12 sequences of 1 to 24 tokens, 460 rows: 19 us in one, 32 in two).
+// Short sequences are those of up to 16 rows, or up to 32 where more than 16 heads share a cached one, so that
+// decoding stays among them (15 decoding sequences and a chunk of 403, groups of 24: 87 us, 92 with up to 16
+// rows; it loses with 63 of them, 120 and 112, and in groups of 32, 83 and 67).
 //
 // That the sequences divide the tokens is a guess at equal chunks, and a mixture (or a padded batch) may meet
 // it by chance. Both sides, one list and two, 32 heads on 8 of 128 over 1500 to 6000 cached tokens and over 50
