@@ -759,6 +759,81 @@ int intent_paged_attention(const void* q, int64_t T, int64_t HQ, int64_t q_ld,
 size_t intent_paged_attention_workspace_size(int64_t T, int64_t HQ, int64_t HK, int64_t D, int64_t S,
                                              int64_t table_width, int64_t page_size);
 
+/* How a paged cache holds its rows. */
+#define INTENT_CACHE_SAME 0 /* the heads' type */
+#define INTENT_CACHE_FP8 1  /* E4M3FN codes, a scale f32 for each token and head */
+#define INTENT_CACHE_INT4 2 /* 4-bit codes, a pair of f16 for each group of 32 elements */
+
+/*
+ * intent_paged_kv_append into a cache of 4 bits. A token's head is D / 2 bytes
+ * in u8 [pages][HK][page_size][D / 2] and ceil(D / 32) pairs in f16
+ * [pages][HK][page_size][ceil(D / 32)][2] (k_groups_ld, v_groups_ld elements
+ * from a page to the next, even; 4-byte aligned): little-endian words of eight
+ * codes, element e at bit 16 (e mod 2) + 4 (e div 2), and for each group of 32
+ * elements (the last may be shorter) a scale and a lowest value,
+ *   value = lowest + scale * code.
+ * With y clamped to +-61440 (so that lowest + 15 scale is an f16):
+ *   scale = f16((max y - min y) / 15), lowest = f16(min y),
+ *   code = clamp(rint((y - lowest) / scale), 0, 15), 0 where the scale is 0.
+ * A group that holds an infinity or NaN has scale 0 and lowest NaN: it reads as
+ * NaN. Everything else as in intent_paged_kv_append. No reference counterpart.
+ */
+int intent_paged_kv_append_int4(const void* q, int64_t T, int64_t HQ, int64_t q_ld,
+                                const void* k, int64_t HK, int64_t k_ld,
+                                const void* v, int64_t v_ld, int64_t D,
+                                const void* q_weight, const void* k_weight, float eps,
+                                const float* cos_sin, int64_t P, int64_t R, int64_t cos_sin_ld,
+                                int interleaved, const int32_t* positions, const int32_t* slots,
+                                int is_bf16,
+                                void* k_cache, int64_t k_page_ld, void* v_cache, int64_t v_page_ld,
+                                void* k_groups, int64_t k_groups_ld,
+                                void* v_groups, int64_t v_groups_ld,
+                                int64_t pages, int64_t page_size,
+                                void* q_out, int64_t q_out_ld, void* stream);
+
+/*
+ * Reads tokens back out of a paged cache of any format (k_params, v_params: the
+ * scales or groups, not read for INTENT_CACHE_SAME): k_out and v_out [T, HK, D]
+ * of the heads' type get the keys and values of token slots[t] = page *
+ * page_size + place, code times scale or lowest + scale * code in f32, rounded
+ * once. A slot outside the cache (a padded row) gives zeros; slots may repeat.
+ * No reference counterpart.
+ */
+int intent_paged_kv_read(int cache_format,
+                         const void* k_cache, int64_t k_page_ld, const void* v_cache, int64_t v_page_ld,
+                         const void* k_params, int64_t k_params_ld,
+                         const void* v_params, int64_t v_params_ld,
+                         int64_t pages, int64_t HK, int64_t page_size, int64_t D,
+                         const int32_t* slots, int64_t T, int is_bf16,
+                         void* k_out, int64_t k_out_ld, void* v_out, int64_t v_out_ld, void* stream);
+
+/*
+ * intent_paged_attention over a cache of any format, its scores in other forms
+ * where asked for:
+ *   x_t = scale q.k_t;  softcap > 0: x_t = softcap tanh(x_t / softcap);
+ *   slopes f32 [HQ] (finite): x_t = x_t - slopes[head] |p - t|;
+ *   out = sum_t softmax_t(x_t) v_t;
+ *   prefix_lens i32 [S], causal: row p sees t <= p and t < prefix_lens[s] too.
+ * 0 and null leave a form out; with none of them, and without 4 bits, it is
+ * intent_paged_attention. A window bounds the prefix as well. Values in 4 bits
+ * are rounded to f16 for the products, in bf16 too (the queries of bf16, scaled
+ * by a power of two for each row, are exact in f16 or 2^-38 of the row's largest
+ * off). The workspace is that of intent_paged_attention_workspace_size. No
+ * reference counterpart.
+ */
+int intent_biased_paged_attention(const void* q, int64_t T, int64_t HQ, int64_t q_ld,
+                                  int is_bf16, int cache_format,
+                                  const void* k_cache, int64_t k_page_ld, const void* v_cache, int64_t v_page_ld,
+                                  const void* k_params, int64_t k_params_ld,
+                                  const void* v_params, int64_t v_params_ld,
+                                  int64_t pages, int64_t HK, int64_t page_size, int64_t D,
+                                  const int32_t* page_table, int64_t S, int64_t table_width, int64_t table_ld,
+                                  const int32_t* q_offsets, const int32_t* kv_lens,
+                                  float scale, int causal, int64_t window,
+                                  float softcap, const float* slopes, const int32_t* prefix_lens,
+                                  void* out, int64_t out_ld,
+                                  void* workspace, size_t workspace_bytes, void* stream);
+
 /*
  * Repeats a call that the caller keeps as slots: one int64 for each argument
  * before the stream, in the entry's order (pointers and integers as they are, a
@@ -768,6 +843,9 @@ size_t intent_paged_attention_workspace_size(int64_t T, int64_t HQ, int64_t HK, 
 #define INTENT_RECORD_QK_NORM_ROPE 0
 #define INTENT_RECORD_PAGED_KV_APPEND 1
 #define INTENT_RECORD_PAGED_ATTENTION 2
+#define INTENT_RECORD_PAGED_KV_APPEND_INT4 3
+#define INTENT_RECORD_PAGED_KV_READ 4
+#define INTENT_RECORD_BIASED_PAGED_ATTENTION 5
 int intent_amd_replay(int record, const int64_t* slots, int64_t count, void* stream);
 
 #ifdef __cplusplus

@@ -63,6 +63,22 @@ from .definitions import (
     bf16_paged_attention,
     paged_attention_fp8,
     bf16_paged_attention_fp8,
+    paged_kv_append_int4,
+    bf16_paged_kv_append_int4,
+    paged_kv_read,
+    bf16_paged_kv_read,
+    paged_kv_read_fp8,
+    bf16_paged_kv_read_fp8,
+    paged_kv_read_int4,
+    bf16_paged_kv_read_int4,
+    paged_attention_int4,
+    bf16_paged_attention_int4,
+    biased_paged_attention,
+    bf16_biased_paged_attention,
+    biased_paged_attention_fp8,
+    bf16_biased_paged_attention_fp8,
+    biased_paged_attention_int4,
+    bf16_biased_paged_attention_int4,
 )
 from .errors import CompilationStageError, LanguageUseError, NativeLibraryError
 from .interface import DType, PublicInterface, ScalarParameter, ViewKind, ViewParameter
@@ -85,4 +101,9 @@ __all__ = [
     "qk_norm_rope", "bf16_qk_norm_rope", "paged_kv_append", "bf16_paged_kv_append", "paged_kv_append_fp8",
     "bf16_paged_kv_append_fp8", "paged_attention", "bf16_paged_attention", "paged_attention_fp8",
     "bf16_paged_attention_fp8",
+    "paged_kv_append_int4", "bf16_paged_kv_append_int4", "paged_kv_read", "bf16_paged_kv_read", "paged_kv_read_fp8",
+    "bf16_paged_kv_read_fp8", "paged_kv_read_int4", "bf16_paged_kv_read_int4", "paged_attention_int4",
+    "bf16_paged_attention_int4", "biased_paged_attention", "bf16_biased_paged_attention",
+    "biased_paged_attention_fp8", "bf16_biased_paged_attention_fp8", "biased_paged_attention_int4",
+    "bf16_biased_paged_attention_int4",
 ]

@@ -95,6 +95,11 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "intent_paged_attention": ([P, I64, I64, I64, INT, INT, P, I64, P, I64, P, I64, P, I64, I64, I64, I64, I64, P, I64,
                                 I64, I64, P, P, F32, INT, I64, P, I64, P, SIZE, P], INT),
     "intent_paged_attention_workspace_size": ([I64, I64, I64, I64, I64, I64, I64], SIZE),
+    "intent_paged_kv_append_int4": ([P, I64, I64, I64, P, I64, I64, P, I64, I64, P, P, F32, P, I64, I64, I64, INT, P, P,
+                                     INT, P, I64, P, I64, P, I64, P, I64, I64, I64, P, I64, P], INT),
+    "intent_paged_kv_read": ([INT, P, I64, P, I64, P, I64, P, I64, I64, I64, I64, I64, P, I64, INT, P, I64, P, I64, P], INT),
+    "intent_biased_paged_attention": ([P, I64, I64, I64, INT, INT, P, I64, P, I64, P, I64, P, I64, I64, I64, I64, I64, P,
+                                       I64, I64, I64, P, P, F32, INT, I64, F32, P, P, P, I64, P, SIZE, P], INT),
     "intent_amd_replay": ([INT, P, I64, P], INT),
     "intent_hbm_read_probe": ([P, I64, INT, INT, P, I64, P], INT),
     "intent_mfma_peak_probe": ([INT, I64, I64, P, P], INT),
@@ -168,7 +173,9 @@ class _Slots:
 
 
 RECORDS = {entry: _Slots(number, entry)
-           for number, entry in enumerate(("intent_qk_norm_rope", "intent_paged_kv_append", "intent_paged_attention"))}
+           for number, entry in enumerate(("intent_qk_norm_rope", "intent_paged_kv_append", "intent_paged_attention",
+                                           "intent_paged_kv_append_int4", "intent_paged_kv_read",
+                                           "intent_biased_paged_attention"))}
 
 
 def call_packed(entry: str, arguments: tuple, stream: int) -> None:

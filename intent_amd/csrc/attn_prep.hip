@@ -7,7 +7,10 @@
 //            a' = a cos - b sin, b' = b cos + a sin, cos and sin of the token's position
 //   cache:   the row as it is (f16 / bf16), or E4M3FN codes with a scale for each token and head,
 //            s = max(absmax, 1e-12) / 448, code = e4m3fn(clamp(y / s, +-448)): the groupwise FP8
-//            quantizer's rule with one group for each head
+//            quantizer's rule with one group for each head; or 4 bits (cache4.h), y clamped to +-61440,
+//            s = f16((max - min) / 15), m = f16(min) of each group of 32 elements,
+//            code = clamp(rint((y - m) / s), 0, 15). s and m are rounded before the codes are found, so that
+//            these make up for it; the clamp keeps m + 15 s inside f16.
 //
 // All of it in f32; each result is rounded once, when it is stored (y is not rounded between
 // the norm, the rotation and the encoding). Values are neither normed nor rotated.
@@ -22,6 +25,7 @@
 // latencies (position, table row, store).
 #include "common.h"
 #include "internal.h"
+#include "paged_cache.h"
 
 namespace {
 
@@ -45,11 +49,18 @@ struct PrepArgs {
   int HQ, HK, D, R, P, heads, items_per_token, interleaved, page_shift, slot_count;
 };
 
-enum Mode { kKeysOut = 0, kCacheSame = 1, kCacheFp8 = 2 };
+enum Mode { kKeysOut = -1, kCacheSame = intent::kCacheSame, kCacheFp8 = intent::kCacheFp8, kCacheInt4 = intent::kCacheInt4 };
 
 // The larger of two floats without a sign, by their bits: NaN is the largest.
 INTENT_DEVICE float magnitude_max(float a, float b) {
   return bit_cast<float>(max(bit_cast<uint32_t>(a), bit_cast<uint32_t>(b)));
+}
+
+// Reductions over the four lanes of a group of 32 elements.
+template <typename F>
+INTENT_DEVICE float quad_reduce(float v, F join) {
+  v = join(v, dpp_f32<0xB1>(v));     // quad_perm [1,0,3,2]
+  return join(v, dpp_f32<0x4E>(v));  // quad_perm [2,3,0,1]
 }
 
 // Sum or maximum over the LPR lanes of a group.
@@ -197,6 +208,42 @@ __global__ __launch_bounds__(256) void attn_prep_kernel(const PrepArgs a) {
       if constexpr (MODE == kCacheSame) {
         uint16_t* cache = (uint16_t*)(is_v ? a.v_cache : a.k_cache);
         if (mine && slot >= 0) store16(cache + cache_row(a, slot, head, page_ld, a.D) + c * 8, narrow<kBf16>(x));
+      } else if constexpr (MODE == kCacheInt4) {
+        constexpr float kMost = 61440.0f;
+        float low = INFINITY, high = -INFINITY, size = 0.f;
+        if (mine) {  // a group's missing lanes, behind the last element, leave its ends alone
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            size = magnitude_max(size, fabsf(x[j]));
+            x[j] = fminf(fmaxf(x[j], -kMost), kMost);
+            low = fminf(low, x[j]), high = fmaxf(high, x[j]);
+          }
+        }
+        low = quad_reduce(low, [](float p, float q) { return fminf(p, q); });
+        high = quad_reduce(high, [](float p, float q) { return fmaxf(p, q); });
+        size = quad_reduce(size, [](float p, float q) { return magnitude_max(p, q); });
+        // a group that holds an infinity or NaN reads as NaN throughout
+        const bool good = size < INFINITY;
+        const f16 scale = good ? (f16)__fdiv_rn(high - low, 15.0f) : (f16)0.f;
+        const f16 lowest = good ? (f16)low : bit_cast<f16>((uint16_t)0x7e00);
+        uint32_t word = 0;
+        if ((float)scale > 0.f) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float t = rintf(__fdiv_rn(x[j] - (float)lowest, (float)scale));
+            word |= (uint32_t)fminf(fmaxf(t, 0.f), 15.f) << intent::code_bit(j);
+          }
+        }
+        if (slot >= 0 && mine) {
+          const int row = a.D / 2, groups = (a.D + intent::kGroup4 - 1) / intent::kGroup4;
+          uint8_t* cache = (uint8_t*)(is_v ? a.v_cache : a.k_cache);
+          *(uint32_t*)(cache + cache_row(a, slot, head, page_ld, row) + c * 4) = word;
+          if (c % 4 == 0) {
+            uint32_t* pairs = (uint32_t*)(is_v ? a.v_scales : a.k_scales);
+            pairs[cache_row(a, slot, head, is_v ? a.vs_page : a.ks_page, groups) + c / 4] =
+                (uint32_t)bit_cast<uint16_t>(scale) | (uint32_t)bit_cast<uint16_t>(lowest) << 16;
+          }
+        }
       } else {
         float amax = 0.f;
 #pragma unroll
@@ -233,7 +280,7 @@ int launch(PrepArgs a, int64_t T, hipStream_t stream) {
   const int64_t blocks = (a.items + 256 / LPR - 1) / (256 / LPR);
   hipLaunchKernelGGL((attn_prep_kernel<kBf16, MODE, LPR, RPG>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
   static const intent::KernelName name("attn_prep_kernel<%s%s, %d lanes, %d heads>", kBf16 ? "bf16" : "f16",
-                                       MODE == kCacheFp8 ? ", fp8 cache" : MODE == kCacheSame ? ", cache" : "", LPR, RPG);
+                                       MODE == kKeysOut ? "" : MODE == kCacheSame ? ", cache" : intent::cache_name(MODE), LPR, RPG);
   return intent::launch_status(name.text);
 }
 
@@ -322,6 +369,49 @@ extern "C" int intent_qk_norm_rope(const void* q, int64_t T, int64_t HQ, int64_t
                  : launch_lanes<false, kKeysOut>(a, T, (hipStream_t)stream);
 }
 
+namespace {
+
+int append(PrepArgs& a, int64_t T, const void* v, int64_t v_ld, const intent::Cache& c, const int32_t* slots, int is_bf16,
+           hipStream_t stream) {
+  const int64_t HK = a.HK, D = a.D;
+  if (HK > 0) {
+    INTENT_REQUIRE(c.page_size > 0 && (c.page_size & (c.page_size - 1)) == 0, INTENT_ERR_UNSUPPORTED,
+                   "the page size must be a power of two, got %lld", (long long)c.page_size);
+    INTENT_REQUIRE(v && slots, INTENT_ERR_INVALID_ARGUMENT, "null pointer argument");
+    INTENT_REQUIRE(T == 1 || v_ld >= HK * D, INTENT_ERR_INVALID_ARGUMENT, "token stride smaller than the heads");
+    INTENT_REQUIRE(intent::aligned16(v) && (T == 1 || v_ld % 8 == 0), INTENT_ERR_ALIGNMENT,
+                   "v must be 16-byte aligned with a token stride %% 8 == 0");
+    if (c.pages > 0)
+      if (const int status = intent::check_cache(c, D)) return status;
+  }
+  const intent::RowSizes sizes = intent::row_sizes(c.format, D);
+  a.v = (const uint16_t*)v, a.v_ld = v_ld, a.slots = slots;
+  a.k_cache = (void*)c.k, a.v_cache = (void*)c.v, a.k_page = c.k_page_ld, a.v_page = c.v_page_ld;
+  a.k_scales = (float*)c.k_params, a.v_scales = (float*)c.v_params;
+  a.ks_page = c.k_params_ld / sizes.each, a.vs_page = c.v_params_ld / sizes.each;
+  a.page_shift = c.page_size > 0 ? __builtin_ctzll((unsigned long long)c.page_size) : 0;
+  a.slot_count = (int)(c.pages * c.page_size);
+  a.heads = a.HQ + 2 * a.HK;
+  switch (c.format) {
+    case kCacheInt4:
+      return is_bf16 ? launch_lanes<true, kCacheInt4>(a, T, stream) : launch_lanes<false, kCacheInt4>(a, T, stream);
+    case kCacheFp8:
+      return is_bf16 ? launch_lanes<true, kCacheFp8>(a, T, stream) : launch_lanes<false, kCacheFp8>(a, T, stream);
+    default:
+      return is_bf16 ? launch_lanes<true, kCacheSame>(a, T, stream) : launch_lanes<false, kCacheSame>(a, T, stream);
+  }
+}
+
+int check_extents(int64_t pages, int64_t page_size) {
+  INTENT_REQUIRE(pages >= 0 && page_size >= 0 && pages <= INT32_MAX && page_size <= INT32_MAX &&
+                     pages * page_size <= INT32_MAX,
+                 INTENT_ERR_INVALID_ARGUMENT, "bad cache extents (%lld pages of %lld)", (long long)pages,
+                 (long long)page_size);
+  return INTENT_OK;
+}
+
+}  // namespace
+
 extern "C" int intent_paged_kv_append(const void* q, int64_t T, int64_t HQ, int64_t q_ld, const void* k, int64_t HK,
                                       int64_t k_ld, const void* v, int64_t v_ld, int64_t D, const void* q_weight,
                                       const void* k_weight, float eps, const float* cos_sin, int64_t P, int64_t R,
@@ -335,39 +425,29 @@ extern "C" int intent_paged_kv_append(const void* q, int64_t T, int64_t HQ, int6
   if (const int status = check_heads(a, q, T, HQ, q_ld, k, HK, k_ld, D, q_weight, k_weight, eps, cos_sin, P, R,
                                      cos_sin_ld, interleaved, positions, q_out, q_out_ld))
     return status;
-  INTENT_REQUIRE(pages >= 0 && page_size >= 0 && pages <= INT32_MAX && page_size <= INT32_MAX &&
-                     pages * page_size <= INT32_MAX,
-                 INTENT_ERR_INVALID_ARGUMENT, "bad cache extents (%lld pages of %lld)", (long long)pages,
-                 (long long)page_size);
+  if (const int status = check_extents(pages, page_size)) return status;
   if (T == 0 || D == 0 || HQ + HK == 0) return INTENT_OK;
-  if (HK > 0) {
-    INTENT_REQUIRE(page_size > 0 && (page_size & (page_size - 1)) == 0, INTENT_ERR_UNSUPPORTED,
-                   "the page size must be a power of two, got %lld", (long long)page_size);
-    INTENT_REQUIRE(v && slots, INTENT_ERR_INVALID_ARGUMENT, "null pointer argument");
-    INTENT_REQUIRE(T == 1 || v_ld >= HK * D, INTENT_ERR_INVALID_ARGUMENT, "token stride smaller than the heads");
-    INTENT_REQUIRE(intent::aligned16(v) && (T == 1 || v_ld % 8 == 0), INTENT_ERR_ALIGNMENT,
-                   "v must be 16-byte aligned with a token stride %% 8 == 0");
-    if (pages > 0) {
-      INTENT_REQUIRE(k_cache && v_cache && (!cache_is_fp8 || (k_scales && v_scales)), INTENT_ERR_INVALID_ARGUMENT,
-                     "null pointer argument");
-      INTENT_REQUIRE(pages == 1 || (k_page_ld >= HK * page_size * D && v_page_ld >= HK * page_size * D &&
-                                    (!cache_is_fp8 || (k_scales_ld >= HK * page_size && v_scales_ld >= HK * page_size))),
-                     INTENT_ERR_INVALID_ARGUMENT, "page stride smaller than the page");
-      const int64_t step = cache_is_fp8 ? 16 : 8;
-      INTENT_REQUIRE(intent::aligned16(k_cache) && intent::aligned16(v_cache) &&
-                         (pages == 1 || (k_page_ld % step == 0 && v_page_ld % step == 0)) &&
-                         (!cache_is_fp8 || (intent::aligned4(k_scales) && intent::aligned4(v_scales))),
-                     INTENT_ERR_ALIGNMENT, "the cache must be 16-byte aligned with page strides of whole 16 bytes");
-    }
-  }
-  a.v = (const uint16_t*)v, a.v_ld = v_ld, a.slots = slots;
-  a.k_cache = k_cache, a.v_cache = v_cache, a.k_page = k_page_ld, a.v_page = v_page_ld;
-  a.k_scales = k_scales, a.v_scales = v_scales, a.ks_page = k_scales_ld, a.vs_page = v_scales_ld;
-  a.page_shift = page_size > 0 ? __builtin_ctzll((unsigned long long)page_size) : 0;
-  a.slot_count = (int)(pages * page_size);
-  a.heads = a.HQ + 2 * a.HK;
-  hipStream_t st = (hipStream_t)stream;
-  if (cache_is_fp8)
-    return is_bf16 ? launch_lanes<true, kCacheFp8>(a, T, st) : launch_lanes<false, kCacheFp8>(a, T, st);
-  return is_bf16 ? launch_lanes<true, kCacheSame>(a, T, st) : launch_lanes<false, kCacheSame>(a, T, st);
+  const intent::Cache c{cache_is_fp8 ? kCacheFp8 : kCacheSame, k_cache, k_page_ld, v_cache, v_page_ld, k_scales,
+                        k_scales_ld, v_scales, v_scales_ld, pages, HK, page_size};
+  return append(a, T, v, v_ld, c, slots, is_bf16, (hipStream_t)stream);
+}
+
+extern "C" int intent_paged_kv_append_int4(const void* q, int64_t T, int64_t HQ, int64_t q_ld, const void* k, int64_t HK,
+                                           int64_t k_ld, const void* v, int64_t v_ld, int64_t D, const void* q_weight,
+                                           const void* k_weight, float eps, const float* cos_sin, int64_t P, int64_t R,
+                                           int64_t cos_sin_ld, int interleaved, const int32_t* positions,
+                                           const int32_t* slots, int is_bf16, void* k_cache, int64_t k_page_ld,
+                                           void* v_cache, int64_t v_page_ld, void* k_groups, int64_t k_groups_ld,
+                                           void* v_groups, int64_t v_groups_ld, int64_t pages, int64_t page_size,
+                                           void* q_out, int64_t q_out_ld, void* stream) {
+  intent::clear_error();
+  PrepArgs a{};
+  if (const int status = check_heads(a, q, T, HQ, q_ld, k, HK, k_ld, D, q_weight, k_weight, eps, cos_sin, P, R,
+                                     cos_sin_ld, interleaved, positions, q_out, q_out_ld))
+    return status;
+  if (const int status = check_extents(pages, page_size)) return status;
+  if (T == 0 || D == 0 || HQ + HK == 0) return INTENT_OK;
+  const intent::Cache c{kCacheInt4, k_cache, k_page_ld, v_cache, v_page_ld, k_groups, k_groups_ld, v_groups,
+                        v_groups_ld, pages, HK, page_size};
+  return append(a, T, v, v_ld, c, slots, is_bf16, (hipStream_t)stream);
 }

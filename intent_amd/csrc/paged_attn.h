@@ -4,13 +4,18 @@
 // its pages (the new tokens among them, appended before the call). Its row i of n stands at position
 // p = kv_len - n + i and sees the tokens t with
 //   t < kv_len,   t <= p (causal),   t > p - window (window > 0).
-//   out = sum_t w_t v_t / sum_t w_t,   w_t = exp(scale q.k_t - max),   0 where nothing is seen.
+//   out = sum_t w_t v_t / sum_t w_t,   w_t = exp(x_t - max),   0 where nothing is seen,
+//   x_t = scale q.k_t.
+// Biased, each where it is asked for:
+//   x_t = cap tanh(scale q.k_t / cap),   then less slope[head] |p - t|;
+//   t <= p or t < prefix_len (causal): a prefix is seen by every row.
 // Offsets, lengths and page ids come from device memory: they are clamped to the tensors' extents,
 // so a wrong one gives a wrong row and no access outside them.
 #pragma once
 
 #include "common.h"
 #include "internal.h"
+#include "paged_cache.h"
 
 namespace intent {
 
@@ -19,8 +24,8 @@ struct AttnArgs {
   int64_t q_ld;
   const void *k_cache, *v_cache;
   int64_t k_page, v_page;  // elements from a page to the next
-  const float *k_scales, *v_scales;
-  int64_t ks_page, vs_page;
+  const float *k_scales, *v_scales;  // of 8 bits; of 4: the groups' pairs of f16
+  int64_t ks_page, vs_page;          // scales (pairs) from a page to the next
   const int32_t* page_table;
   int64_t table_ld;
   const int32_t *q_offsets, *kv_lens;
@@ -36,6 +41,10 @@ struct AttnArgs {
   int slots;               // parts of split tiles of one head that the workspace holds
   float* partial;          // [slot][HK][tile rows][D] unnormalised sums, then [slot][HK][tile rows][2]
   float* partial_stats;
+  // biased: null and zero where a form is not asked for
+  const float* slopes;  // of a query head, times log2(e) where they are used
+  const int32_t* prefix_lens;
+  float cap_log2;  // cap * log2(e)
 };
 
 // The tiled kernels for one type and cache (paged_attn_*.hip), by the rows of a tile: 16 to 64, whose
@@ -59,9 +68,9 @@ struct AttnJoin {
 int launch_join_f16(const AttnJoin& j, int side, hipStream_t stream);
 int launch_join_bf16(const AttnJoin& j, int side, hipStream_t stream);
 
-// Query rows [start, start + count) and cached tokens of sequence s.
+// Query rows [start, start + count), cached tokens and prefix of sequence s.
 struct Sequence {
-  int start, count, kv;
+  int start, count, kv, front;
 };
 
 INTENT_DEVICE Sequence sequence_of(const AttnArgs& a, int s) {
@@ -69,12 +78,18 @@ INTENT_DEVICE Sequence sequence_of(const AttnArgs& a, int s) {
   r.start = min(max(a.q_offsets[s], 0), a.T);
   r.count = max(min(a.q_offsets[s + 1], a.T) - r.start, 0);
   r.kv = min(max(a.kv_lens[s], 0), a.most_kv);
+  r.front = 0;
   return r;
 }
 
+// The tokens of sequence s that every row sees (a window aside).
+INTENT_DEVICE int prefix_of(const AttnArgs& a, int s) { return a.prefix_lens != nullptr ? max(a.prefix_lens[s], 0) : 0; }
+
 // First and one past the last token that the row at position p sees.
 INTENT_DEVICE int first_seen(const AttnArgs& a, int p) { return a.window > 0 && p >= a.window ? p - a.window + 1 : 0; }
-INTENT_DEVICE int end_seen(const AttnArgs& a, int p, int kv) { return a.causal ? min(max(p + 1, 0), kv) : kv; }
+INTENT_DEVICE int end_seen(const AttnArgs& a, int p, const Sequence& q) {
+  return a.causal ? min(max(p + 1, q.front), q.kv) : q.kv;
+}
 
 // Parts of a tile. One sequence on one cached head would be cut further to fill the GPU, but its join goes through
 // the parts of a row in one workgroup: 131000 tokens take 40 us in 256 parts and 111 in 1024; on two heads 47 and
@@ -143,7 +158,7 @@ INTENT_DEVICE bool span_of(const AttnArgs& a, int tile, int unit_log, int tiles,
   const int before = r.q.kv - r.q.count;
   const int p0 = before + (int)((uint32_t)r.row0 / (uint32_t)a.group);
   const int p1 = before + (int)((uint32_t)(r.row0 + r.rows - 1) / (uint32_t)a.group);
-  const int lo = first_seen(a, p0) & ~63, hi = end_seen(a, p1, r.q.kv);
+  const int lo = first_seen(a, p0) & ~63, hi = end_seen(a, p1, r.q);
   const uint32_t units = hi > lo ? (uint32_t)(hi - lo + (1 << unit_log) - 1) >> unit_log : 0u;
   const uint32_t each = units / (uint32_t)r.splits, more = units - each * (uint32_t)r.splits;
   const uint32_t from = each * split + min((uint32_t)split, more);
@@ -165,7 +180,7 @@ INTENT_DEVICE bool span_of(const AttnArgs& a, int tile, int unit_log, int tiles,
 // Lanes take a sequence each of 64, or of AT times 64 whose extents are all loaded before the first is
 // used: 2048 sequences of 512 tokens take 1245 us with 64 at a time, 935 with 256; one sequence takes 7.1
 // us with 64 and would wait for three useless loads with 256.
-template <int AT>
+template <int AT, bool kBiased>
 INTENT_DEVICE bool find_span_by(const AttnArgs& a, int tile, int unit_log, int item, bool joins, Span& r) {
   const int lane = threadIdx.x & 63;
   Extent e[AT];
@@ -200,7 +215,7 @@ INTENT_DEVICE bool find_span_by(const AttnArgs& a, int tile, int unit_log, int i
         const int at = __builtin_ctzll(past);
         r.s = s0 + i * 64 + at;
         r.q.start = lane_value(e[i].q.start, at), r.q.count = lane_value(e[i].q.count, at);
-        r.q.kv = lane_value(e[i].q.kv, at);
+        r.q.kv = lane_value(e[i].q.kv, at), r.q.front = kBiased ? prefix_of(a, r.s) : 0;
         r.splits = lane_value(splits, at);
         const int local = item - lane_value(up - mine, at), slot = lane_value(kept_up - kept, at);
         return span_of(a, tile, unit_log, lane_value(e[i].tiles, at), local, slot, joins, r);
@@ -213,9 +228,10 @@ INTENT_DEVICE bool find_span_by(const AttnArgs& a, int tile, int unit_log, int i
     for (int i = 0; i < AT; ++i) e[i] = extent_of(a, tile, unit_log, s0 + i * 64 + lane);
   }
 }
+template <bool kBiased>
 INTENT_DEVICE bool find_span(const AttnArgs& a, int tile, int unit_log, int item, bool joins, Span& r) {
-  if (a.S <= 64) return find_span_by<1>(a, tile, unit_log, item, joins, r);
-  return find_span_by<4>(a, tile, unit_log, item, joins, r);
+  if (a.S <= 64) return find_span_by<1, kBiased>(a, tile, unit_log, item, joins, r);
+  return find_span_by<4, kBiased>(a, tile, unit_log, item, joins, r);
 }
 
 // Page of token t (t < most_kv) of sequence s.
@@ -228,6 +244,15 @@ INTENT_DEVICE uint32_t table_entry(const AttnArgs& a, int s, int t) {
   return (uint32_t)a.page_table[(int64_t)s * a.table_ld + (t >> a.page_shift)];
 }
 INTENT_DEVICE uint32_t page_named(const AttnArgs& a, uint32_t entry) { return min(entry, (uint32_t)a.pages - 1u); }
+
+// The score's form in base 2: x times log2(e) in and out. tanh(y) = 1 - 2 / (exp(2 y) + 1): 2^-23 of the cap
+// off at most, the rounding of scores as large as it. exp2 may end at infinity or zero: tanh is 1 or -1 there.
+INTENT_DEVICE float capped(float x, float cap_log2, float rate) {
+  const float e = __builtin_amdgcn_exp2f(x * rate);
+  return __builtin_fmaf(-2.0f * cap_log2, __builtin_amdgcn_rcpf(e + 1.0f), cap_log2);
+}
+// `rate` of capped(): 2 log2(e) / cap_log2.
+INTENT_DEVICE float cap_rate(const AttnArgs& a) { return 2.88539008177792681472f / a.cap_log2; }
 
 // Row of token t of a page and head in a cache with `row` elements for each token.
 INTENT_DEVICE int64_t row_in_cache(const AttnArgs& a, int page, int64_t page_ld, int head, int t, int row) {

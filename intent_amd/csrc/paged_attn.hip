@@ -14,10 +14,13 @@ INTENT_DEVICE float widen1(uint16_t v) {
   else return (float)bit_cast<f16>(v);
 }
 
-template <bool kBf16, bool kFp8>
-INTENT_DEVICE void widen8(const void* p, float (&v)[8]) {
-  if constexpr (kFp8) {
-    const u32x2 raw = *(const u32x2*)p;
+// Elements d .. d + 7 of a token's head in the cache, from its row (and its groups' pairs), without the scale of 8 bits.
+template <bool kBf16, int kCache>
+INTENT_DEVICE void widen8(const char* row, const uint32_t* pairs, int d, float (&v)[8]) {
+  if constexpr (kCache == kCacheInt4) {
+    widen4(*(const uint32_t*)(row + d / 2), pairs[d / kGroup4], v);
+  } else if constexpr (kCache == kCacheFp8) {
+    const u32x2 raw = *(const u32x2*)(row + d);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)raw[j], false);
@@ -25,7 +28,7 @@ INTENT_DEVICE void widen8(const void* p, float (&v)[8]) {
       v[4 * j] = lo[0], v[4 * j + 1] = lo[1], v[4 * j + 2] = hi[0], v[4 * j + 3] = hi[1];
     }
   } else {
-    const u32x4 raw = load16(p);
+    const u32x4 raw = load16(row + d * 2);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       v[2 * j] = widen1<kBf16>((uint16_t)(raw[j] & 0xffffu));
@@ -34,10 +37,17 @@ INTENT_DEVICE void widen8(const void* p, float (&v)[8]) {
   }
 }
 
-template <bool kBf16, bool kFp8>
-INTENT_DEVICE float widen_one(const void* cache, int64_t index) {
-  if constexpr (kFp8) return __builtin_amdgcn_cvt_f32_fp8((int)((const uint8_t*)cache)[index], 0);
-  else return widen1<kBf16>(((const uint16_t*)cache)[index]);
+template <bool kBf16, int kCache>
+INTENT_DEVICE float widen_one(const char* row, const uint32_t* pairs, int d) {
+  if constexpr (kCache == kCacheInt4) {
+    const f16x2 h = bit_cast<f16x2>(pairs[d / kGroup4]);
+    const uint32_t word = *(const uint32_t*)(row + d / 8 * 4);
+    return __builtin_fmaf((float)(word >> code_bit(d) & 15u), (float)h[0], (float)h[1]);
+  } else if constexpr (kCache == kCacheFp8) {
+    return __builtin_amdgcn_cvt_f32_fp8((int)((const uint8_t*)row)[d], 0);
+  } else {
+    return widen1<kBf16>(((const uint16_t*)row)[d]);
+  }
 }
 
 INTENT_DEVICE float wave_max(float v) {
@@ -54,7 +64,7 @@ INTENT_DEVICE float wave_sum(float v) {
 // Any D that is a multiple of 8 up to 512: one wave for each query row. A lane takes one token of 64
 // for the products with the keys, then D / 64 columns of the values, whose tokens the wave goes
 // through one by one; tokens that the row does not see are not read.
-template <bool kBf16, bool kFp8>
+template <bool kBf16, int kCache, bool kBiased>
 __global__ __launch_bounds__(256) void paged_attn_row_kernel(const AttnArgs a) {
   __shared__ float qs[4][512];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -72,14 +82,20 @@ __global__ __launch_bounds__(256) void paged_attn_row_kernel(const AttnArgs a) {
     if (found) s = s0 + __builtin_ctzll(found);
   }
   if (s < 0) return;  // a row of no sequence is left as it is
-  const Sequence seq = sequence_of(a, s);
+  Sequence seq = sequence_of(a, s);
+  if constexpr (kBiased) seq.front = prefix_of(a, s);
   const int p = seq.kv - seq.count + (row - seq.start);
-  const int first = first_seen(a, p), end = end_seen(a, p, seq.kv);
+  const int first = first_seen(a, p), end = end_seen(a, p, seq);
   const uint16_t* q = a.q + (int64_t)row * a.q_ld + (int64_t)head * a.D;
   for (int d = lane; d < a.D; d += 64) qs[wave][d] = widen1<kBf16>(q[d]) * a.scale_log2;
   __builtin_amdgcn_wave_barrier();
 
-  constexpr int kBytes = kFp8 ? 1 : 2;
+  float slope = 0.f;
+  if constexpr (kBiased)
+    if (a.slopes != nullptr) slope = a.slopes[head] * 1.44269504088896340736f;
+  // bytes of a token's head, and its pairs
+  const int row_bytes = kCache == kCacheInt4 ? a.D / 2 : kCache == kCacheFp8 ? a.D : a.D * 2;
+  const int page_bytes = kCache == kCacheSame ? 2 : 1, groups = (a.D + kGroup4 - 1) / kGroup4;
   float acc[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) acc[j] = 0.f;
@@ -90,17 +106,24 @@ __global__ __launch_bounds__(256) void paged_attn_row_kernel(const AttnArgs a) {
     int page = 0;
     if (t < end) {
       page = page_of(a, s, t);
-      const char* k = (const char*)a.k_cache + row_in_cache(a, page, a.k_page, kv_head, t, a.D) * kBytes;
+      const char* k = (const char*)a.k_cache + row_in_cache(a, page, a.k_page * page_bytes, kv_head, t, row_bytes);
+      const uint32_t* pairs = nullptr;
+      if constexpr (kCache == kCacheInt4)
+        pairs = (const uint32_t*)a.k_scales + row_in_cache(a, page, a.ks_page, kv_head, t, groups);
       float sum = 0.f;
       for (int d = 0; d < a.D; d += 8) {
         float kv[8];
-        widen8<kBf16, kFp8>(k + d * kBytes, kv);
+        widen8<kBf16, kCache>(k, pairs, d, kv);
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum = __builtin_fmaf(kv[j], qs[wave][d + j], sum);
       }
-      if constexpr (kFp8) {
+      if constexpr (kCache == kCacheFp8) {
         sum *= a.k_scales[row_in_cache(a, page, a.ks_page, kv_head, t, 1)];
         v_scale = a.v_scales[row_in_cache(a, page, a.vs_page, kv_head, t, 1)];
+      }
+      if constexpr (kBiased) {
+        if (a.cap_log2 != 0.f) sum = capped(sum, a.cap_log2, cap_rate(a));
+        if (a.slopes != nullptr) sum = __builtin_fmaf(-slope, (float)abs(p - t), sum);
       }
       score = sum;
     }
@@ -115,11 +138,15 @@ __global__ __launch_bounds__(256) void paged_attn_row_kernel(const AttnArgs a) {
     const int n = min(end - t0, 64);
     for (int i = 0; i < n; ++i) {
       const float wi = __shfl(wv, i);
-      const int64_t v = row_in_cache(a, __shfl(page, i), a.v_page, kv_head, t0 + i, a.D);
+      const int from = __shfl(page, i);
+      const char* v = (const char*)a.v_cache + row_in_cache(a, from, a.v_page * page_bytes, kv_head, t0 + i, row_bytes);
+      const uint32_t* pairs = nullptr;
+      if constexpr (kCache == kCacheInt4)
+        pairs = (const uint32_t*)a.v_scales + row_in_cache(a, from, a.vs_page, kv_head, t0 + i, groups);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (lane + 64 * j < a.D)
-          acc[j] = __builtin_fmaf(wi, widen_one<kBf16, kFp8>(a.v_cache, v + lane + 64 * j), acc[j]);
+          acc[j] = __builtin_fmaf(wi, widen_one<kBf16, kCache>(v, pairs, lane + 64 * j), acc[j]);
     }
     top = m;
   }
@@ -135,12 +162,25 @@ __global__ __launch_bounds__(256) void paged_attn_row_kernel(const AttnArgs a) {
   }
 }
 
-template <bool kBf16, bool kFp8>
+template <bool kBf16, int kCache, bool kBiased>
 int launch_rows(const AttnArgs& a, hipStream_t stream) {
   const int64_t blocks = ((int64_t)a.T * a.HQ + 3) / 4;
-  hipLaunchKernelGGL((paged_attn_row_kernel<kBf16, kFp8>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
-  static const KernelName name("paged_attn_row_kernel<%s%s>", kBf16 ? "bf16" : "f16", kFp8 ? ", fp8 cache" : "");
+  hipLaunchKernelGGL((paged_attn_row_kernel<kBf16, kCache, kBiased>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  static const KernelName name("paged_attn_row_kernel<%s%s%s>", kBf16 ? "bf16" : "f16",
+                               cache_name(kCache), kBiased ? ", biased" : "");
   return launch_status(name.text);
+}
+
+template <bool kBf16, int kCache>
+int launch_rows(const AttnArgs& a, bool biased, hipStream_t stream) {
+  return biased ? launch_rows<kBf16, kCache, true>(a, stream) : launch_rows<kBf16, kCache, false>(a, stream);
+}
+int launch_any_rows(const AttnArgs& a, bool bf16, int cache, bool biased, hipStream_t stream) {
+  if (cache == kCacheInt4)
+    return bf16 ? launch_rows<true, kCacheInt4>(a, biased, stream) : launch_rows<false, kCacheInt4>(a, biased, stream);
+  if (cache == kCacheFp8)
+    return bf16 ? launch_rows<true, kCacheFp8>(a, biased, stream) : launch_rows<false, kCacheFp8>(a, biased, stream);
+  return bf16 ? launch_rows<true, kCacheSame>(a, biased, stream) : launch_rows<false, kCacheSame>(a, biased, stream);
 }
 
 // ---- which kernel, and into how many parts --------------------------------------------
@@ -303,15 +343,20 @@ extern "C" size_t intent_paged_attention_workspace_size(int64_t T, int64_t HQ, i
   return need;
 }
 
-extern "C" int intent_paged_attention(const void* q, int64_t T, int64_t HQ, int64_t q_ld, int is_bf16,
-                                      int cache_is_fp8, const void* k_cache, int64_t k_page_ld, const void* v_cache,
-                                      int64_t v_page_ld, const float* k_scales, int64_t k_scales_ld,
-                                      const float* v_scales, int64_t v_scales_ld, int64_t pages, int64_t HK,
-                                      int64_t page_size, int64_t D, const int32_t* page_table, int64_t S,
-                                      int64_t table_width, int64_t table_ld, const int32_t* q_offsets,
-                                      const int32_t* kv_lens, float scale, int causal, int64_t window, void* out,
-                                      int64_t out_ld, void* workspace, size_t workspace_bytes, void* stream) {
-  clear_error();
+namespace {
+
+// What a biased call adds to the scores and the mask; null and zero: nothing.
+struct Forms {
+  float softcap;
+  const float* slopes;
+  const int32_t* prefix_lens;
+};
+
+int attend(const void* q, int64_t T, int64_t HQ, int64_t q_ld, int is_bf16, const Cache& c, int64_t D,
+           const int32_t* page_table, int64_t S, int64_t table_width, int64_t table_ld, const int32_t* q_offsets,
+           const int32_t* kv_lens, float scale, int causal, int64_t window, const Forms& f, void* out, int64_t out_ld,
+           void* workspace, size_t workspace_bytes, void* stream) {
+  const int64_t HK = c.HK, pages = c.pages, page_size = c.page_size;
   INTENT_REQUIRE(T >= 0 && HQ >= 0 && HK >= 0 && D >= 0 && S >= 0 && pages >= 0 && page_size >= 0 && table_width >= 0 &&
                      window >= 0 && T <= INT32_MAX && HQ <= 65536 && HK <= 65536 && S < INT32_MAX &&
                      pages <= INT32_MAX && page_size <= INT32_MAX,
@@ -322,6 +367,10 @@ extern "C" int intent_paged_attention(const void* q, int64_t T, int64_t HQ, int6
   const float scale_log2 = scale * 1.44269504088896340736f;
   INTENT_REQUIRE(__builtin_isfinite(scale_log2), INTENT_ERR_INVALID_ARGUMENT, "scale * log2(e) must be finite, got %g",
                  (double)scale_log2);
+  const float cap_log2 = f.softcap * 1.44269504088896340736f;
+  // a cap so small that 1 / cap is no f32 is none that a score could tell from zero
+  INTENT_REQUIRE(f.softcap == 0.f || (f.softcap >= 0x1p-100f && f.softcap <= 0x1p100f), INTENT_ERR_INVALID_ARGUMENT,
+                 "softcap must be 0 (none) or between 2^-100 and 2^100, got %g", (double)f.softcap);
   INTENT_REQUIRE(HK > 0 && HQ % HK == 0, INTENT_ERR_INVALID_ARGUMENT,
                  "HQ=%lld query heads must be a multiple of the HK=%lld heads of the cache", (long long)HQ,
                  (long long)HK);
@@ -339,34 +388,28 @@ extern "C" int intent_paged_attention(const void* q, int64_t T, int64_t HQ, int6
   INTENT_REQUIRE(T * HQ < ((int64_t)1 << 25), INTENT_ERR_UNSUPPORTED,
                  "T * HQ = %lld rows exceed the %lld a launch covers", (long long)(T * HQ),
                  (long long)((int64_t)1 << 25));
-  INTENT_REQUIRE(q && out && q_offsets && kv_lens && (!any || (k_cache && v_cache && page_table)) &&
-                     (!any || !cache_is_fp8 || (k_scales && v_scales)),
-                 INTENT_ERR_INVALID_ARGUMENT, "null pointer argument");
+  INTENT_REQUIRE(q && out && q_offsets && kv_lens && (!any || page_table), INTENT_ERR_INVALID_ARGUMENT,
+                 "null pointer argument");
   INTENT_REQUIRE(T == 1 || (q_ld >= HQ * D && out_ld >= HQ * D), INTENT_ERR_INVALID_ARGUMENT,
                  "token stride smaller than the heads");
   INTENT_REQUIRE(intent::aligned16(q) && intent::aligned16(out) && (T == 1 || (q_ld % 8 == 0 && out_ld % 8 == 0)),
                  INTENT_ERR_ALIGNMENT, "q and out must be 16-byte aligned with token strides %% 8 == 0");
   if (any) {
-    const int64_t step = cache_is_fp8 ? 16 : 8;
     INTENT_REQUIRE(S == 1 || table_ld >= table_width, INTENT_ERR_INVALID_ARGUMENT, "table stride smaller than the row");
-    INTENT_REQUIRE(pages == 1 || (k_page_ld >= HK * page_size * D && v_page_ld >= HK * page_size * D &&
-                                  (!cache_is_fp8 || (k_scales_ld >= HK * page_size && v_scales_ld >= HK * page_size))),
-                   INTENT_ERR_INVALID_ARGUMENT, "page stride smaller than the page");
-    INTENT_REQUIRE(intent::aligned16(k_cache) && intent::aligned16(v_cache) &&
-                       (pages == 1 || (k_page_ld % step == 0 && v_page_ld % step == 0)) &&
-                       (!cache_is_fp8 || (intent::aligned4(k_scales) && intent::aligned4(v_scales))),
-                   INTENT_ERR_ALIGNMENT, "the cache must be 16-byte aligned with page strides of whole 16 bytes");
+    if (const int status = check_cache(c, D)) return status;
   }
-  INTENT_REQUIRE(!any || pages == 1 || (k_page_ld <= kMostStride && v_page_ld <= kMostStride &&
-                                        k_scales_ld <= kMostStride && v_scales_ld <= kMostStride),
+  INTENT_REQUIRE(!any || pages == 1 || (c.k_page_ld <= kMostStride && c.v_page_ld <= kMostStride &&
+                                        c.k_params_ld <= kMostStride && c.v_params_ld <= kMostStride),
                  INTENT_ERR_UNSUPPORTED, "page stride past 2^32 elements");
   AttnArgs a{};
   a.q = (const uint16_t*)q, a.q_ld = q_ld;
-  a.k_cache = k_cache, a.v_cache = v_cache, a.k_page = k_page_ld, a.v_page = v_page_ld;
-  a.k_scales = k_scales, a.v_scales = v_scales, a.ks_page = k_scales_ld, a.vs_page = v_scales_ld;
-  const int64_t units = cache_is_fp8 ? 16 : 8;
-  a.k_step = (uint32_t)(k_page_ld / units), a.v_step = (uint32_t)(v_page_ld / units);
-  a.ks_step = (uint32_t)k_scales_ld, a.vs_step = (uint32_t)v_scales_ld;
+  a.k_cache = c.k, a.v_cache = c.v, a.k_page = c.k_page_ld, a.v_page = c.v_page_ld;
+  a.k_scales = (const float*)c.k_params, a.v_scales = (const float*)c.v_params;
+  const RowSizes sizes = row_sizes(c.format, D);
+  a.ks_page = c.k_params_ld / sizes.each, a.vs_page = c.v_params_ld / sizes.each;
+  const int64_t units = c.format == kCacheSame ? 8 : 16;
+  a.k_step = (uint32_t)(c.k_page_ld / units), a.v_step = (uint32_t)(c.v_page_ld / units);
+  a.ks_step = (uint32_t)a.ks_page, a.vs_step = (uint32_t)a.vs_page;
   a.page_table = page_table, a.table_ld = table_ld;
   a.q_offsets = q_offsets, a.kv_lens = kv_lens;
   a.out = (uint16_t*)out, a.out_ld = out_ld;
@@ -375,11 +418,46 @@ extern "C" int intent_paged_attention(const void* q, int64_t T, int64_t HQ, int6
   a.pages = any ? (int)pages : 0, a.page_shift = any ? __builtin_ctzll((unsigned long long)page_size) : 0;
   a.most_kv = any ? (int)(table_width * page_size) : 0;
   a.causal = causal != 0, a.window = (int)(window < INT32_MAX ? window : INT32_MAX);
+  a.slopes = f.slopes, a.prefix_lens = f.prefix_lens, a.cap_log2 = cap_log2;
+  const bool biased = cap_log2 != 0.f || f.slopes != nullptr || (f.prefix_lens != nullptr && causal);
   hipStream_t st = (hipStream_t)stream;
-  if (tiled(D)) {
+  if (tiled(D) && c.format != kCacheInt4 && !biased) {
     const bool aligned = workspace != nullptr && intent::aligned16(workspace);
-    return launch_tiled(a, is_bf16 != 0, cache_is_fp8 != 0, aligned ? (float*)workspace : nullptr, workspace_bytes, st);
+    return launch_tiled(a, is_bf16 != 0, c.format == kCacheFp8, aligned ? (float*)workspace : nullptr, workspace_bytes,
+                        st);
   }
-  if (cache_is_fp8) return is_bf16 ? launch_rows<true, true>(a, st) : launch_rows<false, true>(a, st);
-  return is_bf16 ? launch_rows<true, false>(a, st) : launch_rows<false, false>(a, st);
+  return launch_any_rows(a, is_bf16 != 0, c.format, biased, st);
+}
+
+}  // namespace
+
+extern "C" int intent_paged_attention(const void* q, int64_t T, int64_t HQ, int64_t q_ld, int is_bf16,
+                                      int cache_is_fp8, const void* k_cache, int64_t k_page_ld, const void* v_cache,
+                                      int64_t v_page_ld, const float* k_scales, int64_t k_scales_ld,
+                                      const float* v_scales, int64_t v_scales_ld, int64_t pages, int64_t HK,
+                                      int64_t page_size, int64_t D, const int32_t* page_table, int64_t S,
+                                      int64_t table_width, int64_t table_ld, const int32_t* q_offsets,
+                                      const int32_t* kv_lens, float scale, int causal, int64_t window, void* out,
+                                      int64_t out_ld, void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  const Cache c{cache_is_fp8 ? kCacheFp8 : kCacheSame, k_cache, k_page_ld, v_cache, v_page_ld, k_scales, k_scales_ld,
+                v_scales, v_scales_ld, pages, HK, page_size};
+  return attend(q, T, HQ, q_ld, is_bf16, c, D, page_table, S, table_width, table_ld, q_offsets, kv_lens, scale, causal,
+                window, Forms{}, out, out_ld, workspace, workspace_bytes, stream);
+}
+
+extern "C" int intent_biased_paged_attention(
+    const void* q, int64_t T, int64_t HQ, int64_t q_ld, int is_bf16, int cache_format, const void* k_cache,
+    int64_t k_page_ld, const void* v_cache, int64_t v_page_ld, const void* k_params, int64_t k_params_ld,
+    const void* v_params, int64_t v_params_ld, int64_t pages, int64_t HK, int64_t page_size, int64_t D,
+    const int32_t* page_table, int64_t S, int64_t table_width, int64_t table_ld, const int32_t* q_offsets,
+    const int32_t* kv_lens, float scale, int causal, int64_t window, float softcap, const float* slopes,
+    const int32_t* prefix_lens, void* out, int64_t out_ld, void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  INTENT_REQUIRE(cache_format >= INTENT_CACHE_SAME && cache_format <= INTENT_CACHE_INT4, INTENT_ERR_INVALID_ARGUMENT,
+                 "no cache has format %d", cache_format);
+  const Cache c{cache_format, k_cache, k_page_ld, v_cache, v_page_ld, k_params, k_params_ld, v_params, v_params_ld,
+                pages, HK, page_size};
+  return attend(q, T, HQ, q_ld, is_bf16, c, D, page_table, S, table_width, table_ld, q_offsets, kv_lens, scale, causal,
+                window, Forms{softcap, slopes, prefix_lens}, out, out_ld, workspace, workspace_bytes, stream);
 }

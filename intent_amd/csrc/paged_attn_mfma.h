@@ -167,7 +167,7 @@ struct RowView {
 };
 INTENT_DEVICE RowView row_view(const AttnArgs& a, const Span& w, int r) {
   const int p = w.q.kv - w.q.count + (int)((uint32_t)(w.row0 + min(r, w.rows - 1)) / (uint32_t)a.group);
-  return {first_seen(a, p), end_seen(a, p, w.q.kv)};
+  return {first_seen(a, p), end_seen(a, p, w.q)};
 }
 
 INTENT_DEVICE const uint16_t* q_row(const AttnArgs& a, const Span& w, int head, int r) {
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
 
   const int head = blockIdx.x % a.HK;
   Span w;
-  if (!find_span(a, 16 * MT, 7, blockIdx.x / a.HK, false, w)) return;
+  if (!find_span<false>(a, 16 * MT, 7, blockIdx.x / a.HK, false, w)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int col = lane & 15, g = lane >> 4;
 
@@ -570,7 +570,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
 
   const int head = blockIdx.x % a.HK;
   Span w;
-  if (!find_span(a, ROWS, 6, blockIdx.x / a.HK, false, w)) return;
+  if (!find_span<false>(a, ROWS, 6, blockIdx.x / a.HK, false, w)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int col = lane & 31, h = lane >> 5;
   const int r0 = wave * 32;
@@ -954,7 +954,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(int items, int tile, int
     a.partial = j.partial, a.partial_stats = j.partial_stats;
   }
   Span w;
-  if (!find_span(a, tile, unit_log, item, true, w)) return;
+  if (!find_span<false>(a, tile, unit_log, item, true, w)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (w.splits <= FEW) {
     const int c = lane % LANES * 4 < D ? lane % LANES * 4 : 0;

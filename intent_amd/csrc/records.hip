@@ -47,6 +47,11 @@ extern "C" int intent_amd_replay(int record, const int64_t* slots, int64_t count
       return call_slots<intent_paged_kv_append>(intent_paged_kv_append, slots, count, stream);
     case INTENT_RECORD_PAGED_ATTENTION:
       return call_slots<intent_paged_attention>(intent_paged_attention, slots, count, stream);
+    case INTENT_RECORD_PAGED_KV_APPEND_INT4:
+      return call_slots<intent_paged_kv_append_int4>(intent_paged_kv_append_int4, slots, count, stream);
+    case INTENT_RECORD_PAGED_KV_READ: return call_slots<intent_paged_kv_read>(intent_paged_kv_read, slots, count, stream);
+    case INTENT_RECORD_BIASED_PAGED_ATTENTION:
+      return call_slots<intent_biased_paged_attention>(intent_biased_paged_attention, slots, count, stream);
     default: return intent::fail(INTENT_ERR_INVALID_ARGUMENT, "no entry has record number %d", record);
   }
 }

@@ -1395,35 +1395,52 @@ def _append_check(env: dict) -> None:
     _page_check(env)
 
 
-def _cache_params(dt: str, fp8: bool, access: ViewKind) -> tuple:
-    cache = "f8e4m3fn" if fp8 else dt
-    params = tuple(Param(f"{name}_cache", cache, ("PAGES", "HK", "PAGE", "D"), access, leading_stride=True)
+# A cache's format: the suffix of its operators, INTENT_CACHE_* and what it holds.
+_FORMATS = {"same": ("", 0, ""),
+            "fp8": ("_fp8", 1, "E4M3FN codes with a scale per token and head, max(absmax, 1e-12) / 448"),
+            "int4": ("_int4", 2, "4-bit codes with (scale, lowest) f16 per 32 elements, ((max - min) / 15, min): value = "
+                                 "lowest + scale * code, element e of eight at bit 16 (e % 2) + 4 (e // 2) of a word")}
+
+
+def _cache_params(dt: str, cache: str, access: ViewKind, d: Dim = "D", half: Dim = lambda env: env["D"] // 2) -> tuple:
+    element, row = {"same": (dt, d), "fp8": ("f8e4m3fn", d), "int4": ("u8", half)}[cache]
+    params = tuple(Param(f"{name}_cache", element, ("PAGES", "HK", "PAGE", row), access, leading_stride=True)
                    for name in ("k", "v"))
-    if fp8:
+    if cache == "fp8":
         params += tuple(Param(f"{name}_scales", "f32", ("PAGES", "HK", "PAGE"), access, leading_stride=True)
                         for name in ("k", "v"))
+    if cache == "int4":
+        params += tuple(Param(f"{name}_groups", "f16", ("PAGES", "HK", "PAGE", lambda env: (_head_size(env) + 31) // 32, 2),
+                              access, leading_stride=True) for name in ("k", "v"))
     return params
 
 
-def _cache_arguments(v: dict, fp8: bool) -> tuple:
+def _head_size(env: dict) -> int:
+    return env["D"] if "D" in env else 2 * env["HALF"]
+
+
+def _cache_arguments(v: dict, cache: str) -> tuple:
     k, kv = v["k_cache"], v["v_cache"]
-    scales = (_ptr(v["k_scales"]), _ld(v["k_scales"]), _ptr(v["v_scales"]), _ld(v["v_scales"])) if fp8 else (0, 0, 0, 0)
-    return (_ptr(k), _ld(k), _ptr(kv), _ld(kv), *scales)
+    beside = {"same": None, "fp8": "scales", "int4": "groups"}[cache]
+    if beside is None:
+        return (_ptr(k), _ld(k), _ptr(kv), _ld(kv), 0, 0, 0, 0)
+    kp, vp = v["k_" + beside], v["v_" + beside]
+    return (_ptr(k), _ld(k), _ptr(kv), _ld(kv), _ptr(kp), _ld(kp), _ptr(vp), _ld(vp))
 
 
-_CACHE_DOC = "E4M3FN codes with a scale per token and head, max(absmax, 1e-12) / 448"
+def _append_definition(dt: str, cache: str) -> KernelDefinition:
+    suffix, number, held = _FORMATS[cache]
 
-
-def _append_definition(dt: str, fp8: bool) -> KernelDefinition:
     def call(v: dict, env: dict, scratch) -> tuple:
         first, rest = _heads_arguments(v, env)
         value, q_out = v["v"], v["q_out"]
-        return "intent_paged_kv_append", (
-            *first, _ptr(value), _ld(value), *rest, _ptr(v["slots"]), int(dt == "bf16"), int(fp8),
-            *_cache_arguments(v, fp8), env["PAGES"], env["PAGE"], _ptr(q_out), _ld(q_out))
+        entry, kind = ("intent_paged_kv_append_int4", ()) if cache == "int4" else ("intent_paged_kv_append", (number,))
+        return entry, (
+            *first, _ptr(value), _ld(value), *rest, _ptr(v["slots"]), int(dt == "bf16"), *kind,
+            *_cache_arguments(v, cache), env["PAGES"], env["PAGE"], _ptr(q_out), _ld(q_out))
 
     return KernelDefinition(
-        name=_prefix(dt) + "paged_kv_append" + ("_fp8" if fp8 else ""),
+        name=_prefix(dt) + "paged_kv_append" + suffix,
         params=(
             Param("q", dt, ("T", "HQ", "D"), leading_stride=True),
             Param("k", dt, ("T", "HK", "D"), leading_stride=True),
@@ -1433,23 +1450,65 @@ def _append_definition(dt: str, fp8: bool) -> KernelDefinition:
             Param("cos_sin", "f32", ("P", "R"), leading_stride=True),
             Param("positions", "i32", ("T",)),
             Param("slots", "i32", ("T",)),
-            *_cache_params(dt, fp8, INOUT),
+            *_cache_params(dt, cache, INOUT),
             Param("q_out", dt, ("T", "HQ", "D"), OUT, leading_stride=True),
         ),
         **_one_call(call),
         constexprs=dict(_HEADS_CONSTEXPRS),
         check=_append_check,
-        reference="examples/kernels/quantization/fp8.py:11-39 (the quantizer's rule, one group for each head)" if fp8 else
+        reference="examples/kernels/quantization/fp8.py:11-39 (the quantizer's rule, one group for each head)" if cache == "fp8" else
                   "no kernel of the reference's quantized path; the producer of the paged attention's cache",
         doc="q_out, and keys as qk_norm_rope, values as they are, at token slots[t] (page * PAGE + place) of the cache"
-            + (f": {_CACHE_DOC}" if fp8 else "") + "; a negative slot (padding) or one past the cache is skipped",
+            + (f": {held}" if held else "") + "; a negative slot (padding) or one past the cache is skipped",
     )
 
 
-paged_kv_append = _append_definition("f16", False)
-bf16_paged_kv_append = _append_definition("bf16", False)
-paged_kv_append_fp8 = _append_definition("f16", True)
-bf16_paged_kv_append_fp8 = _append_definition("bf16", True)
+paged_kv_append = _append_definition("f16", "same")
+bf16_paged_kv_append = _append_definition("bf16", "same")
+paged_kv_append_fp8 = _append_definition("f16", "fp8")
+bf16_paged_kv_append_fp8 = _append_definition("bf16", "fp8")
+paged_kv_append_int4 = _append_definition("f16", "int4")
+bf16_paged_kv_append_int4 = _append_definition("bf16", "int4")
+
+
+def _read_check(env: dict) -> None:
+    D = _head_size(env)
+    if D % 8 or D > 512:
+        raise NotImplementedError(f"D ({D}) must be a multiple of 8 up to 512")
+    _page_check(env)
+
+
+def _read_definition(dt: str, cache: str) -> KernelDefinition:
+    suffix, number, held = _FORMATS[cache]
+
+    def call(v: dict, env: dict, scratch) -> tuple:
+        k, kv = v["k_out"], v["v_out"]
+        return "intent_paged_kv_read", (number, *_cache_arguments(v, cache), env["PAGES"], env["HK"], env["PAGE"],
+                                        _head_size(env), _ptr(v["slots"]), env["T"], int(dt == "bf16"), _ptr(k), _ld(k),
+                                        _ptr(kv), _ld(kv))
+
+    return KernelDefinition(
+        name=_prefix(dt) + "paged_kv_read" + suffix,
+        params=(
+            *_cache_params(dt, cache, IN, half="HALF"),
+            Param("slots", "i32", ("T",)),
+            Param("k_out", dt, ("T", "HK", _head_size), OUT, leading_stride=True),
+            Param("v_out", dt, ("T", "HK", _head_size), OUT, leading_stride=True),
+        ),
+        **_one_call(call),
+        check=_read_check,
+        reference="no kernel of the reference's quantized path; the inverse of the paged append",
+        doc="keys and values at token slots[t] (page * PAGE + place) of the cache as rows"
+            + (f": {held}" if held else "") + "; zeros for a slot outside the cache (padding)",
+    )
+
+
+paged_kv_read = _read_definition("f16", "same")
+bf16_paged_kv_read = _read_definition("bf16", "same")
+paged_kv_read_fp8 = _read_definition("f16", "fp8")
+bf16_paged_kv_read_fp8 = _read_definition("bf16", "fp8")
+paged_kv_read_int4 = _read_definition("f16", "int4")
+bf16_paged_kv_read_int4 = _read_definition("bf16", "int4")
 
 
 def _attention_check(env: dict) -> None:
@@ -1464,47 +1523,78 @@ def _attention_check(env: dict) -> None:
     _page_check(env)
 
 
+def _biased_check(env: dict) -> None:
+    _attention_check(env)
+    for name, extent, whole in (("slopes", env["SLOPES"], env["HQ"]), ("prefix_lens", env["PREFIXES"], env["S"])):
+        if extent not in (0, whole):
+            raise ValueError(f"{name} must have {whole} elements, or none, got {extent}")
+    cap = float(env["SOFTCAP"])
+    if cap != 0.0 and not 2.0 ** -100 <= cap <= 2.0 ** 100:
+        raise ValueError(f"SOFTCAP must be 0 (none) or between 2^-100 and 2^100, got {cap}")
+
+
 def _attention_scratch(env: dict) -> int:
     return _native.library().intent_paged_attention_workspace_size(
         env["T"], env["HQ"], env["HK"], env["D"], env["S"], env["MAX_PAGES"], env["PAGE"])
 
 
-def _attention_definition(dt: str, fp8: bool) -> KernelDefinition:
+def _attention_definition(dt: str, cache: str, biased: bool = False) -> KernelDefinition:
+    suffix, number, held = _FORMATS[cache]
+    # the entry without forms knows the first two caches
+    general = biased or cache == "int4"
+
     def call(v: dict, env: dict, scratch) -> tuple:
         q, out, table = v["q"], v["out"], v["page_table"]
-        return "intent_paged_attention", (
-            _ptr(q), env["T"], env["HQ"], _ld(q), int(dt == "bf16"), int(fp8), *_cache_arguments(v, fp8), env["PAGES"],
+        forms = ()
+        if biased:
+            forms = (float(env["SOFTCAP"]), _ptr(v["slopes"]) if env["SLOPES"] else 0,
+                     _ptr(v["prefix_lens"]) if env["PREFIXES"] else 0)
+        elif general:
+            forms = (0.0, 0, 0)
+        return "intent_biased_paged_attention" if general else "intent_paged_attention", (
+            _ptr(q), env["T"], env["HQ"], _ld(q), int(dt == "bf16"), number, *_cache_arguments(v, cache), env["PAGES"],
             env["HK"], env["PAGE"], env["D"], _ptr(table), env["S"], env["MAX_PAGES"], _ld(table), _ptr(v["q_offsets"]),
-            _ptr(v["kv_lens"]), float(env["scale"]), int(bool(env["CAUSAL"])), min(int(env["WINDOW"]), 2 ** 31),
+            _ptr(v["kv_lens"]), float(env["scale"]), int(bool(env["CAUSAL"])), min(int(env["WINDOW"]), 2 ** 31), *forms,
             _ptr(out), _ld(out),
             0 if scratch is None else _ptr(scratch), 0 if scratch is None else scratch.numel())
 
     return KernelDefinition(
-        name=_prefix(dt) + "paged_attention" + ("_fp8" if fp8 else ""),
+        name=_prefix(dt) + ("biased_" if biased else "") + "paged_attention" + suffix,
         params=(
             Param("q", dt, ("T", "HQ", "D"), leading_stride=True),
-            *_cache_params(dt, fp8, IN),
+            *_cache_params(dt, cache, IN),
             Param("page_table", "i32", ("S", "MAX_PAGES"), leading_stride=True),
             Param("q_offsets", "i32", ("S_PLUS_1",)),
             Param("kv_lens", "i32", ("S",)),
+            *((Param("slopes", "f32", ("SLOPES",)), Param("prefix_lens", "i32", ("PREFIXES",))) if biased else ()),
             Param("out", dt, ("T", "HQ", "D"), OUT, leading_stride=True),
             Scalar("scale", "f32"),
         ),
         **_one_call(call),
         scratch=_attention_scratch,
-        constexprs={"CAUSAL": True, "WINDOW": 0},
-        check=_attention_check,
+        constexprs={"CAUSAL": True, "WINDOW": 0, **({"SOFTCAP": 0.0} if biased else {})},
+        check=_biased_check if biased else _attention_check,
         reference="no kernel of the reference's quantized path; I.matmul contractions over a paged operand",
         doc="rows q_offsets[s] .. q_offsets[s+1] attend the kv_lens[s] tokens of sequence s's pages (the new ones last): "
             "out = softmax(scale q.k) v over the seen tokens, zeros where none is seen"
-            + (f"; cache: {_CACHE_DOC}" if fp8 else ""),
+            + ("; scores capped by SOFTCAP tanh(x / SOFTCAP), less slopes[head] |p - t| (none with no slopes), the first "
+               "prefix_lens[s] tokens seen by every row (CAUSAL; none with no lengths)" if biased else "")
+            + (f"; cache: {held}" if held else ""),
     )
 
 
-paged_attention = _attention_definition("f16", False)
-bf16_paged_attention = _attention_definition("bf16", False)
-paged_attention_fp8 = _attention_definition("f16", True)
-bf16_paged_attention_fp8 = _attention_definition("bf16", True)
+paged_attention = _attention_definition("f16", "same")
+bf16_paged_attention = _attention_definition("bf16", "same")
+paged_attention_fp8 = _attention_definition("f16", "fp8")
+bf16_paged_attention_fp8 = _attention_definition("bf16", "fp8")
+paged_attention_int4 = _attention_definition("f16", "int4")
+bf16_paged_attention_int4 = _attention_definition("bf16", "int4")
+biased_paged_attention = _attention_definition("f16", "same", biased=True)
+bf16_biased_paged_attention = _attention_definition("bf16", "same", biased=True)
+biased_paged_attention_fp8 = _attention_definition("f16", "fp8", biased=True)
+bf16_biased_paged_attention_fp8 = _attention_definition("bf16", "fp8", biased=True)
+biased_paged_attention_int4 = _attention_definition("f16", "int4", biased=True)
+bf16_biased_paged_attention_int4 = _attention_definition("bf16", "int4", biased=True)
 
 
 ALL_DEFINITIONS = (
@@ -1518,4 +1608,8 @@ ALL_DEFINITIONS = (
     nvfp4_quantize, per_token_int8_quantize, bf16_per_token_int8_quantize,
     qk_norm_rope, bf16_qk_norm_rope, paged_kv_append, bf16_paged_kv_append, paged_kv_append_fp8,
     bf16_paged_kv_append_fp8, paged_attention, bf16_paged_attention, paged_attention_fp8, bf16_paged_attention_fp8,
+    paged_kv_append_int4, bf16_paged_kv_append_int4, paged_kv_read, bf16_paged_kv_read, paged_kv_read_fp8,
+    bf16_paged_kv_read_fp8, paged_kv_read_int4, bf16_paged_kv_read_int4, paged_attention_int4,
+    bf16_paged_attention_int4, biased_paged_attention, bf16_biased_paged_attention, biased_paged_attention_fp8,
+    bf16_biased_paged_attention_fp8, biased_paged_attention_int4, bf16_biased_paged_attention_int4,
 )
