@@ -47,13 +47,13 @@ struct AttnArgs {
   float cap_log2;  // cap * log2(e)
 };
 
-// The tiled kernels for one type and cache (paged_attn_*.hip), by the rows of a tile: 16 to 64, whose
-// tokens are spread over a workgroup's four waves, or 128 or 256, 32 to a wave. `items` workgroups for
-// each cached head.
-int launch_attn_f16(const AttnArgs& a, int items, int rows, hipStream_t stream);
-int launch_attn_bf16(const AttnArgs& a, int items, int rows, hipStream_t stream);
-int launch_attn_f16_fp8(const AttnArgs& a, int items, int rows, hipStream_t stream);
-int launch_attn_bf16_fp8(const AttnArgs& a, int items, int rows, hipStream_t stream);
+// The tiled kernels for one type, cache and form of scores (paged_attn_*.hip), by the rows of a tile: 16 to 64,
+// whose tokens are spread over a workgroup's four waves, or 128 or 256, 32 to a wave. `items` workgroups for each
+// cached head.
+typedef int LaunchAttn(const AttnArgs& a, int items, int rows, hipStream_t stream);
+LaunchAttn launch_attn_f16, launch_attn_bf16, launch_attn_f16_fp8, launch_attn_bf16_fp8, launch_attn_f16_int4,
+    launch_attn_bf16_int4, launch_attn_f16_biased, launch_attn_bf16_biased, launch_attn_f16_fp8_biased,
+    launch_attn_bf16_fp8_biased, launch_attn_f16_int4_biased, launch_attn_bf16_int4_biased;
 
 // One launch for the joins of the split tiles of up to two lists: the rows of each one's tiles, its units of
 // tokens (their logarithm) and workgroups for each cached head (0: no list), and the second list's own
@@ -65,8 +65,8 @@ struct AttnJoin {
   AttnArgs a;
 };
 // with `side` workgroups for the rows of a tile
-int launch_join_f16(const AttnJoin& j, int side, hipStream_t stream);
-int launch_join_bf16(const AttnJoin& j, int side, hipStream_t stream);
+typedef int LaunchJoin(const AttnJoin& j, int side, hipStream_t stream);
+LaunchJoin launch_join_f16, launch_join_bf16, launch_join_f16_biased, launch_join_bf16_biased;
 
 // Query rows [start, start + count), cached tokens and prefix of sequence s.
 struct Sequence {

@@ -281,7 +281,15 @@ size_t part_bytes(const Part& p, int64_t T, int64_t S, int64_t group, int64_t HK
   return (size_t)(slots_bound(p, T, S, group, HK, D, most_kv) * HK * p.rows * (D + 2) * 4);
 }
 
-int launch_tiled(AttnArgs a, bool bf16, bool fp8, float* workspace, size_t bytes, hipStream_t stream) {
+// By cache format, scores biased or not, and heads of bf16 or not.
+LaunchAttn* const kLaunchAttn[3][2][2] = {
+    {{launch_attn_f16, launch_attn_bf16}, {launch_attn_f16_biased, launch_attn_bf16_biased}},
+    {{launch_attn_f16_fp8, launch_attn_bf16_fp8}, {launch_attn_f16_fp8_biased, launch_attn_bf16_fp8_biased}},
+    {{launch_attn_f16_int4, launch_attn_bf16_int4}, {launch_attn_f16_int4_biased, launch_attn_bf16_int4_biased}}};
+LaunchJoin* const kLaunchJoin[2][2] = {{launch_join_f16, launch_join_bf16},
+                                       {launch_join_f16_biased, launch_join_bf16_biased}};
+
+int launch_tiled(AttnArgs a, bool bf16, int cache, bool biased, float* workspace, size_t bytes, hipStream_t stream) {
   const Plan plan = plan_of(a.T, a.S, a.HK, a.group, a.D);
   size_t need = 0;
   for (int i = 0; i < plan.parts; ++i) need += part_bytes(plan.part[i], a.T, a.S, a.group, a.HK, a.D, a.most_kv);
@@ -304,8 +312,7 @@ int launch_tiled(AttnArgs a, bool bf16, bool fp8, float* workspace, size_t bytes
                    "%lld tiles of %d heads exceed the %lld workgroups that a launch covers", (long long)tiles, a.HK,
                    (long long)((int64_t)1 << 23));
     const int items = (int)(tiles + a.target);
-    const auto go = fp8 ? (bf16 ? launch_attn_bf16_fp8 : launch_attn_f16_fp8) : (bf16 ? launch_attn_bf16 : launch_attn_f16);
-    const int status = go(a, items, p.rows, stream);
+    const int status = kLaunchAttn[cache][biased][bf16](a, items, p.rows, stream);
     if (status != INTENT_OK) return status;
     if (!split) continue;
     // a tile is split from one and a half shares on
@@ -326,7 +333,7 @@ int launch_tiled(AttnArgs a, bool bf16, bool fp8, float* workspace, size_t bytes
   const int64_t room = 1024 / ((int64_t)(join.items[0] + join.items[1]) * a.HK), rows = plan.part[0].rows;
   const int64_t side = mean < rows ? mean : rows;
   const int sides = (int)(room < 1 ? 1 : room < side ? room : side);
-  return bf16 ? launch_join_bf16(join, sides, stream) : launch_join_f16(join, sides, stream);
+  return kLaunchJoin[biased][bf16](join, sides, stream);
 }
 
 }  // namespace
@@ -421,10 +428,9 @@ int attend(const void* q, int64_t T, int64_t HQ, int64_t q_ld, int is_bf16, cons
   a.slopes = f.slopes, a.prefix_lens = f.prefix_lens, a.cap_log2 = cap_log2;
   const bool biased = cap_log2 != 0.f || f.slopes != nullptr || (f.prefix_lens != nullptr && causal);
   hipStream_t st = (hipStream_t)stream;
-  if (tiled(D) && c.format != kCacheInt4 && !biased) {
+  if (tiled(D)) {
     const bool aligned = workspace != nullptr && intent::aligned16(workspace);
-    return launch_tiled(a, is_bf16 != 0, c.format == kCacheFp8, aligned ? (float*)workspace : nullptr, workspace_bytes,
-                        st);
+    return launch_tiled(a, is_bf16 != 0, c.format, biased, aligned ? (float*)workspace : nullptr, workspace_bytes, st);
   }
   return launch_any_rows(a, is_bf16 != 0, c.format, biased, st);
 }

@@ -1,8 +1,8 @@
-// The tiled attention kernels (paged_attn_mfma.h) of one type of heads and cache.
+// The tiled attention kernels (paged_attn_mfma.h) of one type of heads, cache and form of scores.
 #include "paged_attn_mfma.h"
 
 int intent::launch_attn_bf16(const AttnArgs& a, int items, int rows, hipStream_t stream) {
-  return attn::launch_any<true, false>(a, items, rows, stream);
+  return attn::launch_any<true, kCacheSame>(a, items, rows, stream);
 }
 
 int intent::launch_join_bf16(const AttnJoin& j, int side, hipStream_t stream) {

@@ -45,6 +45,15 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 // A cached token's row or scale: global addresses, so that the loads count on vmcnt alone.
 typedef const __attribute__((address_space(1))) char* global_bytes;
 INTENT_DEVICE global_bytes as_global(const void* p) { return (global_bytes)p; }
+// Bytes of a token's head in the cache, and scales (or pairs of f16) beside it.
+template <int kCache, int D>
+constexpr int cached_bytes() {
+  return kCache == kCacheInt4 ? D / 2 : kCache == kCacheFp8 ? D : D * 2;
+}
+template <int kCache, int D>
+constexpr int cached_params() {
+  return kCache == kCacheInt4 ? D / kGroup4 : 1;
+}
 // Rows (of kRowBytes) of a head from token t on, t and the page uniform or not.
 template <int kRowBytes>
 INTENT_DEVICE global_bytes cached_rows(const AttnArgs& a, const void* base, uint32_t page, uint32_t step, int head,
@@ -52,13 +61,16 @@ INTENT_DEVICE global_bytes cached_rows(const AttnArgs& a, const void* base, uint
   const uint32_t row = ((uint32_t)head << a.page_shift) + ((uint32_t)t & ((1u << a.page_shift) - 1u));
   return as_global(base) + ((uint64_t)page * step + (uint64_t)row * (kRowBytes / 16)) * 16;
 }
+// Their scales or pairs, kParams of them to a token.
+template <int kParams>
 INTENT_DEVICE global_bytes cached_scales(const AttnArgs& a, const float* base, uint32_t page, uint32_t step, int head,
                                          int t) {
   const uint32_t row = ((uint32_t)head << a.page_shift) + ((uint32_t)t & ((1u << a.page_shift) - 1u));
-  return as_global(base) + ((uint64_t)page * step + row) * 4;
+  return as_global(base) + ((uint64_t)page * step + (uint64_t)row * kParams) * 4;
 }
 INTENT_DEVICE float load_float(global_bytes p) { return *(const __attribute__((address_space(1))) float*)p; }
 INTENT_DEVICE u32x4 load16(global_bytes p) { return *(const __attribute__((address_space(1))) u32x4*)p; }
+INTENT_DEVICE uint32_t load4(global_bytes p) { return *(const __attribute__((address_space(1))) uint32_t*)p; }
 INTENT_DEVICE u32x2 load8(global_bytes p) { return *(const __attribute__((address_space(1))) u32x2*)p; }
 
 template <bool kBf16>
@@ -120,14 +132,23 @@ INTENT_DEVICE u32x4 only_finite(u32x4 v, bool& found) {
   return v;
 }
 
-// One cached value, its scale left out.
-template <bool kBf16, bool kFp8>
-INTENT_DEVICE float cached_value(const void* row, int d) {
-  if constexpr (kFp8) return __builtin_amdgcn_cvt_f32_fp8((int)((const uint8_t*)row)[d], 0);
-  else if constexpr (kBf16) return bit_cast<float>((uint32_t)((const uint16_t*)row)[d] << 16);
-  else return (float)((const f16*)row)[d];
+// Element d of token t of a page and head in the values, as it goes into the product (8 bits: times its scale).
+template <bool kBf16, int kCache, int D>
+INTENT_DEVICE float cached_value(const AttnArgs& a, int page, int head, int t, int d) {
+  constexpr int kRow = cached_bytes<kCache, D>(), kParams = cached_params<kCache, D>();
+  const char* row = (const char*)cached_rows<kRow>(a, a.v_cache, page, a.v_step, head, t);
+  const char* params = (const char*)cached_scales<kParams>(a, a.v_scales, page, a.vs_step, head, t);
+  if constexpr (kCache == kCacheInt4) {
+    const f16x2 pair = bit_cast<f16x2>(((const uint32_t*)params)[d / kGroup4]);
+    return (float)__builtin_elementwise_fma((f16)(int)(((const uint32_t*)row)[d / 8] >> code_bit(d) & 15u), pair[0], pair[1]);
+  } else if constexpr (kCache == kCacheFp8) {
+    return __builtin_amdgcn_cvt_f32_fp8((int)((const uint8_t*)row)[d], 0) * *(const float*)params;
+  } else if constexpr (kBf16) {
+    return bit_cast<float>((uint32_t)((const uint16_t*)row)[d] << 16);
+  } else {
+    return (float)((const f16*)row)[d];
+  }
 }
-
 INTENT_DEVICE u32x2 read_transposed(const char* lds) {
   return bit_cast<u32x2>(__builtin_amdgcn_ds_read_tr16_b64_v4i16(
       (__attribute__((address_space(3))) s16x4*)(__attribute__((address_space(3))) char*)lds));
@@ -161,13 +182,13 @@ INTENT_DEVICE float scale_exponent(float v) {
   return fmaxf(__builtin_amdgcn_logf(fabsf(v)), kLift<kBf16> - 100.0f);
 }
 
-// Where one query row of a tile (column r of S^T) stands: the tokens lo <= t < hi that it sees.
+// Where one query row of a tile (column r of S^T) stands: its position and the tokens lo <= t < hi that it sees.
 struct RowView {
-  int lo, hi;
+  int lo, hi, p;
 };
 INTENT_DEVICE RowView row_view(const AttnArgs& a, const Span& w, int r) {
   const int p = w.q.kv - w.q.count + (int)((uint32_t)(w.row0 + min(r, w.rows - 1)) / (uint32_t)a.group);
-  return {first_seen(a, p), end_seen(a, p, w.q)};
+  return {first_seen(a, p), end_seen(a, p, w.q), p};
 }
 
 INTENT_DEVICE const uint16_t* q_row(const AttnArgs& a, const Span& w, int head, int r) {
@@ -185,9 +206,39 @@ INTENT_DEVICE u32x4 signed_query(const AttnArgs& a, u32x4 v) {
   return u32x4{v[0] ^ flip, v[1] ^ flip, v[2] ^ flip, v[3] ^ flip};
 }
 
+// The slope of a query row's head in base 2.
+INTENT_DEVICE float slope_of(const AttnArgs& a, const Span& w, int head, int r) {
+  if (a.slopes == nullptr) return 0.f;
+  const int row = w.row0 + min(r, w.rows - 1);
+  return a.slopes[head * a.group + (int)((uint32_t)row % (uint32_t)a.group)] * 1.44269504088896340736f;
+}
+
+// Queries of bf16 for products in f16 (a cache of 4 bits): a row is taken times a power of two that brings its
+// largest element to 2^14 .. 2^15, so that elements down to 2^-28 of that are exact and smaller ones are 2^-39 of
+// it off at most. `high`: the row's largest element's bits without its sign. An infinity or NaN stays one.
+INTENT_DEVICE int query_exponent(uint32_t high) { return min(268 - (int)(high >> 7), 253); }  // biased
+INTENT_DEVICE u32x4 query_f16(u32x4 v, int exponent) {
+  const float by = bit_cast<float>((uint32_t)exponent << 23);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    v[e] = pack2<false>(bit_cast<float>(v[e] << 16) * by, bit_cast<float>(v[e] & 0xffff0000u) * by);
+  return v;
+}
+INTENT_DEVICE uint32_t magnitude(u32x4 v) {
+  uint32_t high = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) high = max(high, max(v[e] & 0x7fffu, v[e] >> 16 & 0x7fffu));
+  return high;
+}
+
 // The size of the scale; instead of zero the smallest f32, which moves no finite score by more than 2^-20 and
 // leaves a masked one at -inf.
 INTENT_DEVICE float scale_of(const AttnArgs& a) { return fmaxf(fabsf(a.scale_log2), 0x1p-149f); }
+
+// The scale of a row that query_f16 took times 2^(exponent - 127); nor is this ever zero.
+INTENT_DEVICE float scale_behind(float scale, int exponent) {
+  return fmaxf(scale * bit_cast<float>((uint32_t)(254 - exponent) << 23), 0x1p-149f);
+}
 
 INTENT_DEVICE float max_across16(float v) {
   const auto r = __builtin_amdgcn_permlane16_swap(bit_cast<uint32_t>(v), bit_cast<uint32_t>(v), false, false);
@@ -206,6 +257,25 @@ INTENT_DEVICE float sum_across32(float v) {
   return bit_cast<float>(r[0]) + bit_cast<float>(r[1]);
 }
 
+// Eight codes of 4 bits as eight f16: 1024 + code and 1024 + 16 code come out of one bitwise operation each, less
+// their 1024 (exact), times the scale plus the lowest value (one rounding).
+INTENT_DEVICE u32x4 widen_codes4(uint32_t word, uint32_t pair) {
+  const f16x2 h = bit_cast<f16x2>(pair), s = splat2(h[0]), m = splat2(h[1]);
+  uint32_t magic = 0x64006400u;
+  asm("" : "+v"(magic));  // in a register, so that mask and magic are one v_bfi_b32
+  const uint32_t rest = word >> 8;
+  u32x4 r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t from = e < 2 ? word : rest;
+    f16x2 code;
+    if (e % 2 == 0) code = bit_cast<f16x2>(bfi(0x000f000fu, from, magic)) - splat2((f16)1024.f);
+    else code = __builtin_elementwise_fma(bit_cast<f16x2>(bfi(0x00f000f0u, from, magic)), splat2((f16)0.0625f), splat2((f16)-64.f));
+    r[e] = bit_cast<uint32_t>(__builtin_elementwise_fma(code, s, m));
+  }
+  return r;
+}
+
 // ---- few rows: 16 * MT of them, the tokens over the waves -----------------------------------------
 
 // A wave takes 32 tokens of each 128: keys straight into the first product's left operand (a lane holds 8
@@ -217,13 +287,18 @@ INTENT_DEVICE float sum_across32(float v) {
 // 242 us, 5.9 TB/s, where a large copy moves 5.1; 64 of 300 to 8191 tokens in 8 bits (645 MB): 124 us, 5.2
 // TB/s, the lengths being uneven. One sequence of 4096 tokens (17 MB) is a chain of latencies, 7 us and 4
 // for the join.
-template <bool kBf16, bool kFp8, int D, int MT>
+template <bool kBf16, int kCache, bool kBiased, int D, int MT>
 __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 256 ? 2 : 1)
     void attn_rows_kernel(const AttnArgs a) {
+  constexpr bool kFp8 = kCache == kCacheFp8, kInt4 = kCache == kCacheInt4;
+  constexpr bool kMath = kBf16 && !kInt4;              // products in bf16
+  constexpr bool kScaled = kFp8 || kBiased;            // scores are scaled before the softmax
   constexpr int KS = D / 32, DT = D / 16, RB = row_bytes<D>();
-  constexpr bool kWide = !kFp8 || D % 64 == 0;         // 16 bytes a lane and load, else 8 codes
-  constexpr int LOADS = kFp8 && kWide ? D / 64 : KS;   // loads of a token's row
-  constexpr int ELEMS = kFp8 && kWide ? 16 : 8;        // elements of one
+  // elements of a lane's load of a token's row: 16 bytes of them if the row's quarter holds as many
+  constexpr int ELEMS = kInt4 ? (D % 128 == 0 ? 32 : D % 64 == 0 ? 16 : 8) : kFp8 && D % 64 == 0 ? 16 : 8;
+  constexpr int LOADS = D / 4 / ELEMS, CHUNKS = ELEMS / 8;  // loads, and 16 bytes of 16-bit elements of one
+  constexpr int kRow = cached_bytes<kCache, D>(), kParams = cached_params<kCache, D>();
+  constexpr int kLoad = kRow / 4 / LOADS;              // bytes of a load
   constexpr int OB = D + 4;                            // floats of a row in the joining buffer
   constexpr int kLds = 4 * 32 * RB > 4 * 16 * OB * 4 ? 4 * 32 * RB : 4 * 16 * OB * 4;
   __shared__ __attribute__((aligned(16))) char lds[kLds];
@@ -232,7 +307,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
 
   const int head = blockIdx.x % a.HK;
   Span w;
-  if (!find_span<false>(a, 16 * MT, 7, blockIdx.x / a.HK, false, w)) return;
+  if (!find_span<kBiased>(a, 16 * MT, 7, blockIdx.x / a.HK, false, w)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int col = lane & 15, g = lane >> 4;
 
@@ -246,12 +321,29 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
     const uint16_t* row = q_row(a, w, head, m * 16 + col);
 #pragma unroll
     for (int i = 0; i < KS; ++i)
-      q[m][i] = signed_query(a, load16(row + (ELEMS == 16 ? at(i / 2) + (i & 1) * 8 : at(i))));
+      q[m][i] = signed_query(a, load16(row + at(i / CHUNKS) + i % CHUNKS * 8));
   }
   // the tokens that some row sees, and those that all rows see
   const RowView top = row_view(a, w, 0), bottom = row_view(a, w, w.rows - 1);
   const int some_lo = top.lo, some_hi = bottom.hi, all_lo = bottom.lo, all_hi = top.hi;
   const float scale = scale_of(a);
+  float row_scale[MT], slope[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    row_scale[m] = scale;
+    if constexpr (kBf16 && kInt4) {
+      uint32_t high = 0;
+#pragma unroll
+      for (int i = 0; i < KS; ++i) high = max(high, magnitude(q[m][i]));
+      // as floats: integers below 2^15 are exact
+      const int exponent = query_exponent((uint32_t)max_across32(max_across16((float)high)));
+#pragma unroll
+      for (int i = 0; i < KS; ++i) q[m][i] = query_f16(q[m][i], exponent);
+      row_scale[m] = scale_behind(scale, exponent);
+    }
+    if constexpr (kBiased) slope[m] = slope_of(a, w, head, m * 16 + col);
+  }
+  const float rate = kBiased ? cap_rate(a) : 0.f;
 
   f32x4 o[MT][DT];
   float ref[MT], total[MT];
@@ -270,29 +362,29 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
       wave * 32 * RB + read_row * RB + (((col >> 1 & 1) ^ swizzle<RB, false>(read_row)) << 4) + (col & 1) * 8;
 
   u32x4 kr[2][LOADS], vr[2][LOADS];
+  uint32_t kg[2][LOADS], vg[2][LOADS];  // pairs of the codes' groups
   float ks[2], vs[2];
   // Pages of 16 tokens and more: each 16 tokens lie in one. The table's entries of this wave's next 32
   // times 32 tokens are kept one in each lane (a vector load every 32 times: scalar loads would make
   // every wait for LDS a wait for them) and clamped where they are used. Smaller pages: each lane looks
   // up its token's.
-  constexpr int kBytes = kFp8 ? 1 : 2;
   const bool paged = a.page_shift >= 4;
-  const uint32_t lane_at = col * (D * kBytes) + g * ELEMS * kBytes;
+  const uint32_t lane_at = col * kRow + g * kLoad;
   auto clamped = [&](int t) { return min(max(t, some_lo), max(some_hi - 1, 0)); };
   uint32_t entries = 0, next_entries = 0;
   auto batch = [&](int t) { return table_entry(a, w.s, clamped(t + (lane >> 1) * 128 + (lane & 1) * 16)); };
   auto issue = [&](int u, global_bytes k, global_bytes v, global_bytes kp, global_bytes vp) {
+    auto codes = [](global_bytes from) {
+      if constexpr (kLoad == 16) return load16(from);
+      if constexpr (kLoad == 4) return u32x4{load4(from), 0u, 0u, 0u};
+      const u32x2 two = load8(from);
+      return u32x4{two[0], two[1], 0u, 0u};
+    };
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      constexpr int kStep = 4 * ELEMS * kBytes;
-      if constexpr (kWide) {
-        kr[u][i] = load16(k + i * kStep);
-        vr[u][i] = load16(v + i * kStep);
-      } else {
-        const u32x2 kc = load8(k + i * kStep), vc = load8(v + i * kStep);
-        kr[u][i] = u32x4{kc[0], kc[1], 0u, 0u};
-        vr[u][i] = u32x4{vc[0], vc[1], 0u, 0u};
-      }
+      kr[u][i] = codes(k + i * 4 * kLoad);
+      vr[u][i] = codes(v + i * 4 * kLoad);
+      if constexpr (kInt4) kg[u][i] = load4(kp + at(i) / kGroup4 * 4), vg[u][i] = load4(vp + at(i) / kGroup4 * 4);
     }
     if constexpr (kFp8) ks[u] = load_float(kp), vs[u] = load_float(vp);
   };
@@ -306,10 +398,10 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
       for (int u = 0; u < 2; ++u) {
         const uint32_t page = page_named(a, (uint32_t)lane_value((int)entries, place + u));
         const int t16 = t + 16 * u;
-        issue(u, cached_rows<D * kBytes>(a, a.k_cache, page, a.k_step, head, t16) + lane_at,
-              cached_rows<D * kBytes>(a, a.v_cache, page, a.v_step, head, t16) + lane_at,
-              cached_scales(a, a.k_scales, page, a.ks_step, head, t16) + col * 4,
-              cached_scales(a, a.v_scales, page, a.vs_step, head, t16) + col * 4);
+        issue(u, cached_rows<kRow>(a, a.k_cache, page, a.k_step, head, t16) + lane_at,
+              cached_rows<kRow>(a, a.v_cache, page, a.v_step, head, t16) + lane_at,
+              cached_scales<kParams>(a, a.k_scales, page, a.ks_step, head, t16) + col * (4 * kParams),
+              cached_scales<kParams>(a, a.v_scales, page, a.vs_step, head, t16) + col * (4 * kParams));
       }
       place += 2;
     } else {
@@ -318,10 +410,10 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
       for (int u = 0; u < 2; ++u) {
         const int tk = t + 16 * u + col;
         const uint32_t page = page_named(a, table_entry(a, w.s, clamped(tk)));
-        issue(u, cached_rows<D * kBytes>(a, a.k_cache, page, a.k_step, head, tk) + g * ELEMS * kBytes,
-              cached_rows<D * kBytes>(a, a.v_cache, page, a.v_step, head, tk) + g * ELEMS * kBytes,
-              cached_scales(a, a.k_scales, page, a.ks_step, head, tk),
-              cached_scales(a, a.v_scales, page, a.vs_step, head, tk));
+        issue(u, cached_rows<kRow>(a, a.k_cache, page, a.k_step, head, tk) + g * kLoad,
+              cached_rows<kRow>(a, a.v_cache, page, a.v_step, head, tk) + g * kLoad,
+              cached_scales<kParams>(a, a.k_scales, page, a.ks_step, head, tk),
+              cached_scales<kParams>(a, a.v_scales, page, a.vs_step, head, tk));
       }
     }
   };
@@ -345,11 +437,11 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
         if (tk < some_lo || tk >= some_hi) {
           vs[u] = 0.f;
 #pragma unroll
-          for (int i = 0; i < LOADS; ++i) vr[u][i] = u32x4{0u, 0u, 0u, 0u};
+          for (int i = 0; i < LOADS; ++i) vr[u][i] = u32x4{0u, 0u, 0u, 0u}, vg[u][i] = 0u;
         }
       }
     }
-    if (apart(t)) {
+    if (!kInt4 && apart(t)) {
       rarely();
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -370,10 +462,14 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
       for (int i = 0; i < LOADS; ++i) {
         char* row = mine + u * 16 * RB + write_at;
         const int chunk = at(i) / 8;
-        if constexpr (kFp8) {
-          *(u32x4*)(row + ((chunk ^ swz) << 4)) = widen_codes<kBf16>(vr[u][i][0], vr[u][i][1]);
-          if constexpr (kWide)
-            *(u32x4*)(row + (((chunk + 1) ^ swz) << 4)) = widen_codes<kBf16>(vr[u][i][2], vr[u][i][3]);
+        if constexpr (kInt4) {
+#pragma unroll
+          for (int c = 0; c < CHUNKS; ++c)
+            *(u32x4*)(row + (((chunk + c) ^ swz) << 4)) = widen_codes4(vr[u][i][c], vg[u][i]);
+        } else if constexpr (kFp8) {
+#pragma unroll
+          for (int c = 0; c < CHUNKS; ++c)
+            *(u32x4*)(row + (((chunk + c) ^ swz) << 4)) = widen_codes<kBf16>(vr[u][i][2 * c], vr[u][i][2 * c + 1]);
         } else {
           *(u32x4*)(row + ((chunk ^ swz) << 4)) = vr[u][i];
         }
@@ -382,9 +478,20 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
         if (g == 0) {
           scales[wave][0][u * 16 + col] = ks[u] * scale;
           scales[wave][1][u * 16 + col] = vs[u];
-          scales[wave][2][u * 16 + col] = scale_exponent<kBf16>(vs[u]);
+          scales[wave][2][u * 16 + col] = scale_exponent<kMath>(vs[u]);
         }
       }
+    }
+    if (kInt4 && apart(t)) {  // once more, what is not finite left out
+      rarely();
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+#pragma unroll
+          for (int c = 0; c < CHUNKS; ++c)
+            *(u32x4*)(mine + u * 16 * RB + write_at + (((at(i) / 8 + c) ^ swz) << 4)) =
+                only_finite<false, false>(widen_codes4(vr[u][i][c], vg[u][i]), found);
     }
     wave_lds_order();
     f32x4 s[MT][2];
@@ -395,11 +502,12 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
 #pragma unroll
       for (int i = 0; i < KS; ++i) {
         u32x4 k;
-        if constexpr (!kFp8) k = kr[u][i];
-        else if constexpr (kWide) k = widen_codes<kBf16>(kr[u][i / 2][(i & 1) * 2], kr[u][i / 2][(i & 1) * 2 + 1]);
-        else k = widen_codes<kBf16>(kr[u][i][0], kr[u][i][1]);
+        const int l = i / CHUNKS, c = i % CHUNKS;
+        if constexpr (kInt4) k = widen_codes4(kr[u][l][c], kg[u][l]);
+        else if constexpr (kFp8) k = widen_codes<kBf16>(kr[u][l][2 * c], kr[u][l][2 * c + 1]);
+        else k = kr[u][i];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) s[m][u] = mfma16<kBf16>(k, q[m][i], s[m][u]);
+        for (int m = 0; m < MT; ++m) s[m][u] = mfma16<kMath>(k, q[m][i], s[m][u]);
       }
     }
     const int now = t;
@@ -420,7 +528,27 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
     }
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      // the highest score, times the value's scale; s is a score or, with an 8-bit cache, its t
+      if constexpr (kBiased) {
+        if constexpr (!kFp8) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) s[m][u] *= row_scale[m];
+        }
+        if (a.cap_log2 != 0.f) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[m][u][r] = capped(s[m][u][r], a.cap_log2, rate);
+        }
+        if (a.slopes != nullptr) {
+          const float ahead = (float)(now + g * 4 - view[m].p);
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              s[m][u][r] = __builtin_fmaf(-slope[m], fabsf(ahead + (float)(16 * u + r)), s[m][u][r]);
+        }
+      }
+      // the highest score, times the value's scale; s is a score or, scaled already, its t
       float high = -INFINITY;
       if (masked) {
         rarely();
@@ -439,7 +567,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
 #pragma unroll
         for (int r = 0; r < 4; ++r) high = fmaxf(high, kFp8 ? s[m][u][r] + v_exp[u][r] : s[m][u][r]);
       high = max_across32(max_across16(high));
-      if constexpr (!kFp8) high *= scale;
+      if constexpr (!kScaled) high *= row_scale[m];
       if (__any(high > ref[m] + kRise)) {
         const float next = fmaxf(ref[m], high);
         const float keep = __builtin_amdgcn_exp2f(ref[m] - (next == -INFINITY ? 0.f : next));
@@ -448,19 +576,19 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[m][d] *= keep;
       }
-      const float base = (ref[m] == -INFINITY ? 0.f : ref[m]) - kLift<kBf16>;
+      const float base = (ref[m] == -INFINITY ? 0.f : ref[m]) - kLift<kMath>;
       float wt[2][4];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float e = __builtin_amdgcn_exp2f(kFp8 ? s[m][u][r] - base : __builtin_fmaf(s[m][u][r], scale, -base));
+          const float e = __builtin_amdgcn_exp2f(kScaled ? s[m][u][r] - base : __builtin_fmaf(s[m][u][r], row_scale[m], -base));
           total[m] += e;
           wt[u][r] = kFp8 ? e * v_mul[u][r] : e;
         }
       }
-      p[m] = u32x4{pack2<kBf16>(wt[0][0], wt[0][1]), pack2<kBf16>(wt[0][2], wt[0][3]), pack2<kBf16>(wt[1][0], wt[1][1]),
-                   pack2<kBf16>(wt[1][2], wt[1][3])};
+      p[m] = u32x4{pack2<kMath>(wt[0][0], wt[0][1]), pack2<kMath>(wt[0][2], wt[0][3]), pack2<kMath>(wt[1][0], wt[1][1]),
+                   pack2<kMath>(wt[1][2], wt[1][3])};
     }
     // V^T: tokens 4 g .. of the first 16, then of the second
     auto value = [&](int d) {
@@ -472,7 +600,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
     for (int d = 0; d < DT; ++d) {
       const u32x4 v = value(d);
 #pragma unroll
-      for (int m = 0; m < MT; ++m) o[m][d] = mfma16<kBf16>(v, p[m], o[m][d]);
+      for (int m = 0; m < MT; ++m) o[m][d] = mfma16<kMath>(v, p[m], o[m][d]);
     }
     wave_lds_order();
   }
@@ -480,13 +608,11 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
     for (t = w.begin + wave * 32; t < w.end; t += 128) {
       for (int tk = max(t, some_lo); apart(t) && tk < min(t + 32, some_hi); ++tk) {
         const int page = page_of(a, w.s, tk);
-        const char* row = (const char*)a.v_cache + row_in_cache(a, page, a.v_page, head, tk, D) * kBytes;
-        const float times = kFp8 ? a.v_scales[row_in_cache(a, page, a.vs_page, head, tk, 1)] : 1.f;
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float v = cached_value<kBf16, kFp8>(row, d * 16 + g * 4 + r) * times;
+            const float v = cached_value<kBf16, kCache, D>(a, page, head, tk, d * 16 + g * 4 + r);
 #pragma unroll
             for (int m = 0; m < MT; ++m)
               if (tk >= view[m].lo && tk < view[m].hi && !(fabsf(v) < INFINITY)) o[m][d][r] += v;
@@ -552,12 +678,17 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
 // TFLOP/s. What is left: with the loads of the cache taken away it takes 140 us, with the vector work
 // 117, with the products 111; each wave's own chain, not one unit, sets the time. 64 rows to a wave read LDS
 // half as often, but one wave to a SIMD and 1500 copies between the two halves of its registers take 215 us.
-template <bool kBf16, bool kFp8, int D, int WAVES>
+template <bool kBf16, int kCache, bool kBiased, int D, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
     void attn_tile_kernel(const AttnArgs a) {
+  constexpr bool kFp8 = kCache == kCacheFp8, kInt4 = kCache == kCacheInt4;
+  constexpr bool kMath = kBf16 && !kInt4;             // products in bf16
+  constexpr bool kScaled = kFp8 || kBiased;           // scores are scaled before the softmax
   constexpr int KS = D / 16, DT = D / 32, RB = row_bytes<D>();
-  constexpr int CHUNKS = kFp8 ? D / 16 : D / 8;       // 16-byte loads of a token's row
-  constexpr int SPREAD = kFp8 ? RB / 32 : RB / 16;    // lanes that take one (a power of two)
+  constexpr int kRow = cached_bytes<kCache, D>(), kParams = cached_params<kCache, D>();
+  constexpr int CHUNKS = kRow / 16;                   // 16-byte loads of a token's row
+  // lanes that take one (a power of two; four where two would do, so that as many waves load)
+  constexpr int SPREAD = kInt4 ? (RB / 64 < 4 ? 4 : RB / 64) : kFp8 ? RB / 32 : RB / 16;
   constexpr int EACH = 64 / SPREAD;                   // tokens that a wave loads at once
   constexpr int STEP = EACH * WAVES;                  // and the workgroup
   constexpr int LOADS = STEP >= 64 ? 1 : 64 / STEP, ROWS = 32 * WAVES;
@@ -570,7 +701,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
 
   const int head = blockIdx.x % a.HK;
   Span w;
-  if (!find_span<false>(a, ROWS, 6, blockIdx.x / a.HK, false, w)) return;
+  if (!find_span<kBiased>(a, ROWS, 6, blockIdx.x / a.HK, false, w)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int col = lane & 31, h = lane >> 5;
   const int r0 = wave * 32;
@@ -587,6 +718,18 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
   const RowView top = row_view(a, w, r0), bottom = row_view(a, w, r0 + 31);  // of this wave
   const bool idle = r0 >= w.rows;
   const float scale = scale_of(a);
+  float row_scale = scale, slope = 0.f;
+  if constexpr (kBf16 && kInt4) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) most = max(most, magnitude(q[i]));
+    const int exponent = query_exponent((uint32_t)max_across32((float)most));  // as floats: exact
+#pragma unroll
+    for (int i = 0; i < KS; ++i) q[i] = query_f16(q[i], exponent);
+    row_scale = scale_behind(scale, exponent);
+  }
+  if constexpr (kBiased) slope = slope_of(a, w, head, r0 + col);
+  const float rate = kBiased ? cap_rate(a) : 0.f;
 
   f32x16 o[DT];
 #pragma unroll
@@ -599,12 +742,12 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
   const int load_token = wave_token + lane / SPREAD, load_chunk = lane % SPREAD;
   const bool loads = load_chunk < CHUNKS && wave * EACH < 64;
   u32x4 kr[LOADS], vr[LOADS];
+  uint32_t kg[LOADS], vg[LOADS];  // pairs of the codes' groups
   float ks = 0.f, vs = 0.f;
   // Pages of EACH tokens and more (16 at most): each load's tokens lie in one, whose id is a scalar.
-  constexpr int kBytes = kFp8 ? 1 : 2;
   const bool paged = (1 << a.page_shift) >= EACH;
   const int chunk = load_chunk < CHUNKS ? load_chunk : 0;
-  const uint32_t lane_at = (lane / SPREAD) * (D * kBytes) + chunk * 16;
+  const uint32_t lane_at = (lane / SPREAD) * kRow + chunk * 16, pair_at = (lane / SPREAD) * (4 * kParams) + chunk * 4;
   // The table's entries of the next `span` times 64 tokens, one in each lane, in two batches (as above).
   const bool one_page = a.page_shift >= 6;  // the 64 tokens in one page
   constexpr int kLoadsLog = LOADS == 1 ? 0 : LOADS == 2 ? 1 : LOADS == 4 ? 2 : 3;
@@ -622,18 +765,25 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
   };
   // Tokens that no row sees are loaded too (a page that is there, whatever it holds): their scores are
   // masked, their values set to zero when they are stored.
-  auto load = [&](u32x4(&fetched)[LOADS], const void* cache, uint32_t step, int t) __attribute__((always_inline)) {
+  auto load = [&](u32x4(&fetched)[LOADS], uint32_t(&pairs)[LOADS], const void* cache, uint32_t step,
+                  const float* params, uint32_t pair_step, int t) __attribute__((always_inline)) {
     const int n = (t - w.begin) >> 6;
     if (one_page) {
       const uint32_t page = page_named(a, entry(n, 0));
-      const global_bytes from = cached_rows<D * kBytes>(a, cache, page, step, head, t + wave_token);
+      const global_bytes from = cached_rows<kRow>(a, cache, page, step, head, t + wave_token);
+      const global_bytes beside = cached_scales<kParams>(a, params, page, pair_step, head, t + wave_token);
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i) fetched[i] = load16(from + i * (STEP * D * kBytes) + lane_at);
+      for (int i = 0; i < LOADS; ++i) {
+        fetched[i] = load16(from + i * (STEP * kRow) + lane_at);
+        if constexpr (kInt4) pairs[i] = load4(beside + i * (STEP * 4 * kParams) + pair_at);
+      }
     } else if (paged) {
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         const uint32_t page = page_named(a, entry(n, i));
-        fetched[i] = load16(cached_rows<D * kBytes>(a, cache, page, step, head, t + i * STEP + wave_token) + lane_at);
+        const int tk = t + i * STEP + wave_token;
+        fetched[i] = load16(cached_rows<kRow>(a, cache, page, step, head, tk) + lane_at);
+        if constexpr (kInt4) pairs[i] = load4(cached_scales<kParams>(a, params, page, pair_step, head, tk) + pair_at);
       }
     } else {
       rarely();
@@ -641,29 +791,33 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
       for (int i = 0; i < LOADS; ++i) {
         const int tk = t + i * STEP + load_token;
         const uint32_t page = page_named(a, table_entry(a, w.s, clamped(tk)));
-        fetched[i] = load16(cached_rows<D * kBytes>(a, cache, page, step, head, tk) + chunk * 16);
+        fetched[i] = load16(cached_rows<kRow>(a, cache, page, step, head, tk) + chunk * 16);
+        if constexpr (kInt4) pairs[i] = load4(cached_scales<kParams>(a, params, page, pair_step, head, tk) + chunk * 4);
       }
     }
   };
-  auto load_keys = [&](int t) __attribute__((always_inline)) { load(kr, a.k_cache, a.k_step, t); };
+  auto load_keys = [&](int t) __attribute__((always_inline)) { load(kr, kg, a.k_cache, a.k_step, a.k_scales, a.ks_step, t); };
   auto load_values = [&](int t) __attribute__((always_inline)) {
-    load(vr, a.v_cache, a.v_step, t);
+    load(vr, vg, a.v_cache, a.v_step, a.v_scales, a.vs_step, t);
     if constexpr (kFp8) {
       if (wave == 0) {
         const int tk = t + lane;
         const uint32_t page = page_named(a, table_entry(a, w.s, clamped(tk)));
-        ks = load_float(cached_scales(a, a.k_scales, page, a.ks_step, head, tk));
-        vs = load_float(cached_scales(a, a.v_scales, page, a.vs_step, head, tk));
+        ks = load_float(cached_scales<1>(a, a.k_scales, page, a.ks_step, head, tk));
+        vs = load_float(cached_scales<1>(a, a.v_scales, page, a.vs_step, head, tk));
       }
     }
   };
-  auto store = [&](char* to, const u32x4(&from)[LOADS]) __attribute__((always_inline)) {
+  auto store = [&](char* to, const u32x4(&from)[LOADS], const uint32_t(&pairs)[LOADS]) __attribute__((always_inline)) {
     if (!loads) return;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int tk = load_token + i * STEP, swz = swizzle<RB, true>(tk);
       char* row = to + tk * RB;
-      if constexpr (kFp8) {
+      if constexpr (kInt4) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) *(u32x4*)(row + ((load_chunk * 4 + c ^ swz) << 4)) = widen_codes4(from[i][c], pairs[i]);
+      } else if constexpr (kFp8) {
         *(u32x4*)(row + ((load_chunk * 2 ^ swz) << 4)) = widen_codes<kBf16>(from[i][0], from[i][1]);
         *(u32x4*)(row + (((load_chunk * 2 + 1) ^ swz) << 4)) = widen_codes<kBf16>(from[i][2], from[i][3]);
       } else {
@@ -681,11 +835,11 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         const int tk = t + i * STEP + load_token;
-        if (tk < some_lo || tk >= some_hi) vr[i] = u32x4{0u, 0u, 0u, 0u};
+        if (tk < some_lo || tk >= some_hi) vr[i] = u32x4{0u, 0u, 0u, 0u}, vg[i] = 0u;
       }
       if (t + lane < some_lo || t + lane >= some_hi) vs = 0.f;
     }
-    if (apart(t)) {
+    if (!kInt4 && apart(t)) {
       rarely();
       bool found = false;
 #pragma unroll
@@ -697,12 +851,27 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
       }
       if (found) left_out = 1;
     }
-    store(lds[buffer][1], vr);
+    store(lds[buffer][1], vr, vg);
+    if (kInt4 && apart(t)) {  // once more, what is not finite left out
+      rarely();
+      bool found = false;
+      if (loads) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+          const int tk = load_token + i * STEP;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            *(u32x4*)(lds[buffer][1] + tk * RB + ((load_chunk * 4 + c ^ swizzle<RB, true>(tk)) << 4)) =
+                only_finite<false, false>(widen_codes4(vr[i][c], vg[i]), found);
+        }
+      }
+      if (found) left_out = 1;
+    }
     if constexpr (kFp8) {
       if (wave == 0) {
         scales[buffer][0][lane] = ks * scale;
         scales[buffer][1][lane] = vs;
-        scales[buffer][2][lane] = scale_exponent<kBf16>(vs);
+        scales[buffer][2][lane] = scale_exponent<kMath>(vs);
       }
     }
   };
@@ -722,7 +891,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
     for (int i = 0; i < KS; ++i)
 #pragma unroll
       for (int u = 0; u < 2; ++u)
-        s[u] = mfma32<kBf16>(*(const u32x4*)(keys + u * 32 * RB + (k_at ^ (i * 32))), q[i], s[u]);
+        s[u] = mfma32<kMath>(*(const u32x4*)(keys + u * 32 * RB + (k_at ^ (i * 32))), q[i], s[u]);
   };
 
   // kAhead: of tokens t, values (and scales) in buffer j, their scores in registers; of t + 64, keys in
@@ -737,12 +906,13 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
     load_values(w.begin);
     if constexpr (kAhead) {
       u32x4 second[LOADS];
-      load(second, a.k_cache, a.k_step, w.begin + 64);
-      store(lds[0][0], kr);
+      uint32_t second_pairs[LOADS];
+      load(second, second_pairs, a.k_cache, a.k_step, a.k_scales, a.ks_step, w.begin + 64);
+      store(lds[0][0], kr, kg);
       store_values(0, w.begin);
-      store(lds[1][0], second);
+      store(lds[1][0], second, second_pairs);
     } else {
-      store(lds[0][0], kr);
+      store(lds[0][0], kr, kg);
       store_values(0, w.begin);
     }
   }
@@ -780,6 +950,26 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
             for (int r = 0; r < 4; ++r) s[u][i * 4 + r] *= k_mul[r];
           }
       }
+      if constexpr (kBiased) {
+        if constexpr (!kFp8) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) s[u] *= row_scale;
+        }
+        if (a.cap_log2 != 0.f) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[u][r] = capped(s[u][r], a.cap_log2, rate);
+        }
+        if (a.slopes != nullptr) {
+          const float ahead = (float)(t + h * 4 - view.p);
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              s[u][r] = __builtin_fmaf(-slope, fabsf(ahead + (float)(u * 32 + (r >> 2) * 8 + (r & 3))), s[u][r]);
+        }
+      }
       if (masked) {
         rarely();
         const int lo = view.lo - t - h * 4, hi = view.hi - t - h * 4;
@@ -800,7 +990,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
 #pragma unroll
           for (int r = 0; r < 4; ++r) high = fmaxf(high, kFp8 ? s[u][i * 4 + r] + v_exp[r] : s[u][i * 4 + r]);
         }
-      if constexpr (!kFp8) high *= scale;
+      if constexpr (!kScaled) high *= row_scale;
       high = max_across32(high);
       if (__any(high > ref + kRise)) {
         rarely();
@@ -813,7 +1003,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[d][r] *= keep;
       }
-      const float base = (ref == -INFINITY ? 0.f : ref) - kLift<kBf16>;
+      const float base = (ref == -INFINITY ? 0.f : ref) - kLift<kMath>;
       // Sixteen steps, each with the weights of two tokens, its part of the next tokens' products with the
       // queries (kAhead; of what lies in that buffer behind the last tokens, too: not used then) and, four
       // steps behind, of the products with these values, so that the matrix unit works through all of them.
@@ -844,7 +1034,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
         for (int n = 0; n < V_ALL; ++n) {
           if (n < from || n >= to) continue;
           if (n + V_AHEAD < V_ALL) vf[n + V_AHEAD] = value(n + V_AHEAD);
-          o[n % DT] = mfma32<kBf16>(vf[n], p[n / DT], o[n % DT]);
+          o[n % DT] = mfma32<kMath>(vf[n], p[n / DT], o[n % DT]);
         }
       };
       float sums[2] = {0.f, 0.f};
@@ -854,7 +1044,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
 #pragma unroll
           for (int n = i * S_ALL / 16; n < (i + 1) * S_ALL / 16; ++n) {
             if (n + K_AHEAD < S_ALL) kf[n + K_AHEAD] = key(n + K_AHEAD);
-            after[n & 1] = mfma32<kBf16>(kf[n], q[n >> 1], after[n & 1]);
+            after[n & 1] = mfma32<kMath>(kf[n], q[n >> 1], after[n & 1]);
           }
         }
         if (i == 3) {
@@ -868,11 +1058,11 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float x = s[i / 8][i % 8 * 2 + e];
-          const float y = __builtin_amdgcn_exp2f(kFp8 ? x - base : __builtin_fmaf(x, scale, -base));
+          const float y = __builtin_amdgcn_exp2f(kScaled ? x - base : __builtin_fmaf(x, row_scale, -base));
           sums[e] += y;
           wt[e] = kFp8 ? y * v_mul[i % 2 * 2 + e] : y;
         }
-        p[i / 4][i % 4] = pack2<kBf16>(wt[0], wt[1]);
+        p[i / 4][i % 4] = pack2<kMath>(wt[0], wt[1]);
         __builtin_amdgcn_sched_barrier(0);
       };
 #pragma unroll
@@ -883,7 +1073,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
     }
     if (more) {
       store_values(j ^ 1, t + 64);
-      store(lds[kAhead ? j : j ^ 1][0], kr);
+      store(lds[kAhead ? j : j ^ 1][0], kr, kg);
     }
     __syncthreads();
   }
@@ -892,14 +1082,12 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
     for (int t = w.begin; t < w.end; t += 64) {
       for (int tk = max(t, some_lo); apart(t) && tk < min(t + 64, some_hi); ++tk) {
         const int page = page_of(a, w.s, tk);
-        const char* row = (const char*)a.v_cache + row_in_cache(a, page, a.v_page, head, tk, D) * kBytes;
-        const float times = kFp8 ? a.v_scales[row_in_cache(a, page, a.vs_page, head, tk, 1)] : 1.f;
         const bool seen = tk >= view.lo && tk < view.hi;
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const float v = cached_value<kBf16, kFp8>(row, d * 32 + (r >> 2) * 8 + h * 4 + (r & 3)) * times;
+            const float v = cached_value<kBf16, kCache, D>(a, page, head, tk, d * 32 + (r >> 2) * 8 + h * 4 + (r & 3));
             if (seen && !(fabsf(v) < INFINITY)) o[d][r] += v;
           }
         }
@@ -939,7 +1127,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
 // their way. What the first list needs to be found comes before the struct, where the kernel has it in
 // registers when it starts. A launch and a chain of four latencies: 4.2 to 4.8 us for one tile of 32 parts;
 // one launch for the tiles of a mixture's two lists 7.2 us, where two took 11.4.
-template <bool kBf16, int D>
+template <bool kBf16, bool kBiased, int D>
 __global__ __launch_bounds__(256) void attn_join_kernel(int items, int tile, int unit_log, const AttnJoin j) {
   constexpr int E = (D + 63) / 64, AHEAD = 8, FEW = 16;
   constexpr int LANES = D == 96 ? 32 : D / 4, TOGETHER = 64 / LANES;  // lanes of a row, rows of a wave
@@ -954,7 +1142,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(int items, int tile, int
     a.partial = j.partial, a.partial_stats = j.partial_stats;
   }
   Span w;
-  if (!find_span<false>(a, tile, unit_log, item, true, w)) return;
+  if (!find_span<kBiased>(a, tile, unit_log, item, true, w)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (w.splits <= FEW) {
     const int c = lane % LANES * 4 < D ? lane % LANES * 4 : 0;
@@ -1053,58 +1241,60 @@ __global__ __launch_bounds__(256) void attn_join_kernel(int items, int tile, int
 }
 
 // ROWS up to 64: rows of the first kernel; 128 or 256: of the second's four or eight waves.
-template <bool kBf16, bool kFp8, int D, int ROWS>
+template <bool kBf16, int kCache, bool kBiased, int D, int ROWS>
 int launch(const AttnArgs& a, int items, hipStream_t stream) {
   const unsigned groups = (unsigned)items * (unsigned)a.HK;
   constexpr bool kFew = ROWS <= 64;
   if constexpr (kFew)
-    hipLaunchKernelGGL((attn_rows_kernel<kBf16, kFp8, D, ROWS / 16>), dim3(groups), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((attn_rows_kernel<kBf16, kCache, kBiased, D, ROWS / 16>), dim3(groups), dim3(256), 0, stream, a);
   else
-    hipLaunchKernelGGL((attn_tile_kernel<kBf16, kFp8, D, ROWS / 32>), dim3(groups), dim3(ROWS * 2), 0, stream, a);
-  static const KernelName name("attn_%s_kernel<%s%s, D %d, %d rows>", kFew ? "rows" : "tile", kBf16 ? "bf16" : "f16",
-                               kFp8 ? ", fp8 cache" : "", D, ROWS);
+    hipLaunchKernelGGL((attn_tile_kernel<kBf16, kCache, kBiased, D, ROWS / 32>), dim3(groups), dim3(ROWS * 2), 0, stream,
+                       a);
+  static const KernelName name("attn_%s_kernel<%s%s%s, D %d, %d rows>", kFew ? "rows" : "tile", kBf16 ? "bf16" : "f16",
+                               cache_name(kCache), kBiased ? ", biased" : "", D, ROWS);
   return launch_status(name.text);
 }
 
-template <bool kBf16, bool kFp8, int D>
+template <bool kBf16, int kCache, bool kBiased, int D>
 int launch_d(const AttnArgs& a, int items, int rows, hipStream_t stream) {
-  if (rows == 16) return launch<kBf16, kFp8, D, 16>(a, items, stream);
+  if (rows == 16) return launch<kBf16, kCache, kBiased, D, 16>(a, items, stream);
   if constexpr (D <= 128) {
-    if (rows == 32) return launch<kBf16, kFp8, D, 32>(a, items, stream);
-    if (rows == 48) return launch<kBf16, kFp8, D, 48>(a, items, stream);
-    if (rows == 64) return launch<kBf16, kFp8, D, 64>(a, items, stream);
-    if (rows == 256) return launch<kBf16, kFp8, D, 256>(a, items, stream);
+    if (rows == 32) return launch<kBf16, kCache, kBiased, D, 32>(a, items, stream);
+    if (rows == 48) return launch<kBf16, kCache, kBiased, D, 48>(a, items, stream);
+    if (rows == 64) return launch<kBf16, kCache, kBiased, D, 64>(a, items, stream);
+    if (rows == 256) return launch<kBf16, kCache, kBiased, D, 256>(a, items, stream);
   }
-  return launch<kBf16, kFp8, D, 128>(a, items, stream);
+  return launch<kBf16, kCache, kBiased, D, 128>(a, items, stream);
 }
 
-template <bool kBf16, bool kFp8>
+template <bool kBf16, int kCache, bool kBiased = false>
 int launch_any(const AttnArgs& a, int items, int rows, hipStream_t stream) {
   switch (a.D) {
-    case 64: return launch_d<kBf16, kFp8, 64>(a, items, rows, stream);
-    case 96: return launch_d<kBf16, kFp8, 96>(a, items, rows, stream);
-    case 128: return launch_d<kBf16, kFp8, 128>(a, items, rows, stream);
-    case 256: return launch_d<kBf16, kFp8, 256>(a, items, rows, stream);
+    case 64: return launch_d<kBf16, kCache, kBiased, 64>(a, items, rows, stream);
+    case 96: return launch_d<kBf16, kCache, kBiased, 96>(a, items, rows, stream);
+    case 128: return launch_d<kBf16, kCache, kBiased, 128>(a, items, rows, stream);
+    case 256: return launch_d<kBf16, kCache, kBiased, 256>(a, items, rows, stream);
     default: return fail(INTENT_ERR_UNSUPPORTED, "no tiled attention kernel for heads of %d", a.D);
   }
 }
 
-template <bool kBf16, int D>
+template <bool kBf16, bool kBiased, int D>
 int launch_join_d(const AttnJoin& j, int side, hipStream_t stream) {
   const unsigned groups = (unsigned)(j.items[0] + j.items[1]) * (unsigned)j.a.HK;
-  hipLaunchKernelGGL((attn_join_kernel<kBf16, D>), dim3(groups, side), dim3(256), 0, stream, j.items[0], j.tile[0],
-                     j.unit_log[0], j);
-  static const KernelName name("attn_join_kernel<%s, D %d> of splits", kBf16 ? "bf16" : "f16", D);
+  hipLaunchKernelGGL((attn_join_kernel<kBf16, kBiased, D>), dim3(groups, side), dim3(256), 0, stream, j.items[0],
+                     j.tile[0], j.unit_log[0], j);
+  static const KernelName name("attn_join_kernel<%s%s, D %d> of splits", kBf16 ? "bf16" : "f16",
+                               kBiased ? ", biased" : "", D);
   return launch_status(name.text);
 }
 
-template <bool kBf16>
+template <bool kBf16, bool kBiased = false>
 int launch_join(const AttnJoin& j, int side, hipStream_t stream) {
   switch (j.a.D) {
-    case 64: return launch_join_d<kBf16, 64>(j, side, stream);
-    case 96: return launch_join_d<kBf16, 96>(j, side, stream);
-    case 128: return launch_join_d<kBf16, 128>(j, side, stream);
-    case 256: return launch_join_d<kBf16, 256>(j, side, stream);
+    case 64: return launch_join_d<kBf16, kBiased, 64>(j, side, stream);
+    case 96: return launch_join_d<kBf16, kBiased, 96>(j, side, stream);
+    case 128: return launch_join_d<kBf16, kBiased, 128>(j, side, stream);
+    case 256: return launch_join_d<kBf16, kBiased, 256>(j, side, stream);
     default: return fail(INTENT_ERR_UNSUPPORTED, "no tiled attention kernel for heads of %d", j.a.D);
   }
 }
