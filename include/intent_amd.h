@@ -818,8 +818,7 @@ int intent_paged_kv_read(int cache_format,
  * intent_paged_attention. A window bounds the prefix as well. Values in 4 bits
  * are rounded to f16 for the products, in bf16 too (the queries of bf16, scaled
  * by a power of two for each row, are exact in f16 or 2^-38 of the row's largest
- * off). The workspace is that of intent_paged_attention_workspace_size. No
- * reference counterpart.
+ * off). Workspace as in intent_paged_attention. No reference counterpart.
  */
 int intent_biased_paged_attention(const void* q, int64_t T, int64_t HQ, int64_t q_ld,
                                   int is_bf16, int cache_format,
@@ -833,6 +832,8 @@ int intent_biased_paged_attention(const void* q, int64_t T, int64_t HQ, int64_t 
                                   float softcap, const float* slopes, const int32_t* prefix_lens,
                                   void* out, int64_t out_ld,
                                   void* workspace, size_t workspace_bytes, void* stream);
+size_t intent_biased_paged_attention_workspace_size(int64_t T, int64_t HQ, int64_t HK, int64_t D, int64_t S,
+                                                    int64_t table_width, int64_t page_size, int cache_format);
 
 /*
  * Repeats a call that the caller keeps as slots: one int64 for each argument

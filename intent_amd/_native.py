@@ -100,6 +100,7 @@ SIGNATURES: dict[str, tuple[list, object]] = {
     "intent_paged_kv_read": ([INT, P, I64, P, I64, P, I64, P, I64, I64, I64, I64, I64, P, I64, INT, P, I64, P, I64, P], INT),
     "intent_biased_paged_attention": ([P, I64, I64, I64, INT, INT, P, I64, P, I64, P, I64, P, I64, I64, I64, I64, I64, P,
                                        I64, I64, I64, P, P, F32, INT, I64, F32, P, P, P, I64, P, SIZE, P], INT),
+    "intent_biased_paged_attention_workspace_size": ([I64, I64, I64, I64, I64, I64, I64, INT], SIZE),
     "intent_amd_replay": ([INT, P, I64, P], INT),
     "intent_hbm_read_probe": ([P, I64, INT, INT, P, I64, P], INT),
     "intent_mfma_peak_probe": ([INT, I64, I64, P, P], INT),

@@ -194,7 +194,12 @@ struct Part {
   // little (four sequences of 60000 to 131000 tokens: 300 us at 512, 235 at 768, 239 at 1536; 64 of 300
   // to 8191 126, 128 and 119 us). One workgroup to a CU loses by a second round (16 sequences of five
   // drafted tokens: 28 us at 256, 34 at 512).
-  int fill(int64_t D) const {
+  //
+  // 4 bits: a CU holds four of 16 rows. Many sequences are evened out by two rounds of them (64 of 300 to 8191
+  // tokens: 87, 89 and 83 us at 1024, 1536 and 2048); few are cut into parts enough by one, and their join costs
+  // more with every part (four of 60000 to 131000: 88, 89 and 90 us, the join 6.0, 7.4 and 10.0).
+  int fill(int64_t D, int cache, int64_t lists) const {
+    if (cache == kCacheInt4 && rows * D <= 2048) return lists >= 256 ? 2048 : 1024;
     if (rows > 64) return rows == 256 || D > 128 ? 256 : 512;
     return D > 128 ? 256 : rows * D <= 2048 ? 1536 : rows * D <= 4096 ? 512 : 256;
   }
@@ -260,16 +265,17 @@ int64_t tiles_bound(const Part& p, int64_t T, int64_t S, int64_t group) {
 // round of a few long shares, so twice as many (111 sequences of 2600 to 7500 tokens on two heads: 612 us
 // with 256 shares, 401 with 512; 128 of them 570 and 434; all of 5000 332 and 360). More tiles to a sequence
 // even out by themselves.
-int64_t target_of(const Part& p, int64_t T, int64_t S, int64_t group, int64_t HK, int64_t D) {
-  const int64_t fill = p.fill(D);
+int64_t target_of(const Part& p, int64_t T, int64_t S, int64_t group, int64_t HK, int64_t D, int cache) {
+  const int64_t fill = p.fill(D, cache, S * HK);
   const bool uneven = D > 128 && p.rows == 128 && T * group <= S * p.rows && S * HK * 2 > fill;
   return (fill * (uneven ? 2 : 1) + HK - 1) / HK;
 }
 
 // Parts of all split tiles of one head: fewer than twice the target (a tile of one and a half shares and
 // more is cut to the nearest number of them), and at most every tile's most.
-int64_t slots_bound(const Part& p, int64_t T, int64_t S, int64_t group, int64_t HK, int64_t D, int64_t most_kv) {
-  const int64_t target = target_of(p, T, S, group, HK, D);
+int64_t slots_bound(const Part& p, int64_t T, int64_t S, int64_t group, int64_t HK, int64_t D, int cache,
+                    int64_t most_kv) {
+  const int64_t target = target_of(p, T, S, group, HK, D, cache);
   int64_t splits = (most_kv + (1 << p.unit_log()) - 1) >> p.unit_log();
   if (splits > kMostSplits) splits = kMostSplits;
   if (splits < 2) return 0;
@@ -277,8 +283,9 @@ int64_t slots_bound(const Part& p, int64_t T, int64_t S, int64_t group, int64_t 
   return all < 2 * target ? all : 2 * target;
 }
 
-size_t part_bytes(const Part& p, int64_t T, int64_t S, int64_t group, int64_t HK, int64_t D, int64_t most_kv) {
-  return (size_t)(slots_bound(p, T, S, group, HK, D, most_kv) * HK * p.rows * (D + 2) * 4);
+size_t part_bytes(const Part& p, int64_t T, int64_t S, int64_t group, int64_t HK, int64_t D, int cache,
+                  int64_t most_kv) {
+  return (size_t)(slots_bound(p, T, S, group, HK, D, cache, most_kv) * HK * p.rows * (D + 2) * 4);
 }
 
 // By cache format, scores biased or not, and heads of bf16 or not.
@@ -292,17 +299,17 @@ LaunchJoin* const kLaunchJoin[2][2] = {{launch_join_f16, launch_join_bf16},
 int launch_tiled(AttnArgs a, bool bf16, int cache, bool biased, float* workspace, size_t bytes, hipStream_t stream) {
   const Plan plan = plan_of(a.T, a.S, a.HK, a.group, a.D);
   size_t need = 0;
-  for (int i = 0; i < plan.parts; ++i) need += part_bytes(plan.part[i], a.T, a.S, a.group, a.HK, a.D, a.most_kv);
+  for (int i = 0; i < plan.parts; ++i) need += part_bytes(plan.part[i], a.T, a.S, a.group, a.HK, a.D, cache, a.most_kv);
   AttnJoin join{};
   int lists = 0;
   for (int i = 0; i < plan.parts; ++i) {
     const Part& p = plan.part[i];
-    const int64_t slots = slots_bound(p, a.T, a.S, a.group, a.HK, a.D, a.most_kv);
+    const int64_t slots = slots_bound(p, a.T, a.S, a.group, a.HK, a.D, cache, a.most_kv);
     // one sequence's tiles all attend the same tokens: enough of them even out by themselves
-    const bool many = a.S == 1 && (int64_t)a.T * a.group / p.rows * a.HK >= 2 * p.fill(a.D);
+    const bool many = a.S == 1 && (int64_t)a.T * a.group / p.rows * a.HK >= 2 * p.fill(a.D, cache, a.HK);
     const bool split = slots > 0 && workspace != nullptr && bytes >= need && !many;
     a.min_rows = p.min_rows, a.max_rows = p.max_rows;
-    a.target = split ? (int)target_of(p, a.T, a.S, a.group, a.HK, a.D) : 0;
+    a.target = split ? (int)target_of(p, a.T, a.S, a.group, a.HK, a.D, cache) : 0;
     a.slots = split ? (int)slots : 0;
     a.partial = workspace;
     a.partial_stats = split ? workspace + slots * a.HK * p.rows * a.D : nullptr;
@@ -325,7 +332,7 @@ int launch_tiled(AttnArgs a, bool bf16, int cache, bool biased, float* workspace
     }
     join.tile[lists] = p.rows, join.unit_log[lists] = p.unit_log();
     join.items[lists++] = (int)(tiles < most ? tiles : most);
-    workspace += part_bytes(p, a.T, a.S, a.group, a.HK, a.D, a.most_kv) / 4;
+    workspace += part_bytes(p, a.T, a.S, a.group, a.HK, a.D, cache, a.most_kv) / 4;
   }
   if (lists == 0) return INTENT_OK;
   // workgroups for the rows of a split tile: one for each of a mean sequence, up to 1024 in all
@@ -338,16 +345,22 @@ int launch_tiled(AttnArgs a, bool bf16, int cache, bool biased, float* workspace
 
 }  // namespace
 
-extern "C" size_t intent_paged_attention_workspace_size(int64_t T, int64_t HQ, int64_t HK, int64_t D, int64_t S,
-                                                        int64_t table_width, int64_t page_size) {
+extern "C" size_t intent_biased_paged_attention_workspace_size(int64_t T, int64_t HQ, int64_t HK, int64_t D, int64_t S,
+                                                               int64_t table_width, int64_t page_size,
+                                                               int cache_format) {
   if (T <= 0 || HQ <= 0 || HK <= 0 || S <= 0 || HQ % HK || table_width <= 0 || page_size <= 0 || !tiled(D) ||
       table_width > kMostTokens / page_size || HQ > 65536 || T * HQ >= ((int64_t)1 << 25))
     return 0;
   const Plan plan = plan_of(T, S, HK, HQ / HK, D);
   size_t need = 0;
   for (int i = 0; i < plan.parts; ++i)
-    need += part_bytes(plan.part[i], T, S, HQ / HK, HK, D, table_width * page_size);
+    need += part_bytes(plan.part[i], T, S, HQ / HK, HK, D, cache_format, table_width * page_size);
   return need;
+}
+
+extern "C" size_t intent_paged_attention_workspace_size(int64_t T, int64_t HQ, int64_t HK, int64_t D, int64_t S,
+                                                        int64_t table_width, int64_t page_size) {
+  return intent_biased_paged_attention_workspace_size(T, HQ, HK, D, S, table_width, page_size, INTENT_CACHE_SAME);
 }
 
 namespace {

@@ -258,23 +258,32 @@ INTENT_DEVICE float sum_across32(float v) {
 }
 
 // Eight codes of 4 bits as eight f16: 1024 + code and 1024 + 16 code come out of one bitwise operation each, less
-// their 1024 (exact), times the scale plus the lowest value (one rounding).
-INTENT_DEVICE u32x4 widen_codes4(uint32_t word, uint32_t pair) {
-  const f16x2 h = bit_cast<f16x2>(pair), s = splat2(h[0]), m = splat2(h[1]);
-  uint32_t magic = 0x64006400u;
-  asm("" : "+v"(magic));  // in a register, so that mask and magic are one v_bfi_b32
-  const uint32_t rest = word >> 8;
-  u32x4 r;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const uint32_t from = e < 2 ? word : rest;
-    f16x2 code;
-    if (e % 2 == 0) code = bit_cast<f16x2>(bfi(0x000f000fu, from, magic)) - splat2((f16)1024.f);
-    else code = __builtin_elementwise_fma(bit_cast<f16x2>(bfi(0x00f000f0u, from, magic)), splat2((f16)0.0625f), splat2((f16)-64.f));
-    r[e] = bit_cast<uint32_t>(__builtin_elementwise_fma(code, s, m));
+// their 1024 (exact), times the scale plus the lowest value (one rounding). The constants that an operation takes
+// two of are kept in vector registers.
+struct Codes4 {
+  uint32_t magic;
+  f16x2 minus;
+  INTENT_DEVICE Codes4() {
+    magic = 0x64006400u;
+    uint32_t m = 0xd400d400u;  // -64
+    asm("" : "+v"(magic), "+v"(m));
+    minus = bit_cast<f16x2>(m);
   }
-  return r;
-}
+  INTENT_DEVICE u32x4 widen(uint32_t word, uint32_t pair) const {
+    const f16x2 h = bit_cast<f16x2>(pair), s = splat2(h[0]), m = splat2(h[1]);
+    const uint32_t rest = word >> 8;
+    u32x4 r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t from = e < 2 ? word : rest;
+      f16x2 code;
+      if (e % 2 == 0) code = bit_cast<f16x2>(bfi(0x000f000fu, from, magic)) - splat2((f16)1024.f);
+      else code = __builtin_elementwise_fma(bit_cast<f16x2>(bfi(0x00f000f0u, from, magic)), splat2((f16)0.0625f), minus);
+      r[e] = bit_cast<uint32_t>(__builtin_elementwise_fma(code, s, m));
+    }
+    return r;
+  }
+};
 
 // ---- few rows: 16 * MT of them, the tokens over the waves -----------------------------------------
 
@@ -288,7 +297,7 @@ INTENT_DEVICE u32x4 widen_codes4(uint32_t word, uint32_t pair) {
 // TB/s, the lengths being uneven. One sequence of 4096 tokens (17 MB) is a chain of latencies, 7 us and 4
 // for the join.
 template <bool kBf16, int kCache, bool kBiased, int D, int MT>
-__global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 256 ? 2 : 1)
+__global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? (kCache == kCacheInt4 ? 4 : 3) : MT * D <= 256 ? 2 : 1)
     void attn_rows_kernel(const AttnArgs a) {
   constexpr bool kFp8 = kCache == kCacheFp8, kInt4 = kCache == kCacheInt4;
   constexpr bool kMath = kBf16 && !kInt4;              // products in bf16
@@ -355,6 +364,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
   }
 
   char* mine = lds + wave * 32 * RB;
+  const Codes4 codes4;
   const int write_at = col * RB, swz = swizzle<RB, false>(col);
   // transposing reads: tokens 4 g .. 4 g + 3 of each 16, columns 16 d ..
   const int read_row = g * 4 + (col >> 2);
@@ -388,6 +398,24 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
     }
     if constexpr (kFp8) ks[u] = load_float(kp), vs[u] = load_float(vp);
   };
+  // 4 bits, in one page: buffer loads, whose base is scalar and whose lane offsets stay in two registers (with
+  // addresses of 64 bits for each of the eight loads four waves to a SIMD spill them).
+  const uint32_t pair_at = col * (4 * kParams) + g * ELEMS / kGroup4 * 4;
+  auto issue4 = [&](u32x4(&codes)[LOADS], uint32_t(&pairs)[LOADS], global_bytes rows, global_bytes params) {
+    const auto from = make_rsrc((const void*)rows), beside = make_rsrc((const void*)params);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      if constexpr (kLoad == 16) {
+        codes[i] = __builtin_amdgcn_raw_buffer_load_b128(from, lane_at, i * 4 * kLoad, 0);
+      } else if constexpr (kLoad == 8) {
+        const u32x2 two = __builtin_amdgcn_raw_buffer_load_b64(from, lane_at, i * 4 * kLoad, 0);
+        codes[i] = u32x4{two[0], two[1], 0u, 0u};
+      } else {
+        codes[i] = u32x4{(uint32_t)__builtin_amdgcn_raw_buffer_load_b32(from, lane_at, i * 4 * kLoad, 0), 0u, 0u, 0u};
+      }
+      pairs[i] = __builtin_amdgcn_raw_buffer_load_b32(beside, pair_at, i * (ELEMS / 2), 0);
+    }
+  };
   int place = 0;  // of the entries of the tokens to load next
   // Tokens that no row sees are loaded too (a page that is there, whatever it holds): their scores are
   // masked, their values set to zero when they are stored.
@@ -398,6 +426,13 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
       for (int u = 0; u < 2; ++u) {
         const uint32_t page = page_named(a, (uint32_t)lane_value((int)entries, place + u));
         const int t16 = t + 16 * u;
+        if constexpr (kInt4) {
+          issue4(kr[u], kg[u], cached_rows<kRow>(a, a.k_cache, page, a.k_step, head, t16),
+                 cached_scales<kParams>(a, a.k_scales, page, a.ks_step, head, t16));
+          issue4(vr[u], vg[u], cached_rows<kRow>(a, a.v_cache, page, a.v_step, head, t16),
+                 cached_scales<kParams>(a, a.v_scales, page, a.vs_step, head, t16));
+          continue;
+        }
         issue(u, cached_rows<kRow>(a, a.k_cache, page, a.k_step, head, t16) + lane_at,
               cached_rows<kRow>(a, a.v_cache, page, a.v_step, head, t16) + lane_at,
               cached_scales<kParams>(a, a.k_scales, page, a.ks_step, head, t16) + col * (4 * kParams),
@@ -414,6 +449,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
               cached_rows<kRow>(a, a.v_cache, page, a.v_step, head, tk) + g * kLoad,
               cached_scales<kParams>(a, a.k_scales, page, a.ks_step, head, tk),
               cached_scales<kParams>(a, a.v_scales, page, a.vs_step, head, tk));
+        if constexpr (kInt4) __builtin_amdgcn_sched_barrier(0);  // the addresses of one of them at a time
       }
     }
   };
@@ -465,7 +501,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
         if constexpr (kInt4) {
 #pragma unroll
           for (int c = 0; c < CHUNKS; ++c)
-            *(u32x4*)(row + (((chunk + c) ^ swz) << 4)) = widen_codes4(vr[u][i][c], vg[u][i]);
+            *(u32x4*)(row + (((chunk + c) ^ swz) << 4)) = codes4.widen(vr[u][i][c], vg[u][i]);
         } else if constexpr (kFp8) {
 #pragma unroll
           for (int c = 0; c < CHUNKS; ++c)
@@ -482,16 +518,14 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
         }
       }
     }
-    if (kInt4 && apart(t)) {  // once more, what is not finite left out
+    if (kInt4 && apart(t)) {  // what is not finite taken out again, by the lane that wrote it
       rarely();
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i)
-#pragma unroll
-          for (int c = 0; c < CHUNKS; ++c)
-            *(u32x4*)(mine + u * 16 * RB + write_at + (((at(i) / 8 + c) ^ swz) << 4)) =
-                only_finite<false, false>(widen_codes4(vr[u][i][c], vg[u][i]), found);
+#pragma unroll 1
+      for (int i = 0; i < 2 * LOADS * CHUNKS; ++i) {
+        const int chunk = at(i % (LOADS * CHUNKS) / CHUNKS) / 8 + i % CHUNKS;
+        u32x4* to = (u32x4*)(mine + i / (LOADS * CHUNKS) * 16 * RB + write_at + ((chunk ^ swz) << 4));
+        *to = only_finite<false, false>(*to, found);
+      }
     }
     wave_lds_order();
     f32x4 s[MT][2];
@@ -503,7 +537,7 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? 3 : MT * D <= 25
       for (int i = 0; i < KS; ++i) {
         u32x4 k;
         const int l = i / CHUNKS, c = i % CHUNKS;
-        if constexpr (kInt4) k = widen_codes4(kr[u][l][c], kg[u][l]);
+        if constexpr (kInt4) k = codes4.widen(kr[u][l][c], kg[u][l]);
         else if constexpr (kFp8) k = widen_codes<kBf16>(kr[u][l][2 * c], kr[u][l][2 * c + 1]);
         else k = kr[u][i];
 #pragma unroll
@@ -738,6 +772,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
     for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
   float ref = -INFINITY, total = 0.f;
 
+  const Codes4 codes4;
   const int wave_token = wave * EACH & 63;  // where there are more waves than tokens, those behind idle
   const int load_token = wave_token + lane / SPREAD, load_chunk = lane % SPREAD;
   const bool loads = load_chunk < CHUNKS && wave * EACH < 64;
@@ -816,7 +851,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
       char* row = to + tk * RB;
       if constexpr (kInt4) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) *(u32x4*)(row + ((load_chunk * 4 + c ^ swz) << 4)) = widen_codes4(from[i][c], pairs[i]);
+        for (int c = 0; c < 4; ++c) *(u32x4*)(row + ((load_chunk * 4 + c ^ swz) << 4)) = codes4.widen(from[i][c], pairs[i]);
       } else if constexpr (kFp8) {
         *(u32x4*)(row + ((load_chunk * 2 ^ swz) << 4)) = widen_codes<kBf16>(from[i][0], from[i][1]);
         *(u32x4*)(row + (((load_chunk * 2 + 1) ^ swz) << 4)) = widen_codes<kBf16>(from[i][2], from[i][3]);
@@ -852,18 +887,14 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
       if (found) left_out = 1;
     }
     store(lds[buffer][1], vr, vg);
-    if (kInt4 && apart(t)) {  // once more, what is not finite left out
+    if (kInt4 && apart(t) && loads) {  // what is not finite taken out again, by the lane that wrote it
       rarely();
       bool found = false;
-      if (loads) {
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-          const int tk = load_token + i * STEP;
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            *(u32x4*)(lds[buffer][1] + tk * RB + ((load_chunk * 4 + c ^ swizzle<RB, true>(tk)) << 4)) =
-                only_finite<false, false>(widen_codes4(vr[i][c], vg[i]), found);
-        }
+#pragma unroll 1
+      for (int i = 0; i < LOADS * 4; ++i) {
+        const int tk = load_token + i / 4 * STEP;
+        u32x4* to = (u32x4*)(lds[buffer][1] + tk * RB + ((load_chunk * 4 + i % 4 ^ swizzle<RB, true>(tk)) << 4));
+        *to = only_finite<false, false>(*to, found);
       }
       if (found) left_out = 1;
     }

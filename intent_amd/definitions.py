@@ -1533,9 +1533,9 @@ def _biased_check(env: dict) -> None:
         raise ValueError(f"SOFTCAP must be 0 (none) or between 2^-100 and 2^100, got {cap}")
 
 
-def _attention_scratch(env: dict) -> int:
-    return _native.library().intent_paged_attention_workspace_size(
-        env["T"], env["HQ"], env["HK"], env["D"], env["S"], env["MAX_PAGES"], env["PAGE"])
+def _attention_scratch(number: int) -> Callable[[dict], int]:
+    return lambda env: _native.library().intent_biased_paged_attention_workspace_size(
+        env["T"], env["HQ"], env["HK"], env["D"], env["S"], env["MAX_PAGES"], env["PAGE"], number)
 
 
 def _attention_definition(dt: str, cache: str, biased: bool = False) -> KernelDefinition:
@@ -1571,7 +1571,7 @@ def _attention_definition(dt: str, cache: str, biased: bool = False) -> KernelDe
             Scalar("scale", "f32"),
         ),
         **_one_call(call),
-        scratch=_attention_scratch,
+        scratch=_attention_scratch(number),
         constexprs={"CAUSAL": True, "WINDOW": 0, **({"SOFTCAP": 0.0} if biased else {})},
         check=_biased_check if biased else _attention_check,
         reference="no kernel of the reference's quantized path; I.matmul contractions over a paged operand",
