@@ -19,6 +19,13 @@
 
 namespace intent {
 
+// Forms of scores that a kernel knows; all but the first know prefixes.
+enum ScoreForms { kPlain = 0, kCapped = 1, kSloped = 2, kBoth = 3 };
+
+constexpr const char* form_name(int forms) {
+  return forms == kCapped ? ", capped" : forms == kSloped ? ", sloped" : forms == kBoth ? ", capped and sloped" : "";
+}
+
 struct AttnArgs {
   const uint16_t* q;
   int64_t q_ld;
@@ -52,8 +59,11 @@ struct AttnArgs {
 // cached head.
 typedef int LaunchAttn(const AttnArgs& a, int items, int rows, hipStream_t stream);
 LaunchAttn launch_attn_f16, launch_attn_bf16, launch_attn_f16_fp8, launch_attn_bf16_fp8, launch_attn_f16_int4,
-    launch_attn_bf16_int4, launch_attn_f16_biased, launch_attn_bf16_biased, launch_attn_f16_fp8_biased,
-    launch_attn_bf16_fp8_biased, launch_attn_f16_int4_biased, launch_attn_bf16_int4_biased;
+    launch_attn_bf16_int4, launch_attn_f16_capped, launch_attn_bf16_capped, launch_attn_f16_fp8_capped,
+    launch_attn_bf16_fp8_capped, launch_attn_f16_int4_capped, launch_attn_bf16_int4_capped, launch_attn_f16_sloped,
+    launch_attn_bf16_sloped, launch_attn_f16_fp8_sloped, launch_attn_bf16_fp8_sloped, launch_attn_f16_int4_sloped,
+    launch_attn_bf16_int4_sloped, launch_attn_f16_both, launch_attn_bf16_both, launch_attn_f16_fp8_both,
+    launch_attn_bf16_fp8_both, launch_attn_f16_int4_both, launch_attn_bf16_int4_both;
 
 // One launch for the joins of the split tiles of up to two lists: the rows of each one's tiles, its units of
 // tokens (their logarithm) and workgroups for each cached head (0: no list), and the second list's own
@@ -66,7 +76,7 @@ struct AttnJoin {
 };
 // with `side` workgroups for the rows of a tile
 typedef int LaunchJoin(const AttnJoin& j, int side, hipStream_t stream);
-LaunchJoin launch_join_f16, launch_join_bf16, launch_join_f16_biased, launch_join_bf16_biased;
+LaunchJoin launch_join_f16, launch_join_bf16, launch_join_f16_prefix, launch_join_bf16_prefix;
 
 // Query rows [start, start + count), cached tokens and prefix of sequence s.
 struct Sequence {

@@ -198,9 +198,10 @@ struct Part {
   // 4 bits: a CU holds four of 16 rows. Many sequences are evened out by two rounds of them (64 of 300 to 8191
   // tokens: 87, 89 and 83 us at 1024, 1536 and 2048); few are cut into parts enough by one, and their join costs
   // more with every part (four of 60000 to 131000: 88, 89 and 90 us, the join 6.0, 7.4 and 10.0).
+  // Tiles of 128 rows of heads of 64: 1925 tokens of 24 sequences, 12 heads, kernel and join, 75 us at 512, 71 at 1024.
   int fill(int64_t D, int cache, int64_t lists) const {
     if (cache == kCacheInt4 && rows * D <= 2048) return lists >= 256 ? 2048 : 1024;
-    if (rows > 64) return rows == 256 || D > 128 ? 256 : 512;
+    if (rows > 64) return rows == 256 || D > 128 ? 256 : cache == kCacheInt4 && D == 64 ? 1024 : 512;
     return D > 128 ? 256 : rows * D <= 2048 ? 1536 : rows * D <= 4096 ? 512 : 256;
   }
 };
@@ -288,15 +289,25 @@ size_t part_bytes(const Part& p, int64_t T, int64_t S, int64_t group, int64_t HK
   return (size_t)(slots_bound(p, T, S, group, HK, D, cache, most_kv) * HK * p.rows * (D + 2) * 4);
 }
 
-// By cache format, scores biased or not, and heads of bf16 or not.
-LaunchAttn* const kLaunchAttn[3][2][2] = {
-    {{launch_attn_f16, launch_attn_bf16}, {launch_attn_f16_biased, launch_attn_bf16_biased}},
-    {{launch_attn_f16_fp8, launch_attn_bf16_fp8}, {launch_attn_f16_fp8_biased, launch_attn_bf16_fp8_biased}},
-    {{launch_attn_f16_int4, launch_attn_bf16_int4}, {launch_attn_f16_int4_biased, launch_attn_bf16_int4_biased}}};
+// By cache format, form of scores, and heads of bf16 or not.
+LaunchAttn* const kLaunchAttn[3][4][2] = {
+    {{launch_attn_f16, launch_attn_bf16},
+     {launch_attn_f16_capped, launch_attn_bf16_capped},
+     {launch_attn_f16_sloped, launch_attn_bf16_sloped},
+     {launch_attn_f16_both, launch_attn_bf16_both}},
+    {{launch_attn_f16_fp8, launch_attn_bf16_fp8},
+     {launch_attn_f16_fp8_capped, launch_attn_bf16_fp8_capped},
+     {launch_attn_f16_fp8_sloped, launch_attn_bf16_fp8_sloped},
+     {launch_attn_f16_fp8_both, launch_attn_bf16_fp8_both}},
+    {{launch_attn_f16_int4, launch_attn_bf16_int4},
+     {launch_attn_f16_int4_capped, launch_attn_bf16_int4_capped},
+     {launch_attn_f16_int4_sloped, launch_attn_bf16_int4_sloped},
+     {launch_attn_f16_int4_both, launch_attn_bf16_int4_both}}};
+// With prefixes or without.
 LaunchJoin* const kLaunchJoin[2][2] = {{launch_join_f16, launch_join_bf16},
-                                       {launch_join_f16_biased, launch_join_bf16_biased}};
+                                       {launch_join_f16_prefix, launch_join_bf16_prefix}};
 
-int launch_tiled(AttnArgs a, bool bf16, int cache, bool biased, float* workspace, size_t bytes, hipStream_t stream) {
+int launch_tiled(AttnArgs a, bool bf16, int cache, int forms, float* workspace, size_t bytes, hipStream_t stream) {
   const Plan plan = plan_of(a.T, a.S, a.HK, a.group, a.D);
   size_t need = 0;
   for (int i = 0; i < plan.parts; ++i) need += part_bytes(plan.part[i], a.T, a.S, a.group, a.HK, a.D, cache, a.most_kv);
@@ -319,7 +330,7 @@ int launch_tiled(AttnArgs a, bool bf16, int cache, bool biased, float* workspace
                    "%lld tiles of %d heads exceed the %lld workgroups that a launch covers", (long long)tiles, a.HK,
                    (long long)((int64_t)1 << 23));
     const int items = (int)(tiles + a.target);
-    const int status = kLaunchAttn[cache][biased][bf16](a, items, p.rows, stream);
+    const int status = kLaunchAttn[cache][forms][bf16](a, items, p.rows, stream);
     if (status != INTENT_OK) return status;
     if (!split) continue;
     // a tile is split from one and a half shares on
@@ -340,7 +351,7 @@ int launch_tiled(AttnArgs a, bool bf16, int cache, bool biased, float* workspace
   const int64_t room = 1024 / ((int64_t)(join.items[0] + join.items[1]) * a.HK), rows = plan.part[0].rows;
   const int64_t side = mean < rows ? mean : rows;
   const int sides = (int)(room < 1 ? 1 : room < side ? room : side);
-  return kLaunchJoin[biased][bf16](join, sides, stream);
+  return kLaunchJoin[forms != kPlain][bf16](join, sides, stream);
 }
 
 }  // namespace
@@ -439,13 +450,14 @@ int attend(const void* q, int64_t T, int64_t HQ, int64_t q_ld, int is_bf16, cons
   a.most_kv = any ? (int)(table_width * page_size) : 0;
   a.causal = causal != 0, a.window = (int)(window < INT32_MAX ? window : INT32_MAX);
   a.slopes = f.slopes, a.prefix_lens = f.prefix_lens, a.cap_log2 = cap_log2;
-  const bool biased = cap_log2 != 0.f || f.slopes != nullptr || (f.prefix_lens != nullptr && causal);
+  const bool slopes = f.slopes != nullptr, prefix = f.prefix_lens != nullptr && causal;
+  const int forms = cap_log2 != 0.f ? (slopes ? kBoth : kCapped) : slopes || prefix ? kSloped : kPlain;
   hipStream_t st = (hipStream_t)stream;
   if (tiled(D)) {
     const bool aligned = workspace != nullptr && intent::aligned16(workspace);
-    return launch_tiled(a, is_bf16 != 0, c.format, biased, aligned ? (float*)workspace : nullptr, workspace_bytes, st);
+    return launch_tiled(a, is_bf16 != 0, c.format, forms, aligned ? (float*)workspace : nullptr, workspace_bytes, st);
   }
-  return launch_any_rows(a, is_bf16 != 0, c.format, biased, st);
+  return launch_any_rows(a, is_bf16 != 0, c.format, forms != kPlain, st);
 }
 
 }  // namespace

@@ -285,6 +285,67 @@ struct Codes4 {
   }
 };
 
+// The forms of a row's scores, each in kernels of its own (kForms; a prefix alone runs among the sloped ones):
+//   capped: cap tanh(x / cap) = cap - 2 cap r, r = 1 / (exp(2 x / cap) + 1): a product, an exponential, a sum and a
+//           reciprocal. The softmax does not see the cap that is added to all of them, so a score becomes -r, and 2 cap
+//           log2(e) brings it to base 2 in the exponent's own multiplication;
+//   sloped: scores get their distance, slope |p - t|, in base 2: with all tokens at or before the row it is linear in
+//           t, one operation, and the scale's product adds it.
+// Written as branches of one kernel they cost the tiles of a prompt 10 to 20% by spilled registers.
+template <int kCache, int kForms, int N, int kElements>
+struct Scores {
+  static constexpr bool kFp8 = kCache == kCacheFp8, kCap = (kForms & kCapped) != 0, kSlope = (kForms & kSloped) != 0;
+  // whether they are in base 2 before the softmax takes its maximum
+  static constexpr bool kScaled = kFp8 || kSlope;
+  float in, out;  // capped: what a score is multiplied by before and behind the reciprocal
+  float slope, position;
+
+  INTENT_DEVICE void begin(const AttnArgs& a, float scale, float slope_log2, int p) {
+    in = kCap ? (kFp8 ? cap_rate(a) : scale * cap_rate(a)) : scale;
+    out = kCap ? 2.0f * a.cap_log2 : scale;
+    slope = slope_log2, position = (float)p;
+  }
+  // s: element (u, r) of token t + token(u, r), of which `last` is the greatest; the rows stand at `top` and behind.
+  // k_mul: scales of the keys, with the scores' own.
+  template <typename S, typename Token, typename KMul>
+  INTENT_DEVICE void apply(S (&s)[N], int t, int last, int top, Token token, KMul k_mul) const {
+    if constexpr (kFp8 && !(kSlope && !kCap)) {
+#pragma unroll
+      for (int u = 0; u < N; ++u)
+#pragma unroll
+        for (int r = 0; r < kElements; ++r) s[u][r] *= k_mul(u, r);
+    }
+    if constexpr (kCap) {
+#pragma unroll
+      for (int u = 0; u < N; ++u)
+#pragma unroll
+        for (int r = 0; r < kElements; ++r) {
+          s[u][r] = -__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[u][r] * in) + 1.0f);
+          if constexpr (kFp8 && !kSlope) s[u][r] *= out;
+        }
+    }
+    if constexpr (kSlope) {
+      const float ahead = (float)t - position;
+      auto add = [&](int u, int r, float bias) {
+        s[u][r] = __builtin_fmaf(s[u][r], kFp8 && !kCap ? k_mul(u, r) : out, bias);
+      };
+      if (t + last <= top) {
+        const float first = slope * ahead;
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+          for (int r = 0; r < kElements; ++r) add(u, r, __builtin_fmaf(slope, (float)token(u, r), first));
+      } else {
+        rarely();
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+          for (int r = 0; r < kElements; ++r) add(u, r, -slope * fabsf(ahead + (float)token(u, r)));
+      }
+    }
+  }
+};
+
 // ---- few rows: 16 * MT of them, the tokens over the waves -----------------------------------------
 
 // A wave takes 32 tokens of each 128: keys straight into the first product's left operand (a lane holds 8
@@ -296,12 +357,14 @@ struct Codes4 {
 // 242 us, 5.9 TB/s, where a large copy moves 5.1; 64 of 300 to 8191 tokens in 8 bits (645 MB): 124 us, 5.2
 // TB/s, the lengths being uneven. One sequence of 4096 tokens (17 MB) is a chain of latencies, 7 us and 4
 // for the join.
-template <bool kBf16, int kCache, bool kBiased, int D, int MT>
-__global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? (kCache == kCacheInt4 ? 4 : 3) : MT * D <= 256 ? 2 : 1)
+template <bool kBf16, int kCache, int kForms, int D, int MT>
+__global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? (kCache == kCacheInt4 && MT == 1 ? 4 : 3) : MT * D <= 256 ? 2 : 1)
     void attn_rows_kernel(const AttnArgs a) {
   constexpr bool kFp8 = kCache == kCacheFp8, kInt4 = kCache == kCacheInt4;
   constexpr bool kMath = kBf16 && !kInt4;              // products in bf16
-  constexpr bool kScaled = kFp8 || kBiased;            // scores are scaled before the softmax
+  constexpr bool kBiased = kForms != kPlain;
+  using Form = Scores<kCache, kForms, 2, 4>;
+  constexpr bool kScaled = kFp8 || Form::kScaled;      // scores are scaled before the softmax
   constexpr int KS = D / 32, DT = D / 16, RB = row_bytes<D>();
   // elements of a lane's load of a token's row: 16 bytes of them if the row's quarter holds as many
   constexpr int ELEMS = kInt4 ? (D % 128 == 0 ? 32 : D % 64 == 0 ? 16 : 8) : kFp8 && D % 64 == 0 ? 16 : 8;
@@ -336,7 +399,8 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? (kCache == kCach
   const RowView top = row_view(a, w, 0), bottom = row_view(a, w, w.rows - 1);
   const int some_lo = top.lo, some_hi = bottom.hi, all_lo = bottom.lo, all_hi = top.hi;
   const float scale = scale_of(a);
-  float row_scale[MT], slope[MT];
+  float row_scale[MT];
+  Form forms[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     row_scale[m] = scale;
@@ -350,9 +414,11 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? (kCache == kCach
       for (int i = 0; i < KS; ++i) q[m][i] = query_f16(q[m][i], exponent);
       row_scale[m] = scale_behind(scale, exponent);
     }
-    if constexpr (kBiased) slope[m] = slope_of(a, w, head, m * 16 + col);
+    if constexpr (kBiased) {
+      forms[m].begin(a, row_scale[m], Form::kSlope ? slope_of(a, w, head, m * 16 + col) : 0.f, view[m].p - g * 4);
+      row_scale[m] = forms[m].out;
+    }
   }
-  const float rate = kBiased ? cap_rate(a) : 0.f;
 
   f32x4 o[MT][DT];
   float ref[MT], total[MT];
@@ -547,40 +613,28 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? (kCache == kCach
     const int now = t;
     if (now + 128 < w.end) load_rows(now + 128);
     u32x4 p[MT];
-    f32x4 v_mul[2], v_exp[2];
+    f32x4 k_mul[2], v_mul[2], v_exp[2];
     if constexpr (kFp8) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const f32x4 k_mul = *(const f32x4*)&scales[wave][0][u * 16 + g * 4];
+        k_mul[u] = *(const f32x4*)&scales[wave][0][u * 16 + g * 4];
         v_mul[u] = *(const f32x4*)&scales[wave][1][u * 16 + g * 4];
         v_exp[u] = *(const f32x4*)&scales[wave][2][u * 16 + g * 4];
+        if constexpr (!kBiased) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+          for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) s[m][u][r] *= k_mul[r];
+            for (int r = 0; r < 4; ++r) s[m][u][r] *= k_mul[u][r];
+        }
       }
     }
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       if constexpr (kBiased) {
-        if constexpr (!kFp8) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u) s[m][u] *= row_scale[m];
-        }
-        if (a.cap_log2 != 0.f) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) s[m][u][r] = capped(s[m][u][r], a.cap_log2, rate);
-        }
-        if (a.slopes != nullptr) {
-          const float ahead = (float)(now + g * 4 - view[m].p);
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              s[m][u][r] = __builtin_fmaf(-slope[m], fabsf(ahead + (float)(16 * u + r)), s[m][u][r]);
-        }
+        // the branch, always taken, keeps the forms apart from the products: without it 16 rows of heads of 256 over
+        // 32 caches of 2000 to 8000 tokens take 187 us, with it 174
+        if (!Form::kCap || a.cap_log2 != 0.f) forms[m].apply(s[m], now, 31, top.p, [](int u, int r) { return 16 * u + r; },
+                       [&](int u, int r) { return k_mul[u][r]; });
       }
       // the highest score, times the value's scale; s is a score or, scaled already, its t
       float high = -INFINITY;
@@ -712,17 +766,20 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? (kCache == kCach
 // TFLOP/s. What is left: with the loads of the cache taken away it takes 140 us, with the vector work
 // 117, with the products 111; each wave's own chain, not one unit, sets the time. 64 rows to a wave read LDS
 // half as often, but one wave to a SIMD and 1500 copies between the two halves of its registers take 215 us.
-template <bool kBf16, int kCache, bool kBiased, int D, int WAVES>
+template <bool kBf16, int kCache, int kForms, int D, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
     void attn_tile_kernel(const AttnArgs a) {
   constexpr bool kFp8 = kCache == kCacheFp8, kInt4 = kCache == kCacheInt4;
   constexpr bool kMath = kBf16 && !kInt4;             // products in bf16
-  constexpr bool kScaled = kFp8 || kBiased;           // scores are scaled before the softmax
+  constexpr bool kBiased = kForms != kPlain;
+  using Form = Scores<kCache, kForms, 2, 16>;
+  constexpr bool kScaled = kFp8 || Form::kScaled;     // scores are scaled before the softmax
   constexpr int KS = D / 16, DT = D / 32, RB = row_bytes<D>();
   constexpr int kRow = cached_bytes<kCache, D>(), kParams = cached_params<kCache, D>();
-  constexpr int CHUNKS = kRow / 16;                   // 16-byte loads of a token's row
-  // lanes that take one (a power of two; four where two would do, so that as many waves load)
-  constexpr int SPREAD = kInt4 ? (RB / 64 < 4 ? 4 : RB / 64) : kFp8 ? RB / 32 : RB / 16;
+  constexpr int kLoad = kInt4 && D == 64 ? 8 : 16;    // bytes of a lane's load: rows of 32 bytes take four lanes too
+  constexpr int CHUNKS = kRow / kLoad, WORDS = kLoad / 4;  // loads of a token's row
+  // lanes that take one (a power of two)
+  constexpr int SPREAD = kInt4 ? RB / kLoad / 4 : kFp8 ? RB / 32 : RB / 16;
   constexpr int EACH = 64 / SPREAD;                   // tokens that a wave loads at once
   constexpr int STEP = EACH * WAVES;                  // and the workgroup
   constexpr int LOADS = STEP >= 64 ? 1 : 64 / STEP, ROWS = 32 * WAVES;
@@ -752,7 +809,8 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
   const RowView top = row_view(a, w, r0), bottom = row_view(a, w, r0 + 31);  // of this wave
   const bool idle = r0 >= w.rows;
   const float scale = scale_of(a);
-  float row_scale = scale, slope = 0.f;
+  float row_scale = scale;
+  Form forms;
   if constexpr (kBf16 && kInt4) {
     uint32_t most = 0;
 #pragma unroll
@@ -762,8 +820,10 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
     for (int i = 0; i < KS; ++i) q[i] = query_f16(q[i], exponent);
     row_scale = scale_behind(scale, exponent);
   }
-  if constexpr (kBiased) slope = slope_of(a, w, head, r0 + col);
-  const float rate = kBiased ? cap_rate(a) : 0.f;
+  if constexpr (kBiased) {
+    forms.begin(a, row_scale, Form::kSlope ? slope_of(a, w, head, r0 + col) : 0.f, view.p - h * 4);
+    row_scale = forms.out;
+  }
 
   f32x16 o[DT];
 #pragma unroll
@@ -772,17 +832,24 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
     for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
   float ref = -INFINITY, total = 0.f;
 
+  // 4 bits and eight waves: 64 tokens' rows are one load of four waves, so half of them take the keys and half the
+  // values (each widens half as much before the barrier).
+  constexpr bool kHalves = kInt4 && STEP >= 128;
+  const bool takes_keys = !kHalves || wave < WAVES / 2, takes_values = !kHalves || wave >= WAVES / 2;
   const Codes4 codes4;
   const int wave_token = wave * EACH & 63;  // where there are more waves than tokens, those behind idle
   const int load_token = wave_token + lane / SPREAD, load_chunk = lane % SPREAD;
-  const bool loads = load_chunk < CHUNKS && wave * EACH < 64;
-  u32x4 kr[LOADS], vr[LOADS];
-  uint32_t kg[LOADS], vg[LOADS];  // pairs of the codes' groups
+  const bool loads = load_chunk < CHUNKS && (kHalves || wave * EACH < 64);
+  u32x4 kr[LOADS], other[LOADS];
+  uint32_t kg[LOADS], other_pairs[LOADS];  // pairs of the codes' groups
+  u32x4(&vr)[LOADS] = kHalves ? kr : other;
+  uint32_t(&vg)[LOADS] = kHalves ? kg : other_pairs;
   float ks = 0.f, vs = 0.f;
   // Pages of EACH tokens and more (16 at most): each load's tokens lie in one, whose id is a scalar.
   const bool paged = (1 << a.page_shift) >= EACH;
   const int chunk = load_chunk < CHUNKS ? load_chunk : 0;
-  const uint32_t lane_at = (lane / SPREAD) * kRow + chunk * 16, pair_at = (lane / SPREAD) * (4 * kParams) + chunk * 4;
+  const int group = chunk * (kLoad / 4) * 8 / kGroup4;
+  const uint32_t lane_at = (lane / SPREAD) * kRow + chunk * kLoad, pair_at = (lane / SPREAD) * (4 * kParams) + group * 4;
   // The table's entries of the next `span` times 64 tokens, one in each lane, in two batches (as above).
   const bool one_page = a.page_shift >= 6;  // the 64 tokens in one page
   constexpr int kLoadsLog = LOADS == 1 ? 0 : LOADS == 2 ? 1 : LOADS == 4 ? 2 : 3;
@@ -802,6 +869,11 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
   // masked, their values set to zero when they are stored.
   auto load = [&](u32x4(&fetched)[LOADS], uint32_t(&pairs)[LOADS], const void* cache, uint32_t step,
                   const float* params, uint32_t pair_step, int t) __attribute__((always_inline)) {
+    auto codes = [](global_bytes at) {
+      if constexpr (kLoad == 16) return load16(at);
+      const u32x2 two = load8(at);
+      return u32x4{two[0], two[1], 0u, 0u};
+    };
     const int n = (t - w.begin) >> 6;
     if (one_page) {
       const uint32_t page = page_named(a, entry(n, 0));
@@ -809,7 +881,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
       const global_bytes beside = cached_scales<kParams>(a, params, page, pair_step, head, t + wave_token);
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        fetched[i] = load16(from + i * (STEP * kRow) + lane_at);
+        fetched[i] = codes(from + i * (STEP * kRow) + lane_at);
         if constexpr (kInt4) pairs[i] = load4(beside + i * (STEP * 4 * kParams) + pair_at);
       }
     } else if (paged) {
@@ -817,7 +889,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
       for (int i = 0; i < LOADS; ++i) {
         const uint32_t page = page_named(a, entry(n, i));
         const int tk = t + i * STEP + wave_token;
-        fetched[i] = load16(cached_rows<kRow>(a, cache, page, step, head, tk) + lane_at);
+        fetched[i] = codes(cached_rows<kRow>(a, cache, page, step, head, tk) + lane_at);
         if constexpr (kInt4) pairs[i] = load4(cached_scales<kParams>(a, params, page, pair_step, head, tk) + pair_at);
       }
     } else {
@@ -826,10 +898,14 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
       for (int i = 0; i < LOADS; ++i) {
         const int tk = t + i * STEP + load_token;
         const uint32_t page = page_named(a, table_entry(a, w.s, clamped(tk)));
-        fetched[i] = load16(cached_rows<kRow>(a, cache, page, step, head, tk) + chunk * 16);
-        if constexpr (kInt4) pairs[i] = load4(cached_scales<kParams>(a, params, page, pair_step, head, tk) + chunk * 4);
+        fetched[i] = codes(cached_rows<kRow>(a, cache, page, step, head, tk) + chunk * kLoad);
+        if constexpr (kInt4) pairs[i] = load4(cached_scales<kParams>(a, params, page, pair_step, head, tk) + group * 4);
       }
     }
+  };
+  auto load_share = [&](int keys, int values) __attribute__((always_inline)) {
+    load(kr, kg, takes_keys ? a.k_cache : a.v_cache, takes_keys ? a.k_step : a.v_step,
+         takes_keys ? a.k_scales : a.v_scales, takes_keys ? a.ks_step : a.vs_step, takes_keys ? keys : values);
   };
   auto load_keys = [&](int t) __attribute__((always_inline)) { load(kr, kg, a.k_cache, a.k_step, a.k_scales, a.ks_step, t); };
   auto load_values = [&](int t) __attribute__((always_inline)) {
@@ -851,7 +927,8 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
       char* row = to + tk * RB;
       if constexpr (kInt4) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) *(u32x4*)(row + ((load_chunk * 4 + c ^ swz) << 4)) = codes4.widen(from[i][c], pairs[i]);
+        for (int c = 0; c < WORDS; ++c)
+          *(u32x4*)(row + ((load_chunk * WORDS + c ^ swz) << 4)) = codes4.widen(from[i][c], pairs[i]);
       } else if constexpr (kFp8) {
         *(u32x4*)(row + ((load_chunk * 2 ^ swz) << 4)) = widen_codes<kBf16>(from[i][0], from[i][1]);
         *(u32x4*)(row + (((load_chunk * 2 + 1) ^ swz) << 4)) = widen_codes<kBf16>(from[i][2], from[i][3]);
@@ -891,9 +968,9 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
       rarely();
       bool found = false;
 #pragma unroll 1
-      for (int i = 0; i < LOADS * 4; ++i) {
-        const int tk = load_token + i / 4 * STEP;
-        u32x4* to = (u32x4*)(lds[buffer][1] + tk * RB + ((load_chunk * 4 + i % 4 ^ swizzle<RB, true>(tk)) << 4));
+      for (int i = 0; i < LOADS * WORDS; ++i) {
+        const int tk = load_token + i / WORDS * STEP;
+        u32x4* to = (u32x4*)(lds[buffer][1] + tk * RB + ((load_chunk * WORDS + i % WORDS ^ swizzle<RB, true>(tk)) << 4));
         *to = only_finite<false, false>(*to, found);
       }
       if (found) left_out = 1;
@@ -933,18 +1010,22 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
   f32x16 s[2];
   if (w.begin < w.end) {
     if (paged) entries[0] = batch(w.begin), entries[1] = batch(w.begin + span * 64);
-    load_keys(w.begin);
-    load_values(w.begin);
+    if constexpr (kHalves) {
+      load_share(w.begin, w.begin);
+    } else {
+      load_keys(w.begin);
+      load_values(w.begin);
+    }
     if constexpr (kAhead) {
       u32x4 second[LOADS];
       uint32_t second_pairs[LOADS];
       load(second, second_pairs, a.k_cache, a.k_step, a.k_scales, a.ks_step, w.begin + 64);
-      store(lds[0][0], kr, kg);
-      store_values(0, w.begin);
-      store(lds[1][0], second, second_pairs);
+      if (takes_keys) store(lds[0][0], kr, kg);
+      if (takes_values) store_values(0, w.begin);
+      if (takes_keys) store(lds[1][0], second, second_pairs);
     } else {
-      store(lds[0][0], kr, kg);
-      store_values(0, w.begin);
+      if (takes_keys) store(lds[0][0], kr, kg);
+      if (takes_values) store_values(0, w.begin);
     }
   }
   __syncthreads();
@@ -956,8 +1037,12 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
   for (int t = w.begin; t < w.end; t += 64, j ^= 1) {
     const bool more = t + 64 < w.end;
     if (more) {
-      load_values(t + 64);
-      load_keys(t + (kAhead ? 128 : 64));
+      if constexpr (kHalves) {
+        load_share(t + (kAhead ? 128 : 64), t + 64);
+      } else {
+        load_values(t + 64);
+        load_keys(t + (kAhead ? 128 : 64));
+      }
       const int n = (t + 64 - w.begin) >> 6;
       if (paged && (n & (span - 1)) == span - 1) {  // past a batch: the one behind the other takes its place
         rarely();
@@ -971,7 +1056,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
       const char* values = lds[j][1];
       const bool masked = t < bottom.lo || t + 64 > top.hi;
       float high = -INFINITY;
-      if constexpr (kFp8) {
+      if constexpr (kFp8 && !kBiased) {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -981,26 +1066,9 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
             for (int r = 0; r < 4; ++r) s[u][i * 4 + r] *= k_mul[r];
           }
       }
-      if constexpr (kBiased) {
-        if constexpr (!kFp8) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u) s[u] *= row_scale;
-        }
-        if (a.cap_log2 != 0.f) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[u][r] = capped(s[u][r], a.cap_log2, rate);
-        }
-        if (a.slopes != nullptr) {
-          const float ahead = (float)(t + h * 4 - view.p);
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              s[u][r] = __builtin_fmaf(-slope, fabsf(ahead + (float)(u * 32 + (r >> 2) * 8 + (r & 3))), s[u][r]);
-        }
-      }
+      if constexpr (kBiased)
+        forms.apply(s, t, 63, top.p, [](int u, int r) { return u * 32 + (r >> 2) * 8 + (r & 3); },
+                    [&](int u, int r) { return scales[j][0][u * 32 + (r >> 2) * 8 + h * 4 + (r & 3)]; });
       if (masked) {
         rarely();
         const int lo = view.lo - t - h * 4, hi = view.hi - t - h * 4;
@@ -1103,8 +1171,8 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
       if constexpr (kAhead) s[0] = after[0], s[1] = after[1];
     }
     if (more) {
-      store_values(j ^ 1, t + 64);
-      store(lds[kAhead ? j : j ^ 1][0], kr, kg);
+      if (takes_values) store_values(j ^ 1, t + 64);
+      if (takes_keys) store(lds[kAhead ? j : j ^ 1][0], kr, kg);
     }
     __syncthreads();
   }
@@ -1272,39 +1340,39 @@ __global__ __launch_bounds__(256) void attn_join_kernel(int items, int tile, int
 }
 
 // ROWS up to 64: rows of the first kernel; 128 or 256: of the second's four or eight waves.
-template <bool kBf16, int kCache, bool kBiased, int D, int ROWS>
+template <bool kBf16, int kCache, int kForms, int D, int ROWS>
 int launch(const AttnArgs& a, int items, hipStream_t stream) {
   const unsigned groups = (unsigned)items * (unsigned)a.HK;
   constexpr bool kFew = ROWS <= 64;
   if constexpr (kFew)
-    hipLaunchKernelGGL((attn_rows_kernel<kBf16, kCache, kBiased, D, ROWS / 16>), dim3(groups), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((attn_rows_kernel<kBf16, kCache, kForms, D, ROWS / 16>), dim3(groups), dim3(256), 0, stream, a);
   else
-    hipLaunchKernelGGL((attn_tile_kernel<kBf16, kCache, kBiased, D, ROWS / 32>), dim3(groups), dim3(ROWS * 2), 0, stream,
+    hipLaunchKernelGGL((attn_tile_kernel<kBf16, kCache, kForms, D, ROWS / 32>), dim3(groups), dim3(ROWS * 2), 0, stream,
                        a);
   static const KernelName name("attn_%s_kernel<%s%s%s, D %d, %d rows>", kFew ? "rows" : "tile", kBf16 ? "bf16" : "f16",
-                               cache_name(kCache), kBiased ? ", biased" : "", D, ROWS);
+                               cache_name(kCache), form_name(kForms), D, ROWS);
   return launch_status(name.text);
 }
 
-template <bool kBf16, int kCache, bool kBiased, int D>
+template <bool kBf16, int kCache, int kForms, int D>
 int launch_d(const AttnArgs& a, int items, int rows, hipStream_t stream) {
-  if (rows == 16) return launch<kBf16, kCache, kBiased, D, 16>(a, items, stream);
+  if (rows == 16) return launch<kBf16, kCache, kForms, D, 16>(a, items, stream);
   if constexpr (D <= 128) {
-    if (rows == 32) return launch<kBf16, kCache, kBiased, D, 32>(a, items, stream);
-    if (rows == 48) return launch<kBf16, kCache, kBiased, D, 48>(a, items, stream);
-    if (rows == 64) return launch<kBf16, kCache, kBiased, D, 64>(a, items, stream);
-    if (rows == 256) return launch<kBf16, kCache, kBiased, D, 256>(a, items, stream);
+    if (rows == 32) return launch<kBf16, kCache, kForms, D, 32>(a, items, stream);
+    if (rows == 48) return launch<kBf16, kCache, kForms, D, 48>(a, items, stream);
+    if (rows == 64) return launch<kBf16, kCache, kForms, D, 64>(a, items, stream);
+    if (rows == 256) return launch<kBf16, kCache, kForms, D, 256>(a, items, stream);
   }
-  return launch<kBf16, kCache, kBiased, D, 128>(a, items, stream);
+  return launch<kBf16, kCache, kForms, D, 128>(a, items, stream);
 }
 
-template <bool kBf16, int kCache, bool kBiased = false>
+template <bool kBf16, int kCache, int kForms = kPlain>
 int launch_any(const AttnArgs& a, int items, int rows, hipStream_t stream) {
   switch (a.D) {
-    case 64: return launch_d<kBf16, kCache, kBiased, 64>(a, items, rows, stream);
-    case 96: return launch_d<kBf16, kCache, kBiased, 96>(a, items, rows, stream);
-    case 128: return launch_d<kBf16, kCache, kBiased, 128>(a, items, rows, stream);
-    case 256: return launch_d<kBf16, kCache, kBiased, 256>(a, items, rows, stream);
+    case 64: return launch_d<kBf16, kCache, kForms, 64>(a, items, rows, stream);
+    case 96: return launch_d<kBf16, kCache, kForms, 96>(a, items, rows, stream);
+    case 128: return launch_d<kBf16, kCache, kForms, 128>(a, items, rows, stream);
+    case 256: return launch_d<kBf16, kCache, kForms, 256>(a, items, rows, stream);
     default: return fail(INTENT_ERR_UNSUPPORTED, "no tiled attention kernel for heads of %d", a.D);
   }
 }
