@@ -226,13 +226,26 @@ __global__ __launch_bounds__(256) void attn_prep_kernel(const PrepArgs a) {
         const bool good = size < INFINITY;
         const f16 scale = good ? (f16)__fdiv_rn(high - low, 15.0f) : (f16)0.f;
         const f16 lowest = good ? (f16)low : bit_cast<f16>((uint16_t)0x7e00);
+        // The quotient by a reciprocal, 2^-22 of it off at most (3e-6 where it gives a code of 0 to 15, beyond that it
+        // is clamped); by division where a lane's may lie at the middle of two codes. 8192 tokens of 32 + 8 + 8 heads
+        // of 128 (178 MB): 43.7 us with divisions alone, 41.6 so.
+        const float s = (float)scale, m = (float)lowest;
         uint32_t word = 0;
-        if ((float)scale > 0.f) {
+        if (s > 0.f) {
+          float code[8], off = 0.f;
+          const float inverse = __builtin_amdgcn_rcpf(s);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const float t = rintf(__fdiv_rn(x[j] - (float)lowest, (float)scale));
-            word |= (uint32_t)fminf(fmaxf(t, 0.f), 15.f) << intent::code_bit(j);
+            const float t = (x[j] - m) * inverse;
+            code[j] = rintf(t);
+            off = fmaxf(off, fabsf(t - code[j]));
           }
+          if (off > 0.5f - 0x1p-15f) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) code[j] = rintf(__fdiv_rn(x[j] - m, s));
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) word |= (uint32_t)fminf(fmaxf(code[j], 0.f), 15.f) << intent::code_bit(j);
         }
         if (slot >= 0 && mine) {
           const int row = a.D / 2, groups = (a.D + intent::kGroup4 - 1) / intent::kGroup4;

@@ -42,6 +42,26 @@ class Binding:
     env: dict
     outputs: tuple
     workspace: object = None
+    call: tuple | None = None  # (entry, arguments before the stream) of a known layout; the views are not named then
+
+
+@dataclass(slots=True)
+class _Template:
+    """The call of a known layout with its addresses and scalars left out: where they go."""
+
+    entry: str
+    arguments: list
+    pointers: tuple  # (argument, view: the supplied ones, then the allocated outputs)
+    scratch: tuple   # arguments that take the scratch's address
+    scalars: tuple   # (argument, position among the supplied arguments)
+
+
+class _Probe:
+    """Stands for a view when a layout's call is made out: its strides and extents, and an address of its own."""
+
+    def __init__(self, t, address: int):
+        self.stride, self.dim, self.numel, self.shape = t.stride, t.dim, t.numel, t.shape
+        self.data_ptr = lambda: address
 
 
 @dataclass(slots=True)
@@ -59,6 +79,7 @@ class _Layout:
     pairs: tuple
     workspace: int      # bytes, -1 without one
     scratch: int        # bytes of a launch's own scratch
+    template: _Template | None = None
 
 
 MAX_LAYOUTS = 256  # layouts kept per artifact and calling form; the oldest go first
@@ -82,6 +103,7 @@ class HIPRuntime:
         self._latest: tuple | None = None  # (entry, kernel name bytes) of the latest launch
         self._scalars = {p.name for p in definition.params if isinstance(p, Scalar)}
         self._writable = {p.name for p in definition.params if isinstance(p, Param) and p.access is not ViewKind.IN}
+        self._outputs = {p.name for p in definition.params if isinstance(p, Param) and p.access is ViewKind.OUT}
         self._supplied = tuple(p for p in definition.params if isinstance(p, Scalar) or p.access is not ViewKind.OUT)
         self._layouts: tuple[dict, dict] = ({}, {})  # by calling form: outputs allocated, outputs supplied
         self._home = None
@@ -141,26 +163,39 @@ class HIPRuntime:
                     tensors.append(a)
         else:
             tensors = arguments
+        starts = None
         if known.pairs:
             starts = [t.data_ptr() for t in tensors]
-            for i, j, rows in known.pairs:
-                if (starts[i] < starts[j] + known.spans[j] and starts[j] < starts[i] + known.spans[i]
-                        and not _rows_apart(rows, starts[i], starts[j])):
-                    return None  # _bind names the overlap
-        views = dict(zip(known.names, tensors))
+            if _may_meet(starts, known.spans):
+                for i, j, rows in known.pairs:
+                    if (starts[i] < starts[j] + known.spans[j] and starts[j] < starts[i] + known.spans[i]
+                            and not _rows_apart(rows, starts[i], starts[j])):
+                        return None  # _bind names the overlap
+        outputs = ()
         if known.outputs:
             import torch
 
-            outputs = []
-            for name, shape, dt in known.outputs:
-                t = torch.empty(shape, dtype=dt, device=self._home_device())
-                views[name] = t
-                outputs.append(t)
-            return Binding(views, env, tuple(outputs), self._buffer_of(known.workspace, known.scratch))
-        outputs = ()
-        if supplied_outputs:
-            outputs = tuple(views[p.name] for p in params if p.name not in self._scalars and p.access is ViewKind.OUT)
-        return Binding(views, env, outputs, self._buffer_of(known.workspace, known.scratch))
+            outputs = tuple(torch.empty(shape, dtype=dt, device=self._home_device()) for _, shape, dt in known.outputs)
+        elif supplied_outputs:
+            outputs = tuple(t for t, name in zip(tensors, known.names) if name in self._outputs)
+        workspace = self._buffer_of(known.workspace, known.scratch)
+        template = known.template
+        if template is not None and (workspace is not None or not template.scratch):
+            values = template.arguments.copy()
+            addresses = [t.data_ptr() for t in tensors] if starts is None else starts
+            if known.outputs:
+                addresses += [t.data_ptr() for t in outputs]
+            for at, view in template.pointers:
+                values[at] = addresses[view]
+            for at in template.scratch:
+                values[at] = workspace.data_ptr()
+            for at, position in template.scalars:
+                values[at] = float(arguments[position])
+            return Binding(None, env, outputs, workspace, (template.entry, values))
+        views = dict(zip(known.names, tensors))
+        if known.outputs:
+            views.update((name, t) for (name, _, _), t in zip(known.outputs, outputs))
+        return Binding(views, env, outputs, workspace)
 
     def _remember(self, arguments: tuple, supplied_outputs: bool, binding: Binding, workspace: int, scratch: int) -> None:
         params = self.definition.params if supplied_outputs else self._supplied
@@ -180,7 +215,35 @@ class HIPRuntime:
         if len(known) >= MAX_LAYOUTS:
             for old in list(known)[:MAX_LAYOUTS // 2]:
                 known.pop(old, None)
-        known[key] = _Layout(dict(binding.env), tuple(p.name for p, _ in views), made, spans, pairs, workspace, scratch)
+        template = self._template(params, binding, [p.name for p, _ in views] + [name for name, _, _ in made], scratch)
+        known[key] = _Layout(dict(binding.env), tuple(p.name for p, _ in views), made, spans, pairs, workspace, scratch,
+                             template)
+
+    def _template(self, params: tuple, binding: Binding, names: list, scratch: int) -> _Template | None:
+        """The call that a layout makes, from views and scalars that are told apart by their values; None where the
+        launch is not one call of one entry, or takes a scalar in another form than its own."""
+        definition = self.definition
+        if definition.call is None:
+            return None
+        address = {name: (1 << 60) + 16 * i for i, name in enumerate(names)}
+        env, marks = dict(binding.env), {}
+        for position, p in enumerate(params):
+            if p.name in self._scalars:
+                marks[p.name] = (position, -(1.0 + position) * 2.0 ** -77)
+                env[p.name] = marks[p.name][1]
+        buffer, own = None, 1 << 61
+        if scratch > 0:
+            import torch
+
+            buffer = _Probe(torch.empty(scratch, dtype=torch.uint8, device="meta"), own)
+        entry, arguments = definition.call({n: _Probe(binding.views[n], a) for n, a in address.items()}, env, buffer)
+        index = {a: i for i, a in enumerate(address.values())}
+        at = list(enumerate(arguments))
+        scalars = tuple((n, position) for position, mark in marks.values() for n, v in at if v == mark)
+        if len(scalars) != len(marks):
+            return None
+        return _Template(entry, list(arguments), tuple((n, index[v]) for n, v in at if v in index),
+                         tuple(n for n, v in at if v == own), scalars)
 
     # ---- binding ------------------------------------------------------------
     def _bind(self, arguments: tuple, explicit_outputs: tuple | None, abstract: bool = False) -> Binding:
@@ -327,7 +390,12 @@ class HIPRuntime:
         return self._workspace
 
     def _launch(self, binding: Binding) -> None:
-        entry = self.definition.launch(binding.views, binding.env, _current_stream(self.device), binding.workspace)
+        stream = _current_stream(self.device)
+        if binding.call is not None:
+            entry, arguments = binding.call
+            _native.call_packed(entry, arguments, stream)
+        else:
+            entry = self.definition.launch(binding.views, binding.env, stream, binding.workspace)
         self._latest = (entry, _native.library().intent_amd_last_kernel())
 
     def _replay(self, record) -> None:
@@ -381,6 +449,17 @@ def _span_bytes(t) -> int:
     if t.numel() == 0:
         return 0
     return (sum((extent - 1) * stride for extent, stride in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _may_meet(starts: list, spans: tuple) -> bool:
+    """Whether two of the views of these addresses and lengths share a byte of their spans."""
+    end = 0
+    for start, span in sorted(zip(starts, spans)):
+        if span:
+            if start < end:
+                return True
+            end = start + span
+    return False
 
 
 def _row_pair(a, b) -> tuple | None:

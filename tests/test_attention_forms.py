@@ -863,3 +863,60 @@ def test_replayed_calls_are_checked():
     with pytest.raises(ValueError, match="intent_biased_paged_attention"):  # a cap that no f32 holds
         _native.Record(BA[0], tuple(_biased_args(cap=1e39)[:-1]))(0)
     assert len(_append_args()) == len(_append4_args()) + 1  # without the cache's format
+
+
+CALLS = ["qk_norm_rope", "paged_kv_append", "paged_kv_append_fp8", "paged_kv_append_int4", "paged_kv_read",
+         "paged_kv_read_fp8", "paged_kv_read_int4", "paged_attention", "paged_attention_fp8", "paged_attention_int4",
+         "biased_paged_attention", "biased_paged_attention_fp8", "biased_paged_attention_int4"]
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_known_layouts_make_the_same_call(monkeypatch, name):
+    """The second call of a layout hands over what the first does: addresses, scratch and scalars of its own, in every
+    place that takes them, with no norm, one view given twice, and memory too short for scratch."""
+    cache = "fp8" if name.endswith("_fp8") else "int4" if name.endswith("_int4") else "same"
+    rt = runtime_for(name)
+    rt._home = torch.device("cpu")
+    made = []
+    monkeypatch.setattr(_native, "call_packed", lambda entry, arguments, stream: made.append((entry, list(arguments))))
+    monkeypatch.setattr("intent_amd.runtime._current_stream", lambda device: 0)
+    buffer = torch.zeros(1 << 22, dtype=torch.uint8)
+    monkeypatch.setattr(rt, "_scratch_of", lambda need: None if need > buffer.numel() else buffer[:need])
+
+    def arguments(seed, n):
+        if "attention" in name:
+            q, caches, *rest = _inputs(seed, "f16", cache, [(1, 900), (1, 300 + seed)], 8, 2, 64, 16)
+            forms = (torch.ones(8), torch.zeros(0, dtype=torch.int32)) if "biased" in name else ()
+            return [q, *caches, *rest, *forms], [torch.empty_like(q)], [0.1 * (seed + 1)]
+        heads = _heads(seed, "f16", n, 6, 2, 64, 32, "k")
+        caches = [c.contiguous() for c in _caches(_gen(seed), "f16", cache, 3, 2, 8, 64)]
+        slots = torch.zeros(n, dtype=torch.int32)
+        if "read" in name:
+            return [*caches, slots], [torch.empty(n, 2, 64).half() for _ in range(2)], []
+        out = [torch.empty(n, 6, 64).half()]
+        if "norm" in name:
+            return [heads[0], heads[1], *heads[3:]], out + [torch.empty(n, 2, 64).half()], []
+        return [*heads[:6], slots, slots, *caches], out, []  # positions are the slots
+
+    for seed in (1, 1, 2):
+        ins, outs, scalars = arguments(seed, 5)
+        assert (rt.rebind((*ins, *outs, *scalars), True) is not None) == (len(made) > 0)
+        rt.launch(*ins, *outs, *scalars)
+        bound = rt.rebind((*ins, *outs, *scalars), True)
+        assert bound.call is not None and bound.outputs == tuple(outs)
+        rt.launch_bound(bound)
+        assert made[-1] == made[-2] and (made[-1][1].count(buffer.data_ptr()) == 1) == ("attention" in name)
+        rt.run(*ins, *scalars)
+        again = rt.rebind((*ins, *scalars), False)
+        rt.launch_bound(again)
+        want = rt.definition.call({**{p.name: t for p, t in zip(rt._supplied, ins)},
+                                   **{p.name: t for p, t in zip([p for p in rt.definition.params if p.name in rt._outputs],
+                                                                again.outputs)}},
+                                  again.env, again.workspace)
+        assert made[-1] == (want[0], list(want[1]))
+    if "attention" in name:
+        monkeypatch.setattr(rt, "_scratch_of", lambda need: None)
+        bound = rt.rebind((*ins, *outs, *scalars), True)
+        assert bound.call is None
+        rt.launch_bound(bound)
+        assert made[-1][1][-2:] == [0, 0]
