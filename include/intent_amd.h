@@ -776,7 +776,8 @@ size_t intent_paged_attention_workspace_size(int64_t T, int64_t HQ, int64_t HK, 
  *   scale = f16((max y - min y) / 15), lowest = f16(min y),
  *   code = clamp(rint((y - lowest) / scale), 0, 15), 0 where the scale is 0.
  * A group that holds an infinity or NaN has scale 0 and lowest NaN: it reads as
- * NaN. Everything else as in intent_paged_kv_append. No reference counterpart.
+ * NaN. A slot given twice may end with codes of one token and groups of the
+ * other. Everything else as in intent_paged_kv_append. No reference counterpart.
  */
 int intent_paged_kv_append_int4(const void* q, int64_t T, int64_t HQ, int64_t q_ld,
                                 const void* k, int64_t HK, int64_t k_ld,
@@ -814,7 +815,8 @@ int intent_paged_kv_read(int cache_format,
  *   slopes f32 [HQ] (finite): x_t = x_t - slopes[head] |p - t|;
  *   out = sum_t softmax_t(x_t) v_t;
  *   prefix_lens i32 [S], causal: row p sees t <= p and t < prefix_lens[s] too.
- * 0 and null leave a form out; with none of them, and without 4 bits, it is
+ * A softcap lies between 2^-100 and 4096; a capped score is 2^-21 of it off at
+ * most. 0 and null leave a form out; with none of them, and without 4 bits, it is
  * intent_paged_attention. A window bounds the prefix as well. Values in 4 bits
  * are rounded to f16 for the products, in bf16 too (the queries of bf16, scaled
  * by a power of two for each row, are exact in f16 or 2^-38 of the row's largest

@@ -399,9 +399,9 @@ int attend(const void* q, int64_t T, int64_t HQ, int64_t q_ld, int is_bf16, cons
   INTENT_REQUIRE(__builtin_isfinite(scale_log2), INTENT_ERR_INVALID_ARGUMENT, "scale * log2(e) must be finite, got %g",
                  (double)scale_log2);
   const float cap_log2 = f.softcap * 1.44269504088896340736f;
-  // a cap so small that 1 / cap is no f32 is none that a score could tell from zero
-  INTENT_REQUIRE(f.softcap == 0.f || (f.softcap >= 0x1p-100f && f.softcap <= 0x1p100f), INTENT_ERR_INVALID_ARGUMENT,
-                 "softcap must be 0 (none) or between 2^-100 and 2^100, got %g", (double)f.softcap);
+  // 2^-21 of the cap is what a capped score may be off: 2^-9 at the highest that is taken
+  INTENT_REQUIRE(f.softcap == 0.f || (f.softcap >= 0x1p-100f && f.softcap <= 4096.f), INTENT_ERR_INVALID_ARGUMENT,
+                 "softcap must be 0 (none) or between 2^-100 and 4096, got %g", (double)f.softcap);
   INTENT_REQUIRE(HK > 0 && HQ % HK == 0, INTENT_ERR_INVALID_ARGUMENT,
                  "HQ=%lld query heads must be a multiple of the HK=%lld heads of the cache", (long long)HQ,
                  (long long)HK);

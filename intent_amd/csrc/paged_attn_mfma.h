@@ -301,7 +301,7 @@ struct Scores {
   float slope, position;
 
   INTENT_DEVICE void begin(const AttnArgs& a, float scale, float slope_log2, int p) {
-    in = kCap ? (kFp8 ? cap_rate(a) : scale * cap_rate(a)) : scale;
+    in = kCap ? fminf(kFp8 ? cap_rate(a) : scale * cap_rate(a), 0x1.fffffep127f) : scale;  // 0 times it stays 0
     out = kCap ? 2.0f * a.cap_log2 : scale;
     slope = slope_log2, position = (float)p;
   }

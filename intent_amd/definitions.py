@@ -1529,8 +1529,8 @@ def _biased_check(env: dict) -> None:
         if extent not in (0, whole):
             raise ValueError(f"{name} must have {whole} elements, or none, got {extent}")
     cap = float(env["SOFTCAP"])
-    if cap != 0.0 and not 2.0 ** -100 <= cap <= 2.0 ** 100:
-        raise ValueError(f"SOFTCAP must be 0 (none) or between 2^-100 and 2^100, got {cap}")
+    if cap != 0.0 and not 2.0 ** -100 <= cap <= 4096.0:
+        raise ValueError(f"SOFTCAP must be 0 (none) or between 2^-100 and 4096, got {cap}")
 
 
 def _attention_scratch(number: int) -> Callable[[dict], int]:

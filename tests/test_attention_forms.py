@@ -480,6 +480,61 @@ def test_scores_past_the_cap(gpu, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("cap", [2.0 ** -100, 0.01, 100.0, 4096.0])
+@pytest.mark.parametrize("new,D", [(1, 64), (40, 128), (300, 128), (5, 256), (9, 80)])
+@pytest.mark.parametrize("cache", ["same", "fp8", "int4"])
+def test_caps_of_many_sizes(gpu, cap, new, D, cache):
+    """From caps that leave all scores alike to caps that leave them as they are, with slopes and without."""
+    inputs = _inputs(35, "f16", cache, [(new, new + 150)], 4, 2, D, 16, q_std=4.0)
+    for slopes in (None, torch.tensor([0.5, 0.0, 0.01, 1.0])):
+        want, tol = ref_attention(inputs[0], inputs[1], cache, *inputs[2:], D ** -0.5, True, 0, cap, slopes, fine=True)
+        _close(_attend(inputs, "f16", cache, D ** -0.5, cap=cap, slopes=slopes), want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [0.0, -0.2, 3e-36, 3.0])
+@pytest.mark.parametrize("lens", [[(1, 200)], [(4, 90)], [(80, 200)]], ids=str)
+@pytest.mark.parametrize("cache", ["same", "fp8", "int4"])
+def test_scales(gpu, lens, scale, cache):
+    inputs = _inputs(36, "bf16", cache, lens, 4, 2, 128, 16, q_std=0.5)
+    for forms in ({}, {"cap": 7.0}, {"slopes": torch.tensor([0.5, 0.0, 0.01, -0.02])},
+                  {"cap": 2.0, "slopes": torch.tensor([0.5, 0.0, 0.01, 1.0]), "prefix": torch.tensor([70], dtype=torch.int32)}):
+        want, tol = ref_attention(inputs[0], inputs[1], cache, *inputs[2:], scale, True, 0, fine=True, **forms)
+        _close(_attend(inputs, "bf16", cache, scale, **forms), want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("new", [1, 6, 90])
+def test_int4_queries_that_are_not_finite(gpu, dt, new):
+    """A query that holds an infinity or NaN leaves the other rows alone."""
+    inputs = _inputs(37, dt, "int4", [(new, 120), (new, 40)], 4, 2, 64, 16)
+    want, tol = ref_attention(inputs[0], inputs[1], "int4", *inputs[2:], 0.125, True, 0, fine=True)
+    inputs[0][0, 1, 5], inputs[0][-1, 2, 9] = float("inf"), float("nan")
+    out = _attend(inputs, dt, "int4", 0.125).cpu()
+    bad = torch.zeros(2 * new, 4, dtype=torch.bool)
+    bad[0, 1], bad[-1, 2] = True, True
+    assert bool(out[bad].isnan().any(-1).all())
+    _close(out[~bad], want[~bad], tol[~bad])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens", [[(1, 300)], [(5, 90)], [(80, 200)]], ids=str)
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+def test_int4_pairs_of_many_sizes(gpu, dt, lens):
+    """Scales below zero, zero, of f16's subnormals and large ones; lowest values far off."""
+    inputs = _inputs(38, dt, "int4", lens, 4, 2, 128, 16)
+    for i in (2, 3):
+        pairs = inputs[1][i]
+        pairs[..., 0, 0] = -pairs[..., 0, 0].abs()
+        pairs[..., 1, 0] = 0
+        pairs[..., 2, :] = torch.tensor([3 * 2.0 ** -24, -5 * 2.0 ** -24])
+        pairs[..., 3, :] = torch.tensor([4096.0, -30720.0]) if i == 3 else torch.tensor([1.0, 32.0])
+    want, tol = ref_attention(inputs[0], inputs[1], "int4", *inputs[2:], 0.02, True, 0, fine=True)
+    _close(_attend(inputs, dt, "int4", 0.02), want, tol)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("new", [1, 40, 300])
 def test_long_distances(gpu, new):
     """Slopes so steep that only the nearest tokens count, and none at all for some heads, over a long cache."""
@@ -550,6 +605,29 @@ def test_far_pages(gpu, new, cache):
     slots = torch.arange(pages * PAGE, dtype=torch.int32)
     read = _compile("paged_kv_read", "f16", cache)
     assert all(torch.equal(a, b) for a, b in zip(read.run(*far, slots.cuda()), read.run(*_cuda(*caches), slots.cuda())))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [7, 900])
+def test_keys_and_values_of_one_allocation(gpu, T):
+    """Append, attention and reading over kv[:, 0] and kv[:, 1]: both halves get their own rows, all others stay."""
+    HQ, HK, D, PAGE, pages = 8, 2, 64, 16, 70
+    gen = _gen(45)
+    heads = _heads(46, "bf16", T, HQ, HK, D, 0, "")
+    slots = torch.randperm(pages * PAGE, generator=gen)[:T].to(torch.int32)
+    k, v, kg, vg = _caches(gen, "bf16", "int4", pages, HK, PAGE, D)
+    alone = _cuda(*[c.contiguous() for c in (k, v, kg, vg)])
+    views = [t[:, i] for t in _cuda(torch.stack((k, v), 1), torch.stack((kg, vg), 1)) for i in (0, 1)]
+    append, args = _compile("paged_kv_append", "bf16", "int4"), _cuda(*heads, slots)
+    for _ in range(2):  # bound, and known
+        q_out = append.run(*args, *views)
+    assert torch.equal(q_out, append.run(*args, *alone))
+    assert all(torch.equal(got, want) for got, want in zip(views, alone))
+    rest = _cuda(torch.randperm(pages, generator=gen).to(torch.int32)[None], torch.tensor([0, T], dtype=torch.int32),
+                 torch.tensor([pages * PAGE - 3], dtype=torch.int32))
+    attend, read = _compile("paged_attention", "bf16", "int4"), _compile("paged_kv_read", "bf16", "int4")
+    assert torch.equal(attend.run(q_out, *views, *rest, 0.125), attend.run(q_out, *alone, *rest, 0.125))
+    assert all(torch.equal(a, b) for a, b in zip(read.run(*views, args[-1]), read.run(*alone, args[-1])))
 
 
 @pytest.mark.gpu
@@ -761,7 +839,7 @@ def test_arguments_are_checked():
         change[i] = bad
         with pytest.raises(error, match=match):
             rt.infer_outputs((*change, 0.1))
-    for cap in (-1.0, float("nan"), float("inf"), 1e-40, 1e39):
+    for cap in (-1.0, float("nan"), float("inf"), 1e-40, 5000.0, 1e39):
         with pytest.raises(ValueError, match="SOFTCAP"):
             runtime_for("biased_paged_attention_int4", SOFTCAP=cap).infer_outputs((*flat, 0.1))
     with pytest.raises(ValueError, match="SOFTCAP"):
@@ -837,7 +915,7 @@ A4, RD, BA = ("intent_paged_kv_append_int4", _append4_args), ("intent_paged_kv_r
     (RD, UNSUPPORTED, dict(D=520)), (RD, UNSUPPORTED, dict(page=3)), (RD, UNSUPPORTED, dict(T=1 << 24)),
     (RD, ALIGN, dict(v_ld=132)), (RD, ALIGN, dict(k_out=FAKE + 8)), (RD, ALIGN, dict(vc=FAKE + 4)), (RD, ALIGN, dict(vg_ld=131)),
     (BA, INVALID, dict(format=4)), (BA, INVALID, dict(cap=-1.0)), (BA, INVALID, dict(cap=float("nan"))),
-    (BA, INVALID, dict(cap=float("inf"))), (BA, INVALID, dict(cap=1e-38)), (BA, INVALID, dict(scale=float("nan"))),
+    (BA, INVALID, dict(cap=float("inf"))), (BA, INVALID, dict(cap=1e-38)), (BA, INVALID, dict(cap=4097.0)), (BA, INVALID, dict(scale=float("nan"))),
     (BA, INVALID, dict(kg=None)), (BA, INVALID, dict(vg_ld=64)), (BA, INVALID, dict(HQ=5, q_ld=400, out_ld=400)),
     (BA, INVALID, dict(window=-1)), (BA, INVALID, dict(format=0)), (BA, UNSUPPORTED, dict(page=10)), (BA, UNSUPPORTED, dict(D=36)),
     (BA, ALIGN, dict(kc_ld=1028)), (BA, ALIGN, dict(kg=FAKE + 2)), (BA, ALIGN, dict(vg_ld=129)), (BA, ALIGN, dict(out_ld=260)),
