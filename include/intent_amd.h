@@ -773,7 +773,7 @@ size_t intent_paged_attention_workspace_size(int64_t T, int64_t HQ, int64_t HK, 
  * elements (the last may be shorter) a scale and a lowest value,
  *   value = lowest + scale * code.
  * With y clamped to +-61440 (so that lowest + 15 scale is an f16):
- *   scale = f16((max y - min y) / 15), lowest = f16(min y),
+ *   scale = f16((max y - min y) * f32(1 / 15)), lowest = f16(min y),
  *   code = clamp(rint((y - lowest) / scale), 0, 15), 0 where the scale is 0.
  * A group that holds an infinity or NaN has scale 0 and lowest NaN: it reads as
  * NaN. A slot given twice may end with codes of one token and groups of the

@@ -8,7 +8,7 @@
 //   cache:   the row as it is (f16 / bf16), or E4M3FN codes with a scale for each token and head,
 //            s = max(absmax, 1e-12) / 448, code = e4m3fn(clamp(y / s, +-448)): the groupwise FP8
 //            quantizer's rule with one group for each head; or 4 bits (cache4.h), y clamped to +-61440,
-//            s = f16((max - min) / 15), m = f16(min) of each group of 32 elements,
+//            s = f16((max - min) * f32(1 / 15)), m = f16(min) of each group of 32 elements,
 //            code = clamp(rint((y - m) / s), 0, 15). s and m are rounded before the codes are found, so that
 //            these make up for it; the clamp keeps m + 15 s inside f16.
 //
@@ -224,7 +224,7 @@ __global__ __launch_bounds__(256) void attn_prep_kernel(const PrepArgs a) {
         size = quad_reduce(size, [](float p, float q) { return magnitude_max(p, q); });
         // a group that holds an infinity or NaN reads as NaN throughout
         const bool good = size < INFINITY;
-        const f16 scale = good ? (f16)__fdiv_rn(high - low, 15.0f) : (f16)0.f;
+        const f16 scale = good ? (f16)((high - low) * (1.0f / 15.0f)) : (f16)0.f;
         const f16 lowest = good ? (f16)low : bit_cast<f16>((uint16_t)0x7e00);
         // The quotient by a reciprocal, 2^-22 of it off at most (3e-6 where it gives a code of 0 to 15, beyond that it
         // is clamped); by division where a lane's may lie at the middle of two codes. 8192 tokens of 32 + 8 + 8 heads

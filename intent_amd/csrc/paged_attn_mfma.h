@@ -357,8 +357,20 @@ struct Scores {
 // 242 us, 5.9 TB/s, where a large copy moves 5.1; 64 of 300 to 8191 tokens in 8 bits (645 MB): 124 us, 5.2
 // TB/s, the lengths being uneven. One sequence of 4096 tokens (17 MB) is a chain of latencies, 7 us and 4
 // for the join.
+//
+// Waves to a SIMD are what the registers hold. Rows of 4 bits leave more of them, slopes take some back (48 rows, 64
+// sequences of 300 to 8191 tokens on eight heads: of 64 148 us with two waves, 110 with three; of 128 246 with one,
+// 182 with two; 16 rows of 256, on four heads: 170 with one, 109 with two).
+constexpr int rows_waves(int cache, int forms, int D, int mt) {
+  if (cache == kCacheInt4) {
+    const int spare = (forms & kSloped) != 0;
+    return D > 128 ? 2 : mt == 1 ? 4 : mt * D <= 128 ? 3 : mt * D <= 192 ? 3 - spare : mt * D < 384 || D == 128 && mt == 3 ? 2 : mt * D <= 384 ? 2 - spare : 1;
+  }
+  return D > 128 ? 1 : mt * D <= 128 ? 3 : mt * D <= 256 ? 2 : 1;
+}
+
 template <bool kBf16, int kCache, int kForms, int D, int MT>
-__global__ __launch_bounds__(256, D > 128 ? 1 : MT * D <= 128 ? (kCache == kCacheInt4 && MT == 1 ? 4 : 3) : MT * D <= 256 ? 2 : 1)
+__global__ __launch_bounds__(256, rows_waves(kCache, kForms, D, MT))
     void attn_rows_kernel(const AttnArgs a) {
   constexpr bool kFp8 = kCache == kCacheFp8, kInt4 = kCache == kCacheInt4;
   constexpr bool kMath = kBf16 && !kInt4;              // products in bf16

@@ -59,7 +59,7 @@ def quantize4(x):
     x = x.float().clamp(-MOST, MOST)
     parts = x.split(32, -1)
     high, low = (torch.stack([getattr(p, f)(-1) for p in parts], -1) for f in ("amax", "amin"))
-    pairs = torch.stack((((high - low) / 15.0).half(), low.half()), -1)
+    pairs = torch.stack((((high - low) * torch.tensor(1 / 15, dtype=torch.float32)).half(), low.half()), -1)
     scale, lowest = (t.float() for t in spread4(pairs, D))
     code = torch.where(scale > 0, ((x - lowest) / scale).round().clamp(0, 15), 0.0)
     return code, pairs
