@@ -408,6 +408,8 @@ int attend(const void* q, int64_t T, int64_t HQ, int64_t q_ld, int is_bf16, cons
   // 2^-21 of the cap is what a capped score may be off: 2^-9 at the highest that is taken
   INTENT_REQUIRE(f.softcap == 0.f || (f.softcap >= 0x1p-100f && f.softcap <= 4096.f), INTENT_ERR_INVALID_ARGUMENT,
                  "softcap must be 0 (none) or between 2^-100 and 4096, got %g", (double)f.softcap);
+  INTENT_REQUIRE(intent::aligned4(f.slopes) && intent::aligned4(f.prefix_lens), INTENT_ERR_ALIGNMENT,
+                 "slopes and prefix lengths must be 4-byte aligned");
   INTENT_REQUIRE(HK > 0 && HQ % HK == 0, INTENT_ERR_INVALID_ARGUMENT,
                  "HQ=%lld query heads must be a multiple of the HK=%lld heads of the cache", (long long)HQ,
                  (long long)HK);

@@ -298,12 +298,13 @@ struct Scores {
   // whether they are in base 2 before the softmax takes its maximum
   static constexpr bool kScaled = kFp8 || kSlope;
   float in, out;  // capped: what a score is multiplied by before and behind the reciprocal
-  float slope, position;
+  float slope;
+  int position;  // less the lane's first token: distances are exact below 2^24 tokens, wherever they lie
 
   INTENT_DEVICE void begin(const AttnArgs& a, float scale, float slope_log2, int p) {
     in = kCap ? fminf(kFp8 ? cap_rate(a) : scale * cap_rate(a), 0x1.fffffep127f) : scale;  // 0 times it stays 0
     out = kCap ? 2.0f * a.cap_log2 : scale;
-    slope = slope_log2, position = (float)p;
+    slope = slope_log2, position = p;
   }
   // s: element (u, r) of token t + token(u, r), of which `last` is the greatest; the rows stand at `top` and behind.
   // k_mul: scales of the keys, with the scores' own.
@@ -325,7 +326,7 @@ struct Scores {
         }
     }
     if constexpr (kSlope) {
-      const float ahead = (float)t - position;
+      const float ahead = (float)(t - position);
       auto add = [&](int u, int r, float bias) {
         s[u][r] = __builtin_fmaf(s[u][r], kFp8 && !kCap ? k_mul(u, r) : out, bias);
       };

@@ -545,6 +545,25 @@ def test_long_distances(gpu, new):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("cache", ["same", "int4"])
+@pytest.mark.parametrize("new", [1, 40, 300])
+def test_distances_past_24_bits(gpu, new, cache):
+    """Positions that no f32 tells apart: with steep slopes the tokens behind 2^24 others give what they give alone
+    (weights of tokens 1024 and more away are below 2^-1000)."""
+    HQ, HK, D, PAGE, near = 4, 2, 64, 256, 2048
+    q, caches, table, offsets, _ = _inputs(39, "f16", cache, [(new, near)], HQ, HK, D, PAGE, poison=False)
+    slopes = torch.tensor([1.0, 2.0, 1.5, 30.0])
+    far = (1 << 24) + 3 * PAGE
+    long = torch.cat((torch.zeros(1, far // PAGE, dtype=torch.int32), table), 1)
+    # rows whose last tokens are as near as 1024: the others see what lies before
+    want, tol = ref_attention(q, caches, cache, table, offsets, torch.tensor([near], dtype=torch.int32), 0.125, True, 0,
+                              slopes=slopes, fine=True)
+    got = _attend((q, caches, long, offsets, torch.tensor([far + near], dtype=torch.int32)), "f16", cache, 0.125, slopes=slopes)
+    # sums of as many terms of f32, none of which counts but the nearest
+    _close(got, want, tol + 2.0 ** -20)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("biased", [False, True])
 @pytest.mark.parametrize("new,HQ,kv,D", [(1, 4, 20000, 64), (7, 8, 9000, 96), (1, 2, 9000, 256), (352, 8, 5000, 128)])
 def test_split_and_unsplit(gpu, new, HQ, kv, D, biased):
@@ -919,6 +938,7 @@ A4, RD, BA = ("intent_paged_kv_append_int4", _append4_args), ("intent_paged_kv_r
     (BA, INVALID, dict(kg=None)), (BA, INVALID, dict(vg_ld=64)), (BA, INVALID, dict(HQ=5, q_ld=400, out_ld=400)),
     (BA, INVALID, dict(window=-1)), (BA, INVALID, dict(format=0)), (BA, UNSUPPORTED, dict(page=10)), (BA, UNSUPPORTED, dict(D=36)),
     (BA, ALIGN, dict(kc_ld=1028)), (BA, ALIGN, dict(kg=FAKE + 2)), (BA, ALIGN, dict(vg_ld=129)), (BA, ALIGN, dict(out_ld=260)),
+    (BA, ALIGN, dict(slopes=FAKE + 2)), (BA, ALIGN, dict(prefix=FAKE + 1)),
 ])
 def test_entries_refuse(entry, code, change):
     """Every call here fails before any HIP call."""
