@@ -15,6 +15,13 @@
 // maximum of t + log2(scale), w = exp2(t - M) * scale, and only the sum of weights takes exp2(t - M) by
 // itself. The codes are exact in 16 bits.
 //
+// 4 bits are widened to f16, for heads of bf16 too (its packed operations have no counterpart for bf16): lowest +
+// scale code in one rounding, 2^-12 of it off at most where the code itself stands for a thirtieth of the group's
+// range. Scores are then 2^-12 sum |q k| off, weights by as much (f16 heads: 5e-4 of the output against 2e-4 with
+// f32 rows; bf16's own rounding is 17e-4); to leave the scale out of the product would keep the codes exact, but
+// takes an accumulator and a weight for every group. Queries of bf16 are brought into f16's range row by row
+// (query_f16); weights are f16's.
+//
 // The product with the values takes the weights rounded to the heads' type, half a step of it each, like
 // the values beside them; the sums of weights are those before the rounding. bf16 has the exponents of
 // f32. f16 ends at 2^-24, and a long flat tail behind one token that outweighs it may lie below: there all
@@ -357,7 +364,10 @@ struct Scores {
 // 16 KB (8 KB of 8-bit) under way. Four sequences of 60000 to 131000 tokens, 32 heads sharing 8 (1.42 GB):
 // 242 us, 5.9 TB/s, where a large copy moves 5.1; 64 of 300 to 8191 tokens in 8 bits (645 MB): 124 us, 5.2
 // TB/s, the lengths being uneven. One sequence of 4096 tokens (17 MB) is a chain of latencies, 7 us and 4
-// for the join.
+// for the join. The same in 4 bits: four (442 MB) 85 to 90 us, 5.0 TB/s, 64 (391 MB) 80 to 84 us, 4.8 TB/s, one 5.8 us.
+// There 32 tokens are 300 vector instructions of a wave, two thirds of them to widen the codes, and the vector unit is
+// busy for 56% of the time; four workgroups to a CU or three, and loads by 64-bit addresses or by buffers, make no
+// difference to the long ones.
 //
 // Waves to a SIMD are what the registers hold. Rows of 4 bits leave more of them, slopes take some back (48 rows, 64
 // sequences of 300 to 8191 tokens on eight heads: of 64 148 us with two waves, 110 with three; of 128 246 with one,
@@ -779,6 +789,13 @@ __global__ __launch_bounds__(256, rows_waves(kCache, kForms, D, MT))
 // TFLOP/s. What is left: with the loads of the cache taken away it takes 140 us, with the vector work
 // 117, with the products 111; each wave's own chain, not one unit, sets the time. 64 rows to a wave read LDS
 // half as often, but one wave to a SIMD and 1500 copies between the two halves of its registers take 215 us.
+//
+// Capped scores (4096 tokens of which the first 1000 are a prefix, 141 GFLOP): 208 to 237 us; an exponential and a
+// reciprocal more for each score cost what they take to issue, 43 cycles, also if they stand between the products.
+// 4 bits (1834 + 1862 tokens over 9000 to 16000 others, 911 GFLOP): 1010 to 1050 us, 870 to 900 TFLOP/s. The codes are
+// widened on their way to LDS, 16 bytes of a token to a lane (heads of 64: 8), between a load's arrival and the barrier:
+// keys by four of eight waves and values by the other four, 3% less than both by the first four. Their stores meet four
+// to a bank; to turn them apart costs more registers and selects than it gains (1220 against 1195 us).
 template <bool kBf16, int kCache, int kForms, int D, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
     void attn_tile_kernel(const AttnArgs a) {
