@@ -49,7 +49,12 @@ struct PrepArgs {
   int HQ, HK, D, R, P, heads, items_per_token, interleaved, page_shift, slot_count;
 };
 
-enum Mode { kKeysOut = -1, kCacheSame = intent::kCacheSame, kCacheFp8 = intent::kCacheFp8, kCacheInt4 = intent::kCacheInt4 };
+enum Mode {
+  kKeysOut = -1,
+  kCacheSame = intent::kCacheSame,
+  kCacheFp8 = intent::kCacheFp8,
+  kCacheInt4 = intent::kCacheInt4
+};
 
 // The larger of two floats without a sign, by their bits: NaN is the largest.
 INTENT_DEVICE float magnitude_max(float a, float b) {

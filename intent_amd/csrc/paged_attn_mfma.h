@@ -147,7 +147,8 @@ INTENT_DEVICE float cached_value(const AttnArgs& a, int page, int head, int t, i
   const char* params = (const char*)cached_scales<kParams>(a, a.v_scales, page, a.vs_step, head, t);
   if constexpr (kCache == kCacheInt4) {
     const f16x2 pair = bit_cast<f16x2>(((const uint32_t*)params)[d / kGroup4]);
-    return (float)__builtin_elementwise_fma((f16)(int)(((const uint32_t*)row)[d / 8] >> code_bit(d) & 15u), pair[0], pair[1]);
+    const uint32_t code = ((const uint32_t*)row)[d / 8] >> code_bit(d) & 15u;
+    return (float)__builtin_elementwise_fma((f16)(int)code, pair[0], pair[1]);
   } else if constexpr (kCache == kCacheFp8) {
     return __builtin_amdgcn_cvt_f32_fp8((int)((const uint8_t*)row)[d], 0) * *(const float*)params;
   } else if constexpr (kBf16) {
@@ -375,7 +376,10 @@ struct Scores {
 constexpr int rows_waves(int cache, int forms, int D, int mt) {
   if (cache == kCacheInt4) {
     const int spare = (forms & kSloped) != 0;
-    return D > 128 ? 2 : mt == 1 ? 4 : mt * D <= 128 ? 3 : mt * D <= 192 ? 3 - spare : mt * D < 384 || D == 128 && mt == 3 ? 2 : mt * D <= 384 ? 2 - spare : 1;
+    if (D > 128) return 2;
+    if (mt == 1) return 4;
+    if (mt * D <= 192) return mt * D <= 128 ? 3 : 3 - spare;
+    return mt * D > 384 ? 1 : D == 96 && mt == 4 ? 2 - spare : 2;
   }
   return D > 128 ? 1 : mt * D <= 128 ? 3 : mt * D <= 256 ? 2 : 1;
 }
@@ -656,7 +660,8 @@ __global__ __launch_bounds__(256, rows_waves(kCache, kForms, D, MT))
       if constexpr (kBiased) {
         // the branch, always taken, keeps the forms apart from the products: without it 16 rows of heads of 256 over
         // 32 caches of 2000 to 8000 tokens take 187 us, with it 174
-        if (!Form::kCap || a.cap_log2 != 0.f) forms[m].apply(s[m], now, 31, top.p, [](int u, int r) { return 16 * u + r; },
+        if (!Form::kCap || a.cap_log2 != 0.f)
+          forms[m].apply(s[m], now, 31, top.p, [](int u, int r) { return 16 * u + r; },
                        [&](int u, int r) { return k_mul[u][r]; });
       }
       // the highest score, times the value's scale; s is a score or, scaled already, its t
@@ -693,7 +698,8 @@ __global__ __launch_bounds__(256, rows_waves(kCache, kForms, D, MT))
       for (int u = 0; u < 2; ++u) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float e = __builtin_amdgcn_exp2f(kScaled ? s[m][u][r] - base : __builtin_fmaf(s[m][u][r], row_scale[m], -base));
+          const float e = __builtin_amdgcn_exp2f(kScaled ? s[m][u][r] - base
+                                                         : __builtin_fmaf(s[m][u][r], row_scale[m], -base));
           total[m] += e;
           wt[u][r] = kFp8 ? e * v_mul[u][r] : e;
         }
@@ -937,7 +943,9 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
     load(kr, kg, takes_keys ? a.k_cache : a.v_cache, takes_keys ? a.k_step : a.v_step,
          takes_keys ? a.k_scales : a.v_scales, takes_keys ? a.ks_step : a.vs_step, takes_keys ? keys : values);
   };
-  auto load_keys = [&](int t) __attribute__((always_inline)) { load(kr, kg, a.k_cache, a.k_step, a.k_scales, a.ks_step, t); };
+  auto load_keys = [&](int t) __attribute__((always_inline)) {
+    load(kr, kg, a.k_cache, a.k_step, a.k_scales, a.ks_step, t);
+  };
   auto load_values = [&](int t) __attribute__((always_inline)) {
     load(vr, vg, a.v_cache, a.v_step, a.v_scales, a.vs_step, t);
     if constexpr (kFp8) {

@@ -74,7 +74,7 @@ class _Layout:
 
     env: dict
     names: tuple        # the supplied views, in argument order
-    outputs: tuple      # allocated Out buffers: (name, shape, dtype)
+    outputs: tuple      # allocated Out buffers: (name, shape, strides, dtype)
     spans: tuple
     pairs: tuple
     workspace: int      # bytes, -1 without one
@@ -105,6 +105,8 @@ class HIPRuntime:
         self._writable = {p.name for p in definition.params if isinstance(p, Param) and p.access is not ViewKind.IN}
         self._outputs = {p.name for p in definition.params if isinstance(p, Param) and p.access is ViewKind.OUT}
         self._supplied = tuple(p for p in definition.params if isinstance(p, Scalar) or p.access is not ViewKind.OUT)
+        self._tensor_at = tuple(tuple(i for i, p in enumerate(params) if isinstance(p, Param))
+                                for params in (self._supplied, definition.params))
         self._layouts: tuple[dict, dict] = ({}, {})  # by calling form: outputs allocated, outputs supplied
         self._home = None
 
@@ -128,19 +130,20 @@ class HIPRuntime:
             self._home = torch.device("cuda", self.device)
         return self._home
 
-    def _layout_key(self, params: tuple, arguments: tuple):
-        """Dtypes, devices, shapes and strides of the arguments; None unless all are plain tensors."""
+    def _layout_key(self, arguments: tuple, supplied_outputs: bool):
+        """Dtypes, devices, shapes and strides of the arguments; None unless all are plain strided tensors."""
         import torch
 
+        plain = (torch.Tensor, torch.nn.Parameter)
         key = []
-        for p, a in zip(params, arguments):
-            if p.name in self._scalars:
-                continue
-            if type(a) is not torch.Tensor and type(a) is not torch.nn.Parameter:
-                return None
-            if a.layout is not torch.strided:
-                return None
-            key += (a.dtype, a.device, a.shape, a.stride())
+        try:
+            for at in self._tensor_at[supplied_outputs]:
+                a = arguments[at]
+                if type(a) not in plain:
+                    return None
+                key += (a.dtype, a.device, a.shape, a.stride())
+        except RuntimeError:  # a layout without strides
+            return None
         return tuple(key)
 
     def rebind(self, arguments: tuple, supplied_outputs: bool) -> Binding | None:
@@ -148,7 +151,7 @@ class HIPRuntime:
         params = self.definition.params if supplied_outputs else self._supplied
         if len(arguments) != len(params):
             return None
-        key = self._layout_key(params, arguments)
+        key = self._layout_key(arguments, supplied_outputs)
         known = self._layouts[supplied_outputs].get(key) if key is not None else None
         if known is None:
             return None
@@ -175,7 +178,8 @@ class HIPRuntime:
         if known.outputs:
             import torch
 
-            outputs = tuple(torch.empty(shape, dtype=dt, device=self._home_device()) for _, shape, dt in known.outputs)
+            outputs = tuple(torch.empty_strided(shape, stride, dtype=dt, device=self._home)
+                            for _, shape, stride, dt in known.outputs)
         elif supplied_outputs:
             outputs = tuple(t for t, name in zip(tensors, known.names) if name in self._outputs)
         workspace = self._buffer_of(known.workspace, known.scratch)
@@ -194,12 +198,12 @@ class HIPRuntime:
             return Binding(None, env, outputs, workspace, (template.entry, values))
         views = dict(zip(known.names, tensors))
         if known.outputs:
-            views.update((name, t) for (name, _, _), t in zip(known.outputs, outputs))
+            views.update((out[0], t) for out, t in zip(known.outputs, outputs))
         return Binding(views, env, outputs, workspace)
 
     def _remember(self, arguments: tuple, supplied_outputs: bool, binding: Binding, workspace: int, scratch: int) -> None:
         params = self.definition.params if supplied_outputs else self._supplied
-        key = self._layout_key(params, arguments)
+        key = self._layout_key(arguments, supplied_outputs)
         if key is None:
             return
         views = [(p, a) for p, a in zip(params, arguments) if p.name not in self._scalars]
@@ -208,14 +212,15 @@ class HIPRuntime:
                       for i in range(len(views)) for j in range(i + 1, len(views))
                       if spans[i] and spans[j]
                       and (views[i][0].name in self._writable or views[j][0].name in self._writable))
-        made = () if supplied_outputs else tuple((p.name, tuple(binding.views[p.name].shape), binding.views[p.name].dtype)
+        made = () if supplied_outputs else tuple((p.name, tuple(binding.views[p.name].shape), binding.views[p.name].stride(),
+                                                  binding.views[p.name].dtype)
                                                  for p in self.definition.params
                                                  if p.name not in self._scalars and p.access is ViewKind.OUT)
         known = self._layouts[supplied_outputs]
         if len(known) >= MAX_LAYOUTS:
             for old in list(known)[:MAX_LAYOUTS // 2]:
                 known.pop(old, None)
-        template = self._template(params, binding, [p.name for p, _ in views] + [name for name, _, _ in made], scratch)
+        template = self._template(params, binding, [p.name for p, _ in views] + [out[0] for out in made], scratch)
         known[key] = _Layout(dict(binding.env), tuple(p.name for p, _ in views), made, spans, pairs, workspace, scratch,
                              template)
 
