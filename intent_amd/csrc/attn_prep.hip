@@ -229,7 +229,9 @@ __global__ __launch_bounds__(256) void attn_prep_kernel(const PrepArgs a) {
         size = quad_reduce(size, [](float p, float q) { return magnitude_max(p, q); });
         // a group that holds an infinity or NaN reads as NaN throughout
         const bool good = size < INFINITY;
-        const f16 scale = good ? (f16)((high - low) * (1.0f / 15.0f)) : (f16)0.f;
+        float step = (high - low) * (1.0f / 15.0f);
+        asm("" : "+v"(step));  // an f32 before it is an f16, not one rounding of a mixed product
+        const f16 scale = good ? (f16)step : (f16)0.f;
         const f16 lowest = good ? (f16)low : bit_cast<f16>((uint16_t)0x7e00);
         // The quotient by a reciprocal, 2^-22 of it off at most (3e-6 where it gives a code of 0 to 15, beyond that it
         // is clamped); by division where a lane's may lie at the middle of two codes. 8192 tokens of 32 + 8 + 8 heads
