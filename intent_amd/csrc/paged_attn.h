@@ -57,7 +57,8 @@ struct AttnArgs {
 // The tiled kernels for one type, cache and form of scores (paged_attn_*.hip), by the rows of a tile: 16 to 64,
 // whose tokens are spread over a workgroup's four waves, or 128 or 256, 32 to a wave. `items` workgroups for each
 // cached head.
-typedef int LaunchAttn(const AttnArgs& a, int items, int rows, hipStream_t stream);
+// `few`: the list of a mixture's short sequences (16 rows, heads of 64), in the same launch with tiles of 128 rows.
+typedef int LaunchAttn(const AttnArgs& a, int items, int rows, const AttnArgs* few, int few_items, hipStream_t stream);
 LaunchAttn launch_attn_f16, launch_attn_bf16, launch_attn_f16_fp8, launch_attn_bf16_fp8, launch_attn_f16_int4,
     launch_attn_bf16_int4, launch_attn_f16_capped, launch_attn_bf16_capped, launch_attn_f16_fp8_capped,
     launch_attn_bf16_fp8_capped, launch_attn_f16_int4_capped, launch_attn_bf16_int4_capped, launch_attn_f16_sloped,

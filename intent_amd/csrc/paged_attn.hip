@@ -215,6 +215,8 @@ struct Part {
 struct Plan {
   Part part[2];
   int parts;
+  // Both lists in one launch: heads of 64, tiles of 128 rows and of 16 (attn_mixed_kernel).
+  static bool together(int64_t D, int tile, int few) { return D == 64 && tile == 128 && few == 16; }
 };
 
 bool tiled(int64_t D) { return D == 64 || D == 96 || D == 128 || D == 256; }
@@ -230,6 +232,10 @@ bool tiled(int64_t D) { return D == 64 || D == 96 || D == 128 || D == 256; }
 // Short sequences are those of up to 16 rows, or up to 32 where more than 16 heads share a cached one, so that
 // decoding stays among them (15 decoding sequences and a chunk of 403, groups of 24: 87 us, 92 with up to 16
 // rows; it loses with 63 of them, 120 and 112, and in groups of 32, 83 and 67).
+//
+// Heads of 64 take both lists in one launch (24 sequences of 1925 tokens, 14 heads on 2 over a window of 1000: 42 us in
+// two, 36.5 in one), which repays itself from 8192 rows of all heads on: 12 heads of their own over 4 bits 75 us in one
+// list, 69 so; 4 heads of their own (7700 rows) 37 and 39.5.
 //
 // That the sequences divide the tokens is a guess at equal chunks, and a mixture (or a padded batch) may meet
 // it by chance. Both sides, one list and two, 32 heads on 8 of 128 over 1500 to 6000 cached tokens and over 50
@@ -249,7 +255,7 @@ Plan plan_of(int64_t T, int64_t S, int64_t HK, int64_t group, int64_t D) {
   const int64_t all = T * group * HK;
   const int tile = D > 128 ? (all < 4 * 128 ? 16 : 128) : all < 22 * 128 ? 64 : all < 384 * 256 ? 128 : 256;
   Plan p{};
-  if (T > S && T % S != 0 && T * group > 2048) {
+  if (T > S && T % S != 0 && (T * group > 2048 || (p.together(D, tile, few) && all >= 8192))) {
     p.parts = 2;
     p.part[0] = {tile, few, INT32_MAX};
     p.part[1] = {few, 0, few};
@@ -318,7 +324,8 @@ int launch_tiled(AttnArgs a, bool bf16, int cache, int forms, float* workspace, 
   size_t need = 0;
   for (int i = 0; i < plan.parts; ++i) need += part_bytes(plan.part[i], a.T, a.S, a.group, a.HK, a.D, cache, a.most_kv);
   AttnJoin join{};
-  int lists = 0;
+  AttnArgs first{};
+  int lists = 0, first_items = 0;
   for (int i = 0; i < plan.parts; ++i) {
     const Part& p = plan.part[i];
     const int64_t slots = slots_bound(p, a.T, a.S, a.group, a.HK, a.D, cache, a.most_kv);
@@ -336,8 +343,16 @@ int launch_tiled(AttnArgs a, bool bf16, int cache, int forms, float* workspace, 
                    "%lld tiles of %d heads exceed the %lld workgroups that a launch covers", (long long)tiles, a.HK,
                    (long long)((int64_t)1 << 23));
     const int items = (int)(tiles + a.target);
-    const int status = kLaunchAttn[cache][forms][bf16](a, items, p.rows, stream);
-    if (status != INTENT_OK) return status;
+    // the short sequences' list of heads of 64 goes out with the tiles
+    const bool together = plan.parts == 2 && Plan::together(a.D, plan.part[0].rows, plan.part[1].rows);
+    if (together && i == 0) {
+      first = a, first_items = items;
+    } else {
+      LaunchAttn* const go = kLaunchAttn[cache][forms][bf16];
+      const int status = together ? go(first, first_items, 128, &a, items, stream)
+                                  : go(a, items, p.rows, nullptr, 0, stream);
+      if (status != INTENT_OK) return status;
+    }
     if (!split) continue;
     // a tile is split from one and a half shares on
     const int64_t most = a.target * 2 / 3 + 1;

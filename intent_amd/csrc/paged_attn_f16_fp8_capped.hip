@@ -1,6 +1,7 @@
 // The tiled attention kernels (paged_attn_mfma.h) of one type of heads, cache and form of scores.
 #include "paged_attn_mfma.h"
 
-int intent::launch_attn_f16_fp8_capped(const AttnArgs& a, int items, int rows, hipStream_t stream) {
-  return attn::launch_any<false, kCacheFp8, kCapped>(a, items, rows, stream);
+int intent::launch_attn_f16_fp8_capped(const AttnArgs& a, int items, int rows, const AttnArgs* few, int few_items,
+                             hipStream_t stream) {
+  return attn::launch_any<false, kCacheFp8, kCapped>(a, items, rows, few, few_items, stream);
 }

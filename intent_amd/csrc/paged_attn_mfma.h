@@ -385,8 +385,7 @@ constexpr int rows_waves(int cache, int forms, int D, int mt) {
 }
 
 template <bool kBf16, int kCache, int kForms, int D, int MT>
-__global__ __launch_bounds__(256, rows_waves(kCache, kForms, D, MT))
-    void attn_rows_kernel(const AttnArgs a) {
+INTENT_DEVICE void attend_rows(const AttnArgs& a, int block) {
   constexpr bool kFp8 = kCache == kCacheFp8, kInt4 = kCache == kCacheInt4;
   constexpr bool kMath = kBf16 && !kInt4;              // products in bf16
   constexpr bool kBiased = kForms != kPlain;
@@ -404,9 +403,9 @@ __global__ __launch_bounds__(256, rows_waves(kCache, kForms, D, MT))
   __shared__ __attribute__((aligned(16))) float scales[kFp8 ? 4 : 1][3][32];
   __shared__ float stats[4][16][2];
 
-  const int head = blockIdx.x % a.HK;
+  const int head = block % a.HK;
   Span w;
-  if (!find_span<kBiased>(a, 16 * MT, 7, blockIdx.x / a.HK, false, w)) return;
+  if (!find_span<kBiased>(a, 16 * MT, 7, block / a.HK, false, w)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int col = lane & 15, g = lane >> 4;
 
@@ -779,6 +778,11 @@ __global__ __launch_bounds__(256, rows_waves(kCache, kForms, D, MT))
   }
 }
 
+template <bool kBf16, int kCache, int kForms, int D, int MT>
+__global__ __launch_bounds__(256, rows_waves(kCache, kForms, D, MT)) void attn_rows_kernel(const AttnArgs a) {
+  attend_rows<kBf16, kCache, kForms, D, MT>(a, (int)blockIdx.x);
+}
+
 // ---- many rows: 128 or 256, 32 to a wave, all of them over the same tokens ----------------------------
 
 // 64 tokens of keys and values in LDS at a time, in two buffers: the next ones are loaded into
@@ -803,8 +807,7 @@ __global__ __launch_bounds__(256, rows_waves(kCache, kForms, D, MT))
 // keys by four of eight waves and values by the other four, 3% less than both by the first four. Their stores meet four
 // to a bank; to turn them apart costs more registers and selects than it gains (1220 against 1195 us).
 template <bool kBf16, int kCache, int kForms, int D, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
-    void attn_tile_kernel(const AttnArgs a) {
+INTENT_DEVICE void attend_tile(const AttnArgs& a, int block) {
   constexpr bool kFp8 = kCache == kCacheFp8, kInt4 = kCache == kCacheInt4;
   constexpr bool kMath = kBf16 && !kInt4;             // products in bf16
   constexpr bool kBiased = kForms != kPlain;
@@ -826,9 +829,9 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
   __shared__ __attribute__((aligned(16))) float scales[kFp8 ? 2 : 1][3][64];
   __shared__ int left_out;  // values that are not finite were left out of a product
 
-  const int head = blockIdx.x % a.HK;
+  const int head = block % a.HK;
   Span w;
-  if (!find_span<kBiased>(a, ROWS, 6, blockIdx.x / a.HK, false, w)) return;
+  if (!find_span<kBiased>(a, ROWS, 6, block / a.HK, false, w)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int col = lane & 31, h = lane >> 5;
   const int r0 = wave * 32;
@@ -1255,6 +1258,19 @@ __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1)
   }
 }
 
+template <bool kBf16, int kCache, int kForms, int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1) void attn_tile_kernel(const AttnArgs a) {
+  attend_tile<kBf16, kCache, kForms, D, WAVES>(a, (int)blockIdx.x);
+}
+
+// Both lists of a mixture of heads of 64 in one launch, whose registers and LDS let three workgroups of either share a
+// CU: tiles of 128 rows in the first `tiles` workgroups, sequences of up to 16 rows in the others.
+template <bool kBf16, int kCache, int kForms>
+__global__ __launch_bounds__(256, 3) void attn_mixed_kernel(const AttnArgs a, const AttnArgs b, int tiles) {
+  if ((int)blockIdx.x < tiles) attend_tile<kBf16, kCache, kForms, 64, 4>(a, (int)blockIdx.x);
+  else attend_rows<kBf16, kCache, kForms, 64, 1>(b, (int)blockIdx.x - tiles);
+}
+
 // ---- the join of split tiles ---------------------------------------------------------------------
 
 // out = sum_j w_j O_j / sum_j w_j l_j, w_j = exp2(M_j - max M), over the parts of a tile in a fixed order.
@@ -1405,7 +1421,15 @@ int launch_d(const AttnArgs& a, int items, int rows, hipStream_t stream) {
 }
 
 template <bool kBf16, int kCache, int kForms = kPlain>
-int launch_any(const AttnArgs& a, int items, int rows, hipStream_t stream) {
+int launch_any(const AttnArgs& a, int items, int rows, const AttnArgs* few, int few_items, hipStream_t stream) {
+  if (few != nullptr) {
+    const int tiles = items * a.HK;
+    hipLaunchKernelGGL((attn_mixed_kernel<kBf16, kCache, kForms>), dim3((unsigned)tiles + (unsigned)few_items * a.HK),
+                       dim3(256), 0, stream, a, *few, tiles);
+    static const KernelName name("attn_mixed_kernel<%s%s%s>", kBf16 ? "bf16" : "f16", cache_name(kCache),
+                                 form_name(kForms));
+    return launch_status(name.text);
+  }
   switch (a.D) {
     case 64: return launch_d<kBf16, kCache, kForms, 64>(a, items, rows, stream);
     case 96: return launch_d<kBf16, kCache, kForms, 96>(a, items, rows, stream);
