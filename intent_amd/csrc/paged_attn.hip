@@ -200,14 +200,17 @@ struct Part {
   // 2048: 64 sequences of 300 to 8191 tokens 87, 89 and 83 us, four of 60000 to 131000 88, 89 and 90, their join 6.0,
   // 7.4 and 10.0. 48 rows of heads of 64: 64 sequences 116 us at 1536, 110 at 768, six of them 26 at 768, 22 at 512.
   // Tiles of 128 rows of heads of 64: 1925 tokens of 24 sequences, 12 heads, kernel and join, 75 us at 512, 71 at 1024.
+  // The two lists of a mixture of heads of 64 even one another out: the same batch in both, tiles and short sequences
+  // at 1024 and 2048 70 us, at 1024 and 1024 67, at 512 and 1024 65, at 512 and 512 66.
   int fill(int64_t D, int cache, int64_t lists) const {
+    const bool mixture = min_rows > 0 || max_rows != INT32_MAX;
     if (cache == kCacheInt4 && rows <= 64) {
       if (D > 128) return 512;
-      if (rows == 16) return lists >= 256 ? 2048 : 1024;
-      if (rows * D <= 3072 && lists >= 256) return rows * D <= 2048 ? 1536 : 768;
+      if (rows == 16) return lists >= 256 && !(D == 64 && mixture) ? 2048 : 1024;
+      if (rows * D < 4096 && lists >= 256) return rows * D <= 2048 ? 1536 : 768;
       return rows * D <= 2048 ? 768 : rows * D <= 6144 ? 512 : 256;
     }
-    if (rows > 64) return rows == 256 || D > 128 ? 256 : cache == kCacheInt4 && D == 64 ? 1024 : 512;
+    if (rows > 64) return rows == 256 || D > 128 ? 256 : cache == kCacheInt4 && D == 64 && !mixture ? 1024 : 512;
     return D > 128 ? 256 : rows * D <= 2048 ? 1536 : rows * D <= 4096 ? 512 : 256;
   }
 };
