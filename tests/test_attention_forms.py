@@ -385,6 +385,28 @@ def test_biased_paged_attention(gpu, at, cache):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("cache", ["same", "fp8", "int4"])
+@pytest.mark.parametrize("forms", range(5))
+def test_chunks_beside_short_sequences(gpu, forms, cache, dt):
+    """Heads of 64, chunks and sequences on both sides of 16 rows of a head, rows of no sequence before and behind:
+    scores without a form, capped, biased by distance, both, and a prefix alone."""
+    lens = [(1, 3000), (300, 700), (1, 33), (17, 400), (16, 90), (200, 200), (0, 40), (9, 0), (129, 131), (1, 1), (2, 500)]
+    HQ, HK, window = ((12, 12, 0), (14, 2, 150))[(forms + (dt == "f16")) % 2]
+    inputs = list(_inputs(41, dt, cache, lens, HQ, HK, 64, 16, q_std=4.0 if forms in (1, 3) else 1.5, spare=38))
+    inputs[3] = inputs[3] + 20
+    more = {"cap": 20.0 if forms in (1, 3) else 0.0,
+            "slopes": (2.0 ** (-8.0 * torch.arange(1, HQ + 1) / HQ)).float() if forms in (2, 3) else None,
+            "prefix": _prefixes(lens, forms) if forms >= 3 else None}
+    want, tol = ref_attention(inputs[0], inputs[1], cache, *inputs[2:], 0.125, True, window, fine=True, **more)
+    out = torch.full_like(inputs[0], 7.0, device="cuda")
+    got = _attend(inputs, dt, cache, 0.125, True, window, out=out, **more).cpu()
+    inside = ~want.isnan().flatten(1).any(1)
+    assert int(inside.sum()) == sum(n for n, _ in lens) and bool((got[~inside] == 7).all())
+    _close(got[inside], want[inside], tol[inside])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("cache", ["same", "fp8"])
 @pytest.mark.parametrize("lens", [[(1, 900), (1, 33)], [(70, 200)]], ids=str)
 def test_biased_without_forms_is_the_plain_attention(gpu, cache, lens):
