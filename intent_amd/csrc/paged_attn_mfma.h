@@ -384,8 +384,18 @@ constexpr int rows_waves(int cache, int forms, int D, int mt) {
   return D > 128 ? 1 : mt * D <= 128 ? 3 : mt * D <= 256 ? 2 : 1;
 }
 
+// Its LDS: the waves' values, then the joining buffer in their place.
+template <bool kFp8, int D>
+struct RowsShared {
+  static constexpr int OB = D + 4;  // floats of a row in the joining buffer
+  static constexpr int kValues = 4 * 32 * row_bytes<D>(), kJoin = 4 * 16 * OB * 4;
+  __attribute__((aligned(16))) char lds[kValues > kJoin ? kValues : kJoin];
+  __attribute__((aligned(16))) float scales[kFp8 ? 4 : 1][3][32];
+  float stats[4][16][2];
+};
+
 template <bool kBf16, int kCache, int kForms, int D, int MT>
-INTENT_DEVICE void attend_rows(const AttnArgs& a, int block) {
+INTENT_DEVICE void attend_rows(const AttnArgs& a, int block, RowsShared<kCache == kCacheFp8, D>& shared) {
   constexpr bool kFp8 = kCache == kCacheFp8, kInt4 = kCache == kCacheInt4;
   constexpr bool kMath = kBf16 && !kInt4;              // products in bf16
   constexpr bool kBiased = kForms != kPlain;
@@ -397,11 +407,10 @@ INTENT_DEVICE void attend_rows(const AttnArgs& a, int block) {
   constexpr int LOADS = D / 4 / ELEMS, CHUNKS = ELEMS / 8;  // loads, and 16 bytes of 16-bit elements of one
   constexpr int kRow = cached_bytes<kCache, D>(), kParams = cached_params<kCache, D>();
   constexpr int kLoad = kRow / 4 / LOADS;              // bytes of a load
-  constexpr int OB = D + 4;                            // floats of a row in the joining buffer
-  constexpr int kLds = 4 * 32 * RB > 4 * 16 * OB * 4 ? 4 * 32 * RB : 4 * 16 * OB * 4;
-  __shared__ __attribute__((aligned(16))) char lds[kLds];
-  __shared__ __attribute__((aligned(16))) float scales[kFp8 ? 4 : 1][3][32];
-  __shared__ float stats[4][16][2];
+  constexpr int OB = RowsShared<kFp8, D>::OB;
+  auto& lds = shared.lds;
+  auto& scales = shared.scales;
+  auto& stats = shared.stats;
 
   const int head = block % a.HK;
   Span w;
@@ -780,7 +789,8 @@ INTENT_DEVICE void attend_rows(const AttnArgs& a, int block) {
 
 template <bool kBf16, int kCache, int kForms, int D, int MT>
 __global__ __launch_bounds__(256, rows_waves(kCache, kForms, D, MT)) void attn_rows_kernel(const AttnArgs a) {
-  attend_rows<kBf16, kCache, kForms, D, MT>(a, (int)blockIdx.x);
+  __shared__ RowsShared<kCache == kCacheFp8, D> shared;
+  attend_rows<kBf16, kCache, kForms, D, MT>(a, (int)blockIdx.x, shared);
 }
 
 // ---- many rows: 128 or 256, 32 to a wave, all of them over the same tokens ----------------------------
@@ -806,8 +816,15 @@ __global__ __launch_bounds__(256, rows_waves(kCache, kForms, D, MT)) void attn_r
 // widened on their way to LDS, 16 bytes of a token to a lane (heads of 64: 8), between a load's arrival and the barrier:
 // keys by four of eight waves and values by the other four, 3% less than both by the first four. Their stores meet four
 // to a bank; to turn them apart costs more registers and selects than it gains (1220 against 1195 us).
+template <bool kFp8, int D>
+struct TileShared {
+  __attribute__((aligned(16))) char lds[2][2][64 * row_bytes<D>()];
+  __attribute__((aligned(16))) float scales[kFp8 ? 2 : 1][3][64];
+  int left_out;  // values that are not finite were left out of a product
+};
+
 template <bool kBf16, int kCache, int kForms, int D, int WAVES>
-INTENT_DEVICE void attend_tile(const AttnArgs& a, int block) {
+INTENT_DEVICE void attend_tile(const AttnArgs& a, int block, TileShared<kCache == kCacheFp8, D>& shared) {
   constexpr bool kFp8 = kCache == kCacheFp8, kInt4 = kCache == kCacheInt4;
   constexpr bool kMath = kBf16 && !kInt4;             // products in bf16
   constexpr bool kBiased = kForms != kPlain;
@@ -822,12 +839,11 @@ INTENT_DEVICE void attend_tile(const AttnArgs& a, int block) {
   constexpr int EACH = 64 / SPREAD;                   // tokens that a wave loads at once
   constexpr int STEP = EACH * WAVES;                  // and the workgroup
   constexpr int LOADS = STEP >= 64 ? 1 : 64 / STEP, ROWS = 32 * WAVES;
-  constexpr int kTile = 64 * RB;
   // Whether the scores of the next 64 tokens are computed during the softmax of these.
   constexpr bool kAhead = D > 64;
-  __shared__ __attribute__((aligned(16))) char lds[2][2][kTile];
-  __shared__ __attribute__((aligned(16))) float scales[kFp8 ? 2 : 1][3][64];
-  __shared__ int left_out;  // values that are not finite were left out of a product
+  auto& lds = shared.lds;
+  auto& scales = shared.scales;
+  int& left_out = shared.left_out;
 
   const int head = block % a.HK;
   Span w;
@@ -1260,15 +1276,22 @@ INTENT_DEVICE void attend_tile(const AttnArgs& a, int block) {
 
 template <bool kBf16, int kCache, int kForms, int D, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, D == 64 ? 3 : D <= 128 ? 2 : 1) void attn_tile_kernel(const AttnArgs a) {
-  attend_tile<kBf16, kCache, kForms, D, WAVES>(a, (int)blockIdx.x);
+  __shared__ TileShared<kCache == kCacheFp8, D> shared;
+  attend_tile<kBf16, kCache, kForms, D, WAVES>(a, (int)blockIdx.x, shared);
 }
 
 // Both lists of a mixture of heads of 64 in one launch, whose registers and LDS let three workgroups of either share a
-// CU: tiles of 128 rows in the first `tiles` workgroups, sequences of up to 16 rows in the others.
+// CU: tiles of 128 rows in the first `tiles` workgroups, sequences of up to 16 rows in the others. The two take the same
+// LDS: side by side they are 53764 bytes with 8 bits, of which a CU holds two (six chunks of 300 to 700 tokens over 500
+// to 3000, 16 heads on 8: 90 us, 74 so; 127 decoding sequences and a chunk of 600, 32 heads on 8: 122 and 100).
 template <bool kBf16, int kCache, int kForms>
 __global__ __launch_bounds__(256, 3) void attn_mixed_kernel(const AttnArgs a, const AttnArgs b, int tiles) {
-  if ((int)blockIdx.x < tiles) attend_tile<kBf16, kCache, kForms, 64, 4>(a, (int)blockIdx.x);
-  else attend_rows<kBf16, kCache, kForms, 64, 1>(b, (int)blockIdx.x - tiles);
+  __shared__ union {
+    TileShared<kCache == kCacheFp8, 64> tile;
+    RowsShared<kCache == kCacheFp8, 64> rows;
+  } shared;
+  if ((int)blockIdx.x < tiles) attend_tile<kBf16, kCache, kForms, 64, 4>(a, (int)blockIdx.x, shared.tile);
+  else attend_rows<kBf16, kCache, kForms, 64, 1>(b, (int)blockIdx.x - tiles, shared.rows);
 }
 
 // ---- the join of split tiles ---------------------------------------------------------------------
