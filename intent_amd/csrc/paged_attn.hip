@@ -237,8 +237,21 @@ bool tiled(int64_t D) { return D == 64 || D == 96 || D == 128 || D == 256; }
 // rows; it loses with 63 of them, 120 and 112, and in groups of 32, 83 and 67).
 //
 // Heads of 64 take both lists in one launch (24 sequences of 1925 tokens, 14 heads on 2 over a window of 1000: 42 us in
-// two, 36.5 in one), which repays itself from 8192 rows of all heads on: 12 heads of their own over 4 bits 75 us in one
-// list, 69 so; 4 heads of their own (7700 rows) 37 and 39.5.
+// two, 36.5 in one), which repays itself below 2048 rows too, from 8192 rows of all heads on (12 heads of their own over
+// 4 bits 75 us in one list, 69 so; 4 heads of their own, 7700 rows, 37 and 39.5), where the mean sequence has more rows
+// than the kernel of few rows takes. Below that one list runs by that kernel, and a second one only takes from it. Of
+// heads of their own unless a number says otherwise, one list and two in us, over 500 to 3000 cached tokens in 16, 8
+// and 4 bits:
+//   20 decoding and three chunks of 300, 16 heads on 8     42 and 38, 58 and 38, 46 and 36
+//   24 of 1 to 600 new tokens, 12 heads                    67 and 57, 87 and 71, 70 and 61
+//   chunks alone, 4 of 300, 32 heads                       56 and 56, 73 and 74, 58 and 63
+//   16 of 10 to 60, 32 heads (mean 35 rows)                64 and 76, 54 and 99, 51 and 79
+//   31 decoding and a chunk of 200, 64 heads (mean 7)      178 and 191, 93 and 115, 79 and 104
+//   64 of 1 to 8 drafted tokens, 32 heads on 8 (mean 18)   58 and 57, 36 and 57, 34 and 44
+// Short caches do not repay it either: 24 of 1 to 600 over 50 to 400 tokens 25 and 29, 31 and 35, 28 and 31; over 200
+// to 800 31 and 31, 40 and 37, 35 and 34. A table of up to 1024 tokens holds nothing longer. What the extents do not
+// tell still loses: a prompt of 1990 beside 30 sequences of one token and no cache, 8 heads, 25 and 29; chunks alone
+// over 4 bits, 8 of 100 to 200 over 2000 to 6000, 16 heads, 66 and 82.
 //
 // That the sequences divide the tokens is a guess at equal chunks, and a mixture (or a padded batch) may meet
 // it by chance. Both sides, one list and two, 32 heads on 8 of 128 over 1500 to 6000 cached tokens and over 50
@@ -252,13 +265,14 @@ bool tiled(int64_t D) { return D == 64 || D == 96 || D == 128 || D == 256; }
 // head over 917 21 and 21; 512 x 4 of eight over 512 22 and 20). Tiles of 256 halve what is loaded for a row
 // but need one and a half rounds of them to even out (4096 x 4 rows of eight heads over 4096: 157 us, 163 in
 // tiles of 128; 2048 x 4 over 2048: 71 and 59).
-Plan plan_of(int64_t T, int64_t S, int64_t HK, int64_t group, int64_t D) {
+Plan plan_of(int64_t T, int64_t S, int64_t HK, int64_t group, int64_t D, int64_t most_kv) {
   const int64_t mean = (T * group + S - 1) / S;
   const int most = D > 128 ? 32 : 64, few = D > 128 || group <= 16 ? 16 : 32;
   const int64_t all = T * group * HK;
   const int tile = D > 128 ? (all < 4 * 128 ? 16 : 128) : all < 22 * 128 ? 64 : all < 384 * 256 ? 128 : 256;
   Plan p{};
-  if (T > S && T % S != 0 && (T * group > 2048 || (p.together(D, tile, few) && all >= 8192))) {
+  const bool repaid = p.together(D, tile, few) && all >= 8192 && mean > most && most_kv > 1024;
+  if (T > S && T % S != 0 && (T * group > 2048 || repaid)) {
     p.parts = 2;
     p.part[0] = {tile, few, INT32_MAX};
     p.part[1] = {few, 0, few};
@@ -323,7 +337,7 @@ LaunchJoin* const kLaunchJoin[2][2] = {{launch_join_f16, launch_join_bf16},
                                        {launch_join_f16_prefix, launch_join_bf16_prefix}};
 
 int launch_tiled(AttnArgs a, bool bf16, int cache, int forms, float* workspace, size_t bytes, hipStream_t stream) {
-  const Plan plan = plan_of(a.T, a.S, a.HK, a.group, a.D);
+  const Plan plan = plan_of(a.T, a.S, a.HK, a.group, a.D, a.most_kv);
   size_t need = 0;
   for (int i = 0; i < plan.parts; ++i) need += part_bytes(plan.part[i], a.T, a.S, a.group, a.HK, a.D, cache, a.most_kv);
   AttnJoin join{};
@@ -386,7 +400,7 @@ extern "C" size_t intent_biased_paged_attention_workspace_size(int64_t T, int64_
   if (T <= 0 || HQ <= 0 || HK <= 0 || S <= 0 || HQ % HK || table_width <= 0 || page_size <= 0 || !tiled(D) ||
       table_width > kMostTokens / page_size || HQ > 65536 || T * HQ >= ((int64_t)1 << 25))
     return 0;
-  const Plan plan = plan_of(T, S, HK, HQ / HK, D);
+  const Plan plan = plan_of(T, S, HK, HQ / HK, D, table_width * page_size);
   size_t need = 0;
   for (int i = 0; i < plan.parts; ++i)
     need += part_bytes(plan.part[i], T, S, HQ / HK, HK, D, cache_format, table_width * page_size);

@@ -5,6 +5,7 @@ from pathlib import Path
 
 import pytest
 
+from intent_amd import _native
 from intent_amd import build as B
 from intent_amd import codeobj_check as C
 
@@ -24,3 +25,29 @@ def test_three_workgroups_of_both_lists_share_a_cu(tmp_path, cache):
     notes = C._run([C._tool("llvm-readelf"), "--notes", str(code)])
     sizes = [int(n) for n in re.findall(r"\.group_segment_fixed_size:\s+(\d+)", notes)]
     assert len(sizes) == 1 and 3 * (-(-sizes[0] // LDS_STEP) * LDS_STEP) <= LDS_OF_A_CU
+
+
+def _scratch(T, S, HQ, HK, cache, tokens=4096):
+    """Bytes for the parts of a batch of heads of 64: two lists of tiles need others than one."""
+    return _native.library().intent_biased_paged_attention_workspace_size(T, HQ, HK, 64, S, tokens // 32, 32, cache)
+
+
+@pytest.mark.parametrize("cache", [0, 1, 2])
+@pytest.mark.parametrize("T,S,HQ,HK", [(301, 100, 32, 32), (101, 40, 128, 8), (301, 64, 32, 8), (561, 16, 32, 32),
+                                       (841, 24, 12, 12), (363, 64, 32, 32), (231, 32, 64, 64)])
+def test_batches_of_few_rows_take_one_list(T, S, HQ, HK, cache):
+    """Drafts, and a small chunk beside decoding sequences: mean sequences of up to 64 rows and up to 2048 rows of a
+    cached head in all take the same plan whether or not the sequences divide the tokens."""
+    assert T % S and T * HQ // HK <= 2048 and T * HQ >= 8192
+    even = T // S * S if -(-(T // S * HQ // HK) // 16) == -(-(-(-T * HQ // HK // S)) // 16) else -(-T // S) * S
+    assert _scratch(T, S, HQ, HK, cache) == _scratch(even, S, HQ, HK, cache)
+
+
+@pytest.mark.parametrize("cache", [0, 1, 2])
+@pytest.mark.parametrize("T,S,HQ,HK", [(1925, 24, 12, 12), (929, 23, 16, 8), (1519, 13, 12, 12), (1921, 24, 14, 2)])
+def test_chunks_beside_decoding_sequences_take_two(T, S, HQ, HK, cache):
+    """Mean sequences of more than 64 rows, where the table holds more than 1024 tokens, or more than 2048 rows."""
+    one = _scratch(T // S * S, S, HQ, HK, cache)
+    assert _scratch(T, S, HQ, HK, cache) != one
+    short = _scratch(T, S, HQ, HK, cache, 1024) != _scratch(T // S * S, S, HQ, HK, cache, 1024)
+    assert short == (T * HQ // HK > 2048)
