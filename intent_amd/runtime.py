@@ -80,6 +80,7 @@ class _Layout:
     workspace: int      # bytes, -1 without one
     scratch: int        # bytes of a launch's own scratch
     template: _Template | None = None
+    made_out: bool = False  # whether `template` is: by the layout's second call, for many a layout comes but once
 
 
 MAX_LAYOUTS = 256  # layouts kept per artifact and calling form; the oldest go first
@@ -183,6 +184,10 @@ class HIPRuntime:
         elif supplied_outputs:
             outputs = tuple(t for t, name in zip(tensors, known.names) if name in self._outputs)
         workspace = self._buffer_of(known.workspace, known.scratch)
+        if not known.made_out:
+            made = tuple(name for name, *_ in known.outputs)
+            views = dict(zip(known.names + made, (*tensors, *outputs) if made else tensors))
+            known.template, known.made_out = self._template(params, views, env, known.scratch), True
         template = known.template
         if template is not None and (workspace is not None or not template.scratch):
             values = template.arguments.copy()
@@ -220,18 +225,16 @@ class HIPRuntime:
         if len(known) >= MAX_LAYOUTS:
             for old in list(known)[:MAX_LAYOUTS // 2]:
                 known.pop(old, None)
-        template = self._template(params, binding, [p.name for p, _ in views] + [out[0] for out in made], scratch)
-        known[key] = _Layout(dict(binding.env), tuple(p.name for p, _ in views), made, spans, pairs, workspace, scratch,
-                             template)
+        known[key] = _Layout(dict(binding.env), tuple(p.name for p, _ in views), made, spans, pairs, workspace, scratch)
 
-    def _template(self, params: tuple, binding: Binding, names: list, scratch: int) -> _Template | None:
+    def _template(self, params: tuple, views: dict, env: dict, scratch: int) -> _Template | None:
         """The call that a layout makes, from views and scalars that are told apart by their values; None where the
         launch is not one call of one entry, or takes a scalar in another form than its own."""
         definition = self.definition
         if definition.call is None:
             return None
-        address = {name: (1 << 60) + 16 * i for i, name in enumerate(names)}
-        env, marks = dict(binding.env), {}
+        address = {name: (1 << 60) + 16 * i for i, name in enumerate(views)}
+        env, marks = dict(env), {}
         for position, p in enumerate(params):
             if p.name in self._scalars:
                 marks[p.name] = (position, -(1.0 + position) * 2.0 ** -77)
@@ -241,7 +244,7 @@ class HIPRuntime:
             import torch
 
             buffer = _Probe(torch.empty(scratch, dtype=torch.uint8, device="meta"), own)
-        entry, arguments = definition.call({n: _Probe(binding.views[n], a) for n, a in address.items()}, env, buffer)
+        entry, arguments = definition.call({n: _Probe(views[n], a) for n, a in address.items()}, env, buffer)
         index = {a: i for i, a in enumerate(address.values())}
         at = list(enumerate(arguments))
         scalars = tuple((n, position) for position, mark in marks.values() for n, v in at if v == mark)

@@ -4,10 +4,12 @@ import shutil
 from pathlib import Path
 
 import pytest
+import torch
 
 from intent_amd import _native
 from intent_amd import build as B
 from intent_amd import codeobj_check as C
+from test_attention import runtime_for
 
 LDS_OF_A_CU, LDS_STEP = 160 * 1024, 1280  # gfx950 gives LDS out in steps of 320 words
 
@@ -51,3 +53,22 @@ def test_chunks_beside_decoding_sequences_take_two(T, S, HQ, HK, cache):
     assert _scratch(T, S, HQ, HK, cache) != one
     short = _scratch(T, S, HQ, HK, cache, 1024) != _scratch(T // S * S, S, HQ, HK, cache, 1024)
     assert short == (T * HQ // HK > 2048)
+
+
+def test_a_layout_that_comes_once_is_not_made_out(monkeypatch):
+    """The call of a layout is made out when it comes again: first calls of a program whose token count changes with
+    every step do not pay for it."""
+    rt = runtime_for("paged_kv_read")
+    rt._home = torch.device("cpu")
+    monkeypatch.setattr(_native, "call_packed", lambda entry, arguments, stream: None)
+    monkeypatch.setattr("intent_amd.runtime._current_stream", lambda device: 0)
+    calls = []
+    monkeypatch.setattr(rt, "_template", lambda *a, make=rt._template: calls.append(a) or make(*a))
+    caches = [torch.zeros(3, 2, 8, 64).half() for _ in range(2)]
+    for n in range(1, 6):
+        rt.run(*caches, torch.zeros(n, dtype=torch.int32))
+    assert not calls
+    for _ in range(3):
+        bound = rt.rebind((*caches, torch.zeros(4, dtype=torch.int32)), False)
+        assert bound.call is not None and bound.outputs[0].shape == (4, 2, 64)
+    assert len(calls) == 1
