@@ -775,6 +775,10 @@ size_t intent_paged_attention_workspace_size(int64_t T, int64_t HQ, int64_t HK, 
  * With y clamped to +-61440 (so that lowest + 15 scale is an f16):
  *   scale = f16((max y - min y) * f32(1 / 15)), lowest = f16(min y),
  *   code = clamp(rint((y - lowest) / scale), 0, 15), 0 where the scale is 0.
+ * A value is max(scale / 2, 2^-11 (|min y| + 15 scale) + 2^-21) off at most: the
+ * second is what rounding the pair to f16 moves a group's ends by, which counts for
+ * groups far off zero (offsets of 100 ranges and more) and for ranges of f16's
+ * subnormals; one of up to 15 * 2^-25 reads as its lowest value.
  * A group that holds an infinity or NaN has scale 0 and lowest NaN: it reads as
  * NaN. A slot given twice may end with codes of one token and groups of the
  * other. Everything else as in intent_paged_kv_append. No reference counterpart.

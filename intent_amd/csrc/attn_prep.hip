@@ -9,8 +9,11 @@
 //            s = max(absmax, 1e-12) / 448, code = e4m3fn(clamp(y / s, +-448)): the groupwise FP8
 //            quantizer's rule with one group for each head; or 4 bits (cache4.h), y clamped to +-61440,
 //            s = f16((max - min) * f32(1 / 15)), m = f16(min) of each group of 32 elements,
-//            code = clamp(rint((y - m) / s), 0, 15). s and m are rounded before the codes are found, so that
-//            these make up for it; the clamp keeps m + 15 s inside f16.
+//            code = clamp(rint((y - m) / s), 0, 15). s and m are rounded before the codes are found: inside
+//            m .. m + 15 s a value is s / 2 off at most, whatever that rounding did. It moves the two ends, by up
+//            to 2^-11 (|min| + 15 s) + 2^-21, and an element past them takes the end: at an offset of 100 times the
+//            range 0.7 of an exact step, of 1000 times 8. A range of up to 15 * 2^-25 rounds to s = 0, and all of
+//            the group reads as m. The clamp to +-61440 keeps m + 15 s inside f16.
 //
 // All of it in f32; each result is rounded once, when it is stored (y is not rounded between
 // the norm, the rotation and the encoding). Values are neither normed nor rotated.

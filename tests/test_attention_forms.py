@@ -193,6 +193,31 @@ def test_paged_kv_append_int4_extremes(gpu):
         assert bool(values[5].half().isfinite().all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+def test_int4_values_are_as_near_as_stated(gpu, dt):
+    """Groups far off zero and of small ranges: half a scale, or what rounding the pair to f16 moves the ends by."""
+    T, HK, D, PAGE, pages = 256, 2, 128, 16, 17
+    gen = _gen(6)
+    offset = 10.0 ** torch.linspace(-8, 4.2, T)[:, None, None] * (1 - 2 * torch.randint(0, 2, (T, HK, 1), generator=gen))
+    reach = 10.0 ** -torch.linspace(0, 4, D // 32).repeat_interleave(32)
+    v = (offset * (1 + torch.rand(T, HK, D, generator=gen) * reach)).to(TYPES[dt])
+    caches, slots = _cuda(*_caches(gen, dt, "int4", pages, HK, PAGE, D)), torch.randperm(pages * PAGE, generator=gen)[:T].to(torch.int32)
+    none = torch.zeros(0, dtype=TYPES[dt])
+    _compile("paged_kv_append", dt, "int4").run(*_cuda(torch.zeros(T, 0, D, dtype=TYPES[dt]), v, v, none, none,
+                                                       torch.zeros(1, 0), slots, slots), *caches)
+    exact = v.double()
+    lowest = torch.stack([p.amin(-1) for p in exact.split(32, -1)], -1).repeat_interleave(32, -1)
+    for i in (0, 1):
+        pairs = _slot_rows(caches[2 + i].cpu(), slots)
+        scale, _ = spread4(pairs, D)
+        bound = torch.maximum(scale / 2, 2.0 ** -11 * (lowest.abs() + 15 * scale) + 2.0 ** -21)
+        # the code is found in f32: 2^-22 of what it is found from
+        off = (values4(_slot_rows(caches[i].cpu(), slots), pairs) - exact).abs()
+        assert bool((off <= bound + exact.abs() * 2.0 ** -22).all())
+        assert bool((scale == 0).any() and (off > scale / 2 * 1.001).any())  # both ends of the bound are met
+
+
 # ---- reading back ----------------------------------------------------------------------
 
 READ_CASES = [
