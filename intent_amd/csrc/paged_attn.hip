@@ -199,6 +199,14 @@ struct Part {
   // into parts enough by one, and their join costs more with every part. 16 rows of heads of 128, at 1024, 1536 and
   // 2048: 64 sequences of 300 to 8191 tokens 87, 89 and 83 us, four of 60000 to 131000 88, 89 and 90, their join 6.0,
   // 7.4 and 10.0. 48 rows of heads of 64: 64 sequences 116 us at 1536, 110 at 768, six of them 26 at 768, 22 at 512.
+  // Half as many as here, as many and twice as many, in us, for 64 sequences of 300 to 8191 tokens and for six of up to
+  // 30000, eight heads (with slopes the same in proportion):
+  //   32 rows of 64    90  82  82   37 31 42     48 of 64   127 107  99   53 41 45     64 of 64   143 163 125   58 48 56
+  //   32 rows of 96   151 133 124   49 44 48     48 of 96   155 161 140   54 50 59     64 of 96   170 187 159   66 59 72
+  //   32 rows of 128  130 145 119   53 42 51     48 of 128  159 178 147   64 54 64     64 of 128  291 291 295  165 81 89
+  //   16 rows of 64    57  59  63   27 26 34     16 of 96   115 111 115   39 39 48     16 of 256  230 227 191   72 64 72
+  // What is left there: 64 sequences on eight heads would take twice the 512; on one head they lose by it, as the six
+  // do (64 rows of 64: 30 us at 512, 43 at 1024).
   // Tiles of 128 rows of heads of 64: 1925 tokens of 24 sequences, 12 heads, kernel and join, 75 us at 512, 71 at 1024.
   // The two lists of a mixture of heads of 64 even one another out: the same batch in both, tiles and short sequences
   // at 1024 and 2048 70 us, at 1024 and 1024 67, at 512 and 1024 65, at 512 and 512 66.
